@@ -6,9 +6,10 @@ after a block fused with its gate and residual scale, forward and backward.
 Where `own` is true, run() makes the framework's calls; where it is false it
 computes the same from elementary torch operations in 32 bits.  Both take the
 operands of prepare().  A packed matrix of R rows and K columns is Q, uint8
-[R, Kp / 2] (two elements a byte, the first in the low four bits), and S,
-uint8 [R, Kp / 32], with Kp = K rounded up to a multiple of 128 and zeros
-behind column K.
+[R, Kp / 2] with Kp = K rounded up to a multiple of 256 (two elements a byte,
+the first in the low four bits), and S, uint8 [ceil(K / 512), R, 4, 4]: the
+scales of 512 columns of a row together, that of its block b (of 32 columns)
+at [b % 4, b / 4].  Elements and scales behind column K are zero.
 """
 from __future__ import annotations
 
@@ -98,8 +99,8 @@ _DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
 _ALPHA, _EPS = 0.875, 1e-5  # residual scale, and the term under the norms' roots
 
 
-def _padded(k: int) -> int:
-    return (k + 127) // 128 * 128
+def _padded(k: int, unit: int = 256) -> int:
+    return (k + unit - 1) // unit * unit
 
 
 def _gate_rows(c: dict) -> int:
@@ -165,7 +166,7 @@ def prepare(case: dict, seed: int) -> dict:
     op, u8, bf, f32 = case["op"], torch.uint8, torch.bfloat16, torch.float32
 
     def packed(rows, cols):
-        return _empty(u8, rows, _padded(cols) // 2), _empty(u8, rows, _padded(cols) // 32)
+        return _empty(u8, rows, _padded(cols) // 2), _empty(u8, _padded(cols, 512) // 512, rows, 4, 4)
 
     if op == "linear":
         s["Xq"], s["Y"] = packed(case["M"], case["K"]), _empty(bf, case["M"], case["N"])
@@ -297,7 +298,7 @@ def _e2m1(device):
 def _quantised(X: torch.Tensor):
     """(Q, S) of a matrix, along its rows."""
     R, K = X.shape
-    x = torch.nn.functional.pad(X.float(), (0, _padded(K) - K)).reshape(R, -1, 32)
+    x = torch.nn.functional.pad(X.float(), (0, _padded(K, 512) - K)).reshape(R, -1, 32)
     amax = x.abs().amax(-1)
     # 2^e scales the block so that its largest value falls into [4, 8); E2M1 ends at 6
     e = torch.where(amax > 0, torch.frexp(amax).exponent - 3, -127).clamp(min=-127)
@@ -306,15 +307,17 @@ def _quantised(X: torch.Tensor):
     # E2M1 steps by 0.5 below 2, by 1 below 4, by 2 below 8; codes 0-3, 4-5, 6-7 (halves to the even code)
     code = torch.where(a < 2, torch.round(a * 2), torch.where(a < 4, torch.round(a) + 2, torch.round(a * 0.5) + 4))
     code = code.clamp(max=7).to(torch.uint8) | ((y < 0) * 8).to(torch.uint8)
-    code = code.reshape(R, -1, 2)
-    return code[..., 0] | (code[..., 1] << 4), (e + 127).to(torch.uint8)
+    code = code.reshape(R, -1, 2)[:, :_padded(K) // 2]
+    S = (e + 127).to(torch.uint8).reshape(R, -1, 4, 4).permute(1, 0, 3, 2)
+    return code[..., 0] | (code[..., 1] << 4), S.contiguous()
 
 
 def _values(Q: torch.Tensor, S: torch.Tensor, K: int) -> torch.Tensor:
     """The fp32 values that a packed matrix stands for."""
-    code = torch.stack((Q & 15, Q >> 4), -1).reshape(Q.shape[0], -1, 32)
-    v = _e2m1(Q.device)[code.int()] * torch.exp2(S.float() - 127).unsqueeze(-1)
-    return v.reshape(Q.shape[0], -1)[:, :K]
+    R = Q.shape[0]
+    code = torch.stack((Q & 15, Q >> 4), -1).reshape(R, -1, 32)
+    scale = torch.exp2(S.float() - 127).permute(1, 0, 3, 2).reshape(R, -1)[:, :code.shape[1]]
+    return (_e2m1(Q.device)[code.int()] * scale.unsqueeze(-1)).reshape(R, -1)[:, :K]
 
 
 def _rounded(X: torch.Tensor) -> torch.Tensor:
@@ -431,7 +434,9 @@ def _exact_values(Q, S, K):
         exponent, mantissa = ((code >> 1) & 3).double(), (code & 1).double()
         size = torch.where(exponent > 0, (1 + mantissa / 2) * torch.exp2(exponent - 1), mantissa / 2)
         out[:, half::2] = torch.where(code >= 8, -size, size)
-    return (out * torch.exp2(S.double() - 127).repeat_interleave(32, 1))[:, :K]
+    block = torch.arange(K, device=Q.device) // 32  # of each column
+    scale = S[block // 16, :, block % 4, block % 16 // 4].t()
+    return out[:, :K] * torch.exp2(scale.double() - 127)
 
 
 def _exact_rounded(X):
