@@ -40,6 +40,9 @@ MIAIE_EUNSUPPORTED = -5
 MIAIE_EFAULT = -6
 B_NN = 0
 B_NT = 1
+F32 = 0   # element types of unpacked matrices (MIAIE_F32, MIAIE_BF16)
+BF16 = 1
+NORM_MAX_COLS = 16384
 
 _ERR_NAMES = {
     MIAIE_EINVAL: "MIAIE_EINVAL",
@@ -56,7 +59,7 @@ class MiaieError(RuntimeError):
         self.code = code
 
 
-_p, _i, _sz, _u64 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64
+_p, _i, _sz, _u64, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64, C.c_float
 _SIGS = {
     "miaie_init": (_i, [C.POINTER(_p), _i]),
     "miaie_init_on_stream": (_i, [C.POINTER(_p), _i, _p]),
@@ -83,6 +86,16 @@ _SIGS = {
     "miaie_conv2d_i8_nhwc": (_i, [_p, _p, _p, _p, _p] + [_i] * 9),
     "miaie_mlp_i8": (_i, [_p, _p, _p, _p, _p, _p] + [_i] * 6),
     "miaie_mlp_i8_noalloc": (_i, [_p, _p, _p, _p, _p] + [_i] * 6),
+    "miaie_mxfp4_q_pitch": (_sz, [_i]),
+    "miaie_mxfp4_q_bytes": (_sz, [_i, _i]),
+    "miaie_mxfp4_s_bytes": (_sz, [_i, _i]),
+    "miaie_quant_mxfp4": (_i, [_p, _p, _i, _i, _i, _i, _p, _p, _p, _p]),
+    "miaie_dequant_mxfp4": (_i, [_p, _p, _p, _p, _i, _i, _i, _i]),
+    "miaie_gemm_mxfp4": (_i, [_p] * 6 + [_i] * 5),
+    "miaie_gemm_mxfp4_rq": (_i, [_p] * 7 + [_i] * 4),
+    "miaie_mlp_mxfp4": (_i, [_p] * 10 + [_i] * 6),
+    "miaie_norm_block": (_i, [_p] * 9 + [_i] * 7 + [_f, _f]),
+    "miaie_norm_block_grad": (_i, [_p] * 15 + [_sz] + [_i] * 7 + [_f]),
     "miaie_fill_i8": (_i, [_p, _p, _sz, _u64]),
     "miaie_plan_gemm_i8": (_i, [_p, _i, _i, _i, _p]),
     "miaie_plan_set_cus": (_i, [_p, _i, C.POINTER(_i)]),
@@ -131,6 +144,17 @@ def plan_conv2d_i8(N, H, W, Cin, Cout, R=3, S=3, stride=1, pad=1) -> str:
     if rc != MIAIE_OK:
         raise MiaieError(rc, load_library().miaie_last_error_string(None).decode())
     return CONV_KERNELS[k.value]
+
+
+def mxfp4_shapes(rows: int, cols: int) -> tuple[tuple[int, int], tuple[int, int, int, int]]:
+    """Shapes of the uint8 arrays Q and S of a packed rows x cols matrix
+    (include/miaie.h, miaie_quant_mxfp4)."""
+    return (rows, (cols + 255) // 256 * 128), ((cols + 511) // 512, rows, 4, 4)
+
+
+def norm_work_bytes(cols: int) -> int:
+    """Bytes of norm_block_grad's work buffer (MIAIE_NORM_WORK_BYTES)."""
+    return 4096 * cols
 
 
 class DeviceBuffer:
@@ -232,6 +256,9 @@ class Context:
         lib = self.lib
         self._f_window, self._f_i32, self._f_rq = lib.miaie_mm_window_i32, lib.miaie_gemm_i8_i32, lib.miaie_gemm_i8_rq
         self._f_bf16, self._f_conv, self._f_mlp = lib.miaie_gemm_bf16_f32, lib.miaie_conv2d_i8_nhwc, lib.miaie_mlp_i8
+        self._f_quant, self._f_dequant, self._f_mx = lib.miaie_quant_mxfp4, lib.miaie_dequant_mxfp4, lib.miaie_gemm_mxfp4
+        self._f_mx_rq, self._f_mlp_mx = lib.miaie_gemm_mxfp4_rq, lib.miaie_mlp_mxfp4
+        self._f_norm, self._f_norm_grad = lib.miaie_norm_block, lib.miaie_norm_block_grad
 
     # -- plumbing
     def _call(self, name: str, *args) -> int:
@@ -391,6 +418,60 @@ class Context:
     def mlp_i8_noalloc(self, X, W1, W2, Y, M, K, F, Nout, s1, s2) -> None:
         """miaie_mlp_i8 with H in the library's own device array (allocates nothing)."""
         self._call("miaie_mlp_i8_noalloc", _addr(X), _addr(W1), _addr(W2), _addr(Y), M, K, F, Nout, s1, s2)
+
+    # -- microscaled 4-bit floating point (packed matrices: mxfp4_shapes)
+    def quant_mxfp4(self, X, R, C, Q, S, Qt=None, St=None, dtype=BF16, ldx=None) -> None:
+        """Pack X (R x C) along its rows (Q, S) and / or its columns (Qt, St)."""
+        rc = self._f_quant(self.handle, _addr(X), dtype, R, C, C if ldx is None else ldx, _addr(Q), _addr(S), _addr(Qt),
+                           _addr(St))
+        if rc:
+            self._raise(rc)
+
+    def dequant_mxfp4(self, Q, S, Y, R, C, dtype=BF16, ldy=None) -> None:
+        rc = self._f_dequant(self.handle, _addr(Q), _addr(S), _addr(Y), dtype, R, C, C if ldy is None else ldy)
+        if rc:
+            self._raise(rc)
+
+    def gemm_mxfp4(self, Aq, As, Bq, Bs, Cm, M, N, K, dtype=F32, ldc=None) -> None:
+        """C = A . B^T, A (M x K) and B (N x K) packed along their rows."""
+        rc = self._f_mx(self.handle, _addr(Aq), _addr(As), _addr(Bq), _addr(Bs), _addr(Cm), dtype, M, N, K,
+                        N if ldc is None else ldc)
+        if rc:
+            self._raise(rc)
+
+    def gemm_mxfp4_rq(self, Aq, As, Bq, Bs, Yq, Ys, M, N, K, relu=False) -> None:
+        """The product packed again, after a ReLU if relu."""
+        rc = self._f_mx_rq(self.handle, _addr(Aq), _addr(As), _addr(Bq), _addr(Bs), _addr(Yq), _addr(Ys), M, N, K,
+                           int(relu))
+        if rc:
+            self._raise(rc)
+
+    def mlp_mxfp4(self, Xq, Xs, W1q, W1s, W2q, W2s, Hq, Hs, Y, M, K, F, Nout, dtype=BF16, ldy=None) -> None:
+        rc = self._f_mlp_mx(self.handle, _addr(Xq), _addr(Xs), _addr(W1q), _addr(W1s), _addr(W2q), _addr(W2s), _addr(Hq),
+                            _addr(Hs), _addr(Y), dtype, M, K, F, Nout, Nout if ldy is None else ldy)
+        if rc:
+            self._raise(rc)
+
+    # -- norms around a block
+    def norm_block(self, x, b, gate, w_after, w_before, out, y, rstd, rows, cols, ldx=None, ldb=None, gate_rows=None,
+                   stream_dtype=BF16, branch_dtype=BF16, alpha=1.0, eps=1e-5) -> None:
+        """out = alpha x + gate w_after b / rms(b); y = w_before out / rms(out)."""
+        rc = self._f_norm(self.handle, _addr(x), _addr(b), _addr(gate), _addr(w_after), _addr(w_before), _addr(out),
+                          _addr(y), _addr(rstd), rows, cols, cols if ldx is None else ldx, cols if ldb is None else ldb,
+                          rows if gate_rows is None else gate_rows, stream_dtype, branch_dtype, alpha, eps)
+        if rc:
+            self._raise(rc)
+
+    def norm_block_grad(self, r, b, gate, w_after, w_before, rstd, dout, dy, dx, db, dgate, dw_after, dw_before, work,
+                        work_bytes, rows, cols, ldx=None, ldb=None, gate_rows=None, stream_dtype=BF16,
+                        branch_dtype=BF16, alpha=1.0) -> None:
+        rc = self._f_norm_grad(self.handle, _addr(r), _addr(b), _addr(gate), _addr(w_after), _addr(w_before),
+                               _addr(rstd), _addr(dout), _addr(dy), _addr(dx), _addr(db), _addr(dgate), _addr(dw_after),
+                               _addr(dw_before), _addr(work), work_bytes, rows, cols, cols if ldx is None else ldx,
+                               cols if ldb is None else ldb, rows if gate_rows is None else gate_rows, stream_dtype,
+                               branch_dtype, alpha)
+        if rc:
+            self._raise(rc)
 
 
 def version() -> str:

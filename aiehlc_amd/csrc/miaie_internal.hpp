@@ -158,6 +158,24 @@ int launch_conv2d_i8(miaie_ctx* ctx, const int8_t* X, const int8_t* W, const uin
                      int8_t* Y, int N, int H, int Wd, int Cin, int Cout, int R, int S, int stride,
                      int pad);
 
+// MXFP4 matrices (quant_mxfp4.hip, gemm_mxfp4.hip) and the norms of a block
+// (norm_block.hip); arguments as in miaie.h, checked by capi_block.hip.
+int launch_quant_mxfp4(miaie_ctx* ctx, const void* X, int dtype, int R, int C, int ldx, uint8_t* Q, uint8_t* S,
+                       uint8_t* Qt, uint8_t* St);
+int launch_dequant_mxfp4(miaie_ctx* ctx, const uint8_t* Q, const uint8_t* S, void* Y, int dtype, int R, int C,
+                         int ldy);
+int launch_gemm_mxfp4(miaie_ctx* ctx, const uint8_t* Aq, const uint8_t* As, const uint8_t* Bq, const uint8_t* Bs,
+                      void* C, int dtype, int M, int N, int K, int ldc);
+int launch_gemm_mxfp4_rq(miaie_ctx* ctx, const uint8_t* Aq, const uint8_t* As, const uint8_t* Bq, const uint8_t* Bs,
+                         uint8_t* Yq, uint8_t* Ys, int M, int N, int K, int relu);
+int launch_norm_block(miaie_ctx* ctx, const void* x, const void* b, const void* gate, const float* w_after,
+                      const float* w_before, void* out, void* y, float* rstd, int rows, int cols, int ldx, int ldb,
+                      int gate_rows, int stream_dtype, int branch_dtype, float alpha, float eps);
+int launch_norm_block_grad(miaie_ctx* ctx, const void* r, const void* b, const void* gate, const float* w_after,
+                           const float* w_before, const float* rstd, const void* dout, const void* dy, void* dx,
+                           void* db, float* dgate, float* dw_after, float* dw_before, float* work, int rows, int cols,
+                           int ldx, int ldb, int gate_rows, int stream_dtype, int branch_dtype, float alpha);
+
 }  // namespace miaie
 
 // Vector types used by the MFMA builtins.

@@ -304,6 +304,111 @@ MIAIE_API int miaie_mlp_i8(miaie_ctx* ctx, const int8_t* X, const int8_t* W1, co
 MIAIE_API int miaie_mlp_i8_noalloc(miaie_ctx* ctx, const int8_t* X, const int8_t* W1, const int8_t* W2, int8_t* Y,
                                    int M, int K, int F, int Nout, int s1, int s2);
 
+/* ---- microscaled 4-bit floating point (MXFP4) --------------------------- */
+
+/* No counterpart in the reference, whose kernels are integer.  An MXFP4
+ * matrix holds 4-bit floats (E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their
+ * negatives) in blocks of 32 along a row that share a power of two (E8M0), as
+ * in the OCP Microscaling Formats specification v1.0.  A matrix of R rows and
+ * K columns is two device arrays, both 16-byte aligned, dense, and zero behind
+ * column K:
+ *   Q  uint8 [R][miaie_mxfp4_q_pitch(K)]: two elements a byte, the even column
+ *      in the low four bits, rows of whole 128-byte lines (256 columns);
+ *   S  uint8 [ceil(K / 512)][R][4][4]: the scales (exponent + 127; 255 is NaN)
+ *      of 512 columns of a row together, that of its block b = 0 .. 15 at
+ *      [b % 4][b / 4], the order in which the matrix instructions take them.
+ *      (From scales stored [R][K / 32]: pad to whole groups of 16, view as
+ *      [R][K / 512][4][4], transpose to [K / 512][R][4][4] with the last two
+ *      axes exchanged.)
+ * Sizes (R, C, M, N, K, F, Nout) are in [1, 2^30]; R times the column groups of
+ * a matrix stays below 2^30. */
+#define MIAIE_F32 0  /* element types of unpacked matrices */
+#define MIAIE_BF16 1 /* raw 16-bit patterns */
+
+/* Bytes of a row of Q, and of the arrays Q and S, of an R x K matrix (0 for
+ * arguments outside the ranges above).  Host functions. */
+MIAIE_API size_t miaie_mxfp4_q_pitch(int K);
+MIAIE_API size_t miaie_mxfp4_q_bytes(int R, int K);
+MIAIE_API size_t miaie_mxfp4_s_bytes(int R, int K);
+
+/* Packs X (R x C row major, row pitch ldx >= C elements, of type dtype).
+ * Along its rows into Q, S (an R x C packed matrix), and / or along its
+ * columns into Qt, St (the packed transpose, C x R); either pair may be NULL.
+ * A product contracts along the packed axis: the forward product of a linear
+ * layer takes X and W packed along their rows, its gradients take dY, W and X
+ * packed along the axis each contracts.
+ * A block's scale is 2^(floor(log2(amax)) - 2), at least 2^-127; its elements
+ * are rounded to nearest, halves to the even code, magnitudes beyond 6 to 6.
+ * A block that holds an infinity or NaN gets scale 255: all of it is NaN. */
+MIAIE_API int miaie_quant_mxfp4(miaie_ctx* ctx, const void* X, int dtype, int R, int C, int ldx, uint8_t* Q,
+                                uint8_t* S, uint8_t* Qt, uint8_t* St);
+
+/* Y = the values of a packed R x C matrix, row major with row pitch ldy >= C
+ * elements, of type dtype (both hold every finite value of scale bytes up to
+ * 252 exactly). */
+MIAIE_API int miaie_dequant_mxfp4(miaie_ctx* ctx, const uint8_t* Q, const uint8_t* S, void* Y, int dtype, int R,
+                                  int C, int ldy);
+
+/* C[m][n] = sum over k of A[m][k] B[n][k]: A (Aq, As) M x K and B (Bq, Bs)
+ * N x K packed along k, fp32 accumulation, C of type dtype with row pitch
+ * ldc >= N elements.  Any M, N, K: single rows stream B once; large products
+ * run on LDS-staged tiles. */
+MIAIE_API int miaie_gemm_mxfp4(miaie_ctx* ctx, const uint8_t* Aq, const uint8_t* As, const uint8_t* Bq,
+                               const uint8_t* Bs, void* C, int dtype, int M, int N, int K, int ldc);
+
+/* The same product packed again along its rows, Y (Yq, Ys) M x N, after a ReLU
+ * if relu != 0: the 4-bit counterpart of miaie_gemm_i8_rq. */
+MIAIE_API int miaie_gemm_mxfp4_rq(miaie_ctx* ctx, const uint8_t* Aq, const uint8_t* As, const uint8_t* Bq,
+                                  const uint8_t* Bs, uint8_t* Yq, uint8_t* Ys, int M, int N, int K, int relu);
+
+/* Chained 4-bit MLP, H = pack(relu(X . W1^T)), Y = H . W2^T: X M x K, W1 F x K,
+ * W2 Nout x F, H M x F packed (Hq, Hs: caller-provided device scratch), Y
+ * M x Nout of type dtype with row pitch ldy >= Nout.  The 4-bit counterpart of
+ * miaie_mlp_i8 (with the weights stored output row by output row). */
+MIAIE_API int miaie_mlp_mxfp4(miaie_ctx* ctx, const uint8_t* Xq, const uint8_t* Xs, const uint8_t* W1q,
+                              const uint8_t* W1s, const uint8_t* W2q, const uint8_t* W2s, uint8_t* Hq, uint8_t* Hs,
+                              void* Y, int dtype, int M, int K, int F, int Nout, int ldy);
+
+/* ---- norms around a block ------------------------------------------------ */
+
+/* No counterpart in the reference.  The norm after a block b = f(y) of a
+ * residual network with its gate and the residual's scale, and the norm before
+ * the next block, in one pass:
+ *   out = alpha * x + gate * w_after * b / rms(b)
+ *   y   = w_before * out / rms(out),       rms(v) = sqrt(mean(v^2) + eps) per row
+ * Without b (NULL; then gate, w_after and out are NULL too, alpha is not used)
+ * only y = w_before * x / rms(x); without y (NULL, w_before too) only out.
+ * x, out (may be the same buffer): rows x cols of type stream_dtype, row pitch
+ * ldx; b, y: of type branch_dtype, row pitch ldb.  gate (NULL: 1): of type
+ * branch_dtype, dense [ceil(rows / gate_rows)][cols], row r using row
+ * r / gate_rows: gate_rows = rows for one vector, the tokens of a sequence for
+ * one per sequence, 1 for one per token.  w_after, w_before: fp32 [cols].
+ * rstd (NULL: not kept): fp32 [2][rows], receives 1 / rms(b) and 1 / rms(out)
+ * (of the norms that run) for the gradient.  out is rounded to its type before
+ * the second norm reads it; all else is fp32.
+ * rows in [1, 2^30], cols in [1, MIAIE_NORM_MAX_COLS], gate_rows >= 1, eps >= 0. */
+#define MIAIE_NORM_MAX_COLS 16384
+MIAIE_API int miaie_norm_block(miaie_ctx* ctx, const void* x, const void* b, const void* gate, const float* w_after,
+                               const float* w_before, void* out, void* y, float* rstd, int rows, int cols, int ldx,
+                               int ldb, int gate_rows, int stream_dtype, int branch_dtype, float alpha, float eps);
+
+/* Its gradient.  r: the stream that the second norm read (out, or x without a
+ * block; not read, and may be NULL, without dy).  dout (NULL: 0): the gradient
+ * of the stream from elsewhere; dy (NULL: no second norm): of y.  Results, each
+ * NULL if not wanted: dx, of type stream_dtype; db, of type branch_dtype;
+ * dgate, fp32, the shape of gate; dw_after, dw_before, fp32 [cols].  dout and dx
+ * have row pitch ldx, dy and db ldb; dx may be dout and db may be dy or b.  Without b the
+ * results but dx and dw_before are NULL, and alpha is not used.
+ * work: device scratch of MIAIE_NORM_WORK_BYTES(cols) for sums over rows (NULL
+ * where dw_after, dw_before and dgate are); the sums are taken in a fixed
+ * order, so equal calls give equal bits. */
+#define MIAIE_NORM_WORK_BYTES(cols) ((size_t)4096 * (size_t)(cols))
+MIAIE_API int miaie_norm_block_grad(miaie_ctx* ctx, const void* r, const void* b, const void* gate,
+                                    const float* w_after, const float* w_before, const float* rstd, const void* dout,
+                                    const void* dy, void* dx, void* db, float* dgate, float* dw_after,
+                                    float* dw_before, void* work, size_t work_bytes, int rows, int cols, int ldx,
+                                    int ldb, int gate_rows, int stream_dtype, int branch_dtype, float alpha);
+
 /* ---- synthetic inputs --------------------------------------------------- */
 
 /* Fill dst[0..n) with the seeded int8 stream of tensor `tensor_id`

@@ -226,6 +226,61 @@ inline void mlp_i8(const Buffer<int8_t>& X, const Buffer<int8_t>& W1, const Buff
   ctx.check(miaie_mlp_i8(ctx.get(), X.data(), W1.data(), W2.data(), H.data(), Y.data(), M, K, F, Nout, s1, s2));
 }
 
+// A packed MXFP4 matrix (miaie.h) of rows x cols.
+struct MxMatrix {
+  MxMatrix(Context& ctx, int rows, int cols)
+      : rows(rows), cols(cols), q(ctx, miaie_mxfp4_q_bytes(rows, cols)), s(ctx, miaie_mxfp4_s_bytes(rows, cols)) {}
+  int rows, cols;
+  Buffer<uint8_t> q, s;
+};
+
+// MIAIE_F32 / MIAIE_BF16 of a buffer's elements (bf16 as raw uint16 bits).
+inline constexpr int dtype_of(const float*) { return MIAIE_F32; }
+inline constexpr int dtype_of(const uint16_t*) { return MIAIE_BF16; }
+
+// Q = X packed along its rows (X dense, Q.rows x Q.cols).
+template <typename T>
+void quant_mxfp4(const Buffer<T>& X, MxMatrix& Q, Context& ctx = Context::current()) {
+  ctx.check(miaie_quant_mxfp4(ctx.get(), X.data(), dtype_of(X.data()), Q.rows, Q.cols, Q.cols, Q.q.data(), Q.s.data(),
+                              nullptr, nullptr));
+}
+
+// Qt = the transpose of X packed along its rows (X dense, Qt.cols x Qt.rows).
+template <typename T>
+void quant_mxfp4_t(const Buffer<T>& X, MxMatrix& Qt, Context& ctx = Context::current()) {
+  ctx.check(miaie_quant_mxfp4(ctx.get(), X.data(), dtype_of(X.data()), Qt.cols, Qt.rows, Qt.rows, nullptr, nullptr,
+                              Qt.q.data(), Qt.s.data()));
+}
+
+// Y = the values of Q.
+template <typename T>
+void dequant_mxfp4(const MxMatrix& Q, Buffer<T>& Y, Context& ctx = Context::current()) {
+  ctx.check(miaie_dequant_mxfp4(ctx.get(), Q.q.data(), Q.s.data(), Y.data(), dtype_of(Y.data()), Q.rows, Q.cols, Q.cols));
+}
+
+// C = A . B^T (A M x K, B N x K).
+template <typename T>
+void gemm_mxfp4(const MxMatrix& A, const MxMatrix& B, Buffer<T>& C, Context& ctx = Context::current()) {
+  ctx.check(miaie_gemm_mxfp4(ctx.get(), A.q.data(), A.s.data(), B.q.data(), B.s.data(), C.data(), dtype_of(C.data()),
+                             A.rows, B.rows, A.cols, B.rows));
+}
+
+// Y = A . B^T packed again, after a ReLU if relu.
+inline void gemm_mxfp4_rq(const MxMatrix& A, const MxMatrix& B, MxMatrix& Y, bool relu = false,
+                          Context& ctx = Context::current()) {
+  ctx.check(miaie_gemm_mxfp4_rq(ctx.get(), A.q.data(), A.s.data(), B.q.data(), B.s.data(), Y.q.data(), Y.s.data(),
+                                A.rows, B.rows, A.cols, relu ? 1 : 0));
+}
+
+// H = pack(relu(X . W1^T)), Y = H . W2^T.
+template <typename T>
+void mlp_mxfp4(const MxMatrix& X, const MxMatrix& W1, const MxMatrix& W2, MxMatrix& H, Buffer<T>& Y,
+               Context& ctx = Context::current()) {
+  ctx.check(miaie_mlp_mxfp4(ctx.get(), X.q.data(), X.s.data(), W1.q.data(), W1.s.data(), W2.q.data(), W2.s.data(),
+                            H.q.data(), H.s.data(), Y.data(), dtype_of(Y.data()), X.rows, X.cols, W1.rows, W2.rows,
+                            W2.rows));
+}
+
 }  // namespace miaie
 
 #endif  // MIAIE_HPP
