@@ -152,11 +152,24 @@ GEMMS = [(1, 1, 1), (1, 16, 32), (1, 4096, 512), (1, 333, 11008), (3, 17, 255), 
          (1024, 1024, 1024)]
 
 
+@pytest.fixture()
+def cus(ctx, request):
+    """Products planned for that many CUs: few tiles are then many."""
+    was = ctx.plan_set_cus(request.param)
+    yield request.param
+    ctx.plan_set_cus(was)
+
+
+# k of 1 to 9 groups of 512 columns and a half, in whole and odd numbers of pairs of k-tiles, on every tile
+GEMMS += [(260, 130, 256 * i) for i in (3, 4, 5, 6, 7, 8, 9, 11, 18)]
+
+
+@pytest.mark.parametrize("cus", [256, 8, 1], indirect=True)
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("shape", GEMMS)
-def test_gemm(ctx, shape, dtype):
+def test_gemm(ctx, shape, dtype, cus):
     M, N, K = shape
-    _say("gemm", M, N, K, dtype)
+    _say("gemm", M, N, K, dtype, "cus", cus)
     rng = np.random.default_rng(M * 31 + N * 7 + K)
     A, B = _operand(rng, M, K, 12), _operand(rng, N, K, 12)
     a, b = mx.values(*A, K), mx.values(*B, K)
@@ -178,12 +191,13 @@ def test_gemm(ctx, shape, dtype):
         x.free()
 
 
+@pytest.mark.parametrize("cus", [256, 8, 1], indirect=True)
 @pytest.mark.parametrize("relu", [False, True])
 @pytest.mark.parametrize("shape", [(1, 1, 1), (1, 96, 300), (3, 33, 64), (16, 255, 512), (17, 257, 1024), (40, 11008, 256),
                                    (70, 513, 2048), (129, 1000, 257), (256, 512, 768), (300, 800, 513), (513, 1025, 1024)])
-def test_packed_product_bit_by_bit(ctx, shape, relu):
+def test_packed_product_bit_by_bit(ctx, shape, relu, cus):
     M, N, K = shape
-    _say("gemm_rq", M, N, K, relu)
+    _say("gemm_rq", M, N, K, relu, "cus", cus)
     rng = np.random.default_rng(M + N + K)
     A, B = _operand(rng, M, K), _operand(rng, N, K)
     a, b = mx.values(*A, K), mx.values(*B, K)
