@@ -8,6 +8,7 @@ using namespace miaie;
 namespace {
 
 constexpr int kMost = 1 << 30;
+constexpr int kMostK = 1 << 26;  // contracted by a product (32-bit offsets of the rows of a tile)
 
 int check_size(miaie_ctx* ctx, const char* fn, const char* name, int v) {
   if (v < 1 || v > kMost) return fail(ctx, MIAIE_EINVAL, "%s: %s=%d outside [1, 2^30]", fn, name, v);
@@ -100,8 +101,8 @@ namespace {
 
 int check_gemm(miaie_ctx* ctx, const char* fn, const uint8_t* Aq, const uint8_t* As, const uint8_t* Bq,
                const uint8_t* Bs, int M, int N, int K) {
-  if (M < 1 || N < 1 || K < 1 || M > kMost || N > kMost || K > kMost)
-    return fail(ctx, MIAIE_EINVAL, "%s: M=%d N=%d K=%d must all be in [1, 2^30]", fn, M, N, K);
+  if (M < 1 || N < 1 || K < 1 || M > kMost || N > kMost || K > kMostK)
+    return fail(ctx, MIAIE_EINVAL, "%s: M=%d N=%d K=%d must be in [1, 2^30], K in [1, 2^26]", fn, M, N, K);
   MIAIE_TRY(check_packed(ctx, fn, "A", Aq, As, M, K));
   return check_packed(ctx, fn, "B", Bq, Bs, N, K);
 }
@@ -134,10 +135,9 @@ extern "C" int miaie_mlp_mxfp4(miaie_ctx* ctx, const uint8_t* Xq, const uint8_t*
   MIAIE_TRY(enter(ctx));
   MIAIE_CHECK_NOT_NULL(ctx, Y);
   MIAIE_TRY(check_dtype(ctx, __func__, "dtype", dtype));
-  MIAIE_TRY(check_size(ctx, __func__, "M", M));
-  MIAIE_TRY(check_size(ctx, __func__, "K", K));
-  MIAIE_TRY(check_size(ctx, __func__, "F", F));
-  MIAIE_TRY(check_size(ctx, __func__, "Nout", Nout));
+  if (M < 1 || K < 1 || F < 1 || Nout < 1 || M > kMost || Nout > kMost || K > kMostK || F > kMostK)
+    return fail(ctx, MIAIE_EINVAL, "%s: M=%d K=%d F=%d Nout=%d must be in [1, 2^30], K and F in [1, 2^26]", __func__, M, K,
+                F, Nout);
   MIAIE_TRY(check_packed(ctx, __func__, "X", Xq, Xs, M, K));
   MIAIE_TRY(check_packed(ctx, __func__, "W1", W1q, W1s, F, K));
   MIAIE_TRY(check_packed(ctx, __func__, "W2", W2q, W2s, Nout, F));

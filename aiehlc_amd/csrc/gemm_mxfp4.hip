@@ -11,6 +11,7 @@
 // n = 4 (l / 16) + 0..3 of its 16 x 16 block: whole vectors of a row of C, and
 // for a packed result the eight lanes' values of a block of 32 columns are one
 // row's.
+#include <algorithm>
 #include <type_traits>
 
 #include "gfx950_ops.hpp"
@@ -75,24 +76,25 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v) {
 
 // Packs NB blocks (columns 32 nb ..) of row m, of which this lane holds in
 // acc[2 k] and acc[2 k + 1] columns 4 fg + e and 16 + 4 fg + e of block k.  Columns
-// from N on become zeros.  Lane fg writes block fg whole: the lanes' four codes
-// of each half are exchanged as a 4 x 4 transpose.
-template <int NB, bool RELU>
+// from N on become zeros (WHOLE: there are none).  Lane fg writes block fg whole:
+// the lanes' four codes of each half are exchanged as a 4 x 4 transpose.
+// Maxima that keep NaN: a block with one becomes NaN, through a ReLU too.
+template <int NB, bool RELU, bool WHOLE>
 __device__ __forceinline__ void store_blocks(const Args& p, int m, int nb, int fg, const v4f* acc) {
   uint32_t q[4] = {0, 0, 0, 0}, s[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int k = 0; k < NB; ++k) {
-    float x[8];
-    uint32_t amax = 0;
+    float x[8], amax = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int n = 32 * (nb + k) + (e >> 2) * 16 + 4 * fg + (e & 3);
-      float v = acc[2 * k + (e >> 2)][e & 3];
-      if (RELU) v = v < 0.f ? 0.f : v;  // (keeps NaN)
-      x[e] = n < p.N ? v : 0.f;
-      amax = max(amax, abs_bits(x[e]));
+      x[e] = acc[2 * k + (e >> 2)][e & 3];
+      if (RELU) x[e] = __builtin_elementwise_maximum(x[e], 0.f);
+      if (!WHOLE) x[e] = 32 * (nb + k) + (e >> 2) * 16 + 4 * fg + (e & 3) < p.N ? x[e] : 0.f;
     }
-    s[k] = scale_of(row_max(amax));
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+      amax = __builtin_elementwise_maximum(__builtin_elementwise_maximum(amax, fabsf(x[e])), fabsf(x[e + 1]));
+    s[k] = scale_of(row_max(__float_as_uint(amax)));
     q[k] = pack8(x, scale_f32(s[k]));
   }
   swap32(q[0], q[2]);
@@ -112,87 +114,154 @@ __device__ __forceinline__ void store_blocks(const Args& p, int m, int nb, int f
 }
 
 // ---------------------------------------------------------------- few rows
-// A workgroup of W waves owns 16 MI rows and 32 columns; the waves share out
-// the 512-column groups of k and add their sums in LDS.  Fragments come
-// straight from memory: a wave reads 256 contiguous bytes of 16 rows of each
-// operand per group.
-template <int MI, int W, Out OUT>
-__global__ __launch_bounds__(64 * W) void gemm_mx_rows(Args p, int tiles_n) {
-  constexpr int NJ = 2;
-  __shared__ v4f part[W > 1 ? W - 1 : 1][MI * NJ][64];
+// A workgroup of up to 16 waves owns 16 MI rows and 16 NJ columns; its waves
+// share out the groups of 512 columns of k and add their sums in LDS, so a
+// product of few rows has thousands of groups in flight at once.  Bound by
+// reading B, every byte of it once.
+//
+// A wave copies its group's 256 bytes of 16 NJ rows of B and of A's rows into a
+// part of LDS of its own (no barriers: it waits for its own copies) and reads
+// the fragments from there.  Loaded straight into registers a fragment load
+// takes 64 bytes of each of 16 rows, half of a line, and a wave's 4 KB of B took
+// 2.7 us with everything in the L2 (1 x 11008 x 4096); a copy takes whole rows.
+// In LDS chunk c (16 bytes) of row r lies at c ^ (r % 16), so the 16 rows of a
+// fragment read cover all banks.  A has 4 AI rows there; fragment rows behind
+// them repeat the last.
+template <int MI, int NJ, int AI, int SLOTS>
+struct RowsGeom {
+  static constexpr int B = 0, A = 4096 * NJ, SB = A + 1024 * AI, SA = SB + 256 * NJ;
+  static constexpr int SLOT = SA + 256 * MI;               // bytes of a group
+  static constexpr int OPS = 4 * NJ + AI + NJ + MI;        // copies of a group
+  static constexpr int SUM = MI * NJ * 1024;               // bytes of a wave's sums
+  static constexpr int REGION = std::max(SLOTS * SLOT, SUM);
+  static constexpr int WAVES = std::min(16, 163840 / REGION);  // at most
+  static_assert(AI <= 4 * MI && OPS <= 63, "rows of A, copies in flight");
+};
+
+template <int MI, int NJ, int AI, int SLOTS, Out OUT>
+__global__ __launch_bounds__((64 * RowsGeom<MI, NJ, AI, SLOTS>::WAVES)) void gemm_mx_rows(Args p, int tiles_n, int waves) {
+  using G = RowsGeom<MI, NJ, AI, SLOTS>;
+  constexpr int REGION = G::REGION;
+  extern __shared__ __attribute__((aligned(1024))) int8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 15, fg = lane >> 4;
-  const int m0 = 16 * MI * (blockIdx.x / tiles_n), n0 = 32 * (blockIdx.x % tiles_n);
-  const size_t pitch = q_pitch(p.K);
-  const int groups = s_groups(p.K), tiles_k = (int)(pitch / 64);  // 128-column steps: an even number
+  const int m0 = 16 * MI * (blockIdx.x / tiles_n), n0 = 16 * NJ * (blockIdx.x % tiles_n);
+  const uint32_t pitch = (uint32_t)q_pitch(p.K);
+  const int groups = s_groups(p.K);
+  const bool half = (pitch / 128) % 2;  // the last group has 256 columns
   v4f acc[MI][NJ];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  const uint8_t *aq[MI], *bq[NJ], *as[MI], *bs[NJ];
+  int8_t* const mine = lds + wave * REGION;
+  const uint32_t mine0 = dev::lds_addr(mine);
+  const dbg::Span aq_span = dbg::span_of(p.Aq), bq_span = dbg::span_of(p.Bq), as_span = dbg::span_of(p.As),
+                  bs_span = dbg::span_of(p.Bs);  // (debug build only)
+  const uint8_t* const a_base = p.Aq + (size_t)m0 * pitch;
+  const uint8_t* const b_base = p.Bq + (size_t)n0 * pitch;
+  // copy x of an operand: rows 4 x .. 4 x + 3, 16 lanes each; rows behind the last
+  // one repeat it.  A last group of 256 columns repeats its first half.
+  const int a_last = p.M - 1 - m0, b_last = p.N - 1 - n0;
+  auto copy = [&](int g, int slot) __attribute__((always_inline)) {
+    const uint32_t to = mine0 + slot * G::SLOT;
+    const uint32_t mask = half && g == groups - 1 ? 7 : 15;
+    auto rows = [&](const uint8_t* base, int x, int last, uint32_t st, const dbg::Span& span) __attribute__((always_inline)) {
+      const int r = 4 * x + fg;
+      const uint32_t off = (uint32_t)min(r, last) * pitch + 16 * ((fr ^ (r & 15)) & mask);
+      dev::gload_lds16(base + 256 * (size_t)g, off, to + st + 1024 * x, span);
+    };
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const size_t m = min(m0 + 16 * i + fr, p.M - 1);
-    aq[i] = p.Aq + m * pitch + 16 * fg;
-    as[i] = p.As + m * 16 + 4 * fg;
-  }
+    for (int x = 0; x < 4 * NJ; ++x) rows(b_base, x, b_last, G::B, bq_span);
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const size_t n = min(n0 + 16 * j + fr, p.N - 1);
-    bq[j] = p.Bq + n * pitch + 16 * fg;
-    bs[j] = p.Bs + n * 16 + 4 * fg;
-  }
-  if (n0 < p.N) {
-    for (int g = wave; g < groups; g += W) {
-      int sa[MI], sb[NJ];
+    for (int x = 0; x < AI; ++x) rows(a_base, x, a_last, G::A, aq_span);
 #pragma unroll
-      for (int i = 0; i < MI; ++i) sa[i] = MIAIE_LD(reinterpret_cast<const int*>(as[i] + (size_t)g * p.M * 16));
+    for (int j = 0; j < NJ; ++j)
+      dev::gload_lds4(p.Bs + ((size_t)g * p.N + n0) * 16, 16 * (uint32_t)min(16 * j + fr, b_last) + 4 * fg,
+                      to + G::SB + 256 * j, bs_span);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) sb[j] = MIAIE_LD(reinterpret_cast<const int*>(bs[j] + (size_t)g * p.N * 16));
-      auto step = [&](auto t_c) {
-        constexpr int t = decltype(t_c)::value;
-        const size_t off = 256 * (size_t)g + 64 * t;
-        v4i a[MI], b[NJ];
+    for (int i = 0; i < MI; ++i)
+      dev::gload_lds4(p.As + ((size_t)g * p.M + m0) * 16, 16 * (uint32_t)min(16 * i + fr, a_last) + 4 * fg,
+                      to + G::SA + 256 * i, as_span);
+  };
+  auto multiply = [&](int g, int slot) __attribute__((always_inline)) {
+    const int8_t* const from = mine + slot * G::SLOT;
+    int sa[MI], sb[NJ];
 #pragma unroll
-        for (int i = 0; i < MI; ++i) a[i] = MIAIE_LD(reinterpret_cast<const v4i*>(aq[i] + off));
+    for (int j = 0; j < NJ; ++j) sb[j] = *reinterpret_cast<const int*>(from + G::SB + 256 * j + 4 * lane);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) b[j] = MIAIE_LD(reinterpret_cast<const v4i*>(bq[j] + off));
+    for (int i = 0; i < MI; ++i) sa[i] = *reinterpret_cast<const int*>(from + G::SA + 256 * i + 4 * lane);
+    auto step = [&](auto t_c) __attribute__((always_inline)) {
+      constexpr int t = decltype(t_c)::value;
+      v4i a[MI], b[NJ];
 #pragma unroll
-        for (int i = 0; i < MI; ++i)
+      for (int j = 0; j < NJ; ++j)
+        b[j] = *reinterpret_cast<const v4i*>(from + G::B + 4096 * j + 256 * fr + 16 * ((4 * t + fg) ^ fr));
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) acc[i][j] = mfma<t>(b[j], a[i], acc[i][j], sb[j], sa[i]);
-      };
-      step(std::integral_constant<int, 0>{});
-      step(std::integral_constant<int, 1>{});
-      if (4 * g + 2 < tiles_k) {
-        step(std::integral_constant<int, 2>{});
-        step(std::integral_constant<int, 3>{});
+      for (int i = 0; i < MI; ++i) {
+        const int r = min(16 * i + fr, 4 * AI - 1);
+        a[i] = *reinterpret_cast<const v4i*>(from + G::A + 256 * r + 16 * ((4 * t + fg) ^ (r & 15)));
       }
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = mfma<t>(b[j], a[i], acc[i][j], sb[j], sa[i]);
+    };
+    step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+    if (half && g == groups - 1) return;
+    step(std::integral_constant<int, 2>{});
+    step(std::integral_constant<int, 3>{});
+  };
+  if (n0 < p.N) {
+    // SLOTS groups in flight; each slot is filled again once its fragments are
+    // in registers
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s)
+      if (wave + s * waves < groups) copy(wave + s * waves, s);
+    int slot = 0;
+    for (int g = wave; g < groups; g += waves) {
+      if (SLOTS > 1 && g + (SLOTS - 1) * waves < groups)
+        dev::wait_vmcnt<(SLOTS - 1) * G::OPS>();
+      else
+        dev::wait_vmcnt<0>();
+      asm volatile("" ::: "memory");
+      multiply(g, slot);
+      const int next = g + SLOTS * waves;
+      if (next < groups) {
+        dev::waitcnt<63, 0>();
+        asm volatile("" ::: "memory");
+        copy(next, slot);
+      }
+      slot = slot + 1 == SLOTS ? 0 : slot + 1;
     }
   }
-  if constexpr (W > 1) {
-    if (wave > 0) {
+  // each wave's sums; row block i (every column block of it) is added up by wave
+  // i % waves
+  if (waves > 1) {
 #pragma unroll
-      for (int f = 0; f < MI * NJ; ++f) part[wave - 1][f][lane] = acc[f / NJ][f % NJ];
-    }
+    for (int f = 0; f < MI * NJ; ++f) *reinterpret_cast<v4f*>(mine + 1024 * f + 16 * lane) = acc[f / NJ][f % NJ];
     __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int w = 0; w < W - 1; ++w)
-#pragma unroll
-      for (int f = 0; f < MI * NJ; ++f) acc[f / NJ][f % NJ] += part[w][f][lane];
   }
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
+    if (i % waves != wave) continue;
+    v4f sum[NJ];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) sum[j] = acc[i][j];
+    for (int w = 1; w < waves; ++w) {
+      const int from = wave + w < waves ? wave + w : wave + w - waves;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) sum[j] += *reinterpret_cast<const v4f*>(lds + from * REGION + 1024 * (i * NJ + j) + 16 * lane);
+    }
     const int m = m0 + 16 * i + fr;
     if constexpr (OUT == OUT_F32 || OUT == OUT_BF16) {
       using T = std::conditional_t<OUT == OUT_F32, float, __bf16>;
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
-        store4(static_cast<T*>(p.C), p.ldc, m, n0 + 16 * j + 4 * fg, p.M, p.N, acc[i][j]);
+        store4(static_cast<T*>(p.C), p.ldc, m, n0 + 16 * j + 4 * fg, p.M, p.N, sum[j]);
     } else {
-      store_blocks<1, OUT == OUT_MX_RELU>(p, m, n0 / 32, fg, acc[i]);
+      store_blocks<NJ / 2, OUT == OUT_MX_RELU, false>(p, m, n0 / 32, fg, sum);
     }
   }
 }
@@ -223,9 +292,8 @@ __global__ __launch_bounds__(64 * W) void gemm_mx_rows(Args p, int tiles_n) {
 //   B k-tile k: half 0 at phi = 2 k - 7 (after the barrier of k-tile k - 4,
 //     whose half 1 had the slot), half 1 at phi = 2 k - 5 (after that of k - 3,
 //     whose half 0 had it);
-//   scales of group q + 1: phase 2 of k-tile 4 q (every wave took those of group
-//     q into registers in phase 2 of k-tile 4 q - 1), taken in phase 2 of k-tile
-//     4 q + 3.
+//   scales of group q + 1: phase 2 of k-tile 4 q (every wave has read those of
+//     group q by its barrier), read from phase 2 of k-tile 4 q + 3 on.
 // What the barrier of k-tile t has to make visible (k-tile t + 1) was sent by
 // phi = 2 t - 3, so the copies of the three phases since may be in flight: at
 // most VM of them (copies of scales in between only make the wait stricter).
@@ -289,7 +357,66 @@ __device__ __forceinline__ void pin(int (&v)[N]) {
     asm volatile("" : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]), "+v"(v[4]), "+v"(v[5]), "+v"(v[6]), "+v"(v[7]));
 }
 
-template <int BM, int BN, Out OUT>
+// The accumulators stay where they are up to this point (the compiler would
+// read all 256 of them at once, and spill).
+template <int NJ>
+__device__ __forceinline__ void hold(v4f (&acc)[NJ]) {
+  static_assert(NJ % 4 == 0, "four at a time");
+#pragma unroll
+  for (int j = 0; j < NJ; j += 4)
+    asm volatile("" : "+a"(acc[j]), "+a"(acc[j + 1]), "+a"(acc[j + 2]), "+a"(acc[j + 3]));
+}
+
+// A wave's quarter at row m0 and column n0 of C.  In bf16 two blocks beside each other are exchanged between lanes fg and fg + 1 of
+// a row, so that each holds eight columns of one block: 16 bytes a lane in either
+// type, at any alignment.  EDGE: some columns of the product's last tiles are
+// behind N.  A kernel of its own, for the branches between the stores: with them
+// the lines of an fp32 C of 256 MB go to memory in parts, 30000 cycles a tile
+// where 17000 do, and with both forms in one kernel the compiler spills
+// accumulators.  Ordinary stores: 64 MB of fp32 tiles leave in 8.8 us, 14 us as
+// non-temporal ones.
+template <bool EDGE, class T, int NI, int NJ>
+__device__ __forceinline__ void store_quarter(T* C, size_t ldc, int m0, int n0, int fr, int fg, int M, int N,
+                                              v4f (&acc)[NI][NJ]) {
+  constexpr int W = 16 / sizeof(T), NB = W / 4;  // columns of a lane, blocks exchanged
+  typedef T V __attribute__((ext_vector_type(W)));
+  using P = At<V, T>;
+  const dbg::Span span = dbg::span_of(C);  // (debug build only)
+  int m = m0 + fr;
+  const int n = n0 + (NB == 1 ? 4 * fg : 16 * (fg & 1) + 8 * (fg >> 1));
+  T* row = C + (size_t)m * ldc + n;
+#pragma unroll
+  for (int i = 0; i < NI; ++i, m += 16, row += 16 * ldc) {
+    if (m < M) {
+#pragma unroll
+      for (int j = 0; j < NJ; j += NB) {
+        V v;
+        if constexpr (NB == 1) {
+          v = acc[i][j];
+        } else {
+          typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+          typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+          const v2u a = __builtin_bit_cast(v2u, __builtin_convertvector(acc[i][j], v4bf));
+          const v2u b = __builtin_bit_cast(v2u, __builtin_convertvector(acc[i][j + 1], v4bf));
+          uint32_t a0 = a[0], a1 = a[1], b0 = b[0], b1 = b[1];
+          swap16(a0, b0);  // (the four lanes of a row are all here)
+          swap16(a1, b1);
+          v = __builtin_bit_cast(V, v4u{a0, a1, b0, b1});
+        }
+        if (!EDGE || n + 16 * j + W <= N) {
+          MIAIE_ST_IN(span, reinterpret_cast<P*>(row + 16 * j), P{v});
+        } else {
+#pragma unroll
+          for (int e = 0; e < W - 1; ++e)
+            if (n + 16 * j + e < N) MIAIE_ST_IN(span, row + 16 * j + e, v[e]);
+        }
+      }
+    }
+    dev::sched_fence();  // (more rows at once spill)
+  }
+}
+
+template <int BM, int BN, Out OUT, bool EDGE>
 __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, int tiles_m, int tiles_n) {
   using G = PipeGeom<BM, BN>;
   constexpr int NI = G::NI, NJ = G::NJ, HI = G::HI, PH = G::PH;
@@ -352,7 +479,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, i
   const int b_fo = B0 + fr * 64 + ((fg ^ b_swz(fr)) << 4);  // (a wave's columns are one half)
   const int sa_fo = S0 + (wm * G::WM + fr) * 16 + 4 * fg, sb_fo = S0 + (BM + wn * G::WN + fr) * 16 + 4 * fg;
   v4i alo[HI], ahi[HI], bs[NJ];
-  int sa[NI], sb[NJ], sa_next[NI], sb_next[NJ];
+  int sa[NI], sb[NJ];
   auto read_a = [&](uint32_t st, int par, int i) __attribute__((always_inline)) -> v4i {
     // (readfirstlane keeps the stage's address in the base register, so that
     // 2048 i is the instruction's offset)
@@ -361,12 +488,8 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, i
   auto read_b = [&](uint32_t st, int j) __attribute__((always_inline)) {
     bs[j] = *reinterpret_cast<const v4i*>(lds + __builtin_amdgcn_readfirstlane(st) + b_fo + 1024 * j);
   };
-  auto read_s = [&](int x) __attribute__((always_inline)) {
-    if (x < NI)
-      sa_next[x] = *reinterpret_cast<const int*>(lds + sa_fo + 256 * x);
-    else
-      sb_next[x - NI] = *reinterpret_cast<const int*>(lds + sb_fo + 256 * (x - NI));
-  };
+  auto read_sa = [&](int i) __attribute__((always_inline)) { sa[i] = *reinterpret_cast<const int*>(lds + sa_fo + 256 * i); };
+  auto read_sb = [&](int j) __attribute__((always_inline)) { sb[j] = *reinterpret_cast<const int*>(lds + sb_fo + 256 * j); };
 
   v4f acc[NI][NJ];
 #pragma unroll
@@ -399,7 +522,9 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, i
     dev::wait_vmcnt<0>();
   dev::barrier();
 #pragma unroll
-  for (int x = 0; x < NI + NJ; ++x) read_s(x);
+  for (int i = 0; i < NI; ++i) read_sa(i);
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) read_sb(j);
 #pragma unroll
   for (int j = 0; j < NJ; ++j) read_b(wn * G::B_HALF, j);
 #pragma unroll
@@ -416,51 +541,59 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, i
   };
   int t = 0;
 
+  constexpr int A_STEP = PH * 3 / (4 * HI);  // phase 1's reads of A, evenly over three quarters of it
   // k-tile t: D k-tiles before the last; PAR = t % 2 and, where it is known at
-  // compile time, T4 = t % 4 (else -1: the registers of scales are then shifted
-  // by a pair's two bytes for the second pair of a group)
+  // compile time, T4 = t % 4.  Each matrix instruction first, then, in its
+  // shadow, what goes with it.
   auto tile = [&](auto par_c, auto t4_c, auto d_c) __attribute__((always_inline)) {
     constexpr int PAR = decltype(par_c)::value, T4 = decltype(t4_c)::value, D = decltype(d_c)::value;
     constexpr int BYTE = T4 >= 0 ? T4 : PAR;
     constexpr int NA = G::a_copies(D), NB = G::b_copies(D);
     constexpr bool NEXT = D >= 1;
+    uint32_t b_next = 0, cp0 = 0, cp1 = 0;
 #pragma unroll
     for (int x = 0; x < PH; ++x) {
       const int j = x / HI, i = dev::snake_j<HI>(x);
       mfma_in_place<BYTE>(acc[i][j], bs[j], alo[i], sb[j], sa[i]);
-      if (x < HI) ahi[x] = read_a(st0, PAR, HI + x);
+      dev::sched_fence();
+      if (x % A_STEP == 1 && x / A_STEP < HI) ahi[x / A_STEP] = read_a(st0, PAR, HI + x / A_STEP);
 #pragma unroll
       for (int c = 0; c < NA; ++c)
-        if (c * PH / (NA > 0 ? NA : 1) == x) copy_a(a_src, st2, G::A_CP * PAR + c);
+        if (2 + c * PH / (NA > 0 ? NA : 1) == x) copy_a(a_src, st2, G::A_CP * PAR + c);
+      if (x == PH / 2 + 1) {
+        // phase 2's slots: of k-tile t + 1, of (t + 4, half 0) and of (t + 3, half 1)
+        b_next = slot_at(2 + wn), cp0 = slot_at(1), cp1 = slot_at(0);
+        asm volatile("" : "+s"(b_next), "+s"(cp0), "+s"(cp1));
+      }
       dev::sched_fence();
     }
     dev::waitcnt<G::vm(D), 0>();
     dev::barrier();
     const uint32_t st_next = PAR == 0 ? st0 : st1;
-    const uint32_t b_next = slot_at(2 + wn);
-    const uint32_t cp0 = slot_at(1), cp1 = slot_at(0);  // (2 (t + 4)) % 7, (2 (t + 3) + 1) % 7
 #pragma unroll
     for (int x = 0; x < PH; ++x) {
       const int j = x / HI, i = dev::snake_j<HI>(x);
       mfma_in_place<BYTE>(acc[HI + i][j], bs[j], ahi[i], sb[j], sa[HI + i]);
+      dev::sched_fence();
 #pragma unroll
       for (int c = 0; c < NB; ++c)
-        if (c * PH / (NB > 0 ? NB : 1) == x) {
+        if (2 + c * PH / (NB > 0 ? NB : 1) == x) {
           if (c < G::B_CP)
             copy_b(b_src, cp1, 1, c);
           else
             copy_b(b_src + 64, cp0, 0, c - G::B_CP);
         }
       if constexpr (T4 == 0 || (T4 < 0 && PAR == 0)) {
-        if (x == 0 && (t & 3) == 0 && t + 4 < KT) copy_s(t / 4 + 1);
+        if (x == PH - 1 && (t & 3) == 0 && t + 4 < KT) copy_s(t / 4 + 1);
       }
       if constexpr (NEXT) {
-        if (x < HI) alo[x] = read_a(st_next, 1 - PAR, x);
-        if (x % HI == HI - 1) read_b(b_next, j);  // last use of k-tile t's fragment j
-        // (where t % 4 may be 1 these are not taken, and read again at 3)
-        if constexpr (T4 == 3 || (T4 < 0 && PAR == 1)) {
-#pragma unroll
-          for (int r = x * (NI + NJ) / PH; r < (x + 1) * (NI + NJ) / PH; ++r) read_s(r);
+        if (x % HI == HI / 2 - 1 && x / HI < HI) alo[x / HI] = read_a(st_next, 1 - PAR, x / HI);
+        // registers of k-tile t are read again after their last use
+        if (x % HI == HI - 1) read_b(b_next, j);
+        if constexpr (T4 == 3) {
+          if (x < HI) read_sa(x);
+          if (x % HI == HI - 1) read_sb(j);
+          if (x >= PH - HI) read_sa(HI + i);
         }
       }
       dev::sched_fence();
@@ -476,14 +609,21 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, i
       a_src += 128;
     }
   };
-  // The scales of the pair that starts: the group's (phase 2 of the k-tile
-  // before read them), or the next two bytes of those.  Three wait states between
+  // The scales of a pair whose place in its group is not known at compile time:
+  // the group's, or the next two bytes of those.  Three wait states between
   // these instructions and the first that takes the registers.
-  auto take_scales = [&](bool shift) __attribute__((always_inline)) {
+  auto take_scales = [&]() __attribute__((always_inline)) {
+    if (t & 2) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) sa[i] = shift ? (int)((uint32_t)sa[i] >> 16) : sa_next[i];
+      for (int i = 0; i < NI; ++i) sa[i] = (int)((uint32_t)sa[i] >> 16);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) sb[j] = shift ? (int)((uint32_t)sb[j] >> 16) : sb_next[j];
+      for (int j = 0; j < NJ; ++j) sb[j] = (int)((uint32_t)sb[j] >> 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) read_sa(i);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) read_sb(j);
+    }
     pin(sa);
     pin(sb);
     asm volatile("s_nop 2" ::: "memory");
@@ -496,48 +636,48 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, i
   // steady k-tiles, then the last six.  (With branches of whole tails for 2, 4
   // and 6 left the register allocator moves the accumulators through memory.)
   while (t + 10 <= KT) {
-    take_scales(false);
     tile(P0{}, std::integral_constant<int, 0>{}, DS{});
     tile(P1{}, std::integral_constant<int, 1>{}, DS{});
     tile(P0{}, std::integral_constant<int, 2>{}, DS{});
     tile(P1{}, std::integral_constant<int, 3>{}, DS{});
   }
   while (t + 6 < KT) {
-    take_scales(t & 2);
+    take_scales();
     tile(P0{}, TR{}, DS{});
     tile(P1{}, TR{}, DS{});
   }
   if (KT >= 6) {
-    take_scales(t & 2);
+    take_scales();
     tile(P0{}, TR{}, std::integral_constant<int, 5>{});
     tile(P1{}, TR{}, std::integral_constant<int, 4>{});
   }
   if (KT >= 4) {
-    take_scales(t & 2);
+    take_scales();
     tile(P0{}, TR{}, std::integral_constant<int, 3>{});
     tile(P1{}, TR{}, std::integral_constant<int, 2>{});
   }
-  take_scales(t & 2);
+  take_scales();
   tile(P0{}, TR{}, std::integral_constant<int, 1>{});
   tile(P1{}, TR{}, std::integral_constant<int, 0>{});
   // the last results are readable after 18 wait states at most
   dev::sched_fence();
   asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < NI; ++i) hold(acc[i]);  // (read behind the wait)
   dev::sched_fence();
 
   // ---- acc[i][j]: row 16 i + fr and columns 16 j + 4 fg + 0..3 of the wave's quarter
   const int mw = m0 + wm * G::WM, nw = n0 + wn * G::WN;
   if constexpr (OUT == OUT_F32 || OUT == OUT_BF16) {
     using T = std::conditional_t<OUT == OUT_F32, float, __bf16>;
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        store4(static_cast<T*>(p.C), p.ldc, mw + 16 * i + fr, nw + 16 * j + 4 * fg, p.M, p.N, acc[i][j]);
+    store_quarter<EDGE>(static_cast<T*>(p.C), p.ldc, mw, nw, fr, fg, p.M, p.N, acc);
   } else {
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      store_blocks<NJ / 2, OUT == OUT_MX_RELU>(p, mw + 16 * i + fr, nw / 32, fg, acc[i]);
+      if (n0 + BN <= p.N)
+        store_blocks<NJ / 2, OUT == OUT_MX_RELU, true>(p, mw + 16 * i + fr, nw / 32, fg, acc[i]);
+      else
+        store_blocks<NJ / 2, OUT == OUT_MX_RELU, false>(p, mw + 16 * i + fr, nw / 32, fg, acc[i]);
       dev::sched_fence();  // (more rows at once spill)
     }
     if (tn == tiles_n - 1) {  // zeros up to the end of the last 512 columns
@@ -555,29 +695,113 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, i
   }
 }
 
-// Tiles and workgroups of a launch; HIP takes fewer than 2^32 threads.
 template <int BM, int BN, Out OUT>
 int run_pipe(miaie_ctx* ctx, const Args& p) {
   const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
-  const hipError_t e = launch<gemm_mx_pipe<BM, BN, OUT>>(ctx->device, dim3((unsigned)tiles_m * tiles_n), dim3(256), 0,
-                                                         ctx->stream, p, tiles_m, tiles_n);
+  hipError_t e = hipSuccess;
+  auto go = [&](auto k) {
+    e = launch<decltype(k)::value>(ctx->device, dim3((unsigned)tiles_m * tiles_n), dim3(256), 0, ctx->stream, p, tiles_m,
+                                   tiles_n);
+  };
+  if ((OUT == OUT_F32 || OUT == OUT_BF16) && p.N % BN)
+    go(kernel_t<gemm_mx_pipe<BM, BN, OUT, OUT == OUT_F32 || OUT == OUT_BF16>>{});
+  else
+    go(kernel_t<gemm_mx_pipe<BM, BN, OUT, false>>{});
   return check_launch(ctx, e, "gemm_mx_pipe");
+}
+
+template <int MI, int NJ, int AI, int SLOTS, Out OUT>
+int run_rows(miaie_ctx* ctx, const Args& p) {
+  using G = RowsGeom<MI, NJ, AI, SLOTS>;
+  // (a packed result has zeros up to the end of its last 512 columns)
+  const int cols = OUT == OUT_MX || OUT == OUT_MX_RELU ? 512 * s_groups(p.N) : p.N;
+  const int tiles_n = (cols + 16 * NJ - 1) / (16 * NJ);
+  const long tiles = (p.M + 16l * MI - 1) / (16 * MI) * tiles_n;
+  const int groups = s_groups(p.K);
+  // as many waves as share the groups evenly, up to 16 and to what fits the LDS
+  const int each = (groups + G::WAVES - 1) / G::WAVES, waves = (groups + each - 1) / each;
+  if (tiles * waves >= 1l << 26) return fail(ctx, MIAIE_EINVAL, "gemm_mxfp4: M=%d N=%d too large", p.M, p.N);
+  const hipError_t e = launch<gemm_mx_rows<MI, NJ, AI, SLOTS, OUT>>(ctx->device, dim3((unsigned)tiles), dim3(64 * waves),
+                                                                    (size_t)waves * G::REGION, ctx->stream, p, tiles_n, waves);
+  return check_launch(ctx, e, "gemm_mx_rows");
+}
+
+// ------------------------------------------------------------ choice of kernel
+// The kernel with the lowest estimated time.  Few rows: a CU copies about 42
+// bytes a ns into LDS with its waves' groups in flight, so the workgroups of one
+// CU take that time for all their groups (within 15% of 46 measured products of
+// 1 to 100 rows, 4 to 26 us).  Large products: cycles of a workgroup's start, of a
+// k-tile and of its end as measured on the tiles (a k-tile of 256 x 256 has 64
+// instructions of 16 cycles on each wave), the clock 2.3 GHz with a part of the
+// CUs at work and about 1.9 under the power limit.  128 x 128 tiles fit a CU
+// twice, and then take 960 cycles for both where one takes 540.
+struct Choice {
+  double us = 1e30;
+  int kernel = -1;
+};
+void consider(Choice& best, int kernel, double us) {
+  if (us < best.us) best = Choice{us, kernel};
+}
+
+double rows_us(long M, long cols, int groups, int mi, int nj, int slot, int cus) {
+  const long tiles = ((M + 16 * mi - 1) / (16 * mi)) * ((cols + 16 * nj - 1) / (16 * nj));
+  return 1.2 + (double)((tiles + cus - 1) / cus) * groups * slot / 42e3;
+}
+
+double pipe_us(long M, long N, int k_tiles, int bm, int bn, double start, double tile, double end, int cus) {
+  const long tiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+  const long rounds = (tiles + cus - 1) / cus;
+  const double ghz = 2 * tiles < cus ? 2.35e3 : 1.9e3;
+  if (bm == 128 && rounds > 1) return 1.0 + (double)((rounds + 1) / 2) * (1600 + start + end + 960.0 * k_tiles) / ghz;
+  return 1.0 + (double)rounds * (start + end + tile * k_tiles) / ghz;
 }
 
 template <Out OUT>
 int run(miaie_ctx* ctx, const Args& p) {
-  if (p.M > 64 && q_pitch(p.K) < (1u << 24)) {
-    const long tiles = ((p.M + 255l) / 256) * ((p.N + 255l) / 256);
-    if (tiles < 1l << 22) return 3 * tiles >= 2 * ctx->cus ? run_pipe<256, 256, OUT>(ctx, p) : run_pipe<128, 128, OUT>(ctx, p);
+  constexpr bool packed = OUT == OUT_MX || OUT == OUT_MX_RELU;
+  const int groups = s_groups(p.K), k_tiles = (int)(q_pitch(p.K) / 64), cus = ctx->cus;
+  const long cols = packed ? 512l * s_groups(p.N) : p.N;
+  Choice c;
+#define MIAIE_MX_ROWS(MI, NJ, AI) RowsGeom<MI, NJ, AI, 1>::SLOT
+  if (p.M <= 4)
+    consider(c, 0, rows_us(p.M, cols, groups, 1, 1 + packed, packed ? MIAIE_MX_ROWS(1, 2, 1) : MIAIE_MX_ROWS(1, 1, 1), cus));
+  else if (!packed)
+    consider(c, 1, rows_us(p.M, cols, groups, 1, 1, MIAIE_MX_ROWS(1, 1, 4), cus));
+  consider(c, 2, rows_us(p.M, cols, groups, 1, 2, MIAIE_MX_ROWS(1, 2, 4), cus));
+  consider(c, 3, rows_us(p.M, cols, groups, 1, 4, MIAIE_MX_ROWS(1, 4, 4), cus));
+  if (p.M > 16) {
+    if (!packed) consider(c, 4, rows_us(p.M, cols, groups, 2, 1, MIAIE_MX_ROWS(2, 1, 8), cus));
+    consider(c, 5, rows_us(p.M, cols, groups, 2, 2, MIAIE_MX_ROWS(2, 2, 8), cus));
+    consider(c, 6, rows_us(p.M, cols, groups, 2, 4, MIAIE_MX_ROWS(2, 4, 8), cus));
   }
-  // (a packed result has zeros up to the end of its last 512 columns)
-  const int cols = OUT == OUT_MX || OUT == OUT_MX_RELU ? 512 * s_groups(p.N) : p.N;
-  const int tiles_n = (cols + 31) / 32;
-  const long tiles_m = (p.M + 31l) / 32;
-  if (tiles_m * tiles_n >= 1l << 24) return fail(ctx, MIAIE_EINVAL, "gemm_mxfp4: M=%d N=%d too large", p.M, p.N);
-  const hipError_t e = launch<gemm_mx_rows<2, 4, OUT>>(ctx->device, dim3((unsigned)(tiles_m * tiles_n)), dim3(256), 0,
-                                                       ctx->stream, p, tiles_n);
-  return check_launch(ctx, e, "gemm_mx_rows");
+  if (p.M > 32) {
+    consider(c, 7, rows_us(p.M, cols, groups, 4, 2, MIAIE_MX_ROWS(4, 2, 16), cus));
+    consider(c, 8, rows_us(p.M, cols, groups, 4, 4, MIAIE_MX_ROWS(4, 4, 16), cus));
+  }
+#undef MIAIE_MX_ROWS
+  // (a row's offset within a tile in 32 bits, and HIP takes fewer than 2^32 threads)
+  const long tiles = ((p.M + 127l) / 128) * ((p.N + 127l) / 128);
+  if (q_pitch(p.K) < (1u << 24) && tiles < 1l << 23) {
+    const int o = packed ? 2 : OUT == OUT_BF16;
+    constexpr double end[3][3] = {{16500, 7800, 9900}, {8200, 3800, 5800}, {3500, 1850, 3400}};
+    consider(c, 9, pipe_us(p.M, p.N, k_tiles, 128, 128, 2400, 540, end[2][o], cus));
+    consider(c, 10, pipe_us(p.M, p.N, k_tiles, 256, 128, 3400, 840, end[1][o], cus));
+    consider(c, 11, pipe_us(p.M, p.N, k_tiles, 256, 256, 4500, 1320, end[0][o], cus));
+  }
+  switch (c.kernel) {
+    case 0: return run_rows<1, 1 + packed, 1, 1, OUT>(ctx, p);
+    case 1: return run_rows<1, 1 + packed, 4, 1, OUT>(ctx, p);
+    case 2: return run_rows<1, 2, 4, 1, OUT>(ctx, p);
+    case 3: return run_rows<1, 4, 4, 1, OUT>(ctx, p);
+    case 4: return run_rows<2, 1 + packed, 8, 1, OUT>(ctx, p);
+    case 5: return run_rows<2, 2, 8, 1, OUT>(ctx, p);
+    case 6: return run_rows<2, 4, 8, 1, OUT>(ctx, p);
+    case 7: return run_rows<4, 2, 16, 1, OUT>(ctx, p);
+    case 8: return run_rows<4, 4, 16, 1, OUT>(ctx, p);
+    case 9: return run_pipe<128, 128, OUT>(ctx, p);
+    case 10: return run_pipe<256, 128, OUT>(ctx, p);
+    default: return run_pipe<256, 256, OUT>(ctx, p);
+  }
 }
 
 }  // namespace

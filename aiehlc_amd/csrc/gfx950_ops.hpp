@@ -49,6 +49,25 @@ __device__ __forceinline__ void gload_lds16(const void* sbase, uint32_t voff, ui
   asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
 }
 
+// 4-byte global -> LDS copy (global_load_lds_dword): as gload_lds16, lane l's
+// 4 bytes land at LDS address m0 + 4*l.
+__device__ __forceinline__ void gload_lds4(const void* sbase, uint32_t voff, uint32_t m0, dbg::Span span,
+                                           int line = __builtin_LINE(),
+                                           uint32_t file = dbg::file_id(__builtin_FILE_NAME())) {
+#if MIAIE_DEVICE_CHECKS
+  const void* p = static_cast<const char*>(sbase) + voff;
+  if (!dbg::in_span(span, p, 4)) {
+    dbg::report(p, 4, 2, line, file);
+    return;
+  }
+#else
+  (void)span;
+  (void)line;
+  (void)file;
+#endif
+  asm volatile("global_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "{m0}"(m0) : "memory");
+}
+
 // s_waitcnt through the builtin, so that the compiler's own wait insertion
 // sees it (and keeps it: waits written by the program are never dropped).
 // gfx9 encoding: vmcnt[3:0] | expcnt[6:4] | lgkmcnt[11:8] | vmcnt[5:4] at [15:14].

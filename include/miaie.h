@@ -320,8 +320,8 @@ MIAIE_API int miaie_mlp_i8_noalloc(miaie_ctx* ctx, const int8_t* X, const int8_t
  *      (From scales stored [R][K / 32]: pad to whole groups of 16, view as
  *      [R][K / 512][4][4], transpose to [K / 512][R][4][4] with the last two
  *      axes exchanged.)
- * Sizes (R, C, M, N, K, F, Nout) are in [1, 2^30]; R times the column groups of
- * a matrix stays below 2^30. */
+ * Sizes are in [1, 2^30], a size that a product contracts in [1, 2^26]; the rows
+ * times the groups of 512 columns of a matrix stay below 2^30. */
 #define MIAIE_F32 0  /* element types of unpacked matrices */
 #define MIAIE_BF16 1 /* raw 16-bit patterns */
 
