@@ -71,13 +71,31 @@ __device__ __forceinline__ uint32_t pack8(const float (&x)[8], float scale) {
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
-// ---- element types of the unpacked side
-template <class T>
-__device__ __forceinline__ float to_f32(T x) {
-  return (float)x;
+// v of another lane of the same four (CTRL: two bits of source lane for each)
+template <int CTRL>
+__device__ __forceinline__ uint32_t quad_swap(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xf, 0xf, true);
 }
 
-// Eight consecutive elements, n of them inside the row (n >= 1; the rest 0).
+// Eight consecutive elements as they are in memory, n of them inside the row (n >= 1; the rest 0).
+template <class T>
+struct Raw8 {
+  typedef T V __attribute__((ext_vector_type(8)));
+  V v;
+  __device__ __forceinline__ void clear() { v = V{}; }
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if (n >= 8) {
+      using P = At<V, T>;
+      v = MIAIE_LD(reinterpret_cast<const P*>(p)).v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < n ? MIAIE_LD(p + i) : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
+};
+
+// The same as fp32.
 template <class T>
 __device__ __forceinline__ void load8(const T* p, int n, float (&x)[8]) {
   typedef T V __attribute__((ext_vector_type(8)));

@@ -26,26 +26,39 @@ namespace miaie {
 namespace {
 
 using mx::load8;
+using mx::Raw8;
 using mx::store8;
 
+// Sum over a wave, in every lane: within sixteens by lane permutations that are
+// part of the addition, then across them.
+template <int CTRL>
+__device__ __forceinline__ float add_lane(float v) {
+  return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-  return v;
+  v = add_lane<0xB1>(v);   // lane 1 0 3 2 of a four
+  v = add_lane<0x4E>(v);   // 2 3 0 1
+  v = add_lane<0x141>(v);  // the other four of eight (mirrored)
+  v = add_lane<0x140>(v);  // the other eight of sixteen
+  const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r16[0]) + __uint_as_float(r16[1]);
+  const auto r32 = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r32[0]) + __uint_as_float(r32[1]);
 }
 
-// Sum over a row of THREADS threads: a wave, or the workgroup (red: one float
-// per wave; every thread of the workgroup calls it the same number of times).
-template <int THREADS>
+// Sum over a row of TPR threads, a wave or several (red: one float for each
+// wave of the workgroup, all of whose threads call it the same number of times).
+template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* red, int tid) {
   v = wave_sum(v);
-  if constexpr (THREADS > 64) {
+  if constexpr (TPR > 64) {
     __syncthreads();  // the last sum has been read
     if ((tid & 63) == 0) red[tid >> 6] = v;
     __syncthreads();
-    v = red[0];
+    const float* mine = red + tid / TPR * (TPR / 64);
+    v = mine[0];
 #pragma unroll
-    for (int w = 1; w < THREADS / 64; ++w) v += red[w];
+    for (int w = 1; w < TPR / 64; ++w) v += mine[w];
   }
   return v;
 }
@@ -66,55 +79,66 @@ struct Fwd {
 };
 
 // TPR threads hold a row, 8 NC columns each; a workgroup of max(TPR, 256)
-// threads has one row (TPR >= 256) or four (TPR = 64).  ST: x and out, BT: b,
-// gate and y.
+// threads takes one row (TPR >= 256) or several.  ST: x and out, BT: b, gate and
+// y.  Everything a row needs is loaded before its first sum: a single row waits
+// for memory once (1 x 4096 bf16 TBD us, 5.4 with the weights and the gate loaded
+// where they are used).
 template <class ST, class BT, int TPR, int NC>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_fwd(Fwd p) {
-  constexpr int RPW = TPR < 256 ? 256 / TPR : 1;
-  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
+  constexpr int THREADS = TPR < 256 ? 256 : TPR, RPW = THREADS / TPR;
+  __shared__ float red[THREADS / 64];
   const int tid = threadIdx.x, t = tid % TPR;
-  // (the threads that share a barrier have the same row)
-  for (int row = blockIdx.x * RPW + tid / TPR; row < p.rows; row += p.stride) {
-    const ST* x = static_cast<const ST*>(p.x) + (size_t)row * p.ldx;
-    float r[NC][8];
+  Raw8<float> w_after[NC], w_before[NC];
+  // (every thread makes the same number of turns: a row's sum is a barrier)
+  for (int row0 = blockIdx.x * RPW; row0 < p.rows; row0 += p.stride) {
+    const int row = row0 + tid / TPR;
+    const bool active = row < p.rows;
+    const size_t xo = (size_t)row * p.ldx, bo = (size_t)row * p.ldb;
+    const BT* gate = p.gate && active ? static_cast<const BT*>(p.gate) + (size_t)(row / p.gate_rows) * p.cols : nullptr;
+    Raw8<BT> b[NC], g[NC];
+    Raw8<ST> x[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int k = 8 * (t + TPR * c);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) r[c][e] = 0.f;
-      if (k < p.cols) load8(x + k, p.cols - k, r[c]);
+      const int k = 8 * (t + TPR * c), n = p.cols - k;
+      b[c].clear(), x[c].clear(), g[c].clear();
+      if (n <= 0 || !active) continue;
+      if (p.b) b[c].load(static_cast<const BT*>(p.b) + bo + k, n);
+      x[c].load(static_cast<const ST*>(p.x) + xo + k, n);
+      if (gate) g[c].load(gate + k, n);
     }
-    if (p.b) {
-      const BT* b = static_cast<const BT*>(p.b) + (size_t)row * p.ldb;
-      float v[NC][8], ss = 0.f;
+    if (row0 == blockIdx.x * RPW) {
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const int k = 8 * (t + TPR * c);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[c][e] = 0.f;
-        if (k < p.cols) load8(b + k, p.cols - k, v[c]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(v[c][e], v[c][e], ss);
+        const int k = 8 * (t + TPR * c), n = p.cols - k;
+        w_after[c].clear(), w_before[c].clear();
+        if (n <= 0) continue;
+        if (p.b) w_after[c].load(p.w_after + k, n);
+        if (p.y) w_before[c].load(p.w_before + k, n);
       }
+    }
+    float r[NC][8];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) r[c][e] = x[c][e];
+    if (p.b) {
+      float ss = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(b[c][e], b[c][e], ss);
       const float ra = 1.f / sqrtf(row_sum<TPR>(ss, red, tid) / (float)p.cols + p.eps);
-      if (p.rstd && t == 0) MIAIE_ST(p.rstd + row, ra);
-      const BT* gate = p.gate ? static_cast<const BT*>(p.gate) + (size_t)(row / p.gate_rows) * p.cols : nullptr;
-      ST* out = static_cast<ST*>(p.out) + (size_t)row * p.ldx;
+      if (p.rstd && t == 0 && active) MIAIE_ST(p.rstd + row, ra);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const int k = 8 * (t + TPR * c);
-        if (k < p.cols) {
-          float w[8], g[8];
-          load8(p.w_after + k, p.cols - k, w);
-          if (gate) load8(gate + k, p.cols - k, g);
+        const int k = 8 * (t + TPR * c), n = p.cols - k;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float n = v[c][e] * ra * w[e];
-            if (gate) n *= g[e];
-            r[c][e] = rounded<ST>(fmaf(p.alpha, r[c][e], n));
-          }
-          store8(out + k, p.cols - k, r[c]);
+        for (int e = 0; e < 8; ++e) {
+          float v = b[c][e] * ra * w_after[c][e];
+          if (gate) v *= g[c][e];
+          r[c][e] = rounded<ST>(fmaf(p.alpha, r[c][e], v));
         }
+        if (n > 0 && active) store8(static_cast<ST*>(p.out) + xo + k, n, r[c]);
       }
     }
     if (p.y) {
@@ -122,21 +146,16 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_fwd(Fwd p) {
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (8 * (t + TPR * c) + e < p.cols) ss = fmaf(r[c][e], r[c][e], ss);
+        for (int e = 0; e < 8; ++e) ss = fmaf(r[c][e], r[c][e], ss);  // (0 behind the last column)
       const float rb = 1.f / sqrtf(row_sum<TPR>(ss, red, tid) / (float)p.cols + p.eps);
-      if (p.rstd && t == 0) MIAIE_ST(p.rstd + p.rows + row, rb);
-      BT* y = static_cast<BT*>(p.y) + (size_t)row * p.ldb;
+      if (p.rstd && t == 0 && active) MIAIE_ST(p.rstd + p.rows + row, rb);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const int k = 8 * (t + TPR * c);
-        if (k < p.cols) {
-          float w[8];
-          load8(p.w_before + k, p.cols - k, w);
+        const int k = 8 * (t + TPR * c), n = p.cols - k;
+        float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] *= r[c][e] * rb;
-          store8(y + k, p.cols - k, w);
-        }
+        for (int e = 0; e < 8; ++e) y[e] = r[c][e] * rb * w_before[c][e];
+        if (n > 0 && active) store8(static_cast<BT*>(p.y) + bo + k, n, y);
       }
     }
   }
@@ -160,47 +179,73 @@ struct Bwd {
 
 // parts > 0: workgroup i has the rows of part i % parts of gate i / parts.
 // parts == 0: the row lanes of all workgroups take gates in turn.
+//
+// 1024 threads, TPR of them to a row: 1024 / TPR rows at a time, so that a CU has
+// 16 waves' loads in flight although the partial sums allow only about one
+// workgroup a CU (4095 x 4096 bf16: TBD us, 125 with four waves a CU).
+constexpr int BWD_THREADS = 1024;
+
 template <class ST, class BT, int TPR, int NC>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_bwd(Bwd p) {
-  constexpr int THREADS = TPR < 256 ? 256 : TPR, RPW = THREADS / TPR;
-  __shared__ float red[TPR > 64 ? TPR / 64 : 1];
-  __shared__ float lanes[RPW > 1 ? (RPW - 1) * TPR * 8 : 1];
+__global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
+  constexpr int RPW = BWD_THREADS / TPR;
+  __shared__ float red[BWD_THREADS / 64];
+  __shared__ float lanes[RPW > 1 ? RPW / 2 * TPR * 8 : 1];
   const int tid = threadIdx.x, t = tid % TPR, lane_row = tid / TPR;
   const size_t cols = p.cols;
   float dwb[NC][8] = {}, dwa[NC][8] = {}, dg[NC][8] = {};
 
-  auto row_grad = [&](int row) {
-    const float ra = p.b ? MIAIE_LD(p.rstd + row) : 0.f, rb = p.dy ? MIAIE_LD(p.rstd + p.rows + row) : 0.f;
-    float dr[NC][8], m[NC][8], tt[NC][8], c1 = 0.f;
+  // The next row's four tensors, on their way while a row is computed (98 -> TBD
+  // registers, TBD -> TBD us for 4095 x 4096 bf16).
+  Raw8<ST> x_r[NC], x_dout[NC];
+  Raw8<BT> x_dy[NC], x_b[NC];
+  auto fetch = [&](int row, bool active) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int k = 8 * (t + TPR * c);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dr[c][e] = m[c][e] = tt[c][e] = 0.f;
-      if (k >= p.cols) continue;
-      if (p.dout) load8(static_cast<const ST*>(p.dout) + (size_t)row * p.ldx + k, p.cols - k, dr[c]);
+      x_r[c].clear(), x_dout[c].clear(), x_dy[c].clear(), x_b[c].clear();
+      if (k >= p.cols || !active) continue;
+      const size_t xo = (size_t)row * p.ldx + k, bo = (size_t)row * p.ldb + k;
       if (p.dy) {
-        float w[8], d[8];
-        load8(static_cast<const ST*>(p.r) + (size_t)row * p.ldx + k, p.cols - k, m[c]);
-        load8(static_cast<const BT*>(p.dy) + (size_t)row * p.ldb + k, p.cols - k, d);
+        x_r[c].load(static_cast<const ST*>(p.r) + xo, p.cols - k);
+        x_dy[c].load(static_cast<const BT*>(p.dy) + bo, p.cols - k);
+      }
+      if (p.dout) x_dout[c].load(static_cast<const ST*>(p.dout) + xo, p.cols - k);
+      if (p.b) x_b[c].load(static_cast<const BT*>(p.b) + bo, p.cols - k);
+    }
+  };
+
+  // (a lane without a row takes part in the sums' barriers)
+  auto row_grad = [&](int row, bool active, int next, bool next_active) {
+    const float ra = p.b && active ? MIAIE_LD(p.rstd + row) : 0.f;
+    const float rb = p.dy && active ? MIAIE_LD(p.rstd + p.rows + row) : 0.f;
+    float dr[NC][8], m[NC][8], tt[NC][8], v[NC][8], c1 = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dr[c][e] = x_dout[c][e], m[c][e] = x_r[c][e], tt[c][e] = x_dy[c][e], v[c][e] = x_b[c][e];
+    fetch(next, next_active);
+    if (p.dy) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int k = 8 * (t + TPR * c);
+        if (k >= p.cols) continue;
+        float w[8];
         load8(p.w_before + k, p.cols - k, w);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 8; ++e) {  // (what is behind the last column is zero)
           m[c][e] *= rb;
-          tt[c][e] = e < p.cols - k ? d[e] * w[e] : 0.f;
-          if (e < p.cols - k) dwb[c][e] = fmaf(d[e], m[c][e], dwb[c][e]);
+          dwb[c][e] = fmaf(tt[c][e], m[c][e], dwb[c][e]);
+          tt[c][e] *= w[e];
           c1 = fmaf(tt[c][e], m[c][e], c1);
         }
       }
-    }
-    if (p.dy) {
       c1 = row_sum<TPR>(c1, red, tid) / (float)p.cols;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e) dr[c][e] = fmaf(rb, tt[c][e] - m[c][e] * c1, dr[c][e]);
     }
-    if (p.dx) {
+    if (p.dx && active) {
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const int k = 8 * (t + TPR * c);
@@ -212,30 +257,25 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_bwd(Bwd p) {
     }
     if (!p.b) return;
     float c2 = 0.f;
-    const BT* gate = p.gate ? static_cast<const BT*>(p.gate) + (size_t)(row / p.gate_rows) * cols : nullptr;
-    // (m becomes n, dr becomes u)
+    const BT* gate = p.gate && active ? static_cast<const BT*>(p.gate) + (size_t)(row / p.gate_rows) * cols : nullptr;
+    // (v becomes n, dr becomes u)
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int k = 8 * (t + TPR * c);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m[c][e] = 0.f;
       if (k >= p.cols) continue;
       float w[8], g[8];
-      load8(static_cast<const BT*>(p.b) + (size_t)row * p.ldb + k, p.cols - k, m[c]);
       load8(p.w_after + k, p.cols - k, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) g[e] = 1.f;
       if (gate) load8(gate + k, p.cols - k, g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        m[c][e] *= ra;
-        const float dn = dr[c][e] * m[c][e];
-        if (e < p.cols - k) {
-          dwa[c][e] = fmaf(dn, g[e], dwa[c][e]);
-          dg[c][e] = fmaf(dn, w[e], dg[c][e]);
-        }
-        dr[c][e] = e < p.cols - k ? dr[c][e] * g[e] * w[e] : 0.f;
-        c2 = fmaf(dr[c][e], m[c][e], c2);
+        v[c][e] *= ra;
+        const float dn = dr[c][e] * v[c][e];
+        dwa[c][e] = fmaf(dn, g[e], dwa[c][e]);
+        dg[c][e] = fmaf(dn, w[e], dg[c][e]);
+        dr[c][e] *= g[e] * w[e];
+        c2 = fmaf(dr[c][e], v[c][e], c2);
       }
     }
     if (!p.db) return;
@@ -245,8 +285,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_bwd(Bwd p) {
       const int k = 8 * (t + TPR * c);
       float d[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) d[e] = ra * (dr[c][e] - m[c][e] * c2);
-      if (k < p.cols) store8(static_cast<BT*>(p.db) + (size_t)row * p.ldb + k, p.cols - k, d);
+      for (int e = 0; e < 8; ++e) d[e] = ra * (dr[c][e] - v[c][e] * c2);
+      if (k < p.cols && active) store8(static_cast<BT*>(p.db) + (size_t)row * p.ldb + k, p.cols - k, d);
     }
   };
 
@@ -254,16 +294,20 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_bwd(Bwd p) {
     const int gate = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
     const int first = gate * p.gate_rows, n = min(p.gate_rows, p.rows - first);
     const int r0 = first + (int)((long)n * part / p.parts), r1 = first + (int)((long)n * (part + 1) / p.parts);
-    for (int row = r0 + lane_row; row < r1; row += RPW) row_grad(row);
+    fetch(r0 + lane_row, r0 + lane_row < r1);
+    for (int row = r0 + lane_row, i = r0; i < r1; i += RPW, row += RPW) row_grad(row, row < r1, row + RPW, row + RPW < r1);
   } else {
-    for (int gate = blockIdx.x * RPW + lane_row; gate < p.groups; gate += p.workgroups * RPW) {
-      const int first = gate * p.gate_rows, last = min(first + p.gate_rows, p.rows);
-      for (int row = first; row < last; ++row) row_grad(row);
+    // (every row lane makes the same number of turns)
+    for (int g0 = blockIdx.x * RPW; g0 < p.groups; g0 += p.workgroups * RPW) {
+      const int gate = g0 + lane_row, first = gate * p.gate_rows;
+      const int n = gate < p.groups ? min(p.gate_rows, p.rows - first) : 0;
+      fetch(first, n > 0);
+      for (int i = 0; i < p.gate_rows; ++i) row_grad(first + i, i < n, first + i + 1, i + 1 < n);
       if (p.want & 4) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           const int k = 8 * (t + TPR * c);
-          if (k < p.cols) store8(p.dgate + gate * cols + k, p.cols - k, dg[c]);
+          if (k < p.cols && n > 0) store8(p.dgate + gate * cols + k, p.cols - k, dg[c]);
 #pragma unroll
           for (int e = 0; e < 8; ++e) dg[c][e] = 0.f;
         }
@@ -271,24 +315,23 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_bwd(Bwd p) {
     }
   }
 
-  // the workgroup's partial sums
+  // the workgroup's partial sums: its row lanes' added in pairs through LDS
   auto put = [&](float(&v)[NC][8], int which) {
     float* dst = p.work + ((size_t)blockIdx.x * 3 + which) * cols;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int k = 8 * (t + TPR * c);
-      if constexpr (RPW > 1) {
-        __syncthreads();
-        if (lane_row > 0) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) lanes[((lane_row - 1) * 8 + e) * TPR + t] = v[c][e];
+      for (int half = RPW / 2; half >= 1; half /= 2) {
+        __syncthreads();
+        if (lane_row >= half && lane_row < 2 * half) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) lanes[((lane_row - half) * 8 + e) * TPR + t] = v[c][e];
         }
         __syncthreads();
-        if (lane_row == 0) {
+        if (lane_row < half) {
 #pragma unroll
-          for (int l = 0; l < RPW - 1; ++l)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[c][e] += lanes[(l * 8 + e) * TPR + t];
+          for (int e = 0; e < 8; ++e) v[c][e] += lanes[(lane_row * 8 + e) * TPR + t];
         }
       }
       if (lane_row == 0 && k < p.cols) store8(dst + k, p.cols - k, v[c]);
@@ -300,12 +343,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_bwd(Bwd p) {
 }
 
 // Sums of partial rows: workgroup (x, y) adds 64 columns of output row y (0:
-// dw_before, 1: dw_after, 2 + g: dgate row g), its four waves a quarter of the
-// partial rows each.
-__global__ __launch_bounds__(256) void norm_join(const float* __restrict__ work, float* __restrict__ dw_before,
-                                                 float* __restrict__ dw_after, float* __restrict__ dgate, int cols,
-                                                 int workgroups, int parts) {
-  __shared__ float sum[4][64];
+// dw_before, 1: dw_after, 2 + g: dgate row g), its 16 waves a sixteenth of the
+// partial rows each, eight loads in flight.
+__global__ __launch_bounds__(1024) void norm_join(const float* __restrict__ work, float* __restrict__ dw_before,
+                                                  float* __restrict__ dw_after, float* __restrict__ dgate, int cols,
+                                                  int workgroups, int parts) {
+  __shared__ float sum[16][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, k = blockIdx.x * 64 + lane;
   const int out = blockIdx.y;
   float* dst = out == 0 ? dw_before : out == 1 ? dw_after : dgate;
@@ -313,12 +356,21 @@ __global__ __launch_bounds__(256) void norm_join(const float* __restrict__ work,
   const int first = out < 2 ? 0 : (out - 2) * parts, n = out < 2 ? workgroups : parts;
   const int which = min(out, 2);
   float s = 0.f;
-  if (k < cols)
-    for (int i = wave; i < n; i += 4) s += MIAIE_LD(work + ((size_t)(first + i) * 3 + which) * cols + k);
+  if (k < cols) {
+    const float* p = work + ((size_t)first * 3 + which) * cols + k;
+    for (int i = wave; i < n; i += 128) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = i + 16 * u < n ? MIAIE_LD(p + (size_t)(i + 16 * u) * 3 * cols) : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += v[u];
+    }
+  }
   sum[wave][lane] = s;
   __syncthreads();
   if (wave == 0 && k < cols) {
-    s = sum[0][lane] + sum[1][lane] + sum[2][lane] + sum[3][lane];
+#pragma unroll
+    for (int w = 1; w < 16; ++w) s += sum[w][lane];
     MIAIE_ST(dst + (out < 2 ? 0 : (size_t)(out - 2) * cols) + k, s);
   }
 }
@@ -326,16 +378,17 @@ __global__ __launch_bounds__(256) void norm_join(const float* __restrict__ work,
 // go(threads per row, 8-column chunks per thread) for rows of `cols` columns
 template <class F>
 void with_row(int cols, F&& go) {
+  using One = std::integral_constant<int, 1>;
   if (cols <= 512)
-    go(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
+    go(std::integral_constant<int, 64>{}, One{});
   else if (cols <= 1024)
-    go(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
+    go(std::integral_constant<int, 128>{}, One{});
   else if (cols <= 2048)
-    go(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
+    go(std::integral_constant<int, 256>{}, One{});
   else if (cols <= 4096)
-    go(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
+    go(std::integral_constant<int, 512>{}, One{});
   else if (cols <= 8192)
-    go(std::integral_constant<int, 512>{}, std::integral_constant<int, 2>{});
+    go(std::integral_constant<int, 1024>{}, One{});
   else
     go(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
 }
@@ -365,7 +418,8 @@ int launch_norm_block(miaie_ctx* ctx, const void* x, const void* b, const void* 
   with_types(stream_dtype, branch_dtype, [&](auto st, auto bt) {
     with_row(cols, [&](auto tpr, auto nc) {
       constexpr int TPR = decltype(tpr)::value, NC = decltype(nc)::value, RPW = TPR < 256 ? 256 / TPR : 1;
-      const int workgroups = std::min((rows + RPW - 1) / RPW, 1 << 20);
+      // (up to about four rows a workgroup, which then loads the weights once)
+      const int turns = (rows + RPW - 1) / RPW, workgroups = std::min(turns, std::max(16 * ctx->cus, 1));
       p.stride = workgroups * RPW;
       e = launch<norm_fwd<typename decltype(st)::type, typename decltype(bt)::type, TPR, NC>>(
           ctx->device, dim3(workgroups), dim3(TPR < 256 ? 256 : TPR), 0, ctx->stream, p);
@@ -385,7 +439,7 @@ int launch_norm_block_grad(miaie_ctx* ctx, const void* r, const void* b, const v
   hipError_t e = hipSuccess;
   with_types(stream_dtype, branch_dtype, [&](auto st, auto bt) {
     with_row(cols, [&](auto tpr, auto nc) {
-      constexpr int TPR = decltype(tpr)::value, NC = decltype(nc)::value, RPW = TPR < 256 ? 256 / TPR : 1;
+      constexpr int TPR = decltype(tpr)::value, NC = decltype(nc)::value, RPW = BWD_THREADS / TPR;
       // at most 256 workgroups (the work buffer holds 341 partial rows of
       // three sums), each with at least one row for every row lane
       constexpr int kMost = 256;
@@ -397,11 +451,11 @@ int launch_norm_block_grad(miaie_ctx* ctx, const void* r, const void* b, const v
         p.workgroups = (int)std::min<long>(kMost, ((long)p.groups + RPW - 1) / RPW);
       }
       e = launch<norm_bwd<typename decltype(st)::type, typename decltype(bt)::type, TPR, NC>>(
-          ctx->device, dim3(p.workgroups), dim3(TPR < 256 ? 256 : TPR), 0, ctx->stream, p);
+          ctx->device, dim3(p.workgroups), dim3(BWD_THREADS), 0, ctx->stream, p);
     });
   });
   if (e == hipSuccess && (dw_before || dw_after || (dgate && p.parts > 0)))
-    e = launch<norm_join>(ctx->device, dim3((cols + 63) / 64, dgate && p.parts > 0 ? 2 + p.groups : 2), dim3(256), 0,
+    e = launch<norm_join>(ctx->device, dim3((cols + 63) / 64, dgate && p.parts > 0 ? 2 + p.groups : 2), dim3(1024), 0,
                           ctx->stream, work, dw_before, dw_after, dgate, cols, p.workgroups, p.parts);
   return check_launch(ctx, e, "norm_bwd");
 }
