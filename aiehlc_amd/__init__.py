@@ -169,6 +169,10 @@ class DeviceBuffer:
     def value(self) -> int:
         return self.ptr
 
+    @property
+    def _as_parameter_(self):  # ctypes takes a buffer where it takes an address
+        return self.ptr or None
+
     def free(self) -> None:
         if self.ptr:
             self.ctx._call("miaie_free", self.ptr)
@@ -420,35 +424,34 @@ class Context:
         self._call("miaie_mlp_i8_noalloc", _addr(X), _addr(W1), _addr(W2), _addr(Y), M, K, F, Nout, s1, s2)
 
     # -- microscaled 4-bit floating point (packed matrices: mxfp4_shapes)
+    # (operands go to ctypes as they are: an address, None or a DeviceBuffer; 0.5 us less for eight of them than
+    # through _addr)
     def quant_mxfp4(self, X, R, C, Q, S, Qt=None, St=None, dtype=BF16, ldx=None) -> None:
         """Pack X (R x C) along its rows (Q, S) and / or its columns (Qt, St)."""
-        rc = self._f_quant(self.handle, _addr(X), dtype, R, C, C if ldx is None else ldx, _addr(Q), _addr(S), _addr(Qt),
-                           _addr(St))
+        rc = self._f_quant(self.handle, X, dtype, R, C, C if ldx is None else ldx, Q, S, Qt, St)
         if rc:
             self._raise(rc)
 
     def dequant_mxfp4(self, Q, S, Y, R, C, dtype=BF16, ldy=None) -> None:
-        rc = self._f_dequant(self.handle, _addr(Q), _addr(S), _addr(Y), dtype, R, C, C if ldy is None else ldy)
+        rc = self._f_dequant(self.handle, Q, S, Y, dtype, R, C, C if ldy is None else ldy)
         if rc:
             self._raise(rc)
 
     def gemm_mxfp4(self, Aq, As, Bq, Bs, Cm, M, N, K, dtype=F32, ldc=None) -> None:
         """C = A . B^T, A (M x K) and B (N x K) packed along their rows."""
-        rc = self._f_mx(self.handle, _addr(Aq), _addr(As), _addr(Bq), _addr(Bs), _addr(Cm), dtype, M, N, K,
-                        N if ldc is None else ldc)
+        rc = self._f_mx(self.handle, Aq, As, Bq, Bs, Cm, dtype, M, N, K, N if ldc is None else ldc)
         if rc:
             self._raise(rc)
 
     def gemm_mxfp4_rq(self, Aq, As, Bq, Bs, Yq, Ys, M, N, K, relu=False) -> None:
         """The product packed again, after a ReLU if relu."""
-        rc = self._f_mx_rq(self.handle, _addr(Aq), _addr(As), _addr(Bq), _addr(Bs), _addr(Yq), _addr(Ys), M, N, K,
-                           int(relu))
+        rc = self._f_mx_rq(self.handle, Aq, As, Bq, Bs, Yq, Ys, M, N, K, int(relu))
         if rc:
             self._raise(rc)
 
     def mlp_mxfp4(self, Xq, Xs, W1q, W1s, W2q, W2s, Hq, Hs, Y, M, K, F, Nout, dtype=BF16, ldy=None) -> None:
-        rc = self._f_mlp_mx(self.handle, _addr(Xq), _addr(Xs), _addr(W1q), _addr(W1s), _addr(W2q), _addr(W2s), _addr(Hq),
-                            _addr(Hs), _addr(Y), dtype, M, K, F, Nout, Nout if ldy is None else ldy)
+        rc = self._f_mlp_mx(self.handle, Xq, Xs, W1q, W1s, W2q, W2s, Hq, Hs, Y, dtype, M, K, F, Nout,
+                            Nout if ldy is None else ldy)
         if rc:
             self._raise(rc)
 
@@ -456,18 +459,18 @@ class Context:
     def norm_block(self, x, b, gate, w_after, w_before, out, y, rstd, rows, cols, ldx=None, ldb=None, gate_rows=None,
                    stream_dtype=BF16, branch_dtype=BF16, alpha=1.0, eps=1e-5) -> None:
         """out = alpha x + gate w_after b / rms(b); y = w_before out / rms(out)."""
-        rc = self._f_norm(self.handle, _addr(x), _addr(b), _addr(gate), _addr(w_after), _addr(w_before), _addr(out),
-                          _addr(y), _addr(rstd), rows, cols, cols if ldx is None else ldx, cols if ldb is None else ldb,
-                          rows if gate_rows is None else gate_rows, stream_dtype, branch_dtype, alpha, eps)
+        rc = self._f_norm(self.handle, x, b, gate, w_after, w_before, out, y, rstd, rows, cols,
+                          cols if ldx is None else ldx, cols if ldb is None else ldb, rows if gate_rows is None else gate_rows,
+                          stream_dtype, branch_dtype, alpha, eps)
         if rc:
             self._raise(rc)
 
     def norm_block_grad(self, r, b, gate, w_after, w_before, rstd, dout, dy, dx, db, dgate, dw_after, dw_before, work,
                         work_bytes, rows, cols, ldx=None, ldb=None, gate_rows=None, stream_dtype=BF16,
                         branch_dtype=BF16, alpha=1.0) -> None:
-        rc = self._f_norm_grad(self.handle, _addr(r), _addr(b), _addr(gate), _addr(w_after), _addr(w_before),
-                               _addr(rstd), _addr(dout), _addr(dy), _addr(dx), _addr(db), _addr(dgate), _addr(dw_after),
-                               _addr(dw_before), _addr(work), work_bytes, rows, cols, cols if ldx is None else ldx,
+        rc = self._f_norm_grad(self.handle, r, b, gate, w_after, w_before,
+                               rstd, dout, dy, dx, db, dgate, dw_after,
+                               dw_before, work, work_bytes, rows, cols, cols if ldx is None else ldx,
                                cols if ldb is None else ldb, rows if gate_rows is None else gate_rows, stream_dtype,
                                branch_dtype, alpha)
         if rc:

@@ -236,32 +236,43 @@ __global__ __launch_bounds__((64 * RowsGeom<MI, NJ, AI, SLOTS>::WAVES)) void gem
       slot = slot + 1 == SLOTS ? 0 : slot + 1;
     }
   }
-  // each wave's sums; row block i (every column block of it) is added up by wave
-  // i % waves
+  // each wave's sums; those of a unit of one or two column blocks are added up
+  // by one wave, eight loads in flight
   if (waves > 1) {
 #pragma unroll
     for (int f = 0; f < MI * NJ; ++f) *reinterpret_cast<v4f*>(mine + 1024 * f + 16 * lane) = acc[f / NJ][f % NJ];
     __syncthreads();
   }
+  constexpr int UN = NJ == 1 ? 1 : 2, UNITS = MI * NJ / UN;
 #pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    if (i % waves != wave) continue;
-    v4f sum[NJ];
+  for (int u = 0; u < UNITS; ++u) {
+    if (u % waves != wave) continue;
+    v4f sum[UN];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) sum[j] = acc[i][j];
-    for (int w = 1; w < waves; ++w) {
-      const int from = wave + w < waves ? wave + w : wave + w - waves;
+    for (int j = 0; j < UN; ++j) sum[j] = acc[u * UN / NJ][u * UN % NJ + j];
+    for (int w0 = 1; w0 < waves; w0 += 8) {
+      v4f part[8][UN];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) sum[j] += *reinterpret_cast<const v4f*>(lds + from * REGION + 1024 * (i * NJ + j) + 16 * lane);
+      for (int w = 0; w < 8; ++w) {
+        const int k = min(w0 + w, waves - 1), from = wave + k < waves ? wave + k : wave + k - waves;
+#pragma unroll
+        for (int j = 0; j < UN; ++j)
+          part[w][j] = *reinterpret_cast<const v4f*>(lds + from * REGION + 1024 * (u * UN + j) + 16 * lane);
+      }
+#pragma unroll
+      for (int w = 0; w < 8; ++w)
+        if (w0 + w < waves)
+#pragma unroll
+          for (int j = 0; j < UN; ++j) sum[j] += part[w][j];
     }
-    const int m = m0 + 16 * i + fr;
+    const int i = u * UN / NJ, j0 = u * UN % NJ, m = m0 + 16 * i + fr;
     if constexpr (OUT == OUT_F32 || OUT == OUT_BF16) {
       using T = std::conditional_t<OUT == OUT_F32, float, __bf16>;
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        store4(static_cast<T*>(p.C), p.ldc, m, n0 + 16 * j + 4 * fg, p.M, p.N, sum[j]);
+      for (int j = 0; j < UN; ++j)
+        store4(static_cast<T*>(p.C), p.ldc, m, n0 + 16 * (j0 + j) + 4 * fg, p.M, p.N, sum[j]);
     } else {
-      store_blocks<NJ / 2, OUT == OUT_MX_RELU, false>(p, m, n0 / 32, fg, sum);
+      store_blocks<1, OUT == OUT_MX_RELU, false>(p, m, (n0 + 16 * j0) / 32, fg, sum);
     }
   }
 }
@@ -416,18 +427,15 @@ __device__ __forceinline__ void store_quarter(T* C, size_t ldc, int m0, int n0, 
   }
 }
 
+// The tile at row m0 and column n0; last: no tile of its rows is behind it.
 template <int BM, int BN, Out OUT, bool EDGE>
-__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, int tiles_m, int tiles_n) {
+__device__ __forceinline__ void pipe_tile(const Args& p, int8_t* lds, int m0, int n0, bool last) {
   using G = PipeGeom<BM, BN>;
   constexpr int NI = G::NI, NJ = G::NJ, HI = G::HI, PH = G::PH;
-  __shared__ __attribute__((aligned(1024))) int8_t lds[G::LDS];
   constexpr int B0 = G::A_REGION, S0 = G::A_REGION + G::B_REGION;
   const uint32_t lds0 = dev::lds_addr(lds);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wn = wave & 1, fr = lane & 15, fg = lane >> 4;
-  int tm, tn;
-  dev::tile_coords<4>(blockIdx.x, tiles_m, tiles_n, tm, tn);
-  const int m0 = tm * BM, n0 = tn * BN;
   const uint32_t pitch = (uint32_t)q_pitch(p.K);
   const int KT = (int)(pitch / 64);  // even
 
@@ -680,7 +688,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, i
         store_blocks<NJ / 2, OUT == OUT_MX_RELU, false>(p, mw + 16 * i + fr, nw / 32, fg, acc[i]);
       dev::sched_fence();  // (more rows at once spill)
     }
-    if (tn == tiles_n - 1) {  // zeros up to the end of the last 512 columns
+    if (last) {  // zeros up to the end of the last 512 columns
       const int first = (n0 + BN) / 32, blocks = 16 * s_groups(p.N) - first;
       const size_t y_pitch = q_pitch(p.N);
       const v4i zero = {0, 0, 0, 0};
@@ -693,6 +701,46 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, i
       }
     }
   }
+}
+
+template <int BM, int BN, Out OUT, bool EDGE>
+__global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, int tiles_m, int tiles_n) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds[PipeGeom<BM, BN>::LDS];
+  int tm, tn;
+  dev::tile_coords<4>(blockIdx.x, tiles_m, tiles_n, tm, tn);
+  pipe_tile<BM, BN, OUT, EDGE>(p, lds, tm * BM, tn * BN, tn == tiles_n - 1);
+}
+
+// 256 x 256 tiles over the first `wide` tile columns, then 256 x 128 tiles: the
+// narrow ones fill the CUs that the last round of wide ones would leave idle
+// (2048 x 11008 x 4096 packed: 344 wide tiles on 256 CUs, 60 us; TBD us as 256 wide
+// and 176 narrow).
+template <Out OUT, bool EDGE>
+__global__ __launch_bounds__(256, 1) void gemm_mx_mixed(Args p, int tiles_m, int wide, int narrow) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds[PipeGeom<256, 256>::LDS];
+  int tm, tn;
+  if ((int)blockIdx.x < tiles_m * wide) {
+    dev::tile_coords<4>(blockIdx.x, tiles_m, wide, tm, tn);
+    pipe_tile<256, 256, OUT, false>(p, lds, tm * 256, tn * 256, false);
+  } else {
+    dev::tile_coords<4>(blockIdx.x - tiles_m * wide, tiles_m, narrow, tm, tn);
+    pipe_tile<256, 128, OUT, EDGE>(p, lds, tm * 256, wide * 256 + tn * 128, tn == narrow - 1);
+  }
+}
+
+template <Out OUT>
+int run_mixed(miaie_ctx* ctx, const Args& p, int wide) {
+  const int tiles_m = (p.M + 255) / 256, narrow = (p.N - 256 * wide + 127) / 128;
+  hipError_t e = hipSuccess;
+  auto go = [&](auto k) {
+    e = launch<decltype(k)::value>(ctx->device, dim3((unsigned)tiles_m * (wide + narrow)), dim3(256), 0, ctx->stream, p,
+                                   tiles_m, wide, narrow);
+  };
+  if ((OUT == OUT_F32 || OUT == OUT_BF16) && p.N % 128)
+    go(kernel_t<gemm_mx_mixed<OUT, OUT == OUT_F32 || OUT == OUT_BF16>>{});
+  else
+    go(kernel_t<gemm_mx_mixed<OUT, false>>{});
+  return check_launch(ctx, e, "gemm_mx_mixed");
 }
 
 template <int BM, int BN, Out OUT>
@@ -738,22 +786,32 @@ int run_rows(miaie_ctx* ctx, const Args& p) {
 struct Choice {
   double us = 1e30;
   int kernel = -1;
+  int wide = 0;  // tile columns of 256 (mixed tiles)
 };
 void consider(Choice& best, int kernel, double us) {
-  if (us < best.us) best = Choice{us, kernel};
+  if (us < best.us) best = Choice{us, kernel, 0};
 }
 
-double rows_us(long M, long cols, int groups, int mi, int nj, int slot, int cus) {
-  const long tiles = ((M + 16 * mi - 1) / (16 * mi)) * ((cols + 16 * nj - 1) / (16 * nj));
-  return 1.2 + (double)((tiles + cus - 1) / cus) * groups * slot / 42e3;
+template <int MI, int NJ, int AI>
+double rows_us(long M, long cols, int groups, int cus) {
+  using G = RowsGeom<MI, NJ, AI, 1>;
+  const long tiles = ((M + 16 * MI - 1) / (16 * MI)) * ((cols + 16 * NJ - 1) / (16 * NJ));
+  return 1.2 + 0.02 * G::OPS + (double)((tiles + cus - 1) / cus) * groups * G::SLOT / 42e3;
 }
 
-double pipe_us(long M, long N, int k_tiles, int bm, int bn, double start, double tile, double end, int cus) {
-  const long tiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+// Cycles of a workgroup on a tile: its start, a k-tile, its end (fp32, bf16, packed).
+struct TileCycles {
+  int bm;
+  double start, k_tile, end[3];
+};
+constexpr TileCycles kTiles[] = {{256, 4500, 1320, {16500, 7800, 9900}}, {256, 3400, 840, {8200, 3800, 5800}},
+                                 {128, 2400, 540, {3500, 1850, 3400}}};
+
+double pipe_us(long tiles, int k_tiles, const TileCycles& t, double end, int cus) {
   const long rounds = (tiles + cus - 1) / cus;
   const double ghz = 2 * tiles < cus ? 2.35e3 : 1.9e3;
-  if (bm == 128 && rounds > 1) return 1.0 + (double)((rounds + 1) / 2) * (1600 + start + end + 960.0 * k_tiles) / ghz;
-  return 1.0 + (double)rounds * (start + end + tile * k_tiles) / ghz;
+  if (t.bm == 128 && rounds > 1) return 1.0 + (double)((rounds + 1) / 2) * (1600 + t.start + end + 960.0 * k_tiles) / ghz;
+  return 1.0 + (double)rounds * (t.start + end + t.k_tile * k_tiles) / ghz;
 }
 
 template <Out OUT>
@@ -762,45 +820,62 @@ int run(miaie_ctx* ctx, const Args& p) {
   const int groups = s_groups(p.K), k_tiles = (int)(q_pitch(p.K) / 64), cus = ctx->cus;
   const long cols = packed ? 512l * s_groups(p.N) : p.N;
   Choice c;
-#define MIAIE_MX_ROWS(MI, NJ, AI) RowsGeom<MI, NJ, AI, 1>::SLOT
-  if (p.M <= 4)
-    consider(c, 0, rows_us(p.M, cols, groups, 1, 1 + packed, packed ? MIAIE_MX_ROWS(1, 2, 1) : MIAIE_MX_ROWS(1, 1, 1), cus));
-  else if (!packed)
-    consider(c, 1, rows_us(p.M, cols, groups, 1, 1, MIAIE_MX_ROWS(1, 1, 4), cus));
-  consider(c, 2, rows_us(p.M, cols, groups, 1, 2, MIAIE_MX_ROWS(1, 2, 4), cus));
-  consider(c, 3, rows_us(p.M, cols, groups, 1, 4, MIAIE_MX_ROWS(1, 4, 4), cus));
+  if (p.M <= 4) {
+    consider(c, 0, rows_us<1, 1 + packed, 1>(p.M, cols, groups, cus));
+  } else if (p.M <= 8) {
+    if (!packed) consider(c, 1, rows_us<1, 1, 2>(p.M, cols, groups, cus));
+    consider(c, 2, rows_us<1, 2, 2>(p.M, cols, groups, cus));
+    consider(c, 3, rows_us<1, 4, 2>(p.M, cols, groups, cus));
+  } else {
+    if (!packed) consider(c, 4, rows_us<1, 1, 4>(p.M, cols, groups, cus));
+    consider(c, 5, rows_us<1, 2, 4>(p.M, cols, groups, cus));
+    consider(c, 6, rows_us<1, 4, 4>(p.M, cols, groups, cus));
+  }
   if (p.M > 16) {
-    if (!packed) consider(c, 4, rows_us(p.M, cols, groups, 2, 1, MIAIE_MX_ROWS(2, 1, 8), cus));
-    consider(c, 5, rows_us(p.M, cols, groups, 2, 2, MIAIE_MX_ROWS(2, 2, 8), cus));
-    consider(c, 6, rows_us(p.M, cols, groups, 2, 4, MIAIE_MX_ROWS(2, 4, 8), cus));
+    if (!packed) consider(c, 7, rows_us<2, 1, 8>(p.M, cols, groups, cus));
+    consider(c, 8, rows_us<2, 2, 8>(p.M, cols, groups, cus));
+    consider(c, 9, rows_us<2, 4, 8>(p.M, cols, groups, cus));
   }
   if (p.M > 32) {
-    consider(c, 7, rows_us(p.M, cols, groups, 4, 2, MIAIE_MX_ROWS(4, 2, 16), cus));
-    consider(c, 8, rows_us(p.M, cols, groups, 4, 4, MIAIE_MX_ROWS(4, 4, 16), cus));
+    consider(c, 10, rows_us<4, 2, 16>(p.M, cols, groups, cus));
+    consider(c, 11, rows_us<4, 4, 16>(p.M, cols, groups, cus));
   }
-#undef MIAIE_MX_ROWS
   // (a row's offset within a tile in 32 bits, and HIP takes fewer than 2^32 threads)
   const long tiles = ((p.M + 127l) / 128) * ((p.N + 127l) / 128);
   if (q_pitch(p.K) < (1u << 24) && tiles < 1l << 23) {
-    const int o = packed ? 2 : OUT == OUT_BF16;
-    constexpr double end[3][3] = {{16500, 7800, 9900}, {8200, 3800, 5800}, {3500, 1850, 3400}};
-    consider(c, 9, pipe_us(p.M, p.N, k_tiles, 128, 128, 2400, 540, end[2][o], cus));
-    consider(c, 10, pipe_us(p.M, p.N, k_tiles, 256, 128, 3400, 840, end[1][o], cus));
-    consider(c, 11, pipe_us(p.M, p.N, k_tiles, 256, 256, 4500, 1320, end[0][o], cus));
+    constexpr int o = packed ? 2 : OUT == OUT_BF16;
+    consider(c, 12, pipe_us(tiles, k_tiles, kTiles[2], kTiles[2].end[o], cus));
+    const long tiles_m = (p.M + 255l) / 256, wide = (p.N + 255l) / 256;
+    consider(c, 13, pipe_us(tiles_m * ((p.N + 127l) / 128), k_tiles, kTiles[1], kTiles[1].end[o], cus));
+    consider(c, 14, pipe_us(tiles_m * wide, k_tiles, kTiles[0], kTiles[0].end[o], cus));
+    // whole rounds of wide tiles, then narrow ones
+    if (tiles_m * wide > cus && tiles_m <= cus && tiles_m * wide < 8l * cus) {
+      const long first = tiles_m * wide / cus * cus / tiles_m;  // wide tile columns
+      const long narrow = tiles_m * ((p.N - 256 * first + 127) / 128);
+      if (first > 0 && narrow > 0) {
+        const double us = pipe_us(tiles_m * first, k_tiles, kTiles[0], kTiles[0].end[o], cus) - 1.0 +
+                          pipe_us(narrow, k_tiles, kTiles[1], kTiles[1].end[o], cus);
+        if (us < c.us) c = Choice{us, 15, (int)first};
+      }
+    }
   }
   switch (c.kernel) {
     case 0: return run_rows<1, 1 + packed, 1, 1, OUT>(ctx, p);
-    case 1: return run_rows<1, 1 + packed, 4, 1, OUT>(ctx, p);
-    case 2: return run_rows<1, 2, 4, 1, OUT>(ctx, p);
-    case 3: return run_rows<1, 4, 4, 1, OUT>(ctx, p);
-    case 4: return run_rows<2, 1 + packed, 8, 1, OUT>(ctx, p);
-    case 5: return run_rows<2, 2, 8, 1, OUT>(ctx, p);
-    case 6: return run_rows<2, 4, 8, 1, OUT>(ctx, p);
-    case 7: return run_rows<4, 2, 16, 1, OUT>(ctx, p);
-    case 8: return run_rows<4, 4, 16, 1, OUT>(ctx, p);
-    case 9: return run_pipe<128, 128, OUT>(ctx, p);
-    case 10: return run_pipe<256, 128, OUT>(ctx, p);
-    default: return run_pipe<256, 256, OUT>(ctx, p);
+    case 1: return run_rows<1, 1 + packed, 2, 1, OUT>(ctx, p);
+    case 2: return run_rows<1, 2, 2, 1, OUT>(ctx, p);
+    case 3: return run_rows<1, 4, 2, 1, OUT>(ctx, p);
+    case 4: return run_rows<1, 1 + packed, 4, 1, OUT>(ctx, p);
+    case 5: return run_rows<1, 2, 4, 1, OUT>(ctx, p);
+    case 6: return run_rows<1, 4, 4, 1, OUT>(ctx, p);
+    case 7: return run_rows<2, 1 + packed, 8, 1, OUT>(ctx, p);
+    case 8: return run_rows<2, 2, 8, 1, OUT>(ctx, p);
+    case 9: return run_rows<2, 4, 8, 1, OUT>(ctx, p);
+    case 10: return run_rows<4, 2, 16, 1, OUT>(ctx, p);
+    case 11: return run_rows<4, 4, 16, 1, OUT>(ctx, p);
+    case 12: return run_pipe<128, 128, OUT>(ctx, p);
+    case 13: return run_pipe<256, 128, OUT>(ctx, p);
+    case 14: return run_pipe<256, 256, OUT>(ctx, p);
+    default: return run_mixed<OUT>(ctx, p, c.wide);
   }
 }
 
