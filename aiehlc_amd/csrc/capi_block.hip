@@ -44,7 +44,7 @@ int check_packed(miaie_ctx* ctx, const char* fn, const char* name, const uint8_t
 // One workgroup packs 64 rows of a packed transpose (quant_mxfp4.hip), and HIP
 // takes fewer than 2^32 threads.
 int check_transpose(miaie_ctx* ctx, const char* fn, int R, int C) {
-  if ((long)mx::s_groups(R) * (((long)C + 63) / 64) >= 1l << 23)
+  if ((long)mx::s_groups(R) * 8 * mx::s_groups(C) >= 1l << 23)
     return fail(ctx, MIAIE_EINVAL, "%s: R=%d C=%d too large to pack along the columns", fn, R, C);
   return MIAIE_OK;
 }

@@ -41,6 +41,8 @@ __global__ __launch_bounds__(256) void quant_rows(const T* __restrict__ X, uint8
   }
 }
 
+typedef uint16_t v2us __attribute__((ext_vector_type(2)));
+
 // Two adjacent columns of one row; the second is absent in the last column of
 // an odd matrix.
 template <class T>
@@ -54,6 +56,14 @@ struct Pair<float> {
       v = MIAIE_LD(reinterpret_cast<const P*>(p)).v;
     else
       v = v2f{MIAIE_LD(p), 0.f};
+  }
+  // exponents of the larger of a row's two magnitudes, two rows
+  __device__ __forceinline__ static uint32_t exponents(const Pair& a, const Pair& b) {
+    return max(abs_bits(a.v[0]), abs_bits(a.v[1])) >> 23 | max(abs_bits(b.v[0]), abs_bits(b.v[1])) >> 23 << 16;
+  }
+  template <int BYTE>
+  __device__ __forceinline__ uint32_t codes(uint32_t q, float scale) const {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, v[0], v[1], scale, BYTE);
   }
   __device__ __forceinline__ static void pack(const Pair (&x)[32], uint32_t (&s)[2], uint32_t (&q)[2][4]) {
     uint32_t a0 = 0, a1 = 0;
@@ -80,9 +90,17 @@ struct Pair<__bf16> {
     else
       v = MIAIE_LD(reinterpret_cast<const uint16_t*>(p));
   }
-  // (magnitudes are compared as 16-bit integers, two columns in one instruction)
+  // (magnitudes are compared as 16-bit integers, two in one instruction)
+  __device__ __forceinline__ static uint32_t exponents(const Pair& a, const Pair& b) {
+    const v2us c0 = __builtin_bit_cast(v2us, __builtin_amdgcn_perm(b.v, a.v, 0x05040100u) & 0x7fff7fffu);
+    const v2us c1 = __builtin_bit_cast(v2us, __builtin_amdgcn_perm(b.v, a.v, 0x07060302u) & 0x7fff7fffu);
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(c0, c1) >> 7);
+  }
+  template <int BYTE>
+  __device__ __forceinline__ uint32_t codes(uint32_t q, float scale) const {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, __builtin_bit_cast(v2bf, v), scale, BYTE);
+  }
   __device__ __forceinline__ static void pack(const Pair (&x)[32], uint32_t (&s)[2], uint32_t (&q)[2][4]) {
-    typedef uint16_t v2us __attribute__((ext_vector_type(2)));
     v2us a = {0, 0};
 #pragma unroll
     for (int i = 0; i < 32; ++i) a = __builtin_elementwise_max(a, __builtin_bit_cast(v2us, x[i].v & 0x7fff7fffu));
@@ -113,11 +131,19 @@ struct Pair<__bf16> {
 // wave the columns beside them, so every load of a half wave is one row's 128
 // (bf16) or 256 bytes, all 32 are in flight, and no lane needs another's values.
 // The packed rows (256 bytes of 64 columns) leave through LDS in whole lines.
-template <class T>
-__global__ __launch_bounds__(512) void quant_cols(const T* __restrict__ X, uint8_t* __restrict__ Q,
+//
+// ROWS: along the columns' axis too, from the same registers.  A block of 32
+// columns is the 16 lanes of a half wave's half, whose maxima come from four lane
+// permutations, for two rows at a time (only the exponents are needed); the codes
+// leave through LDS, 32 bytes of a row.  (2048 x 4096 bf16: TBD us, TBD in two
+// launches.)
+template <class T, bool ROWS>
+__global__ __launch_bounds__(512) void quant_cols(const T* __restrict__ X, uint8_t* __restrict__ Qt,
+                                                  uint8_t* __restrict__ St, uint8_t* __restrict__ Q,
                                                   uint8_t* __restrict__ S, int R, int C, int ldx, int tiles_c) {
-  constexpr int P = 272;  // bytes of a packed row in LDS
+  constexpr int P = 272, PR = 36;  // bytes of a packed column, and of 64 columns of a packed row, in LDS
   __shared__ __attribute__((aligned(16))) uint8_t lq[64 * P], ls[64 * 16];
+  __shared__ __attribute__((aligned(16))) uint8_t rq[ROWS ? 512 * PR : 16], rs[ROWS ? 2 * 512 : 16];
   const int tid = threadIdx.x, pair = tid & 31, rb = tid >> 5;  // column pair, block of rows
   const int g = blockIdx.x / tiles_c, c0 = 64 * (blockIdx.x % tiles_c), c = c0 + 2 * pair;
   const int r0 = 512 * g + 32 * rb;
@@ -135,6 +161,40 @@ __global__ __launch_bounds__(512) void quant_cols(const T* __restrict__ X, uint8
     *reinterpret_cast<uint4*>(lq + (2 * pair + k) * P + 16 * rb) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
     ls[(2 * pair + k) * 16 + s_byte(rb)] = (uint8_t)s[k];
   }
+  if constexpr (ROWS) {
+    uint32_t scales[8];  // of the block's 32 rows, a byte each
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      uint32_t pairs[2], codes = 0;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        v2us e = __builtin_bit_cast(v2us, Pair<T>::exponents(x[4 * d + 2 * k], x[4 * d + 2 * k + 1]));
+        auto widen = [&](auto ctrl) {
+          e = __builtin_elementwise_max(e, __builtin_bit_cast(v2us, quad_swap<decltype(ctrl)::value>(__builtin_bit_cast(uint32_t, e))));
+        };
+        widen(std::integral_constant<int, 0xB1>{});   // 1 0 3 2 of a four
+        widen(std::integral_constant<int, 0x4E>{});   // 2 3 0 1
+        widen(std::integral_constant<int, 0x141>{});  // the other four of eight
+        widen(std::integral_constant<int, 0x140>{});  // the other eight of sixteen
+        // scale_of: e - 2 from 2 on, 255 for 255
+        const v2us two = {2, 2}, top = {254, 254};
+        const v2us nan = __builtin_elementwise_max(e, top) - top;
+        pairs[k] = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(e, two) - two + nan + nan);
+      }
+      codes = x[4 * d].template codes<0>(codes, scale_f32(pairs[0] & 255));
+      codes = x[4 * d + 1].template codes<1>(codes, scale_f32(pairs[0] >> 16));
+      codes = x[4 * d + 2].template codes<2>(codes, scale_f32(pairs[1] & 255));
+      codes = x[4 * d + 3].template codes<3>(codes, scale_f32(pairs[1] >> 16));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) rq[(32 * rb + 4 * d + k) * PR + pair] = (uint8_t)(codes >> (8 * k));
+      scales[d] = __builtin_amdgcn_perm(pairs[1], pairs[0], 0x06040200u);
+    }
+    if ((pair & 15) == 0) {
+      uint4* to = reinterpret_cast<uint4*>(rs + 512 * (pair >> 4) + 32 * rb);
+      to[0] = make_uint4(scales[0], scales[1], scales[2], scales[3]);
+      to[1] = make_uint4(scales[4], scales[5], scales[6], scales[7]);
+    }
+  }
   __syncthreads();
   const size_t pitch = q_pitch(R);
 #pragma unroll
@@ -142,10 +202,25 @@ __global__ __launch_bounds__(512) void quant_cols(const T* __restrict__ X, uint8
     const int col = 32 * k + (tid >> 4), ch = tid & 15;
     const size_t off = 256 * (size_t)g + 16 * ch;
     if (c0 + col < C && off < pitch)
-      MIAIE_ST(reinterpret_cast<uint4*>(Q + (size_t)(c0 + col) * pitch + off), *reinterpret_cast<const uint4*>(lq + col * P + 16 * ch));
+      MIAIE_ST(reinterpret_cast<uint4*>(Qt + (size_t)(c0 + col) * pitch + off), *reinterpret_cast<const uint4*>(lq + col * P + 16 * ch));
   }
   if (tid < 64 && c0 + tid < C)
-    MIAIE_ST(reinterpret_cast<uint4*>(S + ((size_t)g * C + c0 + tid) * 16), *reinterpret_cast<const uint4*>(ls + 16 * tid));
+    MIAIE_ST(reinterpret_cast<uint4*>(St + ((size_t)g * C + c0 + tid) * 16), *reinterpret_cast<const uint4*>(ls + 16 * tid));
+  if constexpr (ROWS) {
+    const int row = 512 * g + tid;
+    if (row < R) {
+      const size_t row_pitch = q_pitch(C);
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(rq + tid * PR);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if ((size_t)c0 / 2 + 16 * k < row_pitch)
+          MIAIE_ST(reinterpret_cast<uint4*>(Q + row * row_pitch + c0 / 2 + 16 * k),
+                   make_uint4(from[4 * k], from[4 * k + 1], from[4 * k + 2], from[4 * k + 3]));
+        const int block = c0 / 32 + k;
+        MIAIE_ST(S + ((size_t)(block >> 4) * R + row) * 16 + s_byte(block), rs[512 * k + tid]);
+      }
+    }
+  }
 }
 
 // One wave unpacks 512 columns of a row (8192 x 8192 to bf16: 25.6 us).
@@ -178,14 +253,17 @@ int launch_quant_mxfp4(miaie_ctx* ctx, const void* X, int dtype, int R, int C, i
   auto go = [&](auto t) {
     using T = typename decltype(t)::type;
     const T* x = static_cast<const T*>(X);
-    if (Q) {
+    if (Q && Qt) {  // (the rows' form has zeros up to the end of its last 512 columns)
+      const int tiles_c = 8 * s_groups(C);
+      e = launch<quant_cols<T, true>>(ctx->device, dim3((unsigned)s_groups(R) * tiles_c), dim3(512), 0, ctx->stream, x, Qt,
+                                      St, Q, S, R, C, ldx, tiles_c);
+    } else if (Q) {
       const int units = R * s_groups(C), grid = wave_grid(units);
       e = launch<quant_rows<T>>(ctx->device, dim3(grid), dim3(256), 0, ctx->stream, x, Q, S, R, C, ldx, units, 4 * grid);
-    }
-    if (Qt && e == hipSuccess) {
+    } else {
       const int tiles_c = (C + 63) / 64;
-      e = launch<quant_cols<T>>(ctx->device, dim3((unsigned)s_groups(R) * tiles_c), dim3(512), 0, ctx->stream, x, Qt,
-                                St, R, C, ldx, tiles_c);
+      e = launch<quant_cols<T, false>>(ctx->device, dim3((unsigned)s_groups(R) * tiles_c), dim3(512), 0, ctx->stream, x, Qt,
+                                       St, nullptr, nullptr, R, C, ldx, tiles_c);
     }
   };
   if (dtype == MIAIE_BF16)
