@@ -23,8 +23,14 @@
 //                   buffers each), every context's output checked against
 //                   the first's
 //   mlp M K F N     chained int8 MLP, golden on sampled rows
+//   block M D F     a 4-bit feed-forward block of a residual network (no
+//                   counterpart in the reference): norm, conversion to MXFP4,
+//                   4-bit MLP, norm with gate and residual, and the norm before
+//                   the next block; golden in double on sampled rows
+#include <algorithm>
 #include <atomic>
 #include <chrono>
+#include <cmath>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -344,10 +350,129 @@ int run_mlp(miaie::Context& ctx, int M, int K, int F, int Nout) {
   return report(mismatches, "mlp");
 }
 
+// ---- the 4-bit block ----
+uint16_t to_bf16(float v) {
+  uint32_t u;
+  memcpy(&u, &v, 4);
+  return (uint16_t)((u + 0x7fff + ((u >> 16) & 1)) >> 16);
+}
+float from_bf16(uint16_t h) {
+  const uint32_t u = (uint32_t)h << 16;
+  float v;
+  memcpy(&v, &u, 4);
+  return v;
+}
+
+// v rounded to MXFP4 in blocks of 32, in place.
+void round_mxfp4(std::vector<double>& v) {
+  static const double grid[] = {0, 0.5, 1, 1.5, 2, 3, 4, 6};
+  for (size_t b = 0; b < v.size(); b += 32) {
+    const size_t n = std::min<size_t>(32, v.size() - b);
+    double amax = 0;
+    for (size_t i = 0; i < n; ++i) amax = std::max(amax, std::fabs(v[b + i]));
+    const double scale = amax > 0 ? std::exp2(std::floor(std::log2(amax)) - 2) : 1;
+    for (size_t i = 0; i < n; ++i) {
+      const double a = std::fabs(v[b + i]) / scale;
+      int c = 0;
+      while (c < 7 && (c % 2 ? a >= (grid[c] + grid[c + 1]) / 2 : a > (grid[c] + grid[c + 1]) / 2)) ++c;
+      v[b + i] = std::copysign(grid[c] * scale, v[b + i]);
+    }
+  }
+}
+
+double inverse_rms(const std::vector<double>& v, double eps) {
+  double s = 0;
+  for (double x : v) s += x * x;
+  return 1 / std::sqrt(s / (double)v.size() + eps);
+}
+
+int run_block(miaie::Context& ctx, int M, int D, int F) {
+  auto values = [](size_t n, uint64_t id, float size, float mean) {
+    const std::vector<int8_t> r = seeded_i8(n, id);
+    std::vector<float> v(n);
+    for (size_t i = 0; i < n; ++i) v[i] = mean + size * (float)r[i] / 64.f;
+    return v;
+  };
+  auto bf16 = [](const std::vector<float>& v) {
+    std::vector<uint16_t> h(v.size());
+    for (size_t i = 0; i < v.size(); ++i) h[i] = to_bf16(v[i]);
+    return h;
+  };
+  auto buffer = [&](const auto& v) {
+    miaie::Buffer<typename std::decay_t<decltype(v)>::value_type> b(ctx, v.size());
+    b.move_in(v);
+    return b;
+  };
+  const miaie::NormShape shape{M, D, 0.875f, 1e-5f, (M + 1) / 2};  // a gate row for each half of the tokens
+  const std::vector<uint16_t> x = bf16(values((size_t)M * D, 1, 1.f, 0.f)), gate = bf16(values((size_t)2 * D, 2, 0.2f, 1.f));
+  const std::vector<float> w1 = values((size_t)F * D, 3, 1.f / std::sqrt((float)D), 0.f),
+                           w2 = values((size_t)D * F, 4, 1.f / std::sqrt((float)F), 0.f), wb = values(D, 5, 0.1f, 1.f),
+                           wa = values(D, 6, 0.1f, 1.f), wn = values(D, 7, 0.1f, 1.f);
+  auto dx = buffer(x), dgate = buffer(gate);
+  auto d1 = buffer(w1), d2 = buffer(w2), dwb = buffer(wb), dwa = buffer(wa), dwn = buffer(wn);
+  // the weights are packed once
+  miaie::MxMatrix W1(ctx, F, D), W2(ctx, D, F), X(ctx, M, D), H(ctx, M, F);
+  miaie::quant_mxfp4(d1, W1, ctx);
+  miaie::quant_mxfp4(d2, W2, ctx);
+  miaie::Buffer<uint16_t> y(ctx, (size_t)M * D), b(ctx, (size_t)M * D), out(ctx, (size_t)M * D), next(ctx, (size_t)M * D);
+  // the block, queued as a whole
+  miaie::norm_before(dx, dwb, y, shape, nullptr, ctx);
+  miaie::quant_mxfp4(y, X, ctx);
+  miaie::mlp_mxfp4(X, W1, W2, H, b, ctx);
+  miaie::norm_block(dx, b, &dgate, dwa, &dwn, out, &next, shape, nullptr, ctx);
+  if (!ctx.wait(kDeadlineMs)) return 2;
+  const std::vector<uint16_t> got_out = out.move_out(), got_next = next.move_out();
+  // weights as the products see them
+  auto rounded_rows = [](const std::vector<float>& w, int rows, int cols) {
+    std::vector<double> r;
+    r.reserve(w.size());
+    for (int i = 0; i < rows; ++i) {
+      std::vector<double> row(w.begin() + (size_t)i * cols, w.begin() + (size_t)(i + 1) * cols);
+      round_mxfp4(row);
+      r.insert(r.end(), row.begin(), row.end());
+    }
+    return r;
+  };
+  const std::vector<double> v1 = rounded_rows(w1, F, D), v2 = rounded_rows(w2, D, F);
+  // A value may differ by its own rounding, and by the few codes whose rounding
+  // an fp32 sum turns the other way: 2% of the row's size.
+  int mismatches = 0;
+  for (int i : {0, M / 2, M - 1}) {
+    std::vector<double> r(D), h(F), o(D);
+    for (int k = 0; k < D; ++k) r[k] = from_bf16(x[(size_t)i * D + k]);
+    std::vector<double> yr = r;
+    const double rb = inverse_rms(r, shape.eps);
+    for (int k = 0; k < D; ++k) yr[k] = from_bf16(to_bf16((float)(r[k] * rb * wb[k])));
+    round_mxfp4(yr);
+    for (int f = 0; f < F; ++f) {
+      double s = 0;
+      for (int k = 0; k < D; ++k) s += yr[k] * v1[(size_t)f * D + k];
+      h[f] = std::max(s, 0.0);
+    }
+    round_mxfp4(h);
+    for (int k = 0; k < D; ++k) {
+      double s = 0;
+      for (int f = 0; f < F; ++f) s += h[f] * v2[(size_t)k * F + f];
+      o[k] = from_bf16(to_bf16((float)s));
+    }
+    const double ra = inverse_rms(o, shape.eps);
+    for (int k = 0; k < D; ++k)
+      o[k] = shape.alpha * r[k] + from_bf16(gate[(size_t)(i / shape.gate_rows) * D + k]) * wa[k] * o[k] * ra;
+    const double ro = inverse_rms(o, shape.eps);
+    for (int k = 0; k < D; ++k) {
+      const double n = o[k] * ro * wn[k];
+      mismatches += !(std::fabs(from_bf16(got_out[(size_t)i * D + k]) - o[k]) <= 0.02 * std::max(1 / ro, std::fabs(o[k])));
+      mismatches += !(std::fabs(from_bf16(got_next[(size_t)i * D + k]) - n) <= 0.02 * std::max(1.0, std::fabs(n)));
+    }
+  }
+  return report(mismatches, "block");
+}
+
 int usage() {
   fprintf(stderr,
           "usage: miaie_examples mm [n 8|16] [base] | perf | nokernelload | multi_tile | seq_full_col | vek385 |\n"
-          "                      gemm M N K shift | conv [reps] [streams] | mlp M K F N\n");
+          "                      gemm M N K shift | conv [reps] [streams] | mlp M K F N |\n"
+          "                      block M D F\n");
   return 64;
 }
 
@@ -373,6 +498,7 @@ int main(int argc, char** argv) {
     if (cmd == "gemm") return run_gemm(ctx, arg(2, 4096), arg(3, 4096), arg(4, 4096), arg(5, 10));
     if (cmd == "conv") return run_conv(ctx, arg(2, 0), arg(3, 1));
     if (cmd == "mlp") return run_mlp(ctx, arg(2, 256), arg(3, 4096), arg(4, 11008), arg(5, 4096));
+    if (cmd == "block") return run_block(ctx, arg(2, 96), arg(3, 1024), arg(4, 4096));
     return usage();
   } catch (const miaie::Error& e) {
     fprintf(stderr, "miaie error %d: %s\n", e.code(), e.what());

@@ -281,6 +281,35 @@ void mlp_mxfp4(const MxMatrix& X, const MxMatrix& W1, const MxMatrix& W2, MxMatr
                             W2.rows));
 }
 
+// Row counts, sizes and constants of the norms around a block (miaie_norm_block).
+struct NormShape {
+  int rows, cols;
+  float alpha = 1.f, eps = 1e-5f;
+  int gate_rows = 0;  // rows that share a gate row; 0: all of them
+};
+
+// y = w_before * x / rms(x).
+template <typename S, typename B>
+void norm_before(const Buffer<S>& x, const Buffer<float>& w_before, Buffer<B>& y, const NormShape& n,
+                 Buffer<float>* rstd = nullptr, Context& ctx = Context::current()) {
+  ctx.check(miaie_norm_block(ctx.get(), x.data(), nullptr, nullptr, nullptr, w_before.data(), nullptr, y.data(),
+                             rstd ? rstd->data() : nullptr, n.rows, n.cols, n.cols, n.cols, n.rows,
+                             dtype_of(x.data()), dtype_of(y.data()), n.alpha, n.eps));
+}
+
+// out = alpha x + gate * w_after * b / rms(b) and, with w_before and y, the
+// norm before the next block, y = w_before * out / rms(out).  gate (nullable):
+// ceil(rows / gate_rows) x cols.
+template <typename S, typename B>
+void norm_block(const Buffer<S>& x, const Buffer<B>& b, const Buffer<B>* gate, const Buffer<float>& w_after,
+                const Buffer<float>* w_before, Buffer<S>& out, Buffer<B>* y, const NormShape& n,
+                Buffer<float>* rstd = nullptr, Context& ctx = Context::current()) {
+  ctx.check(miaie_norm_block(ctx.get(), x.data(), b.data(), gate ? gate->data() : nullptr, w_after.data(),
+                             w_before ? w_before->data() : nullptr, out.data(), y ? y->data() : nullptr,
+                             rstd ? rstd->data() : nullptr, n.rows, n.cols, n.cols, n.cols,
+                             n.gate_rows ? n.gate_rows : n.rows, dtype_of(x.data()), dtype_of(b.data()), n.alpha, n.eps));
+}
+
 }  // namespace miaie
 
 #endif  // MIAIE_HPP

@@ -374,3 +374,81 @@ def test_refusals(ctx):
     refused(m, *[p] * 9, 5, 4, 4, 4, 4, 4, text="dtype=5")
     ctx.wait(10_000)
     d.free()
+
+
+def test_two_streams_share_nothing(ctx):
+    """Contexts on two streams, their calls interleaved without waiting: no call uses memory of the library's."""
+    M, K, N = 16, 2048, 512
+    _say("two streams")
+    rng = np.random.default_rng(6)
+    ctxs = [ctx, mi.Context(0)]
+    try:
+        work = []
+        for c in ctxs:
+            A, B = _operand(rng, M, K), _operand(rng, N, K)
+            bufs = [c.upload(v) for v in (*A, *B)]
+            outs = [c.empty((M, N), np.float32) for _ in range(4)]
+            c.wait(60_000)
+            work.append((c, mx.values(*A, K), mx.values(*B, K), bufs, outs))
+        for i in range(4):
+            for c, _, _, bufs, outs in work:
+                c.gemm_mxfp4(*bufs, outs[i], M, N, K)
+        for c, a, b, bufs, outs in work:
+            c.wait(60_000)
+            for o in outs:
+                assert (np.abs(c.download(o) - a @ b.T) <= mx.product_bound(a, b)).all()
+            for x in (*bufs, *outs):
+                x.free()
+    finally:
+        ctxs[1].close()
+
+
+def test_captured_by_the_caller():
+    """A caller's own HIP graph of a block's calls, replayed on another stream beside eager calls of the context,
+    every replay against the eager result."""
+    from hip_capture import Capture
+
+    _say("caller's capture")
+    cap = Capture()
+    try:
+        c = cap.ctx
+        M, K, F = 12, 300, 700
+        rng = np.random.default_rng(11)
+        W1, W2 = _operand(rng, F, K), _operand(rng, K, F)
+        w = [c.upload(v) for v in (*W1, *W2)]
+        X, wn = c.empty((M, K), np.float32), c.upload(np.float32(1 + 0.1 * rng.standard_normal(K)))
+        q, h = _packed(c, M, K), _packed(c, M, F)
+        b, out, y, rstd = (c.empty(s, np.float32) for s in ((M, K), (M, K), (M, K), (2, M)))
+        dw, work = [c.empty((K,), np.float32) for _ in range(2)], c.empty((1024 * K,), np.float32)
+        dx, db = c.empty((M, K), np.float32), c.empty((M, K), np.float32)
+        kw = {"stream_dtype": mi.F32, "branch_dtype": mi.F32}
+
+        def block():
+            c.quant_mxfp4(X, M, K, *q, dtype=mi.F32)
+            c.mlp_mxfp4(*q, *w, *h, b, M, K, F, K, dtype=mi.F32)
+            c.norm_block(X, b, None, wn, wn, out, y, rstd, M, K, **kw)
+            c.norm_block_grad(out, b, None, wn, wn, rstd, X, b, dx, db, None, *dw, work, mi.norm_work_bytes(K), M, K, **kw)
+
+        results = (out, y, dx, db, *dw)
+        exe, grids = cap.record(block)
+        assert len(grids) == 6  # conversion, two products, norms, their gradient and the sums of its parts
+        for i in range(4):
+            x = np.float32(rng.standard_normal((M, K)))
+            c.copy_h2d(X, x)
+            cap.sync()
+            cap.replay(exe)
+            cap.sync()
+            got = [c.download(r) for r in results]
+            block()
+            cap.sync()
+            for g, r in zip(got, results):
+                assert np.array_equal(g, c.download(r)), i
+            v = mx.values(*mx.pack(x), K)
+            hv = mx.values(*mx.pack(np.maximum(v @ mx.values(*W1, K).T, 0)), F)
+            want = hv @ mx.values(*W2, F).T
+            assert np.abs(c.download(b) - want).max() <= 0.02 * np.abs(want).max()  # (a code of h may round the other way)
+        cap.ok(cap.hip.hipGraphExecDestroy(exe))
+        for t in (*w, X, wn, *q, *h, b, out, y, rstd, *dw, work, dx, db):
+            t.free()
+    finally:
+        cap.close()

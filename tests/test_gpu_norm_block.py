@@ -280,3 +280,17 @@ def test_refusals(ctx):
     refused(h, p, p, p, p, p, p, p, p, p, p, p, p, p, p, mi._sz(4096 * 8 - 1), *m[1:], text="work_bytes")
     ctx.wait(10_000)
     d.free()
+
+
+def test_example_of_a_whole_block():
+    """aiehlc_amd/harness/miaie_examples block: norm, conversion, 4-bit MLP, norm with gate and residual, through the
+    C++ host surface, against its own golden."""
+    import os
+    import subprocess
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for args in ((), ("5", "200", "333"), ("300", "512", "1000")):
+        print("[case] miaie_examples block", *args, flush=True)
+        r = subprocess.run([os.path.join(root, "aiehlc_amd", "harness", "miaie_examples"), "block", *args], capture_output=True,
+                           text=True, timeout=100)
+        assert r.returncode == 0 and "CPU result matches" in r.stdout, (r.returncode, r.stdout, r.stderr)
