@@ -127,20 +127,20 @@ __device__ __forceinline__ void store_blocks(const Args& p, int m, int nb, int f
 // In LDS chunk c (16 bytes) of row r lies at c ^ (r % 16), so the 16 rows of a
 // fragment read cover all banks.  A has 4 AI rows there; fragment rows behind
 // them repeat the last.
-template <int MI, int NJ, int AI, int SLOTS>
+template <int MI, int NJ, int AI>
 struct RowsGeom {
   static constexpr int B = 0, A = 4096 * NJ, SB = A + 1024 * AI, SA = SB + 256 * NJ;
-  static constexpr int SLOT = SA + 256 * MI;               // bytes of a group
+  static constexpr int GROUP = SA + 256 * MI;              // bytes of a group
   static constexpr int OPS = 4 * NJ + AI + NJ + MI;        // copies of a group
   static constexpr int SUM = MI * NJ * 1024;               // bytes of a wave's sums
-  static constexpr int REGION = std::max(SLOTS * SLOT, SUM);
+  static constexpr int REGION = std::max(GROUP, SUM);
   static constexpr int WAVES = std::min(16, 163840 / REGION);  // at most
-  static_assert(AI <= 4 * MI && OPS <= 63, "rows of A, copies in flight");
+  static_assert(AI <= 4 * MI, "rows of A");
 };
 
-template <int MI, int NJ, int AI, int SLOTS, Out OUT>
-__global__ __launch_bounds__((64 * RowsGeom<MI, NJ, AI, SLOTS>::WAVES)) void gemm_mx_rows(Args p, int tiles_n, int waves) {
-  using G = RowsGeom<MI, NJ, AI, SLOTS>;
+template <int MI, int NJ, int AI, Out OUT>
+__global__ __launch_bounds__((64 * RowsGeom<MI, NJ, AI>::WAVES)) void gemm_mx_rows(Args p, int tiles_n, int waves) {
+  using G = RowsGeom<MI, NJ, AI>;
   constexpr int REGION = G::REGION;
   extern __shared__ __attribute__((aligned(1024))) int8_t lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -163,13 +163,12 @@ __global__ __launch_bounds__((64 * RowsGeom<MI, NJ, AI, SLOTS>::WAVES)) void gem
   // copy x of an operand: rows 4 x .. 4 x + 3, 16 lanes each; rows behind the last
   // one repeat it.  A last group of 256 columns repeats its first half.
   const int a_last = p.M - 1 - m0, b_last = p.N - 1 - n0;
-  auto copy = [&](int g, int slot) __attribute__((always_inline)) {
-    const uint32_t to = mine0 + slot * G::SLOT;
+  auto copy = [&](int g) __attribute__((always_inline)) {
     const uint32_t mask = half && g == groups - 1 ? 7 : 15;
     auto rows = [&](const uint8_t* base, int x, int last, uint32_t st, const dbg::Span& span) __attribute__((always_inline)) {
       const int r = 4 * x + fg;
       const uint32_t off = (uint32_t)min(r, last) * pitch + 16 * ((fr ^ (r & 15)) & mask);
-      dev::gload_lds16(base + 256 * (size_t)g, off, to + st + 1024 * x, span);
+      dev::gload_lds16(base + 256 * (size_t)g, off, mine0 + st + 1024 * x, span);
     };
 #pragma unroll
     for (int x = 0; x < 4 * NJ; ++x) rows(b_base, x, b_last, G::B, bq_span);
@@ -178,29 +177,28 @@ __global__ __launch_bounds__((64 * RowsGeom<MI, NJ, AI, SLOTS>::WAVES)) void gem
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
       dev::gload_lds4(p.Bs + ((size_t)g * p.N + n0) * 16, 16 * (uint32_t)min(16 * j + fr, b_last) + 4 * fg,
-                      to + G::SB + 256 * j, bs_span);
+                      mine0 + G::SB + 256 * j, bs_span);
 #pragma unroll
     for (int i = 0; i < MI; ++i)
       dev::gload_lds4(p.As + ((size_t)g * p.M + m0) * 16, 16 * (uint32_t)min(16 * i + fr, a_last) + 4 * fg,
-                      to + G::SA + 256 * i, as_span);
+                      mine0 + G::SA + 256 * i, as_span);
   };
-  auto multiply = [&](int g, int slot) __attribute__((always_inline)) {
-    const int8_t* const from = mine + slot * G::SLOT;
+  auto multiply = [&](int g) __attribute__((always_inline)) {
     int sa[MI], sb[NJ];
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) sb[j] = *reinterpret_cast<const int*>(from + G::SB + 256 * j + 4 * lane);
+    for (int j = 0; j < NJ; ++j) sb[j] = *reinterpret_cast<const int*>(mine + G::SB + 256 * j + 4 * lane);
 #pragma unroll
-    for (int i = 0; i < MI; ++i) sa[i] = *reinterpret_cast<const int*>(from + G::SA + 256 * i + 4 * lane);
+    for (int i = 0; i < MI; ++i) sa[i] = *reinterpret_cast<const int*>(mine + G::SA + 256 * i + 4 * lane);
     auto step = [&](auto t_c) __attribute__((always_inline)) {
       constexpr int t = decltype(t_c)::value;
       v4i a[MI], b[NJ];
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
-        b[j] = *reinterpret_cast<const v4i*>(from + G::B + 4096 * j + 256 * fr + 16 * ((4 * t + fg) ^ fr));
+        b[j] = *reinterpret_cast<const v4i*>(mine + G::B + 4096 * j + 256 * fr + 16 * ((4 * t + fg) ^ fr));
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
         const int r = min(16 * i + fr, 4 * AI - 1);
-        a[i] = *reinterpret_cast<const v4i*>(from + G::A + 256 * r + 16 * ((4 * t + fg) ^ (r & 15)));
+        a[i] = *reinterpret_cast<const v4i*>(mine + G::A + 256 * r + 16 * ((4 * t + fg) ^ (r & 15)));
       }
 #pragma unroll
       for (int i = 0; i < MI; ++i)
@@ -214,26 +212,17 @@ __global__ __launch_bounds__((64 * RowsGeom<MI, NJ, AI, SLOTS>::WAVES)) void gem
     step(std::integral_constant<int, 3>{});
   };
   if (n0 < p.N) {
-    // SLOTS groups in flight; each slot is filled again once its fragments are
-    // in registers
-#pragma unroll
-    for (int s = 0; s < SLOTS; ++s)
-      if (wave + s * waves < groups) copy(wave + s * waves, s);
-    int slot = 0;
+    // the next group is on its way once this one's fragments are in registers
+    if (wave < groups) copy(wave);
     for (int g = wave; g < groups; g += waves) {
-      if (SLOTS > 1 && g + (SLOTS - 1) * waves < groups)
-        dev::wait_vmcnt<(SLOTS - 1) * G::OPS>();
-      else
-        dev::wait_vmcnt<0>();
+      dev::wait_vmcnt<0>();
       asm volatile("" ::: "memory");
-      multiply(g, slot);
-      const int next = g + SLOTS * waves;
-      if (next < groups) {
+      multiply(g);
+      if (g + waves < groups) {
         dev::waitcnt<63, 0>();
         asm volatile("" ::: "memory");
-        copy(next, slot);
+        copy(g + waves);
       }
-      slot = slot + 1 == SLOTS ? 0 : slot + 1;
     }
   }
   // each wave's sums; those of a unit of one or two column blocks are added up
@@ -758,9 +747,9 @@ int run_pipe(miaie_ctx* ctx, const Args& p) {
   return check_launch(ctx, e, "gemm_mx_pipe");
 }
 
-template <int MI, int NJ, int AI, int SLOTS, Out OUT>
+template <int MI, int NJ, int AI, Out OUT>
 int run_rows(miaie_ctx* ctx, const Args& p) {
-  using G = RowsGeom<MI, NJ, AI, SLOTS>;
+  using G = RowsGeom<MI, NJ, AI>;
   // (a packed result has zeros up to the end of its last 512 columns)
   const int cols = OUT == OUT_MX || OUT == OUT_MX_RELU ? 512 * s_groups(p.N) : p.N;
   const int tiles_n = (cols + 16 * NJ - 1) / (16 * NJ);
@@ -769,7 +758,7 @@ int run_rows(miaie_ctx* ctx, const Args& p) {
   // as many waves as share the groups evenly, up to 16 and to what fits the LDS
   const int each = (groups + G::WAVES - 1) / G::WAVES, waves = (groups + each - 1) / each;
   if (tiles * waves >= 1l << 26) return fail(ctx, MIAIE_EINVAL, "gemm_mxfp4: M=%d N=%d too large", p.M, p.N);
-  const hipError_t e = launch<gemm_mx_rows<MI, NJ, AI, SLOTS, OUT>>(ctx->device, dim3((unsigned)tiles), dim3(64 * waves),
+  const hipError_t e = launch<gemm_mx_rows<MI, NJ, AI, OUT>>(ctx->device, dim3((unsigned)tiles), dim3(64 * waves),
                                                                     (size_t)waves * G::REGION, ctx->stream, p, tiles_n, waves);
   return check_launch(ctx, e, "gemm_mx_rows");
 }
@@ -782,7 +771,9 @@ int run_rows(miaie_ctx* ctx, const Args& p) {
 // k-tile and of its end as measured on the tiles (a k-tile of 256 x 256 has 64
 // instructions of 16 cycles on each wave), the clock 2.3 GHz with a part of the
 // CUs at work and about 1.9 under the power limit.  128 x 128 tiles fit a CU
-// twice, and then take 960 cycles for both where one takes 540.
+// twice, and then take 960 cycles for both where one takes 540.  (A packed result
+// takes no single column block, whose two neighbours a lane needs, and no 64 x 32
+// tiles, which its 512 columns at least never make the quickest.)
 struct Choice {
   double us = 1e30;
   int kernel = -1;
@@ -794,9 +785,9 @@ void consider(Choice& best, int kernel, double us) {
 
 template <int MI, int NJ, int AI>
 double rows_us(long M, long cols, int groups, int cus) {
-  using G = RowsGeom<MI, NJ, AI, 1>;
+  using G = RowsGeom<MI, NJ, AI>;
   const long tiles = ((M + 16 * MI - 1) / (16 * MI)) * ((cols + 16 * NJ - 1) / (16 * NJ));
-  return 1.2 + 0.02 * G::OPS + (double)((tiles + cus - 1) / cus) * groups * G::SLOT / 42e3;
+  return 1.2 + 0.02 * G::OPS + (double)((tiles + cus - 1) / cus) * groups * G::GROUP / 42e3;
 }
 
 // Cycles of a workgroup on a tile: its start, a k-tile, its end (fp32, bf16, packed).
@@ -837,7 +828,7 @@ int run(miaie_ctx* ctx, const Args& p) {
     consider(c, 9, rows_us<2, 4, 8>(p.M, cols, groups, cus));
   }
   if (p.M > 32) {
-    consider(c, 10, rows_us<4, 2, 16>(p.M, cols, groups, cus));
+    if (!packed) consider(c, 10, rows_us<4, 2, 16>(p.M, cols, groups, cus));
     consider(c, 11, rows_us<4, 4, 16>(p.M, cols, groups, cus));
   }
   // (a row's offset within a tile in 32 bits, and HIP takes fewer than 2^32 threads)
@@ -860,18 +851,18 @@ int run(miaie_ctx* ctx, const Args& p) {
     }
   }
   switch (c.kernel) {
-    case 0: return run_rows<1, 1 + packed, 1, 1, OUT>(ctx, p);
-    case 1: return run_rows<1, 1 + packed, 2, 1, OUT>(ctx, p);
-    case 2: return run_rows<1, 2, 2, 1, OUT>(ctx, p);
-    case 3: return run_rows<1, 4, 2, 1, OUT>(ctx, p);
-    case 4: return run_rows<1, 1 + packed, 4, 1, OUT>(ctx, p);
-    case 5: return run_rows<1, 2, 4, 1, OUT>(ctx, p);
-    case 6: return run_rows<1, 4, 4, 1, OUT>(ctx, p);
-    case 7: return run_rows<2, 1 + packed, 8, 1, OUT>(ctx, p);
-    case 8: return run_rows<2, 2, 8, 1, OUT>(ctx, p);
-    case 9: return run_rows<2, 4, 8, 1, OUT>(ctx, p);
-    case 10: return run_rows<4, 2, 16, 1, OUT>(ctx, p);
-    case 11: return run_rows<4, 4, 16, 1, OUT>(ctx, p);
+    case 0: return run_rows<1, 1 + packed, 1, OUT>(ctx, p);
+    case 1: return run_rows<1, 1 + packed, 2, OUT>(ctx, p);
+    case 2: return run_rows<1, 2, 2, OUT>(ctx, p);
+    case 3: return run_rows<1, 4, 2, OUT>(ctx, p);
+    case 4: return run_rows<1, 1 + packed, 4, OUT>(ctx, p);
+    case 5: return run_rows<1, 2, 4, OUT>(ctx, p);
+    case 6: return run_rows<1, 4, 4, OUT>(ctx, p);
+    case 7: return run_rows<2, 1 + packed, 8, OUT>(ctx, p);
+    case 8: return run_rows<2, 2, 8, OUT>(ctx, p);
+    case 9: return run_rows<2, 4, 8, OUT>(ctx, p);
+    case 10: return run_rows<4, packed ? 4 : 2, 16, OUT>(ctx, p);
+    case 11: return run_rows<4, 4, 16, OUT>(ctx, p);
     case 12: return run_pipe<128, 128, OUT>(ctx, p);
     case 13: return run_pipe<256, 128, OUT>(ctx, p);
     case 14: return run_pipe<256, 256, OUT>(ctx, p);
