@@ -92,6 +92,17 @@ struct Raw8 {
       for (int i = 0; i < 8; ++i) v[i] = i < n ? MIAIE_LD(p + i) : (T)0.f;
     }
   }
+  // The values are in the registers from here on: a load is waited for here, not
+  // where the compiler first uses it.
+  __device__ __forceinline__ void arrive() {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(V) / 16; ++i) {
+      v4i w;
+      __builtin_memcpy(&w, reinterpret_cast<const char*>(&v) + 16 * i, 16);
+      asm volatile("" : "+v"(w));
+      __builtin_memcpy(reinterpret_cast<char*>(&v) + 16 * i, &w, 16);
+    }
+  }
   __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
 };
 

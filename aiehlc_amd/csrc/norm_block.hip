@@ -48,11 +48,13 @@ __device__ __forceinline__ float wave_sum(float v) {
 
 // Sum over a row of TPR threads, a wave or several (red: one float for each
 // wave of the workgroup, all of whose threads call it the same number of times).
+// Two sums that take turns each have a red: behind the barrier of the one all
+// have read the other's.  A sum by itself waits first until its last is read.
 template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* red, int tid) {
+__device__ __forceinline__ float row_sum(float v, float* red, int tid, bool alone) {
   v = wave_sum(v);
   if constexpr (TPR > 64) {
-    __syncthreads();  // the last sum has been read
+    if (alone) __syncthreads();
     if ((tid & 63) == 0) red[tid >> 6] = v;
     __syncthreads();
     const float* mine = red + tid / TPR * (TPR / 64);
@@ -86,7 +88,8 @@ struct Fwd {
 template <class ST, class BT, int TPR, int NC>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_fwd(Fwd p) {
   constexpr int THREADS = TPR < 256 ? 256 : TPR, RPW = THREADS / TPR;
-  __shared__ float red[THREADS / 64];
+  __shared__ float red[2][THREADS / 64];
+  const bool alone = !(p.b && p.y);
   const int tid = threadIdx.x, t = tid % TPR;
   Raw8<float> w_after[NC], w_before[NC];
   // (every thread makes the same number of turns: a row's sum is a barrier)
@@ -127,7 +130,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_fwd(Fwd p) {
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(b[c][e], b[c][e], ss);
-      const float ra = 1.f / sqrtf(row_sum<TPR>(ss, red, tid) / (float)p.cols + p.eps);
+      const float ra = 1.f / sqrtf(row_sum<TPR>(ss, red[0], tid, alone) / (float)p.cols + p.eps);
       if (p.rstd && t == 0 && active) MIAIE_ST(p.rstd + row, ra);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -147,7 +150,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_fwd(Fwd p) {
       for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int e = 0; e < 8; ++e) ss = fmaf(r[c][e], r[c][e], ss);  // (0 behind the last column)
-      const float rb = 1.f / sqrtf(row_sum<TPR>(ss, red, tid) / (float)p.cols + p.eps);
+      const float rb = 1.f / sqrtf(row_sum<TPR>(ss, red[1], tid, alone) / (float)p.cols + p.eps);
       if (p.rstd && t == 0 && active) MIAIE_ST(p.rstd + p.rows + row, rb);
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
@@ -182,20 +185,23 @@ struct Bwd {
 //
 // 1024 threads, TPR of them to a row: 1024 / TPR rows at a time, so that a CU has
 // 16 waves' loads in flight although the partial sums allow only about one
-// workgroup a CU (4095 x 4096 bf16: 52 us, 125 with four waves a CU; all seven
-// tensors once at the rate of a large copy are 39).
+// workgroup a CU (four waves a CU took more than twice the time).  4095 x 4096
+// bf16: 47 us, 4.3 TB/s; its six tensors once at the rate of a large copy are 39.
 constexpr int BWD_THREADS = 1024;
 
 template <class ST, class BT, int TPR, int NC>
 __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
   constexpr int RPW = BWD_THREADS / TPR;
-  __shared__ float red[BWD_THREADS / 64];
+  __shared__ float red[2][BWD_THREADS / 64];
+  const bool alone = !(p.dy && p.b && p.db);
   __shared__ float lanes[RPW > 1 ? RPW / 2 * TPR * 8 : 1];
   // Rows of two chunks a thread keep the norms' sums in LDS, each thread its own
   // columns', and fetch no row ahead, so that one row fits the registers (1024 x 16384
   // bf16: 55 us, 143 with the sums and the next row in scratch memory).
   constexpr bool WIDE = NC > 1;
   __shared__ float kept[WIDE ? 2 * NC * 8 * TPR : 1];
+  __shared__ __attribute__((aligned(16))) float weights[WIDE ? 4 : 2 * 8 * TPR];
+  __shared__ __attribute__((aligned(16))) float gates[WIDE ? 4 : 8 * BWD_THREADS];
   const int tid = threadIdx.x, t = tid % TPR, lane_row = tid / TPR;
   const size_t cols = p.cols;
   float dwb[NC][8] = {}, dwa[NC][8] = {}, dg[NC][8] = {};
@@ -205,11 +211,41 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     for (int i = 0; i < 2 * NC * 8; ++i) kept[i * TPR + t] = 0.f;
   }
 
-  // The next row's four tensors, on their way while a row is computed
-  // (112 registers for 98; 4095 x 4096 bf16: 55 us for 60).
+  // The norms' weights in LDS, before's and after's: [which][half of 8][thread][4]
+  // (zeros behind the last column).
+  if constexpr (!WIDE) {
+    for (int i = tid; i < 2 * TPR; i += BWD_THREADS) {
+      const int which = i / TPR, col = i % TPR, k = 8 * col;
+      const float* w = which ? p.w_after : p.w_before;
+      float v[8] = {};
+      if (w && k < p.cols) load8(w + k, p.cols - k, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) weights[((2 * which + e / 4) * TPR + col) * 4 + e % 4] = v[e];
+    }
+    __syncthreads();
+  }
+  auto weight8 = [&](int which, int c, float(&w)[8]) {
+    const int k = 8 * (t + TPR * c);
+    if constexpr (WIDE) {
+      load8((which ? p.w_after : p.w_before) + k, p.cols - k, w);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = weights[((2 * which + e / 4) * TPR + t) * 4 + e % 4];
+    }
+  };
+
+  // The next row's tensors, on their way while a row is computed, which itself
+  // loads nothing: loads return in order, and one of a row's own would wait for all
+  // of the next row's (4095 x 4096 bf16: 47 us, 52 with the gate, the weights and the
+  // reciprocal roots loaded where they are used).
   Raw8<ST> x_r[NC], x_dout[NC];
   Raw8<BT> x_dy[NC], x_b[NC];
+  float x_ra = 0.f, x_rb = 0.f;
   auto fetch = [&](int row, bool active) {
+    if (active) {
+      if (p.b) x_ra = MIAIE_LD(p.rstd + row);
+      if (p.dy) x_rb = MIAIE_LD(p.rstd + p.rows + row);
+    }
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int k = 8 * (t + TPR * c);
@@ -225,11 +261,35 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     }
   };
 
+  // A gate's values, each thread its own columns'.
+  auto open_gate = [&](int gate, bool active) {
+    if (WIDE || !p.gate) return;
+    float v[8] = {};
+    if (active && 8 * t < p.cols) load8(static_cast<const BT*>(p.gate) + gate * cols + 8 * t, p.cols - 8 * t, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gates[(e / 4 * BWD_THREADS + tid) * 4 + e % 4] = v[e];
+  };
+  auto gate8 = [&](int gate, int c, float(&g)[8]) {
+    const int k = 8 * (t + TPR * c);
+    if constexpr (WIDE) {
+      load8(static_cast<const BT*>(p.gate) + gate * cols + k, p.cols - k, g);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] = gates[(e / 4 * BWD_THREADS + tid) * 4 + e % 4];
+    }
+  };
+
+  auto arrive = [&] {
+#pragma unroll
+    for (int c = 0; c < NC; ++c) x_r[c].arrive(), x_dout[c].arrive(), x_dy[c].arrive(), x_b[c].arrive();
+    asm volatile("" : "+v"(x_ra), "+v"(x_rb));
+  };
+
   // (a lane without a row takes part in the sums' barriers)
-  auto row_grad = [&](int row, bool active, int next, bool next_active) {
+  auto row_grad = [&](int row, int gate, bool active, int next, bool next_active) {
     if constexpr (WIDE) fetch(row, active);
-    const float ra = p.b && active ? MIAIE_LD(p.rstd + row) : 0.f;
-    const float rb = p.dy && active ? MIAIE_LD(p.rstd + p.rows + row) : 0.f;
+    if constexpr (!WIDE) arrive();
+    const float ra = active ? x_ra : 0.f, rb = active ? x_rb : 0.f;
     float dr[NC][8], m[NC][8], tt[NC][8], v[NC][8], c1 = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -242,7 +302,7 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
         const int k = 8 * (t + TPR * c);
         if (k >= p.cols) continue;
         float w[8];
-        load8(p.w_before + k, p.cols - k, w);
+        weight8(0, c, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {  // (what is behind the last column is zero)
           m[c][e] *= rb;
@@ -252,7 +312,7 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
           c1 = fmaf(tt[c][e], m[c][e], c1);
         }
       }
-      c1 = row_sum<TPR>(c1, red, tid) / (float)p.cols;
+      c1 = row_sum<TPR>(c1, red[0], tid, alone) / (float)p.cols;
 #pragma unroll
       for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -270,17 +330,16 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     }
     if (!p.b) return;
     float c2 = 0.f;
-    const BT* gate = p.gate && active ? static_cast<const BT*>(p.gate) + (size_t)(row / p.gate_rows) * cols : nullptr;
     // (v becomes n, dr becomes u)
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int k = 8 * (t + TPR * c);
       if (k >= p.cols) continue;
       float w[8], g[8];
-      load8(p.w_after + k, p.cols - k, w);
+      weight8(1, c, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) g[e] = 1.f;
-      if (gate) load8(gate + k, p.cols - k, g);
+      if (p.gate) gate8(gate, c, g);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         v[c][e] *= ra;
@@ -293,7 +352,9 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
       }
     }
     if (!p.db) return;
-    c2 = row_sum<TPR>(c2, red, tid) / (float)p.cols;
+    c2 = row_sum<TPR>(c2, red[1], tid, alone) / (float)p.cols;
+    // (ahead of the last store, for which the next row need not wait)
+    if constexpr (!WIDE) arrive();
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int k = 8 * (t + TPR * c);
@@ -309,14 +370,22 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     const int first = gate * p.gate_rows, n = min(p.gate_rows, p.rows - first);
     const int r0 = first + (int)((long)n * part / p.parts), r1 = first + (int)((long)n * (part + 1) / p.parts);
     if constexpr (!WIDE) fetch(r0 + lane_row, r0 + lane_row < r1);
-    for (int row = r0 + lane_row, i = r0; i < r1; i += RPW, row += RPW) row_grad(row, row < r1, row + RPW, row + RPW < r1);
+    open_gate(gate, true);
+    for (int row = r0 + lane_row, i = r0; i < r1; i += RPW, row += RPW) row_grad(row, gate, row < r1, row + RPW, row + RPW < r1);
   } else {
-    // (every row lane makes the same number of turns)
-    for (int g0 = blockIdx.x * RPW; g0 < p.groups; g0 += p.workgroups * RPW) {
-      const int gate = g0 + lane_row, first = gate * p.gate_rows;
-      const int n = gate < p.groups ? min(p.gate_rows, p.rows - first) : 0;
-      if constexpr (!WIDE) fetch(first, n > 0);
-      for (int i = 0; i < p.gate_rows; ++i) row_grad(first + i, i < n, first + i + 1, i + 1 < n);
+    // (every row lane makes the same number of turns; a gate's last row fetches the
+    // first of the lane's next gate)
+    const int step = p.workgroups * RPW;
+    auto rows_of = [&](int gate) { return gate < p.groups ? min(p.gate_rows, p.rows - gate * p.gate_rows) : 0; };
+    int gate = blockIdx.x * RPW + lane_row, n = rows_of(gate);
+    if constexpr (!WIDE) fetch(gate * p.gate_rows, n > 0);
+    for (int g0 = blockIdx.x * RPW; g0 < p.groups; g0 += step) {
+      const int first = gate * p.gate_rows, then = gate < p.groups - step ? gate + step : p.groups, n_then = rows_of(then);
+      open_gate(gate, n > 0);
+      for (int i = 0; i < p.gate_rows; ++i) {
+        const bool last = i == p.gate_rows - 1;
+        row_grad(first + i, gate, i < n, last ? then * p.gate_rows : first + i + 1, last ? n_then > 0 : i + 1 < n);
+      }
       if (p.want & 4) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
@@ -326,6 +395,7 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
           for (int e = 0; e < 8; ++e) dg[c][e] = 0.f;
         }
       }
+      gate = then, n = n_then;
     }
   }
 
