@@ -145,14 +145,26 @@ __global__ __launch_bounds__(512) void quant_cols(const T* __restrict__ X, uint8
   __shared__ __attribute__((aligned(16))) uint8_t lq[64 * P], ls[64 * 16];
   __shared__ __attribute__((aligned(16))) uint8_t rq[ROWS ? 512 * PR : 16], rs[ROWS ? 2 * 512 : 16];
   const int tid = threadIdx.x, pair = tid & 31, rb = tid >> 5;  // column pair, block of rows
-  const int g = blockIdx.x / tiles_c, c0 = 64 * (blockIdx.x % tiles_c), c = c0 + 2 * pair;
+  int tile = blockIdx.x;
+  if constexpr (ROWS) {
+    // The eight tiles of 512 columns, which write parts of the same lines, on one XCD
+    // (workgroups go round the eight).
+    tile = (tile & ~63) + 8 * (tile & 7) + (tile >> 3 & 7);
+    if (tile >= s_groups(R) * tiles_c) return;
+  }
+  const int g = tile / tiles_c, c0 = 64 * (tile % tiles_c), c = c0 + 2 * pair;
   const int r0 = 512 * g + 32 * rb;
   Pair<T> x[32];
   const T* p = X + (size_t)r0 * ldx + c;
+  if (512 * g + 512 <= R && c0 + 64 <= C) {
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    x[i] = Pair<T>{};
-    if (r0 + i < R && c < C) x[i].load(p + (size_t)i * ldx, c + 1 < C);
+    for (int i = 0; i < 32; ++i) x[i].load(p + (size_t)i * ldx, true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      x[i] = Pair<T>{};
+      if (r0 + i < R && c < C) x[i].load(p + (size_t)i * ldx, c + 1 < C);
+    }
   }
   uint32_t s[2], q[2][4];
   Pair<T>::pack(x, s, q);
@@ -255,8 +267,8 @@ int launch_quant_mxfp4(miaie_ctx* ctx, const void* X, int dtype, int R, int C, i
     const T* x = static_cast<const T*>(X);
     if (Q && Qt) {  // (the rows' form has zeros up to the end of its last 512 columns)
       const int tiles_c = 8 * s_groups(C);
-      e = launch<quant_cols<T, true>>(ctx->device, dim3((unsigned)s_groups(R) * tiles_c), dim3(512), 0, ctx->stream, x, Qt,
-                                      St, Q, S, R, C, ldx, tiles_c);
+      e = launch<quant_cols<T, true>>(ctx->device, dim3(((unsigned)s_groups(R) * tiles_c + 63) / 64 * 64), dim3(512), 0,
+                                      ctx->stream, x, Qt, St, Q, S, R, C, ldx, tiles_c);
     } else if (Q) {
       const int units = R * s_groups(C), grid = wave_grid(units);
       e = launch<quant_rows<T>>(ctx->device, dim3(grid), dim3(256), 0, ctx->stream, x, Q, S, R, C, ldx, units, 4 * grid);
