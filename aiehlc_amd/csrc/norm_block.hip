@@ -194,14 +194,13 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
   constexpr int RPW = BWD_THREADS / TPR;
   __shared__ float red[2][BWD_THREADS / 64];
   const bool alone = !(p.dy && p.b && p.db);
-  __shared__ float lanes[RPW > 1 ? RPW / 2 * TPR * 8 : 1];
   // Rows of two chunks a thread keep the norms' sums in LDS, each thread its own
   // columns', and fetch no row ahead, so that one row fits the registers (1024 x 16384
   // bf16: 55 us, 143 with the sums and the next row in scratch memory).
   constexpr bool WIDE = NC > 1;
   __shared__ float kept[WIDE ? 2 * NC * 8 * TPR : 1];
   __shared__ __attribute__((aligned(16))) float weights[WIDE ? 4 : 2 * 8 * TPR];
-  __shared__ __attribute__((aligned(16))) float gates[WIDE ? 4 : 8 * BWD_THREADS];
+  __shared__ __attribute__((aligned(16))) float gates[WIDE ? 4 : 8 * BWD_THREADS];  // (and the partial sums at the end)
   const int tid = threadIdx.x, t = tid % TPR, lane_row = tid / TPR;
   const size_t cols = p.cols;
   float dwb[NC][8] = {}, dwa[NC][8] = {}, dg[NC][8] = {};
@@ -211,19 +210,6 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     for (int i = 0; i < 2 * NC * 8; ++i) kept[i * TPR + t] = 0.f;
   }
 
-  // The norms' weights in LDS, before's and after's: [which][half of 8][thread][4]
-  // (zeros behind the last column).
-  if constexpr (!WIDE) {
-    for (int i = tid; i < 2 * TPR; i += BWD_THREADS) {
-      const int which = i / TPR, col = i % TPR, k = 8 * col;
-      const float* w = which ? p.w_after : p.w_before;
-      float v[8] = {};
-      if (w && k < p.cols) load8(w + k, p.cols - k, v);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) weights[((2 * which + e / 4) * TPR + col) * 4 + e % 4] = v[e];
-    }
-    __syncthreads();
-  }
   auto weight8 = [&](int which, int c, float(&w)[8]) {
     const int k = 8 * (t + TPR * c);
     if constexpr (WIDE) {
@@ -262,12 +248,17 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
   };
 
   // A gate's values, each thread its own columns'.
-  auto open_gate = [&](int gate, bool active) {
+  auto load_gate = [&](int gate, bool active) {
+    Raw8<BT> g;
+    g.clear();
+    if (!WIDE && p.gate && active && 8 * t < p.cols)
+      g.load(static_cast<const BT*>(p.gate) + gate * cols + 8 * t, p.cols - 8 * t);
+    return g;
+  };
+  auto keep_gate = [&](const Raw8<BT>& g) {
     if (WIDE || !p.gate) return;
-    float v[8] = {};
-    if (active && 8 * t < p.cols) load8(static_cast<const BT*>(p.gate) + gate * cols + 8 * t, p.cols - 8 * t, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) gates[(e / 4 * BWD_THREADS + tid) * 4 + e % 4] = v[e];
+    for (int e = 0; e < 8; ++e) gates[(e / 4 * BWD_THREADS + tid) * 4 + e % 4] = g[e];
   };
   auto gate8 = [&](int gate, int c, float(&g)[8]) {
     const int k = 8 * (t + TPR * c);
@@ -279,6 +270,20 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     }
   };
 
+  // The norms' weights in LDS, before's and after's: [which][half of 8][thread][4]
+  // (zeros behind the last column).
+  auto keep_weights = [&] {
+    if (WIDE) return;
+    for (int i = tid; i < 2 * TPR; i += BWD_THREADS) {
+      const int which = i / TPR, col = i % TPR, k = 8 * col;
+      const float* w = which ? p.w_after : p.w_before;
+      float v[8] = {};
+      if (w && k < p.cols) load8(w + k, p.cols - k, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) weights[((2 * which + e / 4) * TPR + col) * 4 + e % 4] = v[e];
+    }
+    __syncthreads();
+  };
   auto arrive = [&] {
 #pragma unroll
     for (int c = 0; c < NC; ++c) x_r[c].arrive(), x_dout[c].arrive(), x_dy[c].arrive(), x_b[c].arrive();
@@ -370,7 +375,9 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     const int first = gate * p.gate_rows, n = min(p.gate_rows, p.rows - first);
     const int r0 = first + (int)((long)n * part / p.parts), r1 = first + (int)((long)n * (part + 1) / p.parts);
     if constexpr (!WIDE) fetch(r0 + lane_row, r0 + lane_row < r1);
-    open_gate(gate, true);
+    const Raw8<BT> g = load_gate(gate, true);
+    keep_weights();
+    keep_gate(g);
     for (int row = r0 + lane_row, i = r0; i < r1; i += RPW, row += RPW) row_grad(row, gate, row < r1, row + RPW, row + RPW < r1);
   } else {
     // (every row lane makes the same number of turns; a gate's last row fetches the
@@ -379,9 +386,10 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     auto rows_of = [&](int gate) { return gate < p.groups ? min(p.gate_rows, p.rows - gate * p.gate_rows) : 0; };
     int gate = blockIdx.x * RPW + lane_row, n = rows_of(gate);
     if constexpr (!WIDE) fetch(gate * p.gate_rows, n > 0);
+    keep_weights();
     for (int g0 = blockIdx.x * RPW; g0 < p.groups; g0 += step) {
       const int first = gate * p.gate_rows, then = gate < p.groups - step ? gate + step : p.groups, n_then = rows_of(then);
-      open_gate(gate, n > 0);
+      keep_gate(load_gate(gate, n > 0));
       for (int i = 0; i < p.gate_rows; ++i) {
         const bool last = i == p.gate_rows - 1;
         row_grad(first + i, gate, i < n, last ? then * p.gate_rows : first + i + 1, last ? n_then > 0 : i + 1 < n);
@@ -399,26 +407,26 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     }
   }
 
-  // the workgroup's partial sums: its row lanes' added in pairs through LDS
+  // the workgroup's partial sums: its row lanes' added through LDS, a column a thread
   auto put = [&](float(&v)[NC][8], int which) {
     float* dst = p.work + ((size_t)blockIdx.x * 3 + which) * cols;
+    if constexpr (RPW == 1) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int k = 8 * (t + TPR * c);
-#pragma unroll
-      for (int half = RPW / 2; half >= 1; half /= 2) {
-        __syncthreads();
-        if (lane_row >= half && lane_row < 2 * half) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) lanes[((lane_row - half) * 8 + e) * TPR + t] = v[c][e];
-        }
-        __syncthreads();
-        if (lane_row < half) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[c][e] += lanes[(lane_row * 8 + e) * TPR + t];
-        }
+      for (int c = 0; c < NC; ++c) {
+        const int k = 8 * (t + TPR * c);
+        if (k < p.cols) store8(dst + k, p.cols - k, v[c]);
       }
-      if (lane_row == 0 && k < p.cols) store8(dst + k, p.cols - k, v[c]);
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 8; ++e) gates[8 * tid + e] = v[0][e];
+      __syncthreads();
+      for (int k = tid; k < min(p.cols, 8 * TPR); k += BWD_THREADS) {
+        float s = gates[k];
+#pragma unroll
+        for (int r = 1; r < RPW; ++r) s += gates[8 * TPR * r + k];
+        MIAIE_ST(dst + k, s);
+      }
     }
   };
   if constexpr (WIDE) {
