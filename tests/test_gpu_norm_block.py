@@ -55,6 +55,9 @@ CASES = [  # rows, cols, stream, branch, gate_rows (None: no gate), parts
     (4, 16384, "f32", "bf16", 4, "ab"), (3, 16383, "bf16", "f32", 1, "ab"), (1000, 96, "bf16", "bf16", 3, "ab"),
     (2000, 33, "f32", "f32", 2000, "ab"), (50, 1000, "bf16", "bf16", None, "b"), (50, 1000, "f32", "bf16", None, "a"),
     (20, 4096, "bf16", "bf16", 7, "a"),
+    # several turns of a gradient's workgroups: over gates, and over the rows of one gate
+    (600, 4100, "f32", "bf16", 1, "ab"), (1100, 2100, "bf16", "bf16", 2, "ab"), (300, 8200, "bf16", "f32", 1, "ab"),
+    (9000, 33, "f32", "f32", None, "ab"), (1300, 2500, "f32", "f32", 1300, "ab"), (700, 8300, "bf16", "bf16", 350, "ab"),
 ]
 
 
