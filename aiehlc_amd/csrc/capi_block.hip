@@ -41,8 +41,8 @@ int check_packed(miaie_ctx* ctx, const char* fn, const char* name, const uint8_t
   return MIAIE_OK;
 }
 
-// One workgroup of 512 packs 64 rows of a packed transpose, their number rounded
-// up to 64 (quant_mxfp4.hip), and HIP takes fewer than 2^32 threads.
+// 512 threads pack 64 rows of 512 columns of a packed transpose, the workgroups'
+// number rounded up to 64 (quant_mxfp4.hip); HIP takes fewer than 2^32 threads.
 int check_transpose(miaie_ctx* ctx, const char* fn, int R, int C) {
   if ((long)mx::s_groups(R) * 8 * mx::s_groups(C) > (1l << 23) - 64)
     return fail(ctx, MIAIE_EINVAL, "%s: R=%d C=%d too large to pack along the columns", fn, R, C);

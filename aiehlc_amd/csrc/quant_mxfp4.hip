@@ -126,37 +126,43 @@ struct Pair<__bf16> {
   }
 };
 
-// A workgroup of 8 waves packs 512 rows of 64 columns along the rows' axis:
+// A workgroup of four waves packs 256 rows of 64 columns along the rows' axis:
 // each lane has two columns of a block of 32 rows, the other lanes of its half
 // wave the columns beside them, so every load of a half wave is one row's 128
 // (bf16) or 256 bytes, all 32 are in flight, and no lane needs another's values.
-// The packed rows (256 bytes of 64 columns) leave through LDS in whole lines.
+// The packed rows (128 bytes of 64 columns) leave through LDS in whole lines.  A
+// workgroup loads, packs and stores once; 256 rows rather than 512 or 128 leave
+// the fewest idle (4096 x 4096 bf16: 13.2 us, 14.0, 13.7; 1023 x 2049 fp32 along
+// both axes 6.9, 8.4, 7.6).
 //
 // ROWS: along the columns' axis too, from the same registers.  A block of 32
 // columns is the 16 lanes of a half wave's half, whose maxima come from four lane
 // permutations, for two rows at a time (only the exponents are needed); the codes
-// leave through LDS, 32 bytes of a row.  (2048 x 4096 bf16: 13.5 us, 14.4 in
-// two launches that each read x.)
+// leave through LDS, 32 bytes of a row.  (2048 x 4096 bf16: 10.7 us, 14 in two
+// launches that each read x.)
+constexpr int RB = 8;  // blocks of 32 rows
+__host__ __device__ inline int row_tiles(int R) { return s_groups(R) * (16 / RB); }
+
 template <class T, bool ROWS>
-__global__ __launch_bounds__(512) void quant_cols(const T* __restrict__ X, uint8_t* __restrict__ Qt,
-                                                  uint8_t* __restrict__ St, uint8_t* __restrict__ Q,
-                                                  uint8_t* __restrict__ S, int R, int C, int ldx, int tiles_c) {
-  constexpr int P = 272, PR = 36;  // bytes of a packed column, and of 64 columns of a packed row, in LDS
-  __shared__ __attribute__((aligned(16))) uint8_t lq[64 * P], ls[64 * 16];
-  __shared__ __attribute__((aligned(16))) uint8_t rq[ROWS ? 512 * PR : 16], rs[ROWS ? 2 * 512 : 16];
+__global__ __launch_bounds__(32 * RB) void quant_cols(const T* __restrict__ X, uint8_t* __restrict__ Qt,
+                                                      uint8_t* __restrict__ St, uint8_t* __restrict__ Q,
+                                                      uint8_t* __restrict__ S, int R, int C, int ldx, int tiles_c) {
+  constexpr int P = 16 * RB + 16, PR = 36;  // bytes of a packed column, and of 64 columns of a packed row, in LDS
+  __shared__ __attribute__((aligned(16))) uint8_t lq[64 * P], ls[64 * RB];
+  __shared__ __attribute__((aligned(16))) uint8_t rq[ROWS ? 32 * RB * PR : 16], rs[ROWS ? 2 * 32 * RB : 16];
   const int tid = threadIdx.x, pair = tid & 31, rb = tid >> 5;  // column pair, block of rows
   int tile = blockIdx.x;
   if constexpr (ROWS) {
     // The eight tiles of 512 columns, which write parts of the same lines, on one XCD
     // (workgroups go round the eight).
     tile = (tile & ~63) + 8 * (tile & 7) + (tile >> 3 & 7);
-    if (tile >= s_groups(R) * tiles_c) return;
+    if (tile >= row_tiles(R) * tiles_c) return;
   }
-  const int g = tile / tiles_c, c0 = 64 * (tile % tiles_c), c = c0 + 2 * pair;
-  const int r0 = 512 * g + 32 * rb;
+  const int first = 32 * RB * (tile / tiles_c), c0 = 64 * (tile % tiles_c), c = c0 + 2 * pair;
+  const int g = first / 512, b0 = first % 512 / 32, r0 = first + 32 * rb;
   Pair<T> x[32];
   const T* p = X + (size_t)r0 * ldx + c;
-  if (512 * g + 512 <= R && c0 + 64 <= C) {
+  if (first + 32 * RB <= R && c0 + 64 <= C) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) x[i].load(p + (size_t)i * ldx, true);
   } else {
@@ -171,7 +177,7 @@ __global__ __launch_bounds__(512) void quant_cols(const T* __restrict__ X, uint8
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     *reinterpret_cast<uint4*>(lq + (2 * pair + k) * P + 16 * rb) = make_uint4(q[k][0], q[k][1], q[k][2], q[k][3]);
-    ls[(2 * pair + k) * 16 + s_byte(rb)] = (uint8_t)s[k];
+    ls[(2 * pair + k) * RB + 2 * (rb & 3) + (rb >> 2)] = (uint8_t)s[k];  // (as in s_byte)
   }
   if constexpr (ROWS) {
     uint32_t scales[8];  // of the block's 32 rows, a byte each
@@ -202,7 +208,7 @@ __global__ __launch_bounds__(512) void quant_cols(const T* __restrict__ X, uint8
       scales[d] = __builtin_amdgcn_perm(pairs[1], pairs[0], 0x06040200u);
     }
     if ((pair & 15) == 0) {
-      uint4* to = reinterpret_cast<uint4*>(rs + 512 * (pair >> 4) + 32 * rb);
+      uint4* to = reinterpret_cast<uint4*>(rs + 32 * RB * (pair >> 4) + 32 * rb);
       to[0] = make_uint4(scales[0], scales[1], scales[2], scales[3]);
       to[1] = make_uint4(scales[4], scales[5], scales[6], scales[7]);
     }
@@ -211,15 +217,17 @@ __global__ __launch_bounds__(512) void quant_cols(const T* __restrict__ X, uint8
   const size_t pitch = q_pitch(R);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const int col = 32 * k + (tid >> 4), ch = tid & 15;
-    const size_t off = 256 * (size_t)g + 16 * ch;
+    const int col = 32 * k + tid / RB, ch = tid % RB;
+    const size_t off = first / 2 + 16 * ch;
     if (c0 + col < C && off < pitch)
       MIAIE_ST(reinterpret_cast<uint4*>(Qt + (size_t)(c0 + col) * pitch + off), *reinterpret_cast<const uint4*>(lq + col * P + 16 * ch));
   }
-  if (tid < 64 && c0 + tid < C)
-    MIAIE_ST(reinterpret_cast<uint4*>(St + ((size_t)g * C + c0 + tid) * 16), *reinterpret_cast<const uint4*>(ls + 16 * tid));
+  const int col = c0 + tid / 4;  // two blocks' scales of a column a thread
+  if (col < C)
+    MIAIE_ST(reinterpret_cast<uint16_t*>(St + ((size_t)g * C + col) * 16 + 4 * (tid & 3) + b0 / 4),
+             *reinterpret_cast<const uint16_t*>(ls + 2 * tid));
   if constexpr (ROWS) {
-    const int row = 512 * g + tid;
+    const int row = first + tid;
     if (row < R) {
       const size_t row_pitch = q_pitch(C);
       const uint32_t* from = reinterpret_cast<const uint32_t*>(rq + tid * PR);
@@ -229,7 +237,7 @@ __global__ __launch_bounds__(512) void quant_cols(const T* __restrict__ X, uint8
           MIAIE_ST(reinterpret_cast<uint4*>(Q + row * row_pitch + c0 / 2 + 16 * k),
                    make_uint4(from[4 * k], from[4 * k + 1], from[4 * k + 2], from[4 * k + 3]));
         const int block = c0 / 32 + k;
-        MIAIE_ST(S + ((size_t)(block >> 4) * R + row) * 16 + s_byte(block), rs[512 * k + tid]);
+        MIAIE_ST(S + ((size_t)(block >> 4) * R + row) * 16 + s_byte(block), rs[32 * RB * k + tid]);
       }
     }
   }
@@ -267,15 +275,15 @@ int launch_quant_mxfp4(miaie_ctx* ctx, const void* X, int dtype, int R, int C, i
     const T* x = static_cast<const T*>(X);
     if (Q && Qt) {  // (the rows' form has zeros up to the end of its last 512 columns)
       const int tiles_c = 8 * s_groups(C);
-      e = launch<quant_cols<T, true>>(ctx->device, dim3(((unsigned)s_groups(R) * tiles_c + 63) / 64 * 64), dim3(512), 0,
+      e = launch<quant_cols<T, true>>(ctx->device, dim3(((unsigned)row_tiles(R) * tiles_c + 63) / 64 * 64), dim3(32 * RB), 0,
                                       ctx->stream, x, Qt, St, Q, S, R, C, ldx, tiles_c);
     } else if (Q) {
       const int units = R * s_groups(C), grid = wave_grid(units);
       e = launch<quant_rows<T>>(ctx->device, dim3(grid), dim3(256), 0, ctx->stream, x, Q, S, R, C, ldx, units, 4 * grid);
     } else {
       const int tiles_c = (C + 63) / 64;
-      e = launch<quant_cols<T, false>>(ctx->device, dim3((unsigned)s_groups(R) * tiles_c), dim3(512), 0, ctx->stream, x, Qt,
-                                       St, nullptr, nullptr, R, C, ldx, tiles_c);
+      e = launch<quant_cols<T, false>>(ctx->device, dim3((unsigned)row_tiles(R) * tiles_c), dim3(32 * RB), 0, ctx->stream, x,
+                                       Qt, St, nullptr, nullptr, R, C, ldx, tiles_c);
     }
   };
   if (dtype == MIAIE_BF16)
