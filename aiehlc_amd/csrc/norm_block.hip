@@ -84,7 +84,8 @@ struct Fwd {
 // threads takes one row (TPR >= 256) or several.  ST: x and out, BT: b, gate and
 // y.  Everything a row needs is loaded before its first sum: a single row waits
 // for memory once (1 x 4096 bf16 3.6 us, 5.4 with the weights and the gate loaded
-// where they are used).
+// where they are used).  Bound by memory: 8192 x 4096, fp32 stream, bf16 branch in
+// 76 us, 5.3 TB/s.
 template <class ST, class BT, int TPR, int NC>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void norm_fwd(Fwd p) {
   constexpr int THREADS = TPR < 256 ? 256 : TPR, RPW = THREADS / TPR;
@@ -442,7 +443,8 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
 
 // Sums of partial rows: workgroup (x, y) adds 64 columns of output row y (0:
 // dw_before, 1: dw_after, 2 + g: dgate row g), its 16 waves a sixteenth of the
-// partial rows each, eight loads in flight.
+// partial rows each, eight loads in flight (256 partial rows of 3 x 4096: 4.7 us,
+// half of them the launch).
 __global__ __launch_bounds__(1024) void norm_join(const float* __restrict__ work, float* __restrict__ dw_before,
                                                   float* __restrict__ dw_after, float* __restrict__ dgate, int cols,
                                                   int workgroups, int parts) {
