@@ -291,7 +291,8 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
     asm volatile("" : "+v"(x_ra), "+v"(x_rb));
   };
 
-  // (a lane without a row takes part in the sums' barriers)
+  // (a lane without a row takes part in the sums' barriers, and adds nothing to the
+  // sums over rows: its 0 times an infinite weight would make them NaN)
   auto row_grad = [&](int row, int gate, bool active, int next, bool next_active) {
     if constexpr (WIDE) fetch(row, active);
     if constexpr (!WIDE) arrive();
@@ -306,7 +307,7 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const int k = 8 * (t + TPR * c);
-        if (k >= p.cols) continue;
+        if (k >= p.cols || !active) continue;
         float w[8];
         weight8(0, c, w);
 #pragma unroll
@@ -340,7 +341,7 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int k = 8 * (t + TPR * c);
-      if (k >= p.cols) continue;
+      if (k >= p.cols || !active) continue;
       float w[8], g[8];
       weight8(1, c, w);
 #pragma unroll
