@@ -226,6 +226,20 @@ inline void mlp_i8(const Buffer<int8_t>& X, const Buffer<int8_t>& W1, const Buff
   ctx.check(miaie_mlp_i8(ctx.get(), X.data(), W1.data(), W2.data(), H.data(), Y.data(), M, K, F, Nout, s1, s2));
 }
 
+// The 4-bit operators and the norms infer sizes, and refuse (miaie::Error,
+// MIAIE_EINVAL, before anything is queued) operands that do not fit together and
+// buffers shorter than those sizes.
+namespace detail {
+inline void require(bool ok, const char* fn, const char* what) {
+  if (!ok) throw Error(MIAIE_EINVAL, std::string(fn) + ": " + what);
+}
+// rows x cols elements fit the buffer (sizes below 1 are left to the entry point)
+template <typename T>
+bool holds(const Buffer<T>& b, int rows, int cols) {
+  return rows < 1 || cols < 1 || b.size() / (size_t)cols >= (size_t)rows;
+}
+}  // namespace detail
+
 // A packed MXFP4 matrix (miaie.h) of rows x cols.
 struct MxMatrix {
   MxMatrix(Context& ctx, int rows, int cols)
@@ -241,6 +255,7 @@ inline constexpr int dtype_of(const uint16_t*) { return MIAIE_BF16; }
 // Q = X packed along its rows (X dense, Q.rows x Q.cols).
 template <typename T>
 void quant_mxfp4(const Buffer<T>& X, MxMatrix& Q, Context& ctx = Context::current()) {
+  detail::require(detail::holds(X, Q.rows, Q.cols), "quant_mxfp4", "X is smaller than Q");
   ctx.check(miaie_quant_mxfp4(ctx.get(), X.data(), dtype_of(X.data()), Q.rows, Q.cols, Q.cols, Q.q.data(), Q.s.data(),
                               nullptr, nullptr));
 }
@@ -248,6 +263,7 @@ void quant_mxfp4(const Buffer<T>& X, MxMatrix& Q, Context& ctx = Context::curren
 // Qt = the transpose of X packed along its rows (X dense, Qt.cols x Qt.rows).
 template <typename T>
 void quant_mxfp4_t(const Buffer<T>& X, MxMatrix& Qt, Context& ctx = Context::current()) {
+  detail::require(detail::holds(X, Qt.cols, Qt.rows), "quant_mxfp4_t", "X is smaller than Qt");
   ctx.check(miaie_quant_mxfp4(ctx.get(), X.data(), dtype_of(X.data()), Qt.cols, Qt.rows, Qt.rows, nullptr, nullptr,
                               Qt.q.data(), Qt.s.data()));
 }
@@ -255,12 +271,15 @@ void quant_mxfp4_t(const Buffer<T>& X, MxMatrix& Qt, Context& ctx = Context::cur
 // Y = the values of Q.
 template <typename T>
 void dequant_mxfp4(const MxMatrix& Q, Buffer<T>& Y, Context& ctx = Context::current()) {
+  detail::require(detail::holds(Y, Q.rows, Q.cols), "dequant_mxfp4", "Y is smaller than Q");
   ctx.check(miaie_dequant_mxfp4(ctx.get(), Q.q.data(), Q.s.data(), Y.data(), dtype_of(Y.data()), Q.rows, Q.cols, Q.cols));
 }
 
 // C = A . B^T (A M x K, B N x K).
 template <typename T>
 void gemm_mxfp4(const MxMatrix& A, const MxMatrix& B, Buffer<T>& C, Context& ctx = Context::current()) {
+  detail::require(A.cols == B.cols, "gemm_mxfp4", "A and B have rows of different lengths");
+  detail::require(detail::holds(C, A.rows, B.rows), "gemm_mxfp4", "C is smaller than A . B^T");
   ctx.check(miaie_gemm_mxfp4(ctx.get(), A.q.data(), A.s.data(), B.q.data(), B.s.data(), C.data(), dtype_of(C.data()),
                              A.rows, B.rows, A.cols, B.rows));
 }
@@ -268,6 +287,8 @@ void gemm_mxfp4(const MxMatrix& A, const MxMatrix& B, Buffer<T>& C, Context& ctx
 // Y = A . B^T packed again, after a ReLU if relu.
 inline void gemm_mxfp4_rq(const MxMatrix& A, const MxMatrix& B, MxMatrix& Y, bool relu = false,
                           Context& ctx = Context::current()) {
+  detail::require(A.cols == B.cols, "gemm_mxfp4_rq", "A and B have rows of different lengths");
+  detail::require(Y.rows == A.rows && Y.cols == B.rows, "gemm_mxfp4_rq", "Y does not have the shape of A . B^T");
   ctx.check(miaie_gemm_mxfp4_rq(ctx.get(), A.q.data(), A.s.data(), B.q.data(), B.s.data(), Y.q.data(), Y.s.data(),
                                 A.rows, B.rows, A.cols, relu ? 1 : 0));
 }
@@ -276,6 +297,10 @@ inline void gemm_mxfp4_rq(const MxMatrix& A, const MxMatrix& B, MxMatrix& Y, boo
 template <typename T>
 void mlp_mxfp4(const MxMatrix& X, const MxMatrix& W1, const MxMatrix& W2, MxMatrix& H, Buffer<T>& Y,
                Context& ctx = Context::current()) {
+  detail::require(X.cols == W1.cols, "mlp_mxfp4", "X and W1 have rows of different lengths");
+  detail::require(W1.rows == W2.cols, "mlp_mxfp4", "W2's rows do not have W1's number of rows");
+  detail::require(H.rows == X.rows && H.cols == W1.rows, "mlp_mxfp4", "H does not have the shape of X . W1^T");
+  detail::require(detail::holds(Y, X.rows, W2.rows), "mlp_mxfp4", "Y is smaller than H . W2^T");
   ctx.check(miaie_mlp_mxfp4(ctx.get(), X.q.data(), X.s.data(), W1.q.data(), W1.s.data(), W2.q.data(), W2.s.data(),
                             H.q.data(), H.s.data(), Y.data(), dtype_of(Y.data()), X.rows, X.cols, W1.rows, W2.rows,
                             W2.rows));
@@ -286,12 +311,18 @@ struct NormShape {
   int rows, cols;
   float alpha = 1.f, eps = 1e-5f;
   int gate_rows = 0;  // rows that share a gate row; 0: all of them
+  int rows_of_a_gate() const { return gate_rows ? gate_rows : rows; }
+  int gates() const { return gate_rows > 0 ? (int)(((long long)rows + gate_rows - 1) / gate_rows) : 1; }
 };
 
 // y = w_before * x / rms(x).
 template <typename S, typename B>
 void norm_before(const Buffer<S>& x, const Buffer<float>& w_before, Buffer<B>& y, const NormShape& n,
                  Buffer<float>* rstd = nullptr, Context& ctx = Context::current()) {
+  detail::require(detail::holds(x, n.rows, n.cols) && detail::holds(y, n.rows, n.cols), "norm_before",
+                  "x or y is smaller than rows x cols");
+  detail::require(detail::holds(w_before, 1, n.cols), "norm_before", "w_before is shorter than a row");
+  detail::require(!rstd || detail::holds(*rstd, 2, n.rows), "norm_before", "rstd is smaller than 2 x rows");
   ctx.check(miaie_norm_block(ctx.get(), x.data(), nullptr, nullptr, nullptr, w_before.data(), nullptr, y.data(),
                              rstd ? rstd->data() : nullptr, n.rows, n.cols, n.cols, n.cols, n.rows,
                              dtype_of(x.data()), dtype_of(y.data()), n.alpha, n.eps));
@@ -304,10 +335,17 @@ template <typename S, typename B>
 void norm_block(const Buffer<S>& x, const Buffer<B>& b, const Buffer<B>* gate, const Buffer<float>& w_after,
                 const Buffer<float>* w_before, Buffer<S>& out, Buffer<B>* y, const NormShape& n,
                 Buffer<float>* rstd = nullptr, Context& ctx = Context::current()) {
+  detail::require(detail::holds(x, n.rows, n.cols) && detail::holds(b, n.rows, n.cols) &&
+                      detail::holds(out, n.rows, n.cols) && (!y || detail::holds(*y, n.rows, n.cols)),
+                  "norm_block", "x, b, out or y is smaller than rows x cols");
+  detail::require(!gate || detail::holds(*gate, n.gates(), n.cols), "norm_block", "gate is smaller than its rows x cols");
+  detail::require(detail::holds(w_after, 1, n.cols) && (!w_before || detail::holds(*w_before, 1, n.cols)), "norm_block",
+                  "w_after or w_before is shorter than a row");
+  detail::require(!rstd || detail::holds(*rstd, 2, n.rows), "norm_block", "rstd is smaller than 2 x rows");
   ctx.check(miaie_norm_block(ctx.get(), x.data(), b.data(), gate ? gate->data() : nullptr, w_after.data(),
                              w_before ? w_before->data() : nullptr, out.data(), y ? y->data() : nullptr,
-                             rstd ? rstd->data() : nullptr, n.rows, n.cols, n.cols, n.cols,
-                             n.gate_rows ? n.gate_rows : n.rows, dtype_of(x.data()), dtype_of(b.data()), n.alpha, n.eps));
+                             rstd ? rstd->data() : nullptr, n.rows, n.cols, n.cols, n.cols, n.rows_of_a_gate(),
+                             dtype_of(x.data()), dtype_of(b.data()), n.alpha, n.eps));
 }
 
 }  // namespace miaie
