@@ -268,6 +268,15 @@ void quant_mxfp4_t(const Buffer<T>& X, MxMatrix& Qt, Context& ctx = Context::cur
                               Qt.q.data(), Qt.s.data()));
 }
 
+// Both from one read of X.
+template <typename T>
+void quant_mxfp4_both(const Buffer<T>& X, MxMatrix& Q, MxMatrix& Qt, Context& ctx = Context::current()) {
+  detail::require(detail::holds(X, Q.rows, Q.cols), "quant_mxfp4_both", "X is smaller than Q");
+  detail::require(Qt.rows == Q.cols && Qt.cols == Q.rows, "quant_mxfp4_both", "Qt does not have the shape of Q's transpose");
+  ctx.check(miaie_quant_mxfp4(ctx.get(), X.data(), dtype_of(X.data()), Q.rows, Q.cols, Q.cols, Q.q.data(), Q.s.data(),
+                              Qt.q.data(), Qt.s.data()));
+}
+
 // Y = the values of Q.
 template <typename T>
 void dequant_mxfp4(const MxMatrix& Q, Buffer<T>& Y, Context& ctx = Context::current()) {
@@ -346,6 +355,64 @@ void norm_block(const Buffer<S>& x, const Buffer<B>& b, const Buffer<B>* gate, c
                              w_before ? w_before->data() : nullptr, out.data(), y ? y->data() : nullptr,
                              rstd ? rstd->data() : nullptr, n.rows, n.cols, n.cols, n.cols, n.rows_of_a_gate(),
                              dtype_of(x.data()), dtype_of(b.data()), n.alpha, n.eps));
+}
+
+// The gradients that norm_block_grad is to compute; those left NULL are not.
+// dx may be the buffer of dout, db that of dy or b.
+template <typename S, typename B>
+struct NormGrads {
+  Buffer<S>* dx = nullptr;
+  Buffer<B>* db = nullptr;
+  Buffer<float>* dgate = nullptr;     // the shape of gate
+  Buffer<float>* dw_after = nullptr;  // cols
+  Buffer<float>* dw_before = nullptr;
+};
+
+// The gradient of norm_block: r the stream that the second norm read (out of
+// norm_block), rstd as norm_block kept it; dout (nullable: 0) the gradient of the
+// stream from elsewhere, dy (nullable: no second norm; then w_before is not read) of
+// y.  work (nullable unless dgate, dw_after or dw_before is wanted): device scratch
+// of MIAIE_NORM_WORK_BYTES(cols).
+template <typename S, typename B>
+void norm_block_grad(const Buffer<S>& r, const Buffer<B>& b, const Buffer<B>* gate, const Buffer<float>& w_after,
+                     const Buffer<float>* w_before, const Buffer<float>& rstd, const Buffer<S>* dout,
+                     const Buffer<B>* dy, const NormGrads<S, B>& to, Buffer<float>* work, const NormShape& n,
+                     Context& ctx = Context::current()) {
+  auto fits = [](const auto* v, int rows, int cols) { return !v || detail::holds(*v, rows, cols); };
+  detail::require(detail::holds(r, n.rows, n.cols) && detail::holds(b, n.rows, n.cols) && fits(dout, n.rows, n.cols) &&
+                      fits(dy, n.rows, n.cols) && fits(to.dx, n.rows, n.cols) && fits(to.db, n.rows, n.cols),
+                  "norm_block_grad", "r, b, dout, dy, dx or db is smaller than rows x cols");
+  detail::require(fits(gate, n.gates(), n.cols) && fits(to.dgate, n.gates(), n.cols), "norm_block_grad",
+                  "gate or dgate is smaller than its rows x cols");
+  detail::require(detail::holds(w_after, 1, n.cols) && fits(w_before, 1, n.cols) && fits(to.dw_after, 1, n.cols) &&
+                      fits(to.dw_before, 1, n.cols),
+                  "norm_block_grad", "w_after, w_before, dw_after or dw_before is shorter than a row");
+  detail::require(detail::holds(rstd, 2, n.rows), "norm_block_grad", "rstd is smaller than 2 x rows");
+  auto data = [](auto* v) { return v ? v->data() : nullptr; };
+  ctx.check(miaie_norm_block_grad(ctx.get(), r.data(), b.data(), data(gate), w_after.data(), dy ? data(w_before) : nullptr,
+                                  rstd.data(), data(dout), data(dy), data(to.dx), data(to.db), data(to.dgate),
+                                  data(to.dw_after), data(to.dw_before), data(work), work ? work->bytes() : 0, n.rows,
+                                  n.cols, n.cols, n.cols, n.rows_of_a_gate(), dtype_of(r.data()), dtype_of(b.data()),
+                                  n.alpha));
+}
+
+// The gradient of norm_before, added to dout (nullable: 0).
+template <typename S, typename B>
+void norm_before_grad(const Buffer<S>& x, const Buffer<float>& w_before, const Buffer<float>& rstd,
+                      const Buffer<S>* dout, const Buffer<B>& dy, Buffer<S>* dx, Buffer<float>* dw_before,
+                      Buffer<float>* work, const NormShape& n, Context& ctx = Context::current()) {
+  auto fits = [](const auto* v, int rows, int cols) { return !v || detail::holds(*v, rows, cols); };
+  detail::require(detail::holds(x, n.rows, n.cols) && fits(dout, n.rows, n.cols) && detail::holds(dy, n.rows, n.cols) &&
+                      fits(dx, n.rows, n.cols),
+                  "norm_before_grad", "x, dout, dy or dx is smaller than rows x cols");
+  detail::require(detail::holds(w_before, 1, n.cols) && fits(dw_before, 1, n.cols), "norm_before_grad",
+                  "w_before or dw_before is shorter than a row");
+  detail::require(detail::holds(rstd, 2, n.rows), "norm_before_grad", "rstd is smaller than 2 x rows");
+  auto data = [](auto* v) { return v ? v->data() : nullptr; };
+  ctx.check(miaie_norm_block_grad(ctx.get(), x.data(), nullptr, nullptr, nullptr, w_before.data(), rstd.data(), data(dout),
+                                  dy.data(), data(dx), nullptr, nullptr, nullptr, data(dw_before), data(work),
+                                  work ? work->bytes() : 0, n.rows, n.cols, n.cols, n.cols, n.rows, dtype_of(x.data()),
+                                  dtype_of(dy.data()), 1.f));
 }
 
 }  // namespace miaie

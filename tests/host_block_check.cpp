@@ -11,6 +11,7 @@
 
 static std::string last;  // the last compute call: name and sizes
 static int calls = 0;
+static std::vector<const void*> pointers;  // of the last gradient
 
 template <class... I>
 static int called(const char* name, I... sizes) {
@@ -24,7 +25,10 @@ extern "C" {
 int miaie_init(miaie_ctx** ctx, int) { return *ctx = reinterpret_cast<miaie_ctx*>(8), MIAIE_OK; }
 int miaie_finish(miaie_ctx*) { return MIAIE_OK; }
 const char* miaie_last_error_string(const miaie_ctx*) { return "recorded"; }
-int miaie_alloc(miaie_ctx*, size_t, void** p) { return *p = reinterpret_cast<void*>(4096), MIAIE_OK; }  // (never read)
+int miaie_alloc(miaie_ctx*, size_t, void** p) {  // addresses of their own, never read
+  static uintptr_t next = 0;
+  return *p = reinterpret_cast<void*>(next += 4096), MIAIE_OK;
+}
 int miaie_free(miaie_ctx*, void*) { return MIAIE_OK; }
 size_t miaie_mxfp4_q_bytes(int R, int K) { return (size_t)R * ((K + 255) / 256 * 128); }
 size_t miaie_mxfp4_s_bytes(int R, int K) { return (size_t)R * ((K + 511) / 512) * 16; }
@@ -50,6 +54,13 @@ int miaie_norm_block(miaie_ctx*, const void*, const void* b, const void* gate, c
                      float*, int rows, int cols, int ldx, int ldb, int gate_rows, int, int, float, float) {
   return called("norm", rows, cols, ldx, ldb, gate_rows, b != nullptr, gate != nullptr, y != nullptr);
 }
+int miaie_norm_block_grad(miaie_ctx*, const void* r, const void* b, const void* gate, const float* w_after,
+                          const float* w_before, const float* rstd, const void* dout, const void* dy, void* dx, void* db,
+                          float* dgate, float* dw_after, float* dw_before, void* work, size_t work_bytes, int rows, int cols,
+                          int ldx, int ldb, int gate_rows, int stream_dtype, int branch_dtype, float alpha) {
+  pointers = {r, b, gate, w_after, w_before, rstd, dout, dy, dx, db, dgate, dw_after, dw_before, work};
+  return called("grad", work_bytes, rows, cols, ldx, ldb, gate_rows, stream_dtype, branch_dtype, (int)(8 * alpha));
+}
 }
 
 static int failures = 0;
@@ -72,6 +83,10 @@ static void refused(int line, const char* text, F&& f) {
   report(calls == before, line, "an entry point was called");
 }
 
+static void same(int line, const std::vector<const void*>& want) {
+  report(pointers == want, line, "the gradient's buffers are not where they belong");
+}
+
 template <class F>
 static void reaches(int line, const char* want, F&& f) {
   try {
@@ -84,6 +99,7 @@ static void reaches(int line, const char* want, F&& f) {
 
 #define REFUSED(text, call) refused(__LINE__, text, [&] { call; })
 #define REACHES(want, call) reaches(__LINE__, want, [&] { call; })
+#define BUFFERS(...) same(__LINE__, {__VA_ARGS__})
 
 int main() {
   using namespace miaie;
@@ -97,6 +113,10 @@ int main() {
   REFUSED("X is smaller", quant_mxfp4(x1, A));
   REACHES("quant 300 5 5 0 1", quant_mxfp4_t(x, A));
   REFUSED("X is smaller", quant_mxfp4_t(h1, A));
+  MxMatrix At(ctx, 300, 5);
+  REACHES("quant 5 300 300 1 1", quant_mxfp4_both(x, A, At));
+  REFUSED("X is smaller", quant_mxfp4_both(h1, A, At));
+  REFUSED("transpose", quant_mxfp4_both(x, A, longer));
   REACHES("dequant 5 300 300", dequant_mxfp4(A, h));
   REFUSED("Y is smaller", dequant_mxfp4(A, h1));
 
@@ -131,6 +151,32 @@ int main() {
   REFUSED("w_after", norm_block(x, h, &gate, w1, &w, out, &next, two));
   REFUSED("w_after", norm_block(x, h, &gate, w, &w1, out, &next, two));
   REFUSED("rstd", norm_block(x, h, &gate, w, &w, out, &next, two, &rstd1));
+
+  // the gradient: fp32 stream, bf16 branch, gates of two rows (three of them)
+  const NormShape g{5, 300, 0.5f, 1e-5f, 2};
+  Buffer<float> dout(ctx, 1500), dx(ctx, 1500), dgate(ctx, 900), dgate1(ctx, 899), dwa(ctx, 300), dwb(ctx, 300), work(ctx, 1024 * 300);
+  Buffer<uint16_t> dy(ctx, 1500), db(ctx, 1500);
+  const NormGrads<float, uint16_t> all{&dx, &db, &dgate, &dwa, &dwb};
+  REACHES("grad 1228800 5 300 300 300 2 0 1 4",
+          norm_block_grad(x, h, &gate, w, &w, rstd, &dout, &dy, all, &work, g));
+  BUFFERS(x.data(), h.data(), gate.data(), w.data(), w.data(), rstd.data(), dout.data(), dy.data(), dx.data(), db.data(),
+          dgate.data(), dwa.data(), dwb.data(), work.data());
+  const Buffer<uint16_t>* none = nullptr;
+  REACHES("grad 0 5 300 300 300 5 0 1 8",
+          norm_block_grad(x, h, none, w, &w, rstd, &dout, none, NormGrads<float, uint16_t>{&dx, &db}, (Buffer<float>*)nullptr, n));
+  BUFFERS(x.data(), h.data(), nullptr, w.data(), nullptr, rstd.data(), dout.data(), nullptr, dx.data(), db.data(), nullptr,
+          nullptr, nullptr, nullptr);
+  REACHES("grad 1228800 5 300 300 300 5 0 1 8", norm_before_grad(x, w, rstd, &dout, dy, &dx, &dwb, &work, n));
+  BUFFERS(x.data(), nullptr, nullptr, nullptr, w.data(), rstd.data(), dout.data(), dy.data(), dx.data(), nullptr, nullptr,
+          nullptr, dwb.data(), work.data());
+  REFUSED("smaller than rows", norm_block_grad(x, h1, &gate, w, &w, rstd, &dout, &dy, all, &work, g));
+  REFUSED("smaller than rows", norm_block_grad(x, h, &gate, w, &w, rstd, &x1, &dy, all, &work, g));
+  REFUSED("dgate", norm_block_grad(x, h, &gate, w, &w, rstd, &dout, &dy, NormGrads<float, uint16_t>{&dx, &db, &dgate1}, &work, g));
+  REFUSED("dw_after", norm_block_grad(x, h, &gate, w1, &w, rstd, &dout, &dy, all, &work, g));
+  REFUSED("rstd", norm_block_grad(x, h, &gate, w, &w, rstd1, &dout, &dy, all, &work, g));
+  REFUSED("smaller than rows", norm_before_grad(x, w, rstd, &dout, h1, &dx, &dwb, &work, n));
+  REFUSED("dw_before", norm_before_grad(x, w, rstd, &dout, dy, &dx, &w1, &work, n));
+  REFUSED("rstd", norm_before_grad(x, w, rstd1, &dout, dy, &dx, &dwb, &work, n));
 
   std::printf("%d calls, %d failures\n", calls, failures);
   return failures != 0;
