@@ -42,6 +42,7 @@ B_NN = 0
 B_NT = 1
 F32 = 0   # element types of unpacked matrices (MIAIE_F32, MIAIE_BF16)
 BF16 = 1
+MXFP4 = 2  # a packed result, for plan_gemm_mxfp4
 NORM_MAX_COLS = 16384
 
 _ERR_NAMES = {
@@ -94,6 +95,7 @@ _SIGS = {
     "miaie_gemm_mxfp4": (_i, [_p] * 6 + [_i] * 5),
     "miaie_gemm_mxfp4_rq": (_i, [_p] * 7 + [_i] * 4),
     "miaie_mlp_mxfp4": (_i, [_p] * 10 + [_i] * 6),
+    "miaie_plan_gemm_mxfp4": (_i, [_i] * 5 + [_p]),
     "miaie_norm_block": (_i, [_p] * 9 + [_i] * 7 + [_f, _f]),
     "miaie_norm_block_grad": (_i, [_p] * 15 + [_sz] + [_i] * 7 + [_f]),
     "miaie_fill_i8": (_i, [_p, _p, _sz, _u64]),
@@ -191,6 +193,7 @@ def _addr(x) -> int | None:
 KERNEL_TILE64 = 0  # register-staged tiles (GemmPlan.tile_m x tile_n), or the 64x64 kernel for K < 16
 KERNEL_PIPE = 1
 KERNEL_PIPE_MIXED = 2  # 256x256 tiles, then 256x128 tiles over the last columns
+KERNEL_ROWS = 3  # MXFP4 products of few rows
 
 
 class GemmPlan(C.Structure):
@@ -200,6 +203,15 @@ class GemmPlan(C.Structure):
 
     def as_dict(self) -> dict:
         return {f: getattr(self, f) for f, _ in self._fields_}
+
+
+def plan_gemm_mxfp4(M, N, K, out=F32, cus=256) -> dict:
+    """Which kernel an MXFP4 product takes (out: F32, BF16 or MXFP4).  A host function: needs no device."""
+    p = GemmPlan()
+    rc = load_library().miaie_plan_gemm_mxfp4(M, N, K, out, cus, C.byref(p))
+    if rc != MIAIE_OK:
+        raise MiaieError(rc, load_library().miaie_last_error_string(None).decode())
+    return p.as_dict()
 
 
 class Graph:

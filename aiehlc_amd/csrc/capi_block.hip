@@ -31,14 +31,18 @@ int check_elements(miaie_ctx* ctx, const char* fn, const char* name, const void*
   return MIAIE_OK;
 }
 
+int check_rows(miaie_ctx* ctx, const char* fn, const char* name, int R, int K) {
+  if ((long)R * mx::s_groups(K) >= kMost)
+    return fail(ctx, MIAIE_EINVAL, "%s: %s (%d rows of %d columns) is too large", fn, name, R, K);
+  return MIAIE_OK;
+}
+
 // The two arrays of a packed R x K matrix.
 int check_packed(miaie_ctx* ctx, const char* fn, const char* name, const uint8_t* q, const uint8_t* s, int R, int K) {
   if (!q || !s) return fail(ctx, MIAIE_EINVAL, "%s: %s%s is NULL", fn, name, !q ? "q" : "s");
   if (!aligned(q, 16) || !aligned(s, 16))
     return fail(ctx, MIAIE_EINVAL, "%s: %sq and %ss must be 16-byte aligned", fn, name, name);
-  if ((long)R * mx::s_groups(K) >= kMost)
-    return fail(ctx, MIAIE_EINVAL, "%s: %s (%d rows of %d columns) is too large", fn, name, R, K);
-  return MIAIE_OK;
+  return check_rows(ctx, fn, name, R, K);
 }
 
 // 512 threads pack 64 rows of 512 columns of a packed transpose, the workgroups'
@@ -99,15 +103,32 @@ extern "C" int miaie_dequant_mxfp4(miaie_ctx* ctx, const uint8_t* Q, const uint8
 
 namespace {
 
-int check_gemm(miaie_ctx* ctx, const char* fn, const uint8_t* Aq, const uint8_t* As, const uint8_t* Bq,
-               const uint8_t* Bs, int M, int N, int K) {
+int check_gemm_sizes(miaie_ctx* ctx, const char* fn, int M, int N, int K) {
   if (M < 1 || N < 1 || K < 1 || M > kMost || N > kMost || K > kMostK)
     return fail(ctx, MIAIE_EINVAL, "%s: M=%d N=%d K=%d must be in [1, 2^30], K in [1, 2^26]", fn, M, N, K);
+  return MIAIE_OK;
+}
+
+int check_gemm(miaie_ctx* ctx, const char* fn, const uint8_t* Aq, const uint8_t* As, const uint8_t* Bq,
+               const uint8_t* Bs, int M, int N, int K) {
+  MIAIE_TRY(check_gemm_sizes(ctx, fn, M, N, K));
   MIAIE_TRY(check_packed(ctx, fn, "A", Aq, As, M, K));
   return check_packed(ctx, fn, "B", Bq, Bs, N, K);
 }
 
 }  // namespace
+
+extern "C" int miaie_plan_gemm_mxfp4(int M, int N, int K, int out, int cus, miaie_gemm_plan* plan) {
+  if (!plan) return fail(nullptr, MIAIE_EINVAL, "%s: plan is NULL", __func__);
+  MIAIE_TRY(check_gemm_sizes(nullptr, __func__, M, N, K));
+  MIAIE_TRY(check_rows(nullptr, __func__, "A", M, K));
+  MIAIE_TRY(check_rows(nullptr, __func__, "B", N, K));
+  if (out != MIAIE_F32 && out != MIAIE_BF16 && out != MIAIE_MXFP4)
+    return fail(nullptr, MIAIE_EINVAL, "%s: out=%d is none of MIAIE_F32, MIAIE_BF16 and MIAIE_MXFP4", __func__, out);
+  if (out == MIAIE_MXFP4) MIAIE_TRY(check_rows(nullptr, __func__, "Y", M, N));
+  if (cus < 1) return fail(nullptr, MIAIE_EINVAL, "%s: cus=%d must be >= 1", __func__, cus);
+  return plan_gemm_mxfp4(M, N, K, out, cus, plan);
+}
 
 extern "C" int miaie_gemm_mxfp4(miaie_ctx* ctx, const uint8_t* Aq, const uint8_t* As, const uint8_t* Bq,
                                 const uint8_t* Bs, void* C, int dtype, int M, int N, int K, int ldc) {
@@ -144,8 +165,7 @@ extern "C" int miaie_mlp_mxfp4(miaie_ctx* ctx, const uint8_t* Xq, const uint8_t*
   MIAIE_TRY(check_packed(ctx, __func__, "H", Hq, Hs, M, F));
   MIAIE_TRY(check_pitch(ctx, __func__, "ldy", ldy, Nout));
   MIAIE_TRY(check_elements(ctx, __func__, "Y", Y, dtype));
-  MIAIE_TRY(launch_gemm_mxfp4_rq(ctx, Xq, Xs, W1q, W1s, Hq, Hs, M, F, K, 1));
-  return launch_gemm_mxfp4(ctx, Hq, Hs, W2q, W2s, Y, dtype, M, Nout, F, ldy);
+  return launch_mlp_mxfp4(ctx, Xq, Xs, W1q, W1s, W2q, W2s, Hq, Hs, Y, dtype, M, K, F, Nout, ldy);
 }
 
 namespace {

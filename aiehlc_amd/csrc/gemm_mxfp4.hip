@@ -755,19 +755,31 @@ int run_pipe(miaie_ctx* ctx, const Args& p) {
   return check_launch(ctx, e, "gemm_mx_pipe");
 }
 
+// Columns of a result that are written (a packed one has zeros up to the end of its last 512 columns).
+constexpr long written_cols(Out out, int N) {
+  return out == OUT_MX || out == OUT_MX_RELU ? 512l * s_groups(N) : N;
+}
+
+// Tiles and waves of a product on gemm_mx_rows: as many waves as share the groups
+// of 512 columns evenly, up to 16 and to what fits the LDS.
+struct RowsGrid {
+  long tiles_n, tiles;
+  int waves;
+};
+template <int MI, int NJ, int AI>
+RowsGrid rows_grid(long M, long cols, int groups) {
+  using G = RowsGeom<MI, NJ, AI>;
+  const long tiles_n = (cols + 16 * NJ - 1) / (16 * NJ);
+  const int each = (groups + G::WAVES - 1) / G::WAVES;
+  return {tiles_n, (M + 16 * MI - 1) / (16 * MI) * tiles_n, (groups + each - 1) / each};
+}
+
 template <int MI, int NJ, int AI, Out OUT>
 int run_rows(miaie_ctx* ctx, const Args& p) {
-  using G = RowsGeom<MI, NJ, AI>;
-  // (a packed result has zeros up to the end of its last 512 columns)
-  const int cols = OUT == OUT_MX || OUT == OUT_MX_RELU ? 512 * s_groups(p.N) : p.N;
-  const int tiles_n = (cols + 16 * NJ - 1) / (16 * NJ);
-  const long tiles = (p.M + 16l * MI - 1) / (16 * MI) * tiles_n;
-  const int groups = s_groups(p.K);
-  // as many waves as share the groups evenly, up to 16 and to what fits the LDS
-  const int each = (groups + G::WAVES - 1) / G::WAVES, waves = (groups + each - 1) / each;
-  if (tiles * waves >= 1l << 26) return fail(ctx, MIAIE_EINVAL, "gemm_mxfp4: M=%d N=%d too large", p.M, p.N);
-  const hipError_t e = launch<gemm_mx_rows<MI, NJ, AI, OUT>>(ctx->device, dim3((unsigned)tiles), dim3(64 * waves),
-                                                                    (size_t)waves * G::REGION, ctx->stream, p, tiles_n, waves);
+  const RowsGrid g = rows_grid<MI, NJ, AI>(p.M, written_cols(OUT, p.N), s_groups(p.K));
+  const hipError_t e = launch<gemm_mx_rows<MI, NJ, AI, OUT>>(ctx->device, dim3((unsigned)g.tiles), dim3(64 * g.waves),
+                                                                    (size_t)g.waves * RowsGeom<MI, NJ, AI>::REGION, ctx->stream,
+                                                                    p, (int)g.tiles_n, g.waves);
   return check_launch(ctx, e, "gemm_mx_rows");
 }
 
@@ -784,18 +796,20 @@ int run_rows(miaie_ctx* ctx, const Args& p) {
 // tiles, which its 512 columns at least never make the quickest.)
 struct Choice {
   double us = 1e30;
-  int kernel = -1;
-  int wide = 0;  // tile columns of 256 (mixed tiles)
+  int kernel = -1;  // none: no kernel takes a product of that size in one launch
+  int wide = 0;     // tile columns of 256 (mixed tiles)
 };
 void consider(Choice& best, int kernel, double us) {
   if (us < best.us) best = Choice{us, kernel, 0};
 }
+constexpr double kNever = 1e300;
 
 template <int MI, int NJ, int AI>
 double rows_us(long M, long cols, int groups, int cus) {
   using G = RowsGeom<MI, NJ, AI>;
-  const long tiles = ((M + 16 * MI - 1) / (16 * MI)) * ((cols + 16 * NJ - 1) / (16 * NJ));
-  return 1.2 + 0.02 * G::OPS + (double)((tiles + cus - 1) / cus) * groups * G::GROUP / 42e3;
+  const RowsGrid g = rows_grid<MI, NJ, AI>(M, cols, groups);
+  if (g.tiles * g.waves >= 1l << 26) return kNever;  // (HIP takes fewer than 2^32 threads)
+  return 1.2 + 0.02 * G::OPS + (double)((g.tiles + cus - 1) / cus) * groups * G::GROUP / 42e3;
 }
 
 // Cycles of a workgroup on a tile: its start, a k-tile, its end (fp32, bf16, packed).
@@ -814,43 +828,44 @@ double pipe_us(long tiles, int k_tiles, const TileCycles& t, double end, int cus
 }
 
 template <Out OUT>
-int run(miaie_ctx* ctx, const Args& p) {
+Choice choose(int M, int N, int K, int cus) {
   constexpr bool packed = OUT == OUT_MX || OUT == OUT_MX_RELU;
-  const int groups = s_groups(p.K), k_tiles = (int)(q_pitch(p.K) / 64), cus = ctx->cus;
-  const long cols = packed ? 512l * s_groups(p.N) : p.N;
+  const int groups = s_groups(K), k_tiles = (int)(q_pitch(K) / 64);
+  const long cols = written_cols(OUT, N);
   Choice c;
-  if (p.M <= 4) {
-    consider(c, 0, rows_us<1, 1 + packed, 1>(p.M, cols, groups, cus));
-  } else if (p.M <= 8) {
-    if (!packed) consider(c, 1, rows_us<1, 1, 2>(p.M, cols, groups, cus));
-    consider(c, 2, rows_us<1, 2, 2>(p.M, cols, groups, cus));
-    consider(c, 3, rows_us<1, 4, 2>(p.M, cols, groups, cus));
+  if (M <= 4) {
+    consider(c, 0, rows_us<1, 1 + packed, 1>(M, cols, groups, cus));
+  } else if (M <= 8) {
+    if (!packed) consider(c, 1, rows_us<1, 1, 2>(M, cols, groups, cus));
+    consider(c, 2, rows_us<1, 2, 2>(M, cols, groups, cus));
+    consider(c, 3, rows_us<1, 4, 2>(M, cols, groups, cus));
   } else {
-    if (!packed) consider(c, 4, rows_us<1, 1, 4>(p.M, cols, groups, cus));
-    consider(c, 5, rows_us<1, 2, 4>(p.M, cols, groups, cus));
-    consider(c, 6, rows_us<1, 4, 4>(p.M, cols, groups, cus));
+    if (!packed) consider(c, 4, rows_us<1, 1, 4>(M, cols, groups, cus));
+    consider(c, 5, rows_us<1, 2, 4>(M, cols, groups, cus));
+    consider(c, 6, rows_us<1, 4, 4>(M, cols, groups, cus));
   }
-  if (p.M > 16) {
-    if (!packed) consider(c, 7, rows_us<2, 1, 8>(p.M, cols, groups, cus));
-    consider(c, 8, rows_us<2, 2, 8>(p.M, cols, groups, cus));
-    consider(c, 9, rows_us<2, 4, 8>(p.M, cols, groups, cus));
+  if (M > 16) {
+    if (!packed) consider(c, 7, rows_us<2, 1, 8>(M, cols, groups, cus));
+    consider(c, 8, rows_us<2, 2, 8>(M, cols, groups, cus));
+    consider(c, 9, rows_us<2, 4, 8>(M, cols, groups, cus));
   }
-  if (p.M > 32) {
-    if (!packed) consider(c, 10, rows_us<4, 2, 16>(p.M, cols, groups, cus));
-    consider(c, 11, rows_us<4, 4, 16>(p.M, cols, groups, cus));
+  if (M > 32) {
+    if (!packed) consider(c, 10, rows_us<4, 2, 16>(M, cols, groups, cus));
+    consider(c, 11, rows_us<4, 4, 16>(M, cols, groups, cus));
   }
   // (a row's offset within a tile in 32 bits, and HIP takes fewer than 2^32 threads)
-  const long tiles = ((p.M + 127l) / 128) * ((p.N + 127l) / 128);
-  if (q_pitch(p.K) < (1u << 24) && tiles < 1l << 23) {
+  if (q_pitch(K) < (1u << 24)) {
     constexpr int o = packed ? 2 : OUT == OUT_BF16;
-    consider(c, 12, pipe_us(tiles, k_tiles, kTiles[2], kTiles[2].end[o], cus));
-    const long tiles_m = (p.M + 255l) / 256, wide = (p.N + 255l) / 256;
-    consider(c, 13, pipe_us(tiles_m * ((p.N + 127l) / 128), k_tiles, kTiles[1], kTiles[1].end[o], cus));
-    consider(c, 14, pipe_us(tiles_m * wide, k_tiles, kTiles[0], kTiles[0].end[o], cus));
+    constexpr long most = 1l << 24;  // workgroups
+    const long tiles_m = (M + 255l) / 256, wide = (N + 255l) / 256;
+    const long square = ((M + 127l) / 128) * ((N + 127l) / 128), tall = tiles_m * ((N + 127l) / 128);
+    if (square < most) consider(c, 12, pipe_us(square, k_tiles, kTiles[2], kTiles[2].end[o], cus));
+    if (tall < most) consider(c, 13, pipe_us(tall, k_tiles, kTiles[1], kTiles[1].end[o], cus));
+    if (tiles_m * wide < most) consider(c, 14, pipe_us(tiles_m * wide, k_tiles, kTiles[0], kTiles[0].end[o], cus));
     // whole rounds of wide tiles, then narrow ones
-    if (tiles_m * wide > cus && tiles_m <= cus && tiles_m * wide < 8l * cus) {
+    if (tall < most && tiles_m * wide > cus && tiles_m <= cus && tiles_m * wide < 8l * cus) {
       const long first = tiles_m * wide / cus * cus / tiles_m;  // wide tile columns
-      const long narrow = tiles_m * ((p.N - 256 * first + 127) / 128);
+      const long narrow = tiles_m * ((N - 256 * first + 127) / 128);
       if (first > 0 && narrow > 0) {
         const double us = pipe_us(tiles_m * first, k_tiles, kTiles[0], kTiles[0].end[o], cus) - 1.0 +
                           pipe_us(narrow, k_tiles, kTiles[1], kTiles[1].end[o], cus);
@@ -858,24 +873,97 @@ int run(miaie_ctx* ctx, const Args& p) {
       }
     }
   }
+  return c;
+}
+
+// A kernel of the choice as a type.
+template <int MI, int NJ, int AI>
+struct Rows {};
+template <int BM, int BN>
+struct Pipe {};
+struct Mixed {
+  int wide;
+};
+
+template <Out OUT, class F>
+int with_kernel(const Choice& c, F&& go) {
+  constexpr bool packed = OUT == OUT_MX || OUT == OUT_MX_RELU;
   switch (c.kernel) {
-    case 0: return run_rows<1, 1 + packed, 1, OUT>(ctx, p);
-    case 1: return run_rows<1, 1 + packed, 2, OUT>(ctx, p);
-    case 2: return run_rows<1, 2, 2, OUT>(ctx, p);
-    case 3: return run_rows<1, 4, 2, OUT>(ctx, p);
-    case 4: return run_rows<1, 1 + packed, 4, OUT>(ctx, p);
-    case 5: return run_rows<1, 2, 4, OUT>(ctx, p);
-    case 6: return run_rows<1, 4, 4, OUT>(ctx, p);
-    case 7: return run_rows<2, 1 + packed, 8, OUT>(ctx, p);
-    case 8: return run_rows<2, 2, 8, OUT>(ctx, p);
-    case 9: return run_rows<2, 4, 8, OUT>(ctx, p);
-    case 10: return run_rows<4, packed ? 4 : 2, 16, OUT>(ctx, p);
-    case 11: return run_rows<4, 4, 16, OUT>(ctx, p);
-    case 12: return run_pipe<128, 128, OUT>(ctx, p);
-    case 13: return run_pipe<256, 128, OUT>(ctx, p);
-    case 14: return run_pipe<256, 256, OUT>(ctx, p);
-    default: return run_mixed<OUT>(ctx, p, c.wide);
+    case 0: return go(Rows<1, 1 + packed, 1>{});
+    case 1: return go(Rows<1, 1 + packed, 2>{});
+    case 2: return go(Rows<1, 2, 2>{});
+    case 3: return go(Rows<1, 4, 2>{});
+    case 4: return go(Rows<1, 1 + packed, 4>{});
+    case 5: return go(Rows<1, 2, 4>{});
+    case 6: return go(Rows<1, 4, 4>{});
+    case 7: return go(Rows<2, 1 + packed, 8>{});
+    case 8: return go(Rows<2, 2, 8>{});
+    case 9: return go(Rows<2, 4, 8>{});
+    case 10: return go(Rows<4, packed ? 4 : 2, 16>{});
+    case 11: return go(Rows<4, 4, 16>{});
+    case 12: return go(Pipe<128, 128>{});
+    case 13: return go(Pipe<256, 128>{});
+    case 14: return go(Pipe<256, 256>{});
+    default: return go(Mixed{c.wide});
   }
+}
+
+template <Out OUT>
+struct Runner {
+  miaie_ctx* ctx;
+  const Args& p;
+  template <int MI, int NJ, int AI>
+  int operator()(Rows<MI, NJ, AI>) const { return run_rows<MI, NJ, AI, OUT>(ctx, p); }
+  template <int BM, int BN>
+  int operator()(Pipe<BM, BN>) const { return run_pipe<BM, BN, OUT>(ctx, p); }
+  int operator()(Mixed m) const { return run_mixed<OUT>(ctx, p, m.wide); }
+};
+
+template <Out OUT>
+struct Planner {
+  int M, N, K;
+  miaie_gemm_plan* plan;
+  template <int MI, int NJ, int AI>
+  int operator()(Rows<MI, NJ, AI>) const {
+    const RowsGrid g = rows_grid<MI, NJ, AI>(M, written_cols(OUT, N), s_groups(K));
+    *plan = {MIAIE_KERNEL_ROWS, 16 * MI, 16 * NJ, (int)g.tiles, 64 * g.waves};
+    return MIAIE_OK;
+  }
+  template <int BM, int BN>
+  int operator()(Pipe<BM, BN>) const {
+    *plan = {MIAIE_KERNEL_PIPE, BM, BN, (M + BM - 1) / BM * ((N + BN - 1) / BN), 256};
+    return MIAIE_OK;
+  }
+  int operator()(Mixed m) const {
+    *plan = {MIAIE_KERNEL_PIPE_MIXED, 256, 256, (M + 255) / 256 * (m.wide + (N - 256 * m.wide + 127) / 128), 256};
+    return MIAIE_OK;
+  }
+};
+
+int too_large(miaie_ctx* ctx, int M, int N, int K) {
+  return fail(ctx, MIAIE_EINVAL, "gemm_mxfp4: a product of M=%d N=%d K=%d is too large for one launch", M, N, K);
+}
+
+template <Out OUT>
+int run(miaie_ctx* ctx, const Args& p) {
+  const Choice c = choose<OUT>(p.M, p.N, p.K, ctx->cus);
+  return c.kernel < 0 ? too_large(ctx, p.M, p.N, p.K) : with_kernel<OUT>(c, Runner<OUT>{ctx, p});
+}
+
+// Up and down projection, both chosen before either is queued.
+template <Out OUT>
+int run_mlp(miaie_ctx* ctx, const Args& up, const Args& down) {
+  const Choice u = choose<OUT_MX_RELU>(up.M, up.N, up.K, ctx->cus), d = choose<OUT>(down.M, down.N, down.K, ctx->cus);
+  if (u.kernel < 0) return too_large(ctx, up.M, up.N, up.K);
+  if (d.kernel < 0) return too_large(ctx, down.M, down.N, down.K);
+  const int rc = with_kernel<OUT_MX_RELU>(u, Runner<OUT_MX_RELU>{ctx, up});
+  return rc ? rc : with_kernel<OUT>(d, Runner<OUT>{ctx, down});
+}
+
+template <Out OUT>
+int plan(int M, int N, int K, int cus, miaie_gemm_plan* to) {
+  const Choice c = choose<OUT>(M, N, K, cus);
+  return c.kernel < 0 ? too_large(nullptr, M, N, K) : with_kernel<OUT>(c, Planner<OUT>{M, N, K, to});
 }
 
 }  // namespace
@@ -890,6 +978,18 @@ int launch_gemm_mxfp4_rq(miaie_ctx* ctx, const uint8_t* Aq, const uint8_t* As, c
                          uint8_t* Yq, uint8_t* Ys, int M, int N, int K, int relu) {
   const Args p{Aq, As, Bq, Bs, nullptr, Yq, Ys, M, N, K, 0};
   return relu ? run<OUT_MX_RELU>(ctx, p) : run<OUT_MX>(ctx, p);
+}
+
+int launch_mlp_mxfp4(miaie_ctx* ctx, const uint8_t* Xq, const uint8_t* Xs, const uint8_t* W1q, const uint8_t* W1s,
+                     const uint8_t* W2q, const uint8_t* W2s, uint8_t* Hq, uint8_t* Hs, void* Y, int dtype, int M, int K,
+                     int F, int Nout, int ldy) {
+  const Args up{Xq, Xs, W1q, W1s, nullptr, Hq, Hs, M, F, K, 0}, down{Hq, Hs, W2q, W2s, Y, nullptr, nullptr, M, Nout, F, ldy};
+  return dtype == MIAIE_BF16 ? run_mlp<OUT_BF16>(ctx, up, down) : run_mlp<OUT_F32>(ctx, up, down);
+}
+
+int plan_gemm_mxfp4(int M, int N, int K, int out, int cus, miaie_gemm_plan* to) {
+  // (with and without a ReLU a packed product takes the same kernels)
+  return out == MIAIE_MXFP4 ? plan<OUT_MX>(M, N, K, cus, to) : out == MIAIE_BF16 ? plan<OUT_BF16>(M, N, K, cus, to) : plan<OUT_F32>(M, N, K, cus, to);
 }
 
 }  // namespace miaie

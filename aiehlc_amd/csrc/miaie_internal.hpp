@@ -168,6 +168,10 @@ int launch_gemm_mxfp4(miaie_ctx* ctx, const uint8_t* Aq, const uint8_t* As, cons
                       void* C, int dtype, int M, int N, int K, int ldc);
 int launch_gemm_mxfp4_rq(miaie_ctx* ctx, const uint8_t* Aq, const uint8_t* As, const uint8_t* Bq, const uint8_t* Bs,
                          uint8_t* Yq, uint8_t* Ys, int M, int N, int K, int relu);
+int launch_mlp_mxfp4(miaie_ctx* ctx, const uint8_t* Xq, const uint8_t* Xs, const uint8_t* W1q, const uint8_t* W1s,
+                     const uint8_t* W2q, const uint8_t* W2s, uint8_t* Hq, uint8_t* Hs, void* Y, int dtype, int M, int K,
+                     int F, int Nout, int ldy);
+int plan_gemm_mxfp4(int M, int N, int K, int out, int cus, miaie_gemm_plan* to);
 int launch_norm_block(miaie_ctx* ctx, const void* x, const void* b, const void* gate, const float* w_after,
                       const float* w_before, void* out, void* y, float* rstd, int rows, int cols, int ldx, int ldb,
                       int gate_rows, int stream_dtype, int branch_dtype, float alpha, float eps);

@@ -130,6 +130,8 @@ MIAIE_API int miaie_debug_unregister(miaie_ctx* ctx, const void* dev_ptr);
                                      last tile row/column overlaps the one before it) */
 #define MIAIE_KERNEL_PIPE_MIXED 2 /* pipelined kernel, 256x256 tiles over the first columns and 256x128
                                      tiles over the rest, in one launch (tile_m = tile_n = 256) */
+#define MIAIE_KERNEL_ROWS 3       /* MXFP4 products of few rows (miaie_plan_gemm_mxfp4): tile_m x tile_n results a
+                                     workgroup, whose waves share out k */
 
 /* How miaie_gemm_i8_rq would run an M x N x K product on this context with
  * dense 16-byte-aligned NN operands (the tiling planner: the grid
@@ -321,9 +323,12 @@ MIAIE_API int miaie_mlp_i8_noalloc(miaie_ctx* ctx, const int8_t* X, const int8_t
  *      [R][K / 512][4][4], transpose to [K / 512][R][4][4] with the last two
  *      axes exchanged.)
  * Sizes are in [1, 2^30], a size that a product contracts in [1, 2^26]; the rows
- * times the groups of 512 columns of a matrix stay below 2^30. */
+ * times the groups of 512 columns of a matrix stay below 2^30.  One launch each:
+ * ceil(M / 256) ceil(N / 256) of a product stays below 2^24, ceil(R / 512)
+ * ceil(C / 512) of a conversion along the columns at 2^20 - 8 or below. */
 #define MIAIE_F32 0  /* element types of unpacked matrices */
 #define MIAIE_BF16 1 /* raw 16-bit patterns */
+#define MIAIE_MXFP4 2 /* a packed result (miaie_plan_gemm_mxfp4 only) */
 
 /* Bytes of a row of Q, and of the arrays Q and S, of an R x K matrix (0 for
  * arguments outside the ranges above).  Host functions. */
@@ -360,6 +365,14 @@ MIAIE_API int miaie_gemm_mxfp4(miaie_ctx* ctx, const uint8_t* Aq, const uint8_t*
  * if relu != 0: the 4-bit counterpart of miaie_gemm_i8_rq. */
 MIAIE_API int miaie_gemm_mxfp4_rq(miaie_ctx* ctx, const uint8_t* Aq, const uint8_t* As, const uint8_t* Bq,
                                   const uint8_t* Bs, uint8_t* Yq, uint8_t* Ys, int M, int N, int K, int relu);
+
+/* How miaie_gemm_mxfp4 (out: MIAIE_F32, MIAIE_BF16) or miaie_gemm_mxfp4_rq
+ * (MIAIE_MXFP4, with or without the ReLU) runs an M x N x K product planned for
+ * `cus` compute units (256 on an MI355X; miaie_plan_set_cus on a context):
+ * MIAIE_KERNEL_ROWS, MIAIE_KERNEL_PIPE or MIAIE_KERNEL_PIPE_MIXED, each of which
+ * takes any M, N and K.  A host function: needs no context and no device.
+ * MIAIE_EINVAL for sizes that the entry points refuse. */
+MIAIE_API int miaie_plan_gemm_mxfp4(int M, int N, int K, int out, int cus, miaie_gemm_plan* plan);
 
 /* Chained 4-bit MLP, H = pack(relu(X . W1^T)), Y = H . W2^T: X M x K, W1 F x K,
  * W2 Nout x F, H M x F packed (Hq, Hs: caller-provided device scratch), Y
