@@ -519,8 +519,8 @@ int launch_norm_block(miaie_ctx* ctx, const void* x, const void* b, const void* 
   with_types(stream_dtype, branch_dtype, [&](auto st, auto bt) {
     with_row(cols, [&](auto tpr, auto nc) {
       constexpr int TPR = decltype(tpr)::value, NC = decltype(nc)::value, RPW = TPR < 256 ? 256 / TPR : 1;
-      // (up to about four rows a workgroup, which then loads the weights once)
-      const int turns = (rows + RPW - 1) / RPW, workgroups = std::min(turns, std::max(16 * ctx->cus, 1));
+      // (at most 16 workgroups a CU, which load the weights once for all their rows)
+      const int turns = (rows + RPW - 1) / RPW, workgroups = (int)std::min<long>(turns, 16l * ctx->cus);
       p.stride = workgroups * RPW;
       e = launch<norm_fwd<typename decltype(st)::type, typename decltype(bt)::type, TPR, NC>>(
           ctx->device, dim3(workgroups), dim3(TPR < 256 ? 256 : TPR), 0, ctx->stream, p);

@@ -1,5 +1,6 @@
-"""Row lanes without a row in the gradients of the norms around a block, and
-infinities there, against the 64-bit oracle (tests/mx_oracle.py)."""
+"""Edges of the norms around a block: row lanes without a row in their gradients,
+and infinities there, against the 64-bit oracle (tests/mx_oracle.py); the grid
+planned for very many compute units."""
 import numpy as np
 import pytest
 
@@ -49,3 +50,27 @@ def test_infinite_weights_reach_only_the_sums_of_real_rows(ctx, rows, cols, k, w
         _same_where_not_finite(ctx.download(buf).astype(np.float64), want[n], n)
     for b in (*bufs, *g, work):
         b.free()
+
+
+def test_norm_grid_planned_for_very_many_cus():
+    """miaie_plan_set_cus takes any count: 16 workgroups a CU stay within an int."""
+    from hip_capture import Capture
+
+    _say("norm grid")
+    rows, cols = 100, 64
+    cap = Capture()
+    try:
+        c = cap.ctx
+        x, w, y = (c.upload(np.ones(s, np.float32)) for s in ((rows, cols), (cols,), (rows, cols)))
+        grids = []
+        for cus in (256, 1 << 28):
+            c.plan_set_cus(cus)
+            exe, g = cap.record(lambda: c.norm_block(x, None, None, None, w, None, y, None, rows, cols,
+                                                     stream_dtype=mi.F32, branch_dtype=mi.F32))
+            cap.ok(cap.hip.hipGraphExecDestroy(exe))
+            grids.append(g)
+        assert grids[0] == grids[1] == [(25, 1, 1)]  # four rows of 64 threads a workgroup
+        for b in (x, w, y):
+            b.free()
+    finally:
+        cap.close()
