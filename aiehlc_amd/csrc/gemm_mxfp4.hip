@@ -336,7 +336,7 @@ __device__ __forceinline__ int b_swz(int r) { return -(r >> 2) & 3; }
 // form of the instruction writes other registers than it adds to and moves
 // accumulators around: 30 cycles an instruction in a loop of 16 of them,
 // against 17.)  No instruction but a load writes an operand within two
-// instructions before its use (tests/test_mx_asm.py).
+// instructions before its use (tests/test_mx_asm.py, tests/test_block_asm.py).
 template <int T>
 __device__ __forceinline__ void mfma_in_place(v4f& acc, v4i b, v4i a, int sb, int sa) {
 #if MIAIE_DEVICE_CHECKS
@@ -786,14 +786,20 @@ int run_rows(miaie_ctx* ctx, const Args& p) {
 // ------------------------------------------------------------ choice of kernel
 // The kernel with the lowest estimated time.  Few rows: a CU copies about 42
 // bytes a ns into LDS with its waves' groups in flight, so the workgroups of one
-// CU take that time for all their groups (within 15% of 46 measured products of
-// 1 to 100 rows, 4 to 26 us).  Large products: cycles of a workgroup's start, of a
-// k-tile and of its end as measured on the tiles (a k-tile of 256 x 256 has 64
-// instructions of 16 cycles on each wave), the clock 2.3 GHz with a part of the
-// CUs at work and about 1.9 under the power limit.  128 x 128 tiles fit a CU
+// CU take that time for all their groups.  Large products: cycles of a workgroup's
+// start, of a k-tile and of its end as measured on the tiles (a k-tile of 256 x 256
+// has 64 instructions of 16 cycles on each wave), the clock 2.3 GHz with a part of
+// the CUs at work and about 1.9 under the power limit.  128 x 128 tiles fit a CU
 // twice, and then take 960 cycles for both where one takes 540.  (A packed result
 // takes no single column block, whose two neighbours a lane needs, and no 64 x 32
 // tiles, which its 512 columns at least never make the quickest.)
+// The estimates are for the choice, not for the time: against the chosen kernels at
+// 1 to 2048 rows of 4096 x 4096, 11008 x 4096 and 4096 x 11008 (bf16 out) they are
+// 31% low to 10% high below 48 rows, 19% low to 55% high at 48 to 256 (row kernels at
+// K = 11008 are the ones estimated high) and 18% low to 14% high above.  Of those
+// three sizes at 48, 64, 96, 128, 192, 256, 384 and 512 rows, with the row kernels of 16 x 32
+// to 64 x 64 results and the 128 x 128 and 256 x 128 tiles each timed, the chosen
+// one is the quickest in 23 and 4% behind in one.
 struct Choice {
   double us = 1e30;
   int kernel = -1;  // none: no kernel takes a product of that size in one launch

@@ -196,8 +196,12 @@ __global__ __launch_bounds__(BWD_THREADS) void norm_bwd(Bwd p) {
   __shared__ float red[2][BWD_THREADS / 64];
   const bool alone = !(p.dy && p.b && p.db);
   // Rows of two chunks a thread keep the norms' sums in LDS, each thread its own
-  // columns', and fetch no row ahead, so that one row fits the registers (1024 x 16384
-  // bf16: 55 us, 143 with the sums and the next row in scratch memory).
+  // columns', and fetch no row ahead, so that of one row only 14 to 16 registers a
+  // thread (56 to 60 bytes) are in scratch memory.  1024 x 16384 bf16: 68 us with
+  // every tensor from beyond the caches, of which a copy's rate takes 39, and 57 with
+  // those of the call before (143 with the sums and the next row in scratch memory
+  // too); fp32 stream 89 and 84 us.  The rest have none, but for two registers of
+  // fp32 rows of 513 to 4096 columns.
   constexpr bool WIDE = NC > 1;
   __shared__ float kept[WIDE ? 2 * NC * 8 * TPR : 1];
   __shared__ __attribute__((aligned(16))) float weights[WIDE ? 4 : 2 * 8 * TPR];
@@ -541,8 +545,11 @@ int launch_norm_block_grad(miaie_ctx* ctx, const void* r, const void* b, const v
   with_types(stream_dtype, branch_dtype, [&](auto st, auto bt) {
     with_row(cols, [&](auto tpr, auto nc) {
       constexpr int TPR = decltype(tpr)::value, NC = decltype(nc)::value, RPW = BWD_THREADS / TPR;
-      // at most 256 workgroups (the work buffer holds 341 partial rows of
-      // three sums), each with at least one row for every row lane
+      // At most 256 workgroups (the work buffer holds 341 partial rows of three
+      // sums).  Up to 128 gates share them out, each with at least a row of a gate's
+      // gate_rows (there or not) for every row lane; of more, every row lane takes
+      // whole gates, so that few long gates leave CUs idle: 16512 rows of 512 columns
+      // take 20 us in 128 gates and 232 us in 129.
       constexpr int kMost = 256;
       if (p.groups <= kMost / 2) {
         p.parts = (int)std::min<long>(kMost / p.groups, ((long)gate_rows + RPW - 1) / RPW);
