@@ -94,13 +94,13 @@ def draw(rng) -> dict:
         groups = rng.choice((1, 1, 4, 8))
         E = groups * _size(rng, 2, 512 // groups)
         kept = 1 if groups == 1 else rng.randint(1, groups)
-        k = min(rng.randint(1, 8), kept * (E // groups))
+        k = min(rng.randint(2 if grad else 1, 8), kept * (E // groups))  # (a single renormalised weight has no gradient)
         return {"op": op, "T": _size(rng, 1, 8192), "E": E, "k": k, "scoring": scoring, "bias": bias, "groups": groups,
                 "kept": kept, "grad": grad, "masked": masked}
     most_work, most_weights = (2**36, 2**28) if op == "experts" else (2**32, 2**25)
     while True:
         T, E, D = _size(rng, 1, 4096), rng.randint(2, 128), _size(rng, 64, 4096)
-        F, k = 128 * rng.randint(1, 16), rng.randint(1, 8)
+        F, k = 128 * rng.randint(1, 16), rng.randint(2 if op == "experts_grad" else 1, 8)
         if k <= E and E * D * F <= most_weights and T * k * D * F <= most_work and E * T * D * F <= 2**39:
             return {"op": op, "T": T, "E": E, "k": k, "D": D, "F": F, "scoring": scoring, "bias": bias, "masked": masked}
 
