@@ -284,7 +284,7 @@ def _pp(pair):
 
 def _own_route(ctx, c, s):
     groups = c.get("groups", 1)
-    ctx.route_experts(_p(s["logits"]), _p(s.get("bias")), _p(s["idx_"]), _p(s["w_"]), c["T"], c["E"], c["k"],
+    ctx.route_experts(_p(s["logits"]), _p(s.get("bias")), _p(s["idx_"]), _p(s["w_"]), c["T"], c["k"], c["E"],
                       scoring=_SCORING[c["scoring"]], groups=groups, groups_kept=c.get("kept", 1),
                       group_top=min(2, c["E"] // groups) if groups > 1 else 1, renormalize=True, scale=_SCALE)
 
@@ -325,7 +325,7 @@ def _run_own(s: dict):
     T, E, k = c["T"], c["E"], c["k"]
     if op == "route":
         if c["grad"]:
-            ctx.route_experts_grad(_p(s["logits"]), _p(s["idx"]), _p(s["dw"]), _p(s["dlogits_"]), T, E, k,
+            ctx.route_experts_grad(_p(s["logits"]), _p(s["idx"]), _p(s["dw"]), _p(s["dlogits_"]), T, k, E,
                                    scoring=_SCORING[c["scoring"]], renormalize=True, scale=_SCALE)
             return s["dlogits_"]
         _own_route(ctx, c, s)
@@ -343,7 +343,7 @@ def _run_own(s: dict):
     ht, xt, dh = _pp(s["Ht"]), _pp(s["Xt"]), _p(s["dH_"])
     ctx.experts_order(_p(s["idx"]), order, *n)
     ctx.experts_combine_grad(order, _p(s["Y"]), _p(s["dout"]), _p(s["dw_"]), *n, D, dtype=_BF16)
-    ctx.route_experts_grad(_p(s["logits"]), _p(s["idx"]), _p(s["dw_"]), _p(s["dlogits_"]), T, E, k,
+    ctx.route_experts_grad(_p(s["logits"]), _p(s["idx"]), _p(s["dw_"]), _p(s["dlogits_"]), T, k, E,
                            scoring=_SCORING[c["scoring"]], renormalize=True, scale=_SCALE)
     ctx.experts_quant_fp8(order, _p(s["dout"]), _p(s["w"]), *dyq, *dyt, *n, D, dtype=_BF16)
     ctx.experts_quant_fp8(order, _p(s["X"]), None, None, None, *xt, *n, D, dtype=_BF16)
