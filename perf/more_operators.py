@@ -35,7 +35,7 @@ def listed() -> list[dict]:
         # a ragged batch, no size a multiple of anything
         {"name": "linear_ragged", "op": "linear", "M": 333, "K": 1000, "N": 777},
         # a product of kept operands at the size of the bf16 benchmark
-        {"name": "gemm_8192", "op": "gemm", "M": 8192, "K": 8192, "N": 8192, "out": "bf16"},
+        {"name": "gemm_8192", "op": "gemm", "M": 8192, "K": 8192, "N": 8192},
         # gradients of a linear layer: operands quantised along the axis that each product contracts
         {"name": "linear_grad", "op": "linear_grad", "M": 2048, "K": 4096, "N": 4096},
         # quantisation of the benchmark's up-projection weights in blocks of 128 x 128, and their transpose
@@ -78,10 +78,7 @@ def draw(rng) -> dict:
             M, K, N = _size(rng, 1, 8192), _size(rng, 32, 12288), _size(rng, 16, 12288)
             if M * K * N <= (8192**3 if op == "gemm" else 2**36):
                 break
-        case = {"op": op, "M": M, "K": K, "N": N}
-        if op == "gemm":
-            case["out"] = rng.choice(("f32", "bf16"))
-        return case
+        return {"op": op, "M": M, "K": K, "N": N}
     if op == "quant":
         while True:
             R, C = _size(rng, 1, 16384), _size(rng, 1, 16384)
@@ -217,11 +214,11 @@ def prepare(case: dict, seed: int) -> dict:
     if op == "linear":
         s["Xq"], s["C"] = packed(c["M"], c["K"]), _empty(bf, c["M"], c["N"])
     elif op == "gemm":
-        s["C"] = _empty(_DTYPES[c["out"]], c["M"], c["N"])
+        s["C"] = _empty(bf, c["M"], c["N"])
     elif op == "linear_grad":
         M, N, K = c["M"], c["N"], c["K"]
         s["dYq"], s["dYt"], s["Xt"] = packed(M, N), packed(N, M), packed(K, M)
-        s["dX"], s["dW"] = _empty(bf, M, K), _empty(f32, N, K)
+        s["dX"], s["dW"] = _empty(bf, M, K), _empty(bf, N, K)
     elif op == "quant":
         R, C = c["R"], c["C"]
         if c["axis"] != "columns":
@@ -299,7 +296,7 @@ def _run_own(s: dict):
         ctx.gemm_fp8(*xq, *_pp(s["W"]), _p(s["C"]), M, N, K, dtype=_BF16)
         return s["C"]
     if op == "gemm":
-        ctx.gemm_fp8(*_pp(s["A"]), *_pp(s["B"]), _p(s["C"]), c["M"], c["N"], c["K"], dtype=_CODE[s["C"].dtype])
+        ctx.gemm_fp8(*_pp(s["A"]), *_pp(s["B"]), _p(s["C"]), c["M"], c["N"], c["K"], dtype=_BF16)
         return s["C"]
     if op == "linear_grad":
         M, N, K = c["M"], c["N"], c["K"]
@@ -307,7 +304,7 @@ def _run_own(s: dict):
         ctx.quant_fp8(_p(s["dY"]), M, N, *dyq, *dyt, dtype=_BF16)
         ctx.quant_fp8(_p(s["X"]), M, K, None, None, *xt, dtype=_BF16)
         ctx.gemm_fp8(*dyq, *_pp(s["Wt"]), _p(s["dX"]), M, K, N, dtype=_BF16)
-        ctx.gemm_fp8(*dyt, *xt, _p(s["dW"]), N, K, M, b_block=1, dtype=_F32)
+        ctx.gemm_fp8(*dyt, *xt, _p(s["dW"]), N, K, M, b_block=1, dtype=_BF16)
         return s["dX"], s["dW"]
     if op == "quant":
         R, C, X, block = c["R"], c["C"], s["X"], c["block"]
@@ -448,11 +445,11 @@ def _run_plain(s: dict):
         return (_rounded(s["X"]) @ _values(*s["W"], c["N"], c["K"]).t()).to(torch.bfloat16)
     if op == "gemm":
         A, B = _values(*s["A"], c["M"], c["K"], 1), _values(*s["B"], c["N"], c["K"])
-        return (A @ B.t()).to(_DTYPES[c["out"]])
+        return (A @ B.t()).to(torch.bfloat16)
     if op == "linear_grad":
         dX = _rounded(s["dY"]) @ _values(*s["Wt"], c["K"], c["N"]).t()
         dW = _rounded(_columns(s["dY"])) @ _rounded(_columns(s["X"])).t()
-        return dX.to(torch.bfloat16), dW
+        return dX.to(torch.bfloat16), dW.to(torch.bfloat16)
     if op == "quant":
         out = []
         if c["axis"] != "columns":
@@ -505,11 +502,11 @@ def work(case: dict) -> dict:
     c, op = case, case["op"]
     if op in ("linear", "gemm"):
         M, N, K = c["M"], c["N"], c["K"]
-        return {"bytes": (2 if op == "linear" else 1) * M * K + N * K + (4 if c.get("out") == "f32" else 2) * M * N,
+        return {"bytes": (2 if op == "linear" else 1) * M * K + N * K + 2 * M * N,
                 "flops": 2 * M * N * K}
     if op == "linear_grad":
         M, N, K = c["M"], c["N"], c["K"]
-        return {"bytes": 2 * (M * N + M * K) + N * K + 2 * M * K + 4 * N * K, "flops": 4 * M * N * K}
+        return {"bytes": 2 * (M * N + M * K) + N * K + 2 * M * K + 2 * N * K, "flops": 4 * M * N * K}
     if op == "quant":  # the packed matrices, written once, and the values
         n, k = c["R"] * c["C"], 2 if c["axis"] == "both" else 1
         return {"bytes": (2 if c["dtype"] == "bf16" else 4) * n + 3 * k * n, "flops": 0}
