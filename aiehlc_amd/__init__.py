@@ -44,6 +44,10 @@ F32 = 0   # element types of unpacked matrices (MIAIE_F32, MIAIE_BF16)
 BF16 = 1
 MXFP4 = 2  # a packed result, for plan_gemm_mxfp4
 NORM_MAX_COLS = 16384
+SOFTMAX = 0  # scores of route_experts (MIAIE_SOFTMAX, MIAIE_SIGMOID)
+SIGMOID = 1
+MAX_EXPERTS = 1024
+MAX_TOP_K = 64
 
 _ERR_NAMES = {
     MIAIE_EINVAL: "MIAIE_EINVAL",
@@ -98,6 +102,25 @@ _SIGS = {
     "miaie_plan_gemm_mxfp4": (_i, [_i] * 5 + [_p]),
     "miaie_norm_block": (_i, [_p] * 9 + [_i] * 7 + [_f, _f]),
     "miaie_norm_block_grad": (_i, [_p] * 15 + [_sz] + [_i] * 7 + [_f]),
+    "miaie_fp8_q_pitch": (_sz, [_i]),
+    "miaie_fp8_q_bytes": (_sz, [_i, _i]),
+    "miaie_fp8_s_bytes": (_sz, [_i, _i, _i]),
+    "miaie_quant_fp8": (_i, [_p, _p] + [_i] * 5 + [_p] * 4),
+    "miaie_dequant_fp8": (_i, [_p, _p, _p, _i, _p] + [_i] * 4),
+    "miaie_gemm_fp8": (_i, [_p] * 5 + [_i, _p] + [_i] * 5),
+    "miaie_route_experts": (_i, [_p, _p, _i, _p, _p, _p] + [_i] * 9 + [_f]),
+    "miaie_route_experts_grad": (_i, [_p, _p, _i, _p, _p, _p] + [_i] * 7 + [_f]),
+    "miaie_experts_rows": (_sz, [_i] * 3),
+    "miaie_experts_order_bytes": (_sz, [_i] * 3),
+    "miaie_experts_order": (_i, [_p] * 3 + [_i] * 3),
+    "miaie_experts_mlp_fp8": (_i, [_p] * 13 + [_i] * 8),
+    "miaie_experts_gemm_fp8": (_i, [_p] * 7 + [_i] * 8),
+    "miaie_experts_quant_fp8": (_i, [_p] * 3 + [_i] + [_p] * 5 + [_i] * 5),
+    "miaie_experts_swiglu_fp8": (_i, [_p] * 3 + [_i] + [_p] * 4 + [_i] * 5),
+    "miaie_experts_swiglu_grad_fp8": (_i, [_p] * 3 + [_i] + [_p] * 5 + [_i] * 6),
+    "miaie_experts_wgrad_fp8": (_i, [_p] * 7 + [_i] * 7),
+    "miaie_experts_combine": (_i, [_p] * 5 + [_i] * 7),
+    "miaie_experts_combine_grad": (_i, [_p] * 5 + [_i] * 7),
     "miaie_fill_i8": (_i, [_p, _p, _sz, _u64]),
     "miaie_plan_gemm_i8": (_i, [_p, _i, _i, _i, _p]),
     "miaie_plan_set_cus": (_i, [_p, _i, C.POINTER(_i)]),
@@ -152,6 +175,23 @@ def mxfp4_shapes(rows: int, cols: int) -> tuple[tuple[int, int], tuple[int, int,
     """Shapes of the uint8 arrays Q and S of a packed rows x cols matrix
     (include/miaie.h, miaie_quant_mxfp4)."""
     return (rows, (cols + 255) // 256 * 128), ((cols + 511) // 512, rows, 4, 4)
+
+
+def fp8_shapes(rows: int, cols: int, block: int = 1) -> tuple[tuple[int, int], tuple[int, int]]:
+    """Shapes of the arrays Q (uint8) and S (float32) of a packed rows x cols matrix
+    with a scale for 128 columns of `block` rows (include/miaie.h, miaie_quant_fp8)."""
+    blocks = (cols + 127) // 128
+    return (rows, 128 * blocks), (blocks, (rows + block - 1) // block)
+
+
+def experts_rows(tokens: int, top_k: int, experts: int) -> int:
+    """Rows of a matrix over the slots of any routing (miaie_experts_rows; needs no device)."""
+    return load_library().miaie_experts_rows(tokens, top_k, experts)
+
+
+def experts_order_bytes(tokens: int, top_k: int, experts: int) -> int:
+    """Bytes of the order of the slots (miaie_experts_order)."""
+    return load_library().miaie_experts_order_bytes(tokens, top_k, experts)
 
 
 def norm_work_bytes(cols: int) -> int:
@@ -275,6 +315,12 @@ class Context:
         self._f_quant, self._f_dequant, self._f_mx = lib.miaie_quant_mxfp4, lib.miaie_dequant_mxfp4, lib.miaie_gemm_mxfp4
         self._f_mx_rq, self._f_mlp_mx = lib.miaie_gemm_mxfp4_rq, lib.miaie_mlp_mxfp4
         self._f_norm, self._f_norm_grad = lib.miaie_norm_block, lib.miaie_norm_block_grad
+        self._f_quant8, self._f_dequant8, self._f_gemm8 = lib.miaie_quant_fp8, lib.miaie_dequant_fp8, lib.miaie_gemm_fp8
+        self._f_route, self._f_route_grad, self._f_order = lib.miaie_route_experts, lib.miaie_route_experts_grad, lib.miaie_experts_order
+        self._f_x_mlp, self._f_x_gemm, self._f_x_wgrad = lib.miaie_experts_mlp_fp8, lib.miaie_experts_gemm_fp8, lib.miaie_experts_wgrad_fp8
+        self._f_x_quant, self._f_x_glu, self._f_x_glu_grad = (lib.miaie_experts_quant_fp8, lib.miaie_experts_swiglu_fp8,
+                                                              lib.miaie_experts_swiglu_grad_fp8)
+        self._f_x_sum, self._f_x_sum_grad = lib.miaie_experts_combine, lib.miaie_experts_combine_grad
 
     # -- plumbing
     def _call(self, name: str, *args) -> int:
@@ -480,6 +526,75 @@ class Context:
                       dw_before, work, work_bytes, rows, cols, cols if ldx is None else ldx,
                       cols if ldb is None else ldb, rows if gate_rows is None else gate_rows, stream_dtype,
                       branch_dtype, alpha)
+
+    # -- 8-bit floating point with a scale for each block of 128 (packed matrices: fp8_shapes)
+    def quant_fp8(self, X, R, C, Q, S, Qt=None, St=None, block=1, dtype=BF16, ldx=None) -> None:
+        """Pack X (R x C) along its rows (Q, S) and / or its columns (Qt, St)."""
+        self._compute(self._f_quant8, X, dtype, R, C, C if ldx is None else ldx, block, Q, S, Qt, St)
+
+    def dequant_fp8(self, Q, S, Y, R, C, block=1, dtype=BF16, ldy=None) -> None:
+        self._compute(self._f_dequant8, Q, S, block, Y, dtype, R, C, C if ldy is None else ldy)
+
+    def gemm_fp8(self, Aq, As, Bq, Bs, Cm, M, N, K, b_block=128, dtype=F32, ldc=None) -> None:
+        """C = A . B^T, A (M x K, block 1) and B (N x K, block b_block) packed along their rows."""
+        self._compute(self._f_gemm8, Aq, As, Bq, Bs, b_block, Cm, dtype, M, N, K, N if ldc is None else ldc)
+
+    # -- routing of tokens to experts
+    def route_experts(self, logits, bias, idx, w, tokens, top_k, experts, scoring=SOFTMAX, groups=1, groups_kept=1,
+                      group_top=1, renormalize=True, scale=1.0, dtype=F32, ld=None) -> None:
+        """The top_k experts of each token (idx, best first) and their weights w."""
+        self._compute(self._f_route, logits, dtype, bias, idx, w, tokens, top_k, experts, experts if ld is None else ld,
+                      scoring, groups, groups_kept, group_top, int(renormalize), scale)
+
+    def route_experts_grad(self, logits, idx, dw, dlogits, tokens, top_k, experts, scoring=SOFTMAX, renormalize=True,
+                           scale=1.0, dtype=F32, ld=None, ldd=None) -> None:
+        self._compute(self._f_route_grad, logits, dtype, idx, dw, dlogits, tokens, top_k, experts,
+                      experts if ld is None else ld, experts if ldd is None else ldd, scoring, int(renormalize), scale)
+
+    # -- the experts' products over slots (experts_rows, experts_order_bytes)
+    def experts_order(self, idx, order, tokens, top_k, experts) -> None:
+        """The slots of the pairs of a token and a choice, sorted by expert."""
+        self._compute(self._f_order, idx, order, tokens, top_k, experts)
+
+    def experts_mlp_fp8(self, order, w, Xq, Xs, W1q, W1s, W2q, W2s, Hq, Hs, Y, out, tokens, top_k, experts, D, F, Nout,
+                        dtype=BF16, ldo=None) -> None:
+        """out = sum over a token's experts of w * (silu(X . Wg^T) * (X . Wu^T)) . W2^T."""
+        self._compute(self._f_x_mlp, order, w, Xq, Xs, W1q, W1s, W2q, W2s, Hq, Hs, Y, out, dtype, tokens, top_k, experts, D,
+                      F, Nout, Nout if ldo is None else ldo)
+
+    def experts_gemm_fp8(self, order, Aq, As, Bq, Bs, Cm, tokens, top_k, experts, N, K, gather=False, dtype=BF16,
+                         ldc=None) -> None:
+        """C[slot] = A[slot] (gather: A[its token]) . B of its expert, transposed."""
+        self._compute(self._f_x_gemm, order, Aq, As, Bq, Bs, Cm, dtype, tokens, top_k, experts, N, K,
+                      N if ldc is None else ldc, int(gather))
+
+    def experts_quant_fp8(self, order, X, w, Q, S, Qt, St, tokens, top_k, experts, C, dtype=BF16, ldx=None) -> None:
+        """Pack w * X[token] by slot, along the rows and / or along the slots."""
+        self._compute(self._f_x_quant, order, X, dtype, w, Q, S, Qt, St, tokens, top_k, experts, C, C if ldx is None else ldx)
+
+    def experts_swiglu_fp8(self, order, GU, Q, S, Qt, St, tokens, top_k, experts, F, dtype=BF16, ldgu=None) -> None:
+        """Pack silu(gate) * up of GU = (gate, up) likewise."""
+        self._compute(self._f_x_glu, order, GU, dtype, Q, S, Qt, St, tokens, top_k, experts, F, 2 * F if ldgu is None else ldgu)
+
+    def experts_swiglu_grad_fp8(self, order, GU, dH, Q, S, Qt, St, tokens, top_k, experts, F, dtype=BF16, ldgu=None,
+                                ldh=None) -> None:
+        """Pack the gradient of GU from that of silu(gate) * up."""
+        self._compute(self._f_x_glu_grad, order, GU, dtype, dH, Q, S, Qt, St, tokens, top_k, experts, F,
+                      2 * F if ldgu is None else ldgu, F if ldh is None else ldh)
+
+    def experts_wgrad_fp8(self, order, Atq, Ats, Btq, Bts, Cm, tokens, top_k, experts, M, N, dtype=F32, ldc=None) -> None:
+        """Each expert's sum over its slots of A[m][slot] * B[n][slot]."""
+        self._compute(self._f_x_wgrad, order, Atq, Ats, Btq, Bts, Cm, dtype, tokens, top_k, experts, M, N,
+                      N if ldc is None else ldc)
+
+    def experts_combine(self, order, Y, w, out, tokens, top_k, experts, C, dtype=BF16, ldy=None, ldo=None) -> None:
+        """out = sum over a token's slots of w * Y[slot] (w None: of Y[slot])."""
+        self._compute(self._f_x_sum, order, Y, w, out, dtype, tokens, top_k, experts, C, C if ldy is None else ldy,
+                      C if ldo is None else ldo)
+
+    def experts_combine_grad(self, order, Y, dout, dw, tokens, top_k, experts, C, dtype=BF16, ldy=None, ldo=None) -> None:
+        self._compute(self._f_x_sum_grad, order, Y, dout, dw, dtype, tokens, top_k, experts, C, C if ldy is None else ldy,
+                      C if ldo is None else ldo)
 
 
 def version() -> str:

@@ -1,0 +1,746 @@
+// Products of 8-bit floating point matrices with a scale for each block of 128
+// (fp8.hpp) on v_mfma_f32_16x16x128_f8f6f4:
+//   C[m][n] = sum over blocks b of k: Sa[b][m] Sb[b][n] sum_{k in b} A[m][k] B[n][k]
+// dense, over the slots of routed tokens (each expert's rows with its own B), and
+// over each expert's slots as k (the gradients of the experts' weights).
+//
+// An instruction multiplies 128 k, one block: lane l holds 32 of row l % 16 of
+// each operand, the 16-byte chunks l / 16 and 4 + l / 16 (any order of k does that
+// both operands share).  Scales:
+//   B in blocks of 128 x 128 (weights, whose scales may be any fp32): the block's
+//     product starts from zero and is added by a multiply-add per value, with one
+//     factor Sa Sb for a lane's four values;
+//   B with a scale for each row (both operands packed by this library): both
+//     scales are powers of two, the instruction applies them and adds to the
+//     accumulator itself.  In multiply-adds their eight a fragment (a factor a
+//     column) would take as long as the instruction.
+//
+// Operand roles: srcA is the B fragment and srcB the A fragment, so lane l of the
+// result has row m = l % 16 and the four consecutive columns n = 4 (l / 16) + 0..3
+// of its 16 x 16 block: vectors of a row of C, and one scale of A a lane.
+#include <algorithm>
+#include <type_traits>
+
+#include "fp8.hpp"
+#include "gfx950_ops.hpp"
+
+namespace miaie {
+namespace {
+
+using namespace fp8;
+
+enum Mode { DENSE, SLOTS, WGRAD };
+enum Out { OUT_F32, OUT_BF16, OUT_GLU };  // OUT_GLU: silu(gate) up, packed along its rows
+
+struct Args {
+  const uint8_t* Aq;
+  const float* As;
+  const uint8_t* Bq;
+  const float* Bs;
+  void* C;      // OUT_F32, OUT_BF16
+  uint8_t* Hq;  // OUT_GLU
+  float* Hs;
+  int M, N, K, ldc;  // OUT_GLU: N = F, B has 2 F rows; SLOTS: M = the slots' rows; WGRAD: K = those
+  int a_rows;        // rows of A (the stride of its scales)
+  int gather;        // SLOTS: A's rows are tokens
+  Slots s;
+};
+
+__device__ __forceinline__ v4f mfma0(v8i b, v8i a) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, v4f{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+}
+__device__ __forceinline__ v4f mfma_scaled(v8i b, v8i a, v4f acc, int sb, int sa) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(b, a, acc, 0, 0, 0, sb, 0, sa);
+}
+__device__ __forceinline__ v8i join(v4i lo, v4i hi) { return v8i{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]}; }
+
+// 16-byte chunk c of a row's 128 bytes lies at c ^ swz(row): the 16 rows of a
+// fragment read cover all banks.
+__device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
+
+template <class T>
+__device__ __forceinline__ void store4(T* C, size_t ldc, int m, int n, int M, int N, v4f v) {
+  if (m >= M || n >= N) return;
+  typedef T V __attribute__((ext_vector_type(4)));
+  const V r = __builtin_convertvector(v, V);
+  T* p = C + (size_t)m * ldc + n;
+  if (n + 4 <= N) {
+    using P = At<V, T>;
+    MIAIE_ST(reinterpret_cast<P*>(p), P{r});
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (n + e < N) MIAIE_ST(p + e, r[e]);
+  }
+}
+
+// ---------------------------------------------------------------- large tiles
+// A workgroup of WAVES_M x WAVES_N waves owns a BM x BN tile, a wave NI x NJ blocks
+// of 16 x 16.  A step is 128 k: whole 128-byte lines of BM + BN rows and their
+// scales, copied into one of STAGES stages of LDS with no registers in between.
+template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int STAGES_>
+struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, STAGES = STAGES_;
+  static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = 64 * WAVES;
+  static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, NI = WM / 16, NJ = WN / 16;
+  static constexpr int A = 0, B = BM * 128, S = B + BN * 128, STAGE = S + 4 * (BM + BN);
+  static constexpr int A_CP = BM / 8 / WAVES, B_CP = BN / 8 / WAVES;  // copies of a wave in a step
+  static constexpr int S_CP = ((BM + BN) / 64 + WAVES - 1) / WAVES, CP = A_CP + B_CP + S_CP;
+  static constexpr int LDS = STAGES * STAGE;
+  static_assert(A_CP >= 1 && B_CP >= 1 && BM % 64 == 0 && BN % 64 == 0 && STAGE % 128 == 0, "copies of whole waves");
+  static_assert(LDS <= 163840, "LDS of a CU");
+};
+
+// Where a tile's operands are: wave-uniform addresses of step 0, a row's offset for
+// each of a wave's copies.
+struct Operands {
+  const uint8_t *a, *b;
+  const float *as, *bs;
+  size_t as_step, bs_step;  // floats from one step's scales to the next's
+  int steps;
+  int rows, cols;  // of the tile that exist
+};
+
+template <class G, int BBLOCK, bool GLU, class RowA, class RowB, class ScaleB>
+__device__ __forceinline__ void multiply(int8_t* lds, const Operands& o, uint32_t a_pitch, uint32_t b_pitch, RowA row_a, RowB row_b,
+                                         ScaleB scale_b, const dbg::Span& aq_span, const dbg::Span& as_span,
+                                         const dbg::Span& bq_span, const dbg::Span& bs_span, v4f (&acc)[G::NI][G::NJ]) {
+  constexpr int NI = G::NI, NJ = G::NJ;
+  const uint32_t lds0 = dev::lds_addr(lds);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / G::WAVES_N, wn = wave % G::WAVES_N, fr = lane & 15, fg = lane >> 4;
+
+  uint32_t a_off[G::A_CP], b_off[G::B_CP], s_off[G::S_CP];
+#pragma unroll
+  for (int x = 0; x < G::A_CP; ++x) {
+    const int r = 8 * (G::WAVES * x + wave) + (lane >> 3);
+    a_off[x] = row_a(r) * a_pitch + 16 * ((lane & 7) ^ swz(r));
+  }
+#pragma unroll
+  for (int x = 0; x < G::B_CP; ++x) {
+    const int r = 8 * (G::WAVES * x + wave) + (lane >> 3);
+    b_off[x] = row_b(r) * b_pitch + 16 * ((lane & 7) ^ swz(r));
+  }
+  // (scales: every wave makes the same number of copies, the last ones again)
+  int s_row[G::S_CP];
+#pragma unroll
+  for (int x = 0; x < G::S_CP; ++x) {
+    s_row[x] = 64 * ((G::WAVES * x + wave) % ((G::BM + G::BN) / 64));
+    s_off[x] = 4 * (s_row[x] < G::BM ? row_a(s_row[x] + lane) : scale_b(s_row[x] - G::BM + lane));
+  }
+  const uint8_t *a_src = o.a, *b_src = o.b;
+  const float *as_src = o.as, *bs_src = o.bs;
+  auto copy = [&](uint32_t st) __attribute__((always_inline)) {  // the next step's operands
+#pragma unroll
+    for (int x = 0; x < G::A_CP; ++x)
+      dev::gload_lds16(a_src, a_off[x], lds0 + st + G::A + 1024 * (G::WAVES * x + wave), aq_span);
+#pragma unroll
+    for (int x = 0; x < G::B_CP; ++x)
+      dev::gload_lds16(b_src, b_off[x], lds0 + st + G::B + 1024 * (G::WAVES * x + wave), bq_span);
+#pragma unroll
+    for (int x = 0; x < G::S_CP; ++x) {
+      if (s_row[x] < G::BM)
+        dev::gload_lds4(as_src, s_off[x], lds0 + st + G::S + 4 * s_row[x], as_span);
+      else
+        dev::gload_lds4(bs_src, s_off[x], lds0 + st + G::S + 4 * s_row[x], bs_span);
+    }
+    a_src += 128, b_src += 128, as_src += o.as_step, bs_src += o.bs_step;
+  };
+
+  const uint32_t a_fo = G::A + (wm * G::WM + fr) * 128 + ((fg ^ swz(fr)) << 4);
+  const uint32_t b_fo = G::B + (wn * G::WN + fr) * 128 + ((fg ^ swz(fr)) << 4);
+  auto read = [&](uint32_t at, int block) __attribute__((always_inline)) -> v8i {
+    return join(*reinterpret_cast<const v4i*>(lds + at + 2048 * block), *reinterpret_cast<const v4i*>(lds + (at ^ 64) + 2048 * block));
+  };
+  auto scale = [&](uint32_t st, int row) __attribute__((always_inline)) -> float {
+    return *reinterpret_cast<const float*>(lds + st + G::S + 4 * row);
+  };
+  const int KT = o.steps;
+  v8i a[NI], b[2];
+  v4f p[2][NI];
+  float sa[NI], sb[BBLOCK == 1 ? NJ : 2];
+  auto read_scales = [&](uint32_t st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) sa[i] = scale(st, wm * G::WM + 16 * i + fr);
+    if constexpr (BBLOCK == 1) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) sb[j] = scale(st, G::BM + wn * G::WN + 16 * j + fr);
+    } else {
+      sb[0] = scale(st, G::BM + wn * G::WN);
+      sb[1] = GLU ? scale(st, G::BM + wn * G::WN + G::WN / 2) : 0.f;
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < G::STAGES; ++s)
+    if (s < KT) copy(s * G::STAGE);
+  dev::wait_tiles_behind<G::CP, G::STAGES>(min(KT, G::STAGES));
+  dev::barrier();
+  uint32_t st = 0;
+  read_scales(0);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) a[i] = read(a_fo, i);
+  b[0] = read(b_fo, 0);
+
+  for (int t = 0; t < KT; ++t) {
+    const uint32_t next = st + G::STAGE == G::LDS ? 0 : st + G::STAGE;
+    float s[2][NI];
+    int ea[NI], eb[NJ];
+    if constexpr (BBLOCK == 1) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) ea[i] = (int)(__float_as_uint(sa[i]) >> 23);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) eb[j] = (int)(__float_as_uint(sb[j]) >> 23);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        s[0][i] = sa[i] * sb[0];
+        s[1][i] = GLU ? sa[i] * sb[1] : s[0][i];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      if (j + 1 < NJ) b[(j + 1) & 1] = read(b_fo + st, j + 1);
+      if (j == NJ - 1) {
+        // This step's last fragments are in registers: once every wave is here, and
+        // the next step's operands too, its stage takes the copies of step t + STAGES.
+        dev::waitcnt<63, 0>();
+        if (t + 1 < KT) dev::wait_tiles_behind<G::CP, G::STAGES - 1>(min(KT - 1 - t, G::STAGES - 1));
+        dev::barrier();
+        if (t + G::STAGES < KT) copy(st);
+        read_scales(next);
+        b[(j + 1) & 1] = read(b_fo + next, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        if constexpr (BBLOCK == 1) {
+          acc[i][j] = mfma_scaled(b[j & 1], a[i], acc[i][j], eb[j], ea[i]);
+        } else {
+          p[j & 1][i] = mfma0(b[j & 1], a[i]);
+          if (j > 0) {
+            const float f = s[GLU && j - 1 >= NJ / 2][i];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][j - 1][e] = __builtin_fmaf(p[(j - 1) & 1][i][e], f, acc[i][j - 1][e]);
+          }
+        }
+        if (j == NJ - 1) a[i] = read(a_fo + next, i);
+      }
+      dev::sched_fence();
+    }
+    if constexpr (BBLOCK != 1) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          acc[i][NJ - 1][e] = __builtin_fmaf(p[(NJ - 1) & 1][i][e], s[1][i], acc[i][NJ - 1][e]);
+    }
+    static_assert(NJ % 2 == 0, "the next step's first fragment of B in b[0]");
+    st = next;
+  }
+}
+
+// A wave's part at row 0 and column n0 of C (m < M rows, n0 + .. < N columns of it
+// exist).  In bf16 two blocks beside each other are exchanged between the lanes of a
+// row, so that each holds eight columns of one: 16 bytes a lane in either type.
+template <class T, int NI, int NJ>
+__device__ __forceinline__ void store_part(T* C, size_t ldc, int m0, int n0, int M, int N, const v4f (&acc)[NI][NJ]) {
+  const int lane = threadIdx.x & 63, fr = lane & 15, fg = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int m = m0 + 16 * i + fr;
+#pragma unroll
+    for (int j = 0; j < NJ; j += 2) {
+      if constexpr (sizeof(T) == 4) {
+        store4(C, ldc, m, n0 + 16 * j + 4 * fg, M, N, acc[i][j]);
+        store4(C, ldc, m, n0 + 16 * j + 16 + 4 * fg, M, N, acc[i][j + 1]);
+      } else {
+        v2u a = __builtin_bit_cast(v2u, __builtin_convertvector(acc[i][j], v4bf));
+        v2u b = __builtin_bit_cast(v2u, __builtin_convertvector(acc[i][j + 1], v4bf));
+        uint32_t a0 = a[0], a1 = a[1], b0 = b[0], b1 = b[1];
+        swap16(a0, b0);
+        swap16(a1, b1);
+        const v8bf v = __builtin_bit_cast(v8bf, v4u{a0, a1, b0, b1});
+        const int n = n0 + 16 * j + 16 * (fg & 1) + 8 * (fg >> 1);
+        if (m < M) {
+          T* p = C + (size_t)m * ldc + n;
+          if (n + 8 <= N) {
+            using P = At<v8bf, T>;
+            MIAIE_ST(reinterpret_cast<P*>(p), P{v});
+          } else {
+#pragma unroll
+            for (int e = 0; e < 7; ++e)
+              if (n + e < N) MIAIE_ST(p + e, v[e]);
+          }
+        }
+      }
+    }
+    dev::sched_fence();  // (more rows at once take more registers than there are)
+  }
+}
+
+// H = silu(gate) up of a wave's rows, columns j < NJ / 2 gate and the others up of
+// the same H columns; packed along its rows.  A block of 128 columns of H is the
+// workgroup's, so the rows' maxima are joined through LDS.
+template <class G>
+__device__ __forceinline__ void store_glu(const Args& p, int8_t* lds, int slot0, int rows, int f0, v4f (&acc)[G::NI][G::NJ]) {
+  constexpr int NI = G::NI, HJ = G::NJ / 2;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave / G::WAVES_N, wn = wave % G::WAVES_N, fr = lane & 15, fg = lane >> 4;
+  uint32_t* const lmax = reinterpret_cast<uint32_t*>(lds);
+  uint32_t mine[NI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < HJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float h = swiglu(acc[i][j][e], acc[i][j + HJ][e]);
+        acc[i][j][e] = h;
+        m = max(m, abs_bits(h));
+      }
+    mine[i] = max_over_16s(m);
+  }
+  __syncthreads();  // (the last fragments have been read)
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+    if (fg == 0) lmax[wn * G::BM + wm * G::WM + 16 * i + fr] = mine[i];
+  __syncthreads();
+  const size_t h_pitch = pitch(p.N);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int r = wm * G::WM + 16 * i + fr;
+    uint32_t m = 0;
+#pragma unroll
+    for (int w = 0; w < G::WAVES_N; ++w) m = max(m, lmax[w * G::BM + r]);
+    const uint32_t e = scale_of(m);
+    const float inv = inverse_f32(e);
+    uint32_t q[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < HJ; ++j) q[j] = pack4(acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3], inv);
+    uint8_t* row = p.Hq + (size_t)(slot0 + r) * h_pitch + f0 + wn * (G::WN / 2);
+    if constexpr (HJ == 4) {  // the lanes' 4 x 4 dwords transposed: 16 columns of one block a lane
+      swap32(q[0], q[2]);
+      swap32(q[1], q[3]);
+      swap16(q[0], q[1]);
+      swap16(q[2], q[3]);
+      if (r < rows) MIAIE_ST(reinterpret_cast<v4u*>(row + 16 * fg), (v4u{q[0], q[1], q[2], q[3]}));
+    } else {
+      static_assert(HJ == 2 || HJ == 4, "columns of a wave");
+      swap16(q[0], q[1]);
+      if (r < rows) MIAIE_ST(reinterpret_cast<v2u*>(row + 16 * (fg & 1) + 8 * (fg >> 1)), (v2u{q[0], q[1]}));
+    }
+    if (wn == 0 && fg == 0 && r < rows) MIAIE_ST(p.Hs + (size_t)(f0 / 128) * p.M + slot0 + r, scale_f32(e));
+  }
+}
+
+// An expert's tiles are walked blocks of rows first, so that those which share
+// columns of B run beside each other, and the workgroups of one XCD (b % 8) have a
+// contiguous run of all tiles in use: few experts' operands in one L2.  False: no
+// tile is left for this workgroup.
+__device__ __forceinline__ bool slot_tile(const Slots& s, int b, int tiles_n, int& block, int& tn, int& e) {
+  const int tiles = MIAIE_LD(s.start + s.experts) / 128 * tiles_n, each = (tiles + 7) / 8;
+  if (b / 8 >= each) return false;
+  const int logical = b % 8 * each + b / 8;
+  if (logical >= tiles) return false;
+  e = MIAIE_LD(s.expert_of + logical / tiles_n);
+  const int first = MIAIE_LD(s.start + e) / 128, n = (MIAIE_LD(s.count + e) + 127) / 128;
+  const int local = logical - first * tiles_n;
+  block = first + local % n;
+  tn = local / n;
+  return true;
+}
+
+template <class G, Mode MODE, Out OUT, int BBLOCK>
+__global__ __launch_bounds__(G::THREADS) void gemm_tile(Args p, int tiles_m, int tiles_n) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds[G::LDS];
+  constexpr bool GLU = OUT == OUT_GLU;
+  constexpr int COLS = GLU ? G::BN / 2 : G::BN;  // columns of the result
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave / G::WAVES_N, wn = wave % G::WAVES_N;
+  const uint32_t ap = (uint32_t)pitch(p.K), bp = ap;
+  Operands o;
+  int m0, n0, slot0 = 0;
+  size_t to = 0;  // first element of the tile's matrix in C
+  const int b_rows = GLU ? 2 * p.N : p.N;
+  const size_t b_s_rows = BBLOCK == 1 ? (size_t)b_rows : blocks(b_rows);
+  o.a = p.Aq, o.as = p.As, o.b = p.Bq, o.bs = p.Bs;
+  o.steps = (int)blocks(p.K);
+  o.as_step = p.a_rows, o.bs_step = b_s_rows;
+  if constexpr (MODE == DENSE) {
+    int tm, tn;
+    dev::tile_coords<4>(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    m0 = tm * G::BM, n0 = tn * COLS;
+    o.rows = p.M - m0;
+    o.a += (size_t)m0 * ap, o.as += m0;
+  } else if constexpr (MODE == SLOTS) {
+    static_assert(MODE != SLOTS || G::BM == 128, "a block of slots is one expert's");
+    int block, tn, e;
+    if (!slot_tile(p.s, blockIdx.x, tiles_n, block, tn, e)) return;
+    slot0 = 128 * block, m0 = 0, n0 = tn * COLS;
+    o.rows = MIAIE_LD(p.s.start + e) + MIAIE_LD(p.s.count + e) - slot0;
+    if (!p.gather) o.a += (size_t)slot0 * ap, o.as += slot0;
+    o.b += (size_t)e * b_rows * bp, o.bs += (size_t)e * b_s_rows * blocks(p.K);
+    to = (size_t)slot0 * p.ldc;
+  } else {
+    const int each = tiles_m * tiles_n, e = blockIdx.x / each;
+    int tm, tn;
+    dev::tile_coords<4>(blockIdx.x % each, tiles_m, tiles_n, tm, tn);
+    const int first = MIAIE_LD(p.s.start + e);
+    o.steps = (int)blocks(MIAIE_LD(p.s.count + e));
+    m0 = tm * G::BM, n0 = tn * COLS;
+    o.rows = p.M - m0;
+    o.a += (size_t)m0 * ap + first, o.as += (size_t)(first / 128) * p.M + m0;
+    o.b += first, o.bs += (size_t)(first / 128) * b_s_rows;
+    to = (size_t)e * p.M * p.ldc;
+  }
+  o.cols = p.N - n0;
+  o.b += (size_t)n0 * bp;
+  o.bs += BBLOCK == 1 ? n0 : n0 / 128;
+  o.rows = min(o.rows, G::BM), o.cols = min(o.cols, COLS);
+  const dbg::Span aq_span = dbg::span_of(p.Aq), as_span = dbg::span_of(p.As), bq_span = dbg::span_of(p.Bq),
+                  bs_span = dbg::span_of(p.Bs);  // (debug build only)
+  v4f acc[G::NI][G::NJ];
+#pragma unroll
+  for (int i = 0; i < G::NI; ++i)
+#pragma unroll
+    for (int j = 0; j < G::NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+  // rows behind the last one are copies of it, and dropped at the end
+  auto row_a = [&](int r) __attribute__((always_inline)) -> uint32_t {
+    r = min(r, o.rows - 1);
+    if constexpr (MODE == SLOTS) {
+      if (p.gather) return (uint32_t)(MIAIE_LD(p.s.row_of + slot0 + r) / p.s.top_k);
+    }
+    return (uint32_t)r;
+  };
+  // GLU: row r of a wave's part of the stage is a gate's, or the same column's up
+  auto row_b = [&](int r) __attribute__((always_inline)) -> uint32_t {
+    if constexpr (GLU) {
+      const int h = r % G::WN, f = r / G::WN * (G::WN / 2) + h % (G::WN / 2);
+      return (uint32_t)(h < G::WN / 2 ? f : p.N + f);
+    }
+    return (uint32_t)min(r, o.cols - 1);
+  };
+  auto scale_b = [&](int r) __attribute__((always_inline)) -> uint32_t {
+    return BBLOCK == 1 ? row_b(r) : row_b(r) / 128;
+  };
+  if (o.steps > 0)
+    multiply<G, BBLOCK, GLU>(lds, o, ap, bp, row_a, row_b, scale_b, aq_span, as_span, bq_span, bs_span, acc);
+  if constexpr (GLU) {
+    store_glu<G>(p, lds, slot0, o.rows, n0, acc);
+  } else {
+    using T = std::conditional_t<OUT == OUT_F32, float, __bf16>;
+    store_part(static_cast<T*>(p.C) + to, p.ldc, m0 + wm * G::WM, n0 + wn * G::WN, m0 + o.rows, p.N, acc);
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+// A wave copies 256 bytes (two blocks of k, a group) of 16 NJ rows of B and of
+// A's rows into a part of LDS of its own, waits for its own copies (no barriers)
+// and multiplies; the next group is on its way once this one's fragments are in
+// registers.  Bound by reading B, every byte of it once.  Chunk c (16 bytes) of
+// row r lies at c ^ (r % 16).
+template <int MI, int NJ>
+struct RowsGeom {
+  static constexpr int B = 0, A = 4096 * NJ, GROUP = A + 4096 * MI;
+  static constexpr int SUM = MI * NJ * 1024;
+  static constexpr int REGION = GROUP > SUM ? GROUP : SUM;
+};
+
+// acc[i][j] += rows 16 i .. of A times rows of B's j-th sixteen, over the groups
+// first, first + step, ...  a_off, b_off: a lane's offset of the row it copies.
+template <int MI, int NJ, int BBLOCK, class RowA, class RowB>
+__device__ __forceinline__ void multiply_rows(int8_t* mine, const uint8_t* a, const float* as, size_t as_step, const uint8_t* const (&b)[NJ],
+                                              const float* const (&bs)[NJ], size_t bs_step, uint32_t row_pitch, int steps, int rows,
+                                              RowA row_a, RowB row_b, int first, int step, const dbg::Span& aq_span,
+                                              const dbg::Span& bq_span, v4f (&acc)[MI][NJ]) {
+  using G = RowsGeom<MI, NJ>;
+  const int lane = threadIdx.x & 63, fr = lane & 15, fg = lane >> 4;
+  const uint32_t mine0 = dev::lds_addr(mine);
+  const int groups = (steps + 1) / 2;
+  const int a_copies = (min(rows, 16 * MI) + 3) / 4;
+  uint32_t a_off[4 * MI], b_off[4];
+#pragma unroll
+  for (int x = 0; x < 4 * MI; ++x) a_off[x] = row_a(min(4 * x + fg, rows - 1)) * row_pitch;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) b_off[x] = row_b(4 * x + fg) * row_pitch;
+  float sa[2][MI], sb[2][NJ];
+  uint32_t a_row[MI], b_row[4];
+#pragma unroll
+  for (int i = 0; i < MI; ++i) a_row[i] = row_a(min(16 * i + fr, rows - 1));
+  b_row[0] = row_b(fr);
+  auto copy = [&](int g) __attribute__((always_inline)) {
+    const uint32_t mask = 2 * g + 1 < steps ? 15 : 7;  // (half a group: its first block again)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const size_t kb = min(2 * g + k, steps - 1);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) sa[k][i] = MIAIE_LD(as + kb * as_step + a_row[i]);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) sb[k][j] = MIAIE_LD(bs[j] + kb * bs_step + (BBLOCK == 1 ? b_row[0] : 0u));
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        dev::gload_lds16(b[j] + 256 * (size_t)g, b_off[x] + 16 * ((fr ^ (4 * x + fg)) & mask), mine0 + G::B + 4096 * j + 1024 * x, bq_span);
+#pragma unroll
+    for (int x = 0; x < 4 * MI; ++x)
+      if (x < a_copies)
+        dev::gload_lds16(a + 256 * (size_t)g, a_off[x] + 16 * ((fr ^ ((4 * x + fg) & 15)) & mask), mine0 + G::A + 1024 * x, aq_span);
+  };
+  auto half = [&](int k) __attribute__((always_inline)) {
+    v8i fa[MI], fb[NJ];
+    const int c0 = 8 * k + fg, c1 = c0 + 4;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      fb[j] = join(*reinterpret_cast<const v4i*>(mine + G::B + 4096 * j + 256 * fr + 16 * (c0 ^ fr)),
+                   *reinterpret_cast<const v4i*>(mine + G::B + 4096 * j + 256 * fr + 16 * (c1 ^ fr)));
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int r = min(16 * i + fr, 4 * a_copies - 1), x = r & 15;
+      fa[i] = join(*reinterpret_cast<const v4i*>(mine + G::A + 256 * r + 16 * (c0 ^ x)),
+                   *reinterpret_cast<const v4i*>(mine + G::A + 256 * r + 16 * (c1 ^ x)));
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        if constexpr (BBLOCK == 1) {
+          acc[i][j] = mfma_scaled(fb[j], fa[i], acc[i][j], (int)(__float_as_uint(sb[k][j]) >> 23), (int)(__float_as_uint(sa[k][i]) >> 23));
+        } else {
+          const v4f p = mfma0(fb[j], fa[i]);
+          const float f = sa[k][i] * sb[k][j];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(p[e], f, acc[i][j][e]);
+        }
+      }
+  };
+  if (first < groups) copy(first);
+  for (int g = first; g < groups; g += step) {
+    dev::wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    half(0);
+    if (2 * g + 1 < steps) half(1);
+    if (g + step < groups) {
+      dev::waitcnt<63, 0>();
+      asm volatile("" ::: "memory");
+      copy(g + step);
+    }
+  }
+}
+
+// 16 MI rows and 16 NJ columns a workgroup, whose waves share out the groups of k
+// and add their sums in LDS in a fixed order.  SLOTS: a block of 128 slots a
+// workgroup, 16 MI rows at a time (few slots, or B comes out of the L2 again).
+template <int MI, int NJ, Mode MODE, Out OUT, int BBLOCK>
+__global__ __launch_bounds__(1024) void gemm_rows(Args p, int tiles_n, int waves) {
+  using G = RowsGeom<MI, NJ>;
+  extern __shared__ __attribute__((aligned(1024))) int8_t lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 15, fg = lane >> 4;
+  const uint32_t row_pitch = (uint32_t)pitch(p.K);
+  const size_t b_s_rows = BBLOCK == 1 ? (size_t)p.N : blocks(p.N);
+  const uint8_t *a = p.Aq, *b0 = p.Bq;
+  const float *as = p.As, *bs0 = p.Bs;
+  int m0 = 0, n0, rows, slot0 = 0;
+  size_t to = 0;
+  if constexpr (MODE == SLOTS) {
+    int block, tn, e;
+    if (!slot_tile(p.s, blockIdx.x, tiles_n, block, tn, e)) return;
+    slot0 = 128 * block, n0 = 16 * NJ * tn;
+    rows = min(128, MIAIE_LD(p.s.start + e) + MIAIE_LD(p.s.count + e) - slot0);
+    if (!p.gather) a += (size_t)slot0 * row_pitch, as += slot0;
+    b0 += (size_t)e * p.N * row_pitch, bs0 += (size_t)e * b_s_rows * blocks(p.K);
+    to = (size_t)slot0 * p.ldc;
+  } else {
+    m0 = 16 * MI * (blockIdx.x / tiles_n), n0 = 16 * NJ * (blockIdx.x % tiles_n);
+    rows = min(16 * MI, p.M - m0);
+    a += (size_t)m0 * row_pitch, as += m0;
+    to = (size_t)m0 * p.ldc;
+  }
+  b0 += (size_t)n0 * row_pitch, bs0 += BBLOCK == 1 ? n0 : n0 / 128;
+  const uint8_t* b[NJ];
+  const float* bs[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int at = min(16 * j, (p.N - 1 - n0) / 16 * 16);  // (sixteens behind the last column repeat the last)
+    b[j] = b0 + (size_t)at * row_pitch;
+    bs[j] = bs0 + (BBLOCK == 1 ? at : 0);
+  }
+  const dbg::Span aq_span = dbg::span_of(p.Aq), bq_span = dbg::span_of(p.Bq);  // (debug build only)
+  const int last = (p.N - 1 - n0) % 16;  // last row of B's last sixteen
+  const bool whole = n0 + 16 * NJ <= p.N;
+  int8_t* const mine = lds + wave * G::REGION;
+  for (int r0 = 0; r0 < rows; r0 += 16 * MI) {
+    v4f acc[MI][NJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    auto row_a = [&](int r) __attribute__((always_inline)) -> uint32_t {
+      if constexpr (MODE == SLOTS) {
+        if (p.gather) return (uint32_t)(MIAIE_LD(p.s.row_of + slot0 + r0 + r) / p.s.top_k);
+      }
+      return (uint32_t)(r0 + r);
+    };
+    auto row_b = [&](int r) __attribute__((always_inline)) -> uint32_t { return (uint32_t)(whole ? r : min(r, last)); };
+    multiply_rows<MI, NJ, BBLOCK>(mine, a, as, p.a_rows, b, bs, b_s_rows, row_pitch, (int)blocks(p.K), rows - r0, row_a, row_b, wave,
+                                  waves, aq_span, bq_span, acc);
+    if (waves > 1) {
+#pragma unroll
+      for (int f = 0; f < MI * NJ; ++f) *reinterpret_cast<v4f*>(mine + 1024 * f + 16 * lane) = acc[f / NJ][f % NJ];
+      __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < MI * NJ; ++u) {
+      if (u % waves != wave) continue;
+      v4f sum = acc[u / NJ][u % NJ];
+      if (waves > 1) {  // in the order of the waves, whichever of them adds
+        sum = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < waves; ++w) sum += *reinterpret_cast<const v4f*>(lds + w * G::REGION + 1024 * u + 16 * lane);
+      }
+      using T = std::conditional_t<OUT == OUT_F32, float, __bf16>;
+      store4(static_cast<T*>(p.C) + to, p.ldc, r0 + 16 * (u / NJ) + fr, n0 + 16 * (u % NJ) + 4 * fg, rows, p.N, sum);
+    }
+    if (r0 + 16 * MI < rows) __syncthreads();
+  }
+}
+
+// silu(gate) up of 128 columns of H and a block of slots, 16 rows at a time: eight
+// waves, each with 16 gate and 16 up columns over all of k.
+__global__ __launch_bounds__(512) void glu_rows(Args p, int tiles_n) {
+  using G = RowsGeom<1, 2>;
+  __shared__ __attribute__((aligned(1024))) int8_t lds[8 * G::REGION];
+  __shared__ uint32_t lmax[8][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int fr = lane & 15, fg = lane >> 4;
+  const uint32_t row_pitch = (uint32_t)pitch(p.K);
+  const size_t b_s_rows = blocks(2 * (long)p.N);
+  int block, tn, e;
+  if (!slot_tile(p.s, blockIdx.x, tiles_n, block, tn, e)) return;
+  const int slot0 = 128 * block, f0 = 128 * tn;
+  const int rows = min(128, MIAIE_LD(p.s.start + e) + MIAIE_LD(p.s.count + e) - slot0);
+  const uint8_t* a = p.gather ? p.Aq : p.Aq + (size_t)slot0 * row_pitch;
+  const float* as = p.gather ? p.As : p.As + slot0;
+  const uint8_t* const gate = p.Bq + ((size_t)e * 2 * p.N + f0 + 16 * wave) * row_pitch;
+  const uint8_t* const b[2] = {gate, gate + (size_t)p.N * row_pitch};
+  const float* const gate_s = p.Bs + (size_t)e * b_s_rows * blocks(p.K) + f0 / 128;
+  const float* const bs[2] = {gate_s, gate_s + p.N / 128};
+  const dbg::Span aq_span = dbg::span_of(p.Aq), bq_span = dbg::span_of(p.Bq);  // (debug build only)
+  const size_t h_pitch = pitch(p.N);
+  for (int r0 = 0; r0 < rows; r0 += 16) {
+    v4f acc[1][2] = {{v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}}};
+    auto row_a = [&](int r) __attribute__((always_inline)) -> uint32_t {
+      if (p.gather) return (uint32_t)(MIAIE_LD(p.s.row_of + slot0 + r0 + r) / p.s.top_k);
+      return (uint32_t)(r0 + r);
+    };
+    auto row_b = [&](int r) __attribute__((always_inline)) -> uint32_t { return (uint32_t)r; };
+    multiply_rows<1, 2, 128>(lds + wave * G::REGION, a, as, p.a_rows, b, bs, b_s_rows, row_pitch, (int)blocks(p.K), rows - r0, row_a,
+                             row_b, 0, 1, aq_span, bq_span, acc);
+    float h[4];
+    uint32_t m = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      h[x] = swiglu(acc[0][0][x], acc[0][1][x]);
+      m = max(m, abs_bits(h[x]));
+    }
+    m = max_over_16s(m);
+    if (fg == 0) lmax[wave][fr] = m;
+    __syncthreads();
+    m = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max(m, lmax[w][fr]);
+    const uint32_t ex = scale_of(m);
+    if (r0 + fr < rows) {
+      const size_t slot = slot0 + r0 + fr;
+      MIAIE_ST(reinterpret_cast<uint32_t*>(p.Hq + slot * h_pitch + f0 + 16 * wave + 4 * fg), pack4(h[0], h[1], h[2], h[3], inverse_f32(ex)));
+      if (wave == 0 && fg == 0) MIAIE_ST(p.Hs + (size_t)tn * p.M + slot, scale_f32(ex));
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- launches
+using Large = Tile<256, 256, 4, 2, 2>;
+using Block = Tile<128, 256, 2, 4, 3>;
+using Small = Tile<128, 128, 2, 2, 4>;
+
+template <class G, Mode MODE, Out OUT, int BBLOCK>
+int run_tile(miaie_ctx* ctx, const Args& p) {
+  const long tiles_m = (p.M + G::BM - 1l) / G::BM, cols = OUT == OUT_GLU ? G::BN / 2 : G::BN, tiles_n = (p.N + cols - 1) / cols;
+  long grid = tiles_m * tiles_n;
+  if (MODE == WGRAD) grid *= p.s.experts;
+  if (MODE == SLOTS) grid = (grid + 7) / 8 * 8;
+  const hipError_t e = launch<gemm_tile<G, MODE, OUT, BBLOCK>>(ctx->device, dim3((unsigned)grid), dim3(G::THREADS), 0, ctx->stream, p,
+                                                               (int)tiles_m, (int)tiles_n);
+  return check_launch(ctx, e, "gemm_fp8_tile");
+}
+
+template <int MI, int NJ, Mode MODE, Out OUT, int BBLOCK>
+int run_rows(miaie_ctx* ctx, const Args& p) {
+  using G = RowsGeom<MI, NJ>;
+  const int groups = ((int)blocks(p.K) + 1) / 2;
+  const int most = std::min(16, 163840 / G::REGION), each = (groups + most - 1) / most, waves = (groups + each - 1) / each;
+  const long tiles_n = (p.N + 16 * NJ - 1l) / (16 * NJ);
+  const long tiles_m = MODE == SLOTS ? p.M / 128 : (p.M + 16 * MI - 1l) / (16 * MI);
+  const long grid = MODE == SLOTS ? (tiles_m * tiles_n + 7) / 8 * 8 : tiles_m * tiles_n;
+  const hipError_t e = launch<gemm_rows<MI, NJ, MODE, OUT, BBLOCK>>(ctx->device, dim3((unsigned)grid), dim3(64 * waves),
+                                                                    (size_t)waves * G::REGION, ctx->stream, p, (int)tiles_n, waves);
+  return check_launch(ctx, e, "gemm_fp8_rows");
+}
+
+template <Out OUT, int BBLOCK>
+int run_dense(miaie_ctx* ctx, const Args& p) {
+  if (p.M <= 16) return run_rows<1, 1, DENSE, OUT, BBLOCK>(ctx, p);
+  const long large = ((p.M + 255l) / 256) * ((p.N + 255l) / 256);
+  if (large >= 128) return run_tile<Large, DENSE, OUT, BBLOCK>(ctx, p);
+  return run_tile<Small, DENSE, OUT, BBLOCK>(ctx, p);
+}
+
+// Few slots an expert: the waves of gemm_rows and glu_rows have more of B in flight.
+bool few_slots(const Args& p, int cols) {
+  return (long)p.s.tokens * p.s.top_k <= 16l * p.s.experts && p.M / 128 * ((p.N + cols - 1l) / cols) < 1l << 21;
+}
+
+template <Out OUT>
+int run_slots(miaie_ctx* ctx, const Args& p) {
+  if constexpr (OUT == OUT_GLU) {
+    if (few_slots(p, 128)) {
+      const long grid = ((long)p.M / 128 * (p.N / 128) + 7) / 8 * 8;
+      const hipError_t e = launch<glu_rows>(ctx->device, dim3((unsigned)grid), dim3(512), 0, ctx->stream, p, p.N / 128);
+      return check_launch(ctx, e, "glu_rows");
+    }
+  } else {
+    if (few_slots(p, 16)) return run_rows<1, 1, SLOTS, OUT, 128>(ctx, p);
+  }
+  return run_tile<Block, SLOTS, OUT, 128>(ctx, p);
+}
+
+}  // namespace
+
+int launch_gemm_fp8(miaie_ctx* ctx, const uint8_t* Aq, const float* As, const uint8_t* Bq, const float* Bs, int b_block,
+                    void* C, int dtype, int M, int N, int K, int ldc) {
+  const Args p{Aq, As, Bq, Bs, C, nullptr, nullptr, M, N, K, ldc, M, 0, Slots{}};
+  if (b_block == 1) return dtype == MIAIE_BF16 ? run_dense<OUT_BF16, 1>(ctx, p) : run_dense<OUT_F32, 1>(ctx, p);
+  return dtype == MIAIE_BF16 ? run_dense<OUT_BF16, 128>(ctx, p) : run_dense<OUT_F32, 128>(ctx, p);
+}
+
+int launch_experts_gemm_fp8(miaie_ctx* ctx, const fp8::Slots& s, const uint8_t* Aq, const float* As, int gather,
+                            const uint8_t* Bq, const float* Bs, void* C, int dtype, int N, int K, int ldc) {
+  const Args p{Aq, As, Bq, Bs, C, nullptr, nullptr, s.rows, N, K, ldc, gather ? s.tokens : s.rows, gather, s};
+  return dtype == MIAIE_BF16 ? run_slots<OUT_BF16>(ctx, p) : run_slots<OUT_F32>(ctx, p);
+}
+
+int launch_experts_glu_fp8(miaie_ctx* ctx, const fp8::Slots& s, const uint8_t* Xq, const float* Xs, const uint8_t* W1q,
+                           const float* W1s, uint8_t* Hq, float* Hs, int D, int F) {
+  const Args p{Xq, Xs, W1q, W1s, nullptr, Hq, Hs, s.rows, F, D, 0, s.tokens, 1, s};
+  return run_slots<OUT_GLU>(ctx, p);
+}
+
+int launch_experts_wgrad_fp8(miaie_ctx* ctx, const fp8::Slots& s, const uint8_t* Atq, const float* Ats, const uint8_t* Btq,
+                             const float* Bts, void* C, int dtype, int M, int N, int ldc) {
+  const Args p{Atq, Ats, Btq, Bts, C, nullptr, nullptr, M, N, s.rows, ldc, M, 0, s};
+  return dtype == MIAIE_BF16 ? run_tile<Large, WGRAD, OUT_BF16, 1>(ctx, p) : run_tile<Large, WGRAD, OUT_F32, 1>(ctx, p);
+}
+
+}  // namespace miaie

@@ -180,6 +180,41 @@ int launch_norm_block_grad(miaie_ctx* ctx, const void* r, const void* b, const v
                            void* db, float* dgate, float* dw_after, float* dw_before, float* work, int rows, int cols,
                            int ldx, int ldb, int gate_rows, int stream_dtype, int branch_dtype, float alpha);
 
+// 8-bit floating point (quant_fp8.hip, gemm_fp8.hip), routing and the experts'
+// slots (route_experts.hip); arguments as in miaie.h, checked by capi_experts.hip.
+namespace fp8 {
+struct Slots;
+}
+int launch_quant_fp8(miaie_ctx* ctx, const void* X, int dtype, int R, int C, int ldx, int block, uint8_t* Q, float* S,
+                     uint8_t* Qt, float* St);
+int launch_dequant_fp8(miaie_ctx* ctx, const uint8_t* Q, const float* S, int block, void* Y, int dtype, int R, int C,
+                       int ldy);
+int launch_gemm_fp8(miaie_ctx* ctx, const uint8_t* Aq, const float* As, const uint8_t* Bq, const float* Bs, int b_block,
+                    void* C, int dtype, int M, int N, int K, int ldc);
+int launch_route_experts(miaie_ctx* ctx, const void* logits, int dtype, const float* bias, int* idx, float* w, int tokens,
+                         int experts, int top_k, int ld, int scoring, int groups, int groups_kept, int group_top,
+                         int renormalize, float scale);
+int launch_route_experts_grad(miaie_ctx* ctx, const void* logits, int dtype, const int* idx, const float* dw, float* dlogits,
+                              int tokens, int experts, int top_k, int ld, int ldd, int scoring, int renormalize, float scale);
+int launch_experts_order(miaie_ctx* ctx, const fp8::Slots& s, const int* idx);
+int launch_experts_quant_fp8(miaie_ctx* ctx, const fp8::Slots& s, const void* X, int dtype, const float* w, int C, int ldx,
+                             uint8_t* Q, float* S, uint8_t* Qt, float* St);
+int launch_experts_swiglu_fp8(miaie_ctx* ctx, const fp8::Slots& s, const void* GU, int dtype, int F, int ldgu, uint8_t* Q,
+                              float* S, uint8_t* Qt, float* St);
+int launch_experts_swiglu_grad_fp8(miaie_ctx* ctx, const fp8::Slots& s, const void* GU, int dtype, const float* dH, int F,
+                                   int ldgu, int ldh, uint8_t* Q, float* S, uint8_t* Qt, float* St);
+int launch_experts_gemm_fp8(miaie_ctx* ctx, const fp8::Slots& s, const uint8_t* Aq, const float* As, int gather,
+                            const uint8_t* Bq, const float* Bs, void* C, int dtype, int N, int K, int ldc);
+// H = pack(silu(X . Wg^T) * (X . Wu^T)) of the tokens gathered into slots.
+int launch_experts_glu_fp8(miaie_ctx* ctx, const fp8::Slots& s, const uint8_t* Xq, const float* Xs, const uint8_t* W1q,
+                           const float* W1s, uint8_t* Hq, float* Hs, int D, int F);
+int launch_experts_wgrad_fp8(miaie_ctx* ctx, const fp8::Slots& s, const uint8_t* Atq, const float* Ats, const uint8_t* Btq,
+                             const float* Bts, void* C, int dtype, int M, int N, int ldc);
+int launch_experts_combine(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, const float* w, void* out, int dtype, int C,
+                           int ldy, int ldo);
+int launch_experts_combine_grad(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, const void* dout, float* dw, int dtype,
+                                int C, int ldy, int ldo);
+
 }  // namespace miaie
 
 // Vector types used by the MFMA builtins.

@@ -1,0 +1,494 @@
+// Routing of tokens to experts and its gradient, the order of the routed tokens'
+// slots, and the weighted sum over a token's slots with its gradient.
+#include <algorithm>
+
+#include "fp8.hpp"
+
+namespace miaie {
+namespace {
+
+using namespace fp8;
+
+// ---- reductions over a wave, the result in every lane
+template <class V>
+__device__ __forceinline__ V from_dpp(V v, int step) {
+  uint32_t w[sizeof(V) / 4];
+  __builtin_memcpy(w, &v, sizeof(V));
+#pragma unroll
+  for (uint32_t& x : w) {
+    switch (step) {
+      case 0: x = mx::quad_swap<0xB1>(x); break;   // lanes 1 0 3 2
+      case 1: x = mx::quad_swap<0x4E>(x); break;   // lanes 2 3 0 1
+      case 2: x = mx::quad_swap<0x141>(x); break;  // the other four of eight
+      default: x = mx::quad_swap<0x140>(x); break; // the other eight of sixteen
+    }
+  }
+  V r;
+  __builtin_memcpy(&r, w, sizeof(V));
+  return r;
+}
+template <class V, class Op>
+__device__ __forceinline__ V over_wave(V v, Op op) {
+#pragma unroll
+  for (int step = 0; step < 4; ++step) v = op(v, from_dpp(v, step));
+  // the other sixteen, then the other half: swapping a copy leaves one value in each
+#pragma unroll
+  for (int step = 0; step < 2; ++step) {
+    uint32_t a[sizeof(V) / 4], b[sizeof(V) / 4];
+    __builtin_memcpy(a, &v, sizeof(V));
+    __builtin_memcpy(b, &v, sizeof(V));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(V) / 4); ++i) {
+      if (step == 0)
+        swap16(a[i], b[i]);
+      else
+        swap32(a[i], b[i]);
+    }
+    V x, y;
+    __builtin_memcpy(&x, a, sizeof(V));
+    __builtin_memcpy(&y, b, sizeof(V));
+    v = op(x, y);
+  }
+  return v;
+}
+struct Max {
+  __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+  __device__ double operator()(double a, double b) const { return fmax(a, b); }
+};
+struct Add {
+  __device__ float operator()(float a, float b) const { return a + b; }
+  __device__ double operator()(double a, double b) const { return a + b; }
+};
+
+constexpr float kNone = -INFINITY;
+
+template <class T>
+__device__ __forceinline__ float load1(const T* p) {
+  return (float)MIAIE_LD(p);
+}
+
+// A score in 64 bits: two experts' may be next to each other, and the choice
+// between them must not depend on how an exponential is rounded.
+template <bool SIGMOID>
+__device__ __forceinline__ double score_of(float l, float largest, double total) {
+  if (SIGMOID) return 1.0 / (1.0 + exp(-(double)l));
+  return exp((double)l - (double)largest) / total;
+}
+
+struct RouteArgs {
+  const float* bias;
+  int* idx;
+  float* w;
+  int T, E, k, ld, groups, kept, group_top, renormalize;
+  float scale;
+};
+
+// A wave a token, expert lane + 64 p in a lane's p-th place: the experts that equal
+// the largest are found by a ballot a place, the lowest index first.  BY_SCORE: the
+// choice is score + bias in 64 bits, or groups are compared by sums of two; without
+// either the order of the logits is that of the scores, and only the chosen
+// experts' exponentials are needed.
+template <class T, int PER, bool SIGMOID, bool BY_SCORE>
+__global__ __launch_bounds__(256) void route_tokens(const T* __restrict__ logits, RouteArgs a) {
+  using V = std::conditional_t<BY_SCORE, double, float>;
+  __shared__ double lds[BY_SCORE ? 4 * 64 * PER : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blockIdx.x * 4 + wave;
+  if (t >= a.T) return;  // (no barriers: a wave's LDS is its own)
+  const T* row = logits + (size_t)t * a.ld;
+  float l[PER], largest = kNone;
+  bool nan = false;
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int e = lane + 64 * p;
+    l[p] = e < a.E ? load1(row + e) : kNone;
+  }
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    nan |= l[p] != l[p];
+    largest = fmaxf(largest, l[p]);
+  }
+  largest = over_wave(largest, Max{});
+  V c[PER];
+  double total = 1.0;
+  // (without renormalisation a softmax weight needs the sum too)
+  if (!SIGMOID && (BY_SCORE || !a.renormalize)) {
+    double sum = 0.0;
+#pragma unroll
+    for (int p = 0; p < PER; ++p) sum += l[p] > kNone ? exp((double)l[p] - (double)largest) : 0.0;
+    total = over_wave(sum, Add{});
+  }
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int e = lane + 64 * p;
+    if constexpr (BY_SCORE) {
+      c[p] = -(double)INFINITY;
+      if (l[p] != kNone && l[p] == l[p]) {
+        c[p] = score_of<SIGMOID>(l[p], largest, total) + (a.bias ? (double)MIAIE_LD(a.bias + e) : 0.0);
+        if (c[p] != c[p]) nan = true, c[p] = -(double)INFINITY;
+      }
+    } else {
+      c[p] = l[p] == l[p] ? l[p] : kNone;
+    }
+  }
+  // such a token's weights are all NaN (a sum over its slots is, too)
+  nan = __ballot(nan) != 0 || (!SIGMOID && largest == INFINITY);
+  if constexpr (BY_SCORE) {
+    if (a.groups > 1) {
+      double* mine = lds + wave * 64 * PER;
+      const int size = a.E / a.groups;
+#pragma unroll
+      for (int p = 0; p < PER; ++p) mine[lane + 64 * p] = c[p];
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      double of = -(double)INFINITY, second = -(double)INFINITY;
+      if (lane < a.groups)
+        for (int i = 0; i < size; ++i) {
+          // (lanes start at different members: a group's size is often a multiple of the banks)
+          int m = i + lane;
+          m = m < size ? m : m % size;
+          const double v = mine[lane * size + m];
+          second = fmax(second, fmin(of, v));
+          of = fmax(of, v);
+        }
+      if (a.group_top > 1 && second != -(double)INFINITY) of += second;
+      int better = 0;
+      for (int g = 0; g < a.groups; ++g) {
+        const double v = __shfl(of, g);
+        better += v > of || (v == of && g < lane);
+      }
+      const unsigned long long keep = __ballot(lane < a.groups && better < a.kept);
+#pragma unroll
+      for (int p = 0; p < PER; ++p) {
+        const int e = lane + 64 * p;
+        if (e < a.E && !(keep >> (e / size) & 1)) c[p] = -(double)INFINITY;
+      }
+    }
+  }
+  int chosen = -1;  // of lane j: the j-th expert
+  for (int j = 0; j < a.k; ++j) {
+    V best = c[0];
+#pragma unroll
+    for (int p = 1; p < PER; ++p) best = Max{}(best, c[p]);
+    best = over_wave(best, Max{});
+    if (best == (V)-INFINITY) break;
+    int e = -1;
+#pragma unroll
+    for (int p = PER - 1; p >= 0; --p) {
+      const unsigned long long has = __ballot(c[p] == best);
+      if (has) e = 64 * p + __builtin_ctzll(has);
+    }
+#pragma unroll
+    for (int p = 0; p < PER; ++p)
+      if (e == lane + 64 * p) c[p] = (V)-INFINITY;
+    if (lane == j) chosen = e;
+  }
+  double s = 0.0;
+  if (chosen >= 0) s = score_of<SIGMOID>(load1(row + chosen), largest, total);
+  if (a.renormalize) s /= over_wave(s, Add{}) + 1e-20;
+  if (lane < a.k) {
+    MIAIE_ST(a.idx + (size_t)t * a.k + lane, chosen);
+    MIAIE_ST(a.w + (size_t)t * a.k + lane, nan ? NAN : (float)(a.scale * s));
+  }
+}
+
+struct RouteGradArgs {
+  const int* idx;
+  const float* dw;
+  float* dlogits;
+  int T, E, k, ld, ldd, renormalize;
+  float scale;
+};
+
+// A wave a token.  With p the scores, w_j = scale p_j / P, P = sum of the chosen p
+// + 1e-20 (without renormalisation P = 1):
+//   dp_j = scale (dw_j - sum_i dw_i p_i / P) / P,
+//   sigmoid: dl_e = dp_e p_e (1 - p_e); softmax: dl_e = p_e (dp_e - sum_j dp_j p_j),
+// dp_e the sum over the choices of e.  The k choices are computed in 64 bits (their
+// differences cancel), the E experts in 32.
+template <class T, int PER, bool SIGMOID>
+__global__ __launch_bounds__(256) void route_tokens_grad(const T* __restrict__ logits, RouteGradArgs a) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int t = blockIdx.x * 4 + wave;
+  if (t >= a.T) return;
+  const T* row = logits + (size_t)t * a.ld;
+  float l[PER], p[PER], largest = kNone;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) l[i] = lane + 64 * i < a.E ? load1(row + lane + 64 * i) : kNone;
+  int e = -1;
+  float dw = 0.f, le = kNone;
+  if (lane < a.k) {
+    e = MIAIE_LD(a.idx + (size_t)t * a.k + lane);
+    if (e >= a.E) e = -1;
+    if (e >= 0) {
+      dw = MIAIE_LD(a.dw + (size_t)t * a.k + lane);
+      le = load1(row + e);
+    }
+  }
+  double total = 1.0;
+  if (SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) p[i] = 1.f / (1.f + expf(-l[i]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) largest = fmaxf(largest, l[i]);
+    largest = over_wave(largest, Max{});
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      p[i] = l[i] == kNone ? 0.f : expf(l[i] - largest);
+      sum += p[i];
+    }
+    total = over_wave((double)sum, Add{});
+#pragma unroll
+    for (int i = 0; i < PER; ++i) p[i] = l[i] == kNone ? 0.f : p[i] / (float)total;
+  }
+  const double pe = e >= 0 && le != kNone ? score_of<SIGMOID>(le, largest, total) : 0.0;
+  double dp = a.scale * (double)dw;
+  if (a.renormalize) {
+    const double sum = over_wave(pe, Add{}) + 1e-20, dot = over_wave(dw * pe, Add{});
+    dp = a.scale * (dw - dot / sum) / sum;
+  }
+  if (e < 0) dp = 0.0;
+  const float inner = SIGMOID ? 0.f : (float)over_wave(dp * pe, Add{});
+  float d[PER] = {};
+  for (int j = 0; j < a.k; ++j) {
+    const int ej = __shfl(e, j);
+    const float dj = __shfl((float)dp, j);
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (ej == lane + 64 * i) d[i] += dj;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (lane + 64 * i >= a.E) continue;
+    float dl;
+    if (SIGMOID) {  // p (1 - p) = x / (1 + x)^2, x = e^-|l|
+      const float x = expf(-fabsf(l[i]));
+      dl = d[i] * (x / ((1.f + x) * (1.f + x)));
+    } else {
+      dl = p[i] * (d[i] - inner);
+    }
+    MIAIE_ST(a.dlogits + (size_t)t * a.ldd + lane + 64 * i, dl);
+  }
+}
+
+// ---------------------------------------------------------------- the slots' order
+// A stable counting sort by one workgroup: wave w counts its run of the pairs, the
+// experts' counts become their first slots, and each wave places its pairs in turn,
+// 64 at a time, a pair behind those of the same expert in lower lanes.
+constexpr int kOrderWaves = 16;
+__global__ __launch_bounds__(64 * kOrderWaves) void order_slots(const int* __restrict__ idx, int* __restrict__ start,
+                                                                int* __restrict__ count, int* __restrict__ slot_of,
+                                                                int* __restrict__ row_of, int* __restrict__ expert_of,
+                                                                int pairs, int experts, int rows, int bits) {
+  extern __shared__ int at[];  // [waves][experts]: a wave's count of an expert, then its next slot
+  __shared__ int wave_sum[kOrderWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  for (int i = tid; i < kOrderWaves * experts; i += 64 * kOrderWaves) at[i] = 0;
+  for (int i = tid; i < rows / 128; i += 64 * kOrderWaves) MIAIE_ST(expert_of + i, -1);
+  __syncthreads();
+  const int each = (pairs + 64 * kOrderWaves - 1) / (64 * kOrderWaves) * 64, first = wave * each,
+            last = min(pairs, first + each);
+  for (int i = first + lane; i < last; i += 64) {
+    const int e = MIAIE_LD(idx + i);
+    if (e >= 0 && e < experts) atomicAdd(at + wave * experts + e, 1);
+  }
+  __syncthreads();
+  // thread e: the expert's pairs in each wave, and its place among the experts
+  int n = 0;
+  if (tid < experts)
+    for (int w = 0; w < kOrderWaves; ++w) n += at[w * experts + tid];
+  const int padded = (n + 127) / 128 * 128;
+  int upto = padded;
+  for (int d = 1; d < 64; d *= 2) {
+    const int v = __shfl_up(upto, d);
+    if (lane >= d) upto += v;
+  }
+  if (lane == 63) wave_sum[wave] = upto;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) upto += wave_sum[w];
+  const int begin = upto - padded;
+  if (tid < experts) {
+    MIAIE_ST(start + tid, begin);
+    MIAIE_ST(count + tid, n);
+    if (tid == experts - 1) MIAIE_ST(start + experts, upto);
+    for (int b = begin / 128; b < upto / 128; ++b) MIAIE_ST(expert_of + b, tid);
+    for (int r = begin + n; r < upto; ++r) MIAIE_ST(row_of + r, -1);
+    int next = begin;
+    for (int w = 0; w < kOrderWaves; ++w) {
+      const int c = at[w * experts + tid];
+      at[w * experts + tid] = next;
+      next += c;
+    }
+  }
+  __syncthreads();
+  for (int i0 = first; i0 < last; i0 += 64) {
+    const int i = i0 + lane;
+    int e = i < last ? MIAIE_LD(idx + i) : -1;
+    if (e >= experts) e = -1;
+    unsigned long long same = __ballot(e >= 0);
+    for (int b = 0; b < bits; ++b) {
+      const unsigned long long has = __ballot(e >> b & 1);
+      same &= (e >> b & 1) ? has : ~has;
+    }
+    int slot = -1;
+    if (e >= 0) {
+      const int before = __popcll(same & ((1ull << lane) - 1)), base = at[wave * experts + e];
+      slot = base + before;
+      MIAIE_ST(row_of + slot, i);
+      // (every lane has read its expert's place: one instruction for the wave)
+      if (before == 0) at[wave * experts + e] = base + __popcll(same);
+    }
+    if (i < last) MIAIE_ST(slot_of + i, slot);
+  }
+}
+
+// out[t] = sum over the choices j, in their order, of w[t][j] Y[slot]: eight columns
+// a thread.
+template <class T>
+__global__ __launch_bounds__(256) void combine(const T* __restrict__ Y, const float* __restrict__ w, T* __restrict__ out,
+                                               Slots s, int C, int ldy, int ldo, int per_row, long units, long stride) {
+  for (long u = blockIdx.x * 256l + threadIdx.x; u < units; u += stride) {
+    const int t = (int)(u / per_row), c = 8 * (int)(u % per_row);
+    float sum[8] = {};
+    for (int j0 = 0; j0 < s.top_k; j0 += 4) {
+      float y[4][8] = {}, f[4] = {};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j0 + j >= s.top_k) continue;
+        const size_t pair = (size_t)t * s.top_k + j0 + j;
+        const int slot = MIAIE_LD(s.slot_of + pair);
+        f[j] = w ? MIAIE_LD(w + pair) : 1.f;  // (NaN without a slot too)
+        if (slot >= 0) mx::load8(Y + (size_t)slot * ldy + c, C - c, y[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum[i] = __builtin_fmaf(f[j], y[j][i], sum[i]);
+    }
+    mx::store8(out + (size_t)t * ldo + c, C - c, sum);
+  }
+}
+
+// dw[t][j] = <dout[t], Y[slot]>, a wave a pair; 0 without an expert.
+template <class T>
+__global__ __launch_bounds__(256) void combine_grad(const T* __restrict__ Y, const T* __restrict__ dout,
+                                                    float* __restrict__ dw, Slots s, int C, int ldy, int ldo, int pairs) {
+  const int lane = threadIdx.x & 63;
+  const int pair = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (pair >= pairs) return;
+  const int slot = MIAIE_LD(s.slot_of + pair);
+  float sum = 0.f;
+  if (slot >= 0)
+    for (int c = 8 * lane; c < C; c += 512) {
+      float y[8], d[8];
+      mx::load8(Y + (size_t)slot * ldy + c, C - c, y);
+      mx::load8(dout + (size_t)(pair / s.top_k) * ldo + c, C - c, d);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(y[i], d[i], sum);
+    }
+  sum = over_wave(sum, Add{});
+  if (lane == 0) MIAIE_ST(dw + pair, sum);
+}
+
+// f(type of the logits, number of a lane's places)
+template <class F>
+int with_experts(int dtype, int E, F&& f) {
+  auto go = [&](auto t) {
+    if (E <= 64) return f(t, std::integral_constant<int, 1>{});
+    if (E <= 128) return f(t, std::integral_constant<int, 2>{});
+    if (E <= 256) return f(t, std::integral_constant<int, 4>{});
+    if (E <= 512) return f(t, std::integral_constant<int, 8>{});
+    return f(t, std::integral_constant<int, 16>{});
+  };
+  return dtype == MIAIE_BF16 ? go(type_t<__bf16>{}) : go(type_t<float>{});
+}
+
+}  // namespace
+
+int launch_route_experts(miaie_ctx* ctx, const void* logits, int dtype, const float* bias, int* idx, float* w, int tokens,
+                         int experts, int top_k, int ld, int scoring, int groups, int groups_kept, int group_top,
+                         int renormalize, float scale) {
+  const RouteArgs a{bias, idx, w, tokens, experts, top_k, ld, groups, groups_kept, group_top, renormalize, scale};
+  return with_experts(dtype, experts, [&](auto t, auto per) {
+    using T = typename decltype(t)::type;
+    constexpr int PER = decltype(per)::value;
+    hipError_t e = hipSuccess;
+    auto go = [&](auto k) {
+      e = launch<decltype(k)::value>(ctx->device, dim3((tokens + 3u) / 4), dim3(256), 0, ctx->stream,
+                                     static_cast<const T*>(logits), a);
+    };
+    const bool by_score = bias || groups > 1;
+    if (scoring == MIAIE_SIGMOID) {
+      if (by_score)
+        go(kernel_t<route_tokens<T, PER, true, true>>{});
+      else
+        go(kernel_t<route_tokens<T, PER, true, false>>{});
+    } else {
+      if (by_score)
+        go(kernel_t<route_tokens<T, PER, false, true>>{});
+      else
+        go(kernel_t<route_tokens<T, PER, false, false>>{});
+    }
+    return check_launch(ctx, e, "route_tokens");
+  });
+}
+
+int launch_route_experts_grad(miaie_ctx* ctx, const void* logits, int dtype, const int* idx, const float* dw, float* dlogits,
+                              int tokens, int experts, int top_k, int ld, int ldd, int scoring, int renormalize,
+                              float scale) {
+  const RouteGradArgs a{idx, dw, dlogits, tokens, experts, top_k, ld, ldd, renormalize, scale};
+  return with_experts(dtype, experts, [&](auto t, auto per) {
+    using T = typename decltype(t)::type;
+    constexpr int PER = decltype(per)::value;
+    const dim3 grid((tokens + 3u) / 4);
+    const T* l = static_cast<const T*>(logits);
+    const hipError_t e = scoring == MIAIE_SIGMOID
+                             ? launch<route_tokens_grad<T, PER, true>>(ctx->device, grid, dim3(256), 0, ctx->stream, l, a)
+                             : launch<route_tokens_grad<T, PER, false>>(ctx->device, grid, dim3(256), 0, ctx->stream, l, a);
+    return check_launch(ctx, e, "route_tokens_grad");
+  });
+}
+
+int launch_experts_order(miaie_ctx* ctx, const fp8::Slots& s, const int* idx) {
+  int bits = 0;
+  while (1 << bits < s.experts) ++bits;
+  const hipError_t e = launch<order_slots>(ctx->device, dim3(1), dim3(64 * kOrderWaves), sizeof(int) * kOrderWaves * s.experts,
+                                           ctx->stream, idx, const_cast<int*>(s.start), const_cast<int*>(s.count),
+                                           const_cast<int*>(s.slot_of), const_cast<int*>(s.row_of),
+                                           const_cast<int*>(s.expert_of), s.tokens * s.top_k, s.experts, s.rows, bits);
+  return check_launch(ctx, e, "order_slots");
+}
+
+int launch_experts_combine(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, const float* w, void* out, int dtype, int C,
+                           int ldy, int ldo) {
+  const int per_row = (C + 7) / 8;
+  const long units = (long)s.tokens * per_row, grid = std::min((units + 255) / 256, 1l << 22);
+  auto go = [&](auto t) {
+    using T = typename decltype(t)::type;
+    return check_launch(ctx,
+                        launch<combine<T>>(ctx->device, dim3((unsigned)grid), dim3(256), 0, ctx->stream,
+                                           static_cast<const T*>(Y), w, static_cast<T*>(out), s, C, ldy, ldo, per_row, units,
+                                           256 * grid),
+                        "experts_combine");
+  };
+  return dtype == MIAIE_BF16 ? go(type_t<__bf16>{}) : go(type_t<float>{});
+}
+
+int launch_experts_combine_grad(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, const void* dout, float* dw, int dtype,
+                                int C, int ldy, int ldo) {
+  const int pairs = s.tokens * s.top_k;
+  auto go = [&](auto t) {
+    using T = typename decltype(t)::type;
+    return check_launch(ctx,
+                        launch<combine_grad<T>>(ctx->device, dim3((pairs + 3u) / 4), dim3(256), 0, ctx->stream,
+                                                static_cast<const T*>(Y), static_cast<const T*>(dout), dw, s, C, ldy, ldo,
+                                                pairs),
+                        "experts_combine_grad");
+  };
+  return dtype == MIAIE_BF16 ? go(type_t<__bf16>{}) : go(type_t<float>{});
+}
+
+}  // namespace miaie

@@ -422,6 +422,173 @@ MIAIE_API int miaie_norm_block_grad(miaie_ctx* ctx, const void* r, const void* b
                                     float* dw_before, void* work, size_t work_bytes, int rows, int cols, int ldx,
                                     int ldb, int gate_rows, int stream_dtype, int branch_dtype, float alpha);
 
+/* ---- 8-bit floating point with a scale for each block of 128 -------------- */
+
+/* No counterpart in the reference.  A packed matrix of R rows and K columns is
+ * two device arrays, both 16-byte aligned and dense:
+ *   Q  uint8 [R][miaie_fp8_q_pitch(K)]: E4M3 elements (OCP: up to 448, no
+ *      infinities), rows of whole 128-byte lines, zero behind column K;
+ *   S  fp32 [ceil(K / 128)][ceil(R / block)]: the scale of 128 columns of `block`
+ *      rows, block 1 (activations and gradients) or 128 (weights).
+ * Products read any fp32 scale of a 128 x 128 block, and of A beside it; two
+ * operands that both have a scale a row (b_block 1) need powers of two from
+ * 2^-126 to 2^127 or NaN, as miaie_quant_fp8 makes them (of others the exponent
+ * is taken).  The product of two scales is taken in fp32.
+ * R and C of a matrix in [1, 2^30] with ceil(R / 128) ceil(C / 128) below 2^24; M
+ * and N of a product in [1, 2^25] with ceil(M / 256) ceil(N / 256) below 2^23, K
+ * in [1, 2^23]. */
+
+/* Bytes of a row of Q, and of the arrays Q and S, of an R x K matrix (0 for
+ * arguments outside the ranges above).  Host functions. */
+MIAIE_API size_t miaie_fp8_q_pitch(int K);
+MIAIE_API size_t miaie_fp8_q_bytes(int R, int K);
+MIAIE_API size_t miaie_fp8_s_bytes(int R, int K, int block);
+
+/* Packs X (R x C row major, row pitch ldx >= C elements, of type dtype: MIAIE_F32,
+ * MIAIE_BF16).  Along its rows into Q, S (an R x C packed matrix), and / or along
+ * its columns into Qt, St (the packed transpose, C x R); either pair may be NULL.
+ * A block's scale is the smallest power of two that its largest magnitude is at
+ * most 448 times, at least 2^-126; its elements are rounded to nearest, halves to
+ * the even code.  A block that holds an infinity or NaN gets scale NaN: all of it
+ * is NaN, whatever its codes.  With block 128 both forms have the same codes and
+ * scales. */
+MIAIE_API int miaie_quant_fp8(miaie_ctx* ctx, const void* X, int dtype, int R, int C, int ldx, int block, uint8_t* Q,
+                              float* S, uint8_t* Qt, float* St);
+
+/* Y = the values (element times scale, rounded to Y's type) of a packed R x C
+ * matrix, row major with row pitch ldy >= C elements, of type dtype. */
+MIAIE_API int miaie_dequant_fp8(miaie_ctx* ctx, const uint8_t* Q, const float* S, int block, void* Y, int dtype, int R,
+                                int C, int ldy);
+
+/* C[m][n] = sum over k of A[m][k] B[n][k]: A (Aq, As; block 1) M x K and B (Bq,
+ * Bs; block b_block) N x K packed along k, fp32 accumulation, C of type dtype with
+ * row pitch ldc >= N elements.  A linear layer Y = X . W^T with W in blocks of
+ * 128 x 128: forward A = X, B = W; dX: A = dY, B = the packed transpose of W;
+ * dW = dY^T . X: A and B the packed transposes of dY and X, b_block 1. */
+MIAIE_API int miaie_gemm_fp8(miaie_ctx* ctx, const uint8_t* Aq, const float* As, const uint8_t* Bq, const float* Bs,
+                             int b_block, void* C, int dtype, int M, int N, int K, int ldc);
+
+/* ---- routing of tokens to experts ----------------------------------------- */
+
+/* No counterpart in the reference.  logits: tokens x experts, row pitch ld, of type
+ * dtype.  An expert's score is the softmax of its token's logits, or the sigmoid of
+ * its own; bias (NULL: 0; fp32 [experts]) is added to the score for the choice
+ * alone.  The experts are `groups` runs of as many; with more than one group, the
+ * groups_kept best stay, a group being as good as the sum of its group_top (1 or 2;
+ * fewer if it has fewer) best choices.  Of those that stay the top_k best are
+ * written to idx (int32 tokens x top_k, dense), best first, equals by the lower
+ * index, and
+ *   w[j] = scale * score[j] / (sum of the token's chosen scores + 1e-20)
+ * (scale * score[j] if renormalize is 0) to w (fp32 tokens x top_k).  Scores are
+ * computed and compared in 64 bits.
+ * An expert whose logit (or bias) is -infinity is never chosen; where a token has
+ * fewer than top_k others, idx is -1 and w 0 for the rest (all of them for the
+ * padding of a batch).  A NaN among a token's logits or in the choice of an expert
+ * that may be chosen, and +infinity under a softmax, make all its weights NaN; an
+ * expert whose choice is NaN is not chosen.
+ * tokens in [1, 2^25], experts in [1, MIAIE_MAX_EXPERTS], top_k in [1,
+ * MIAIE_MAX_TOP_K], groups in [1, 64] and a divisor of experts, groups_kept in [1,
+ * groups], top_k at most the experts of the groups that stay. */
+#define MIAIE_SOFTMAX 0
+#define MIAIE_SIGMOID 1
+#define MIAIE_MAX_EXPERTS 1024
+#define MIAIE_MAX_TOP_K 64
+MIAIE_API int miaie_route_experts(miaie_ctx* ctx, const void* logits, int dtype, const float* bias, int* idx, float* w,
+                                  int tokens, int top_k, int experts, int ld, int scoring, int groups, int groups_kept,
+                                  int group_top, int renormalize, float scale);
+
+/* Its gradient: dlogits (fp32, tokens x experts, row pitch ldd; every element is
+ * written) from dw (fp32 tokens x top_k), for the choice in idx (entries outside
+ * [0, experts) are no expert; one that is there twice counts twice).  The choice
+ * itself and the bias have none. */
+MIAIE_API int miaie_route_experts_grad(miaie_ctx* ctx, const void* logits, int dtype, const int* idx, const float* dw,
+                                       float* dlogits, int tokens, int top_k, int experts, int ld, int ldd, int scoring,
+                                       int renormalize, float scale);
+
+/* ---- the experts' products ------------------------------------------------- */
+
+/* No counterpart in the reference.  A slot is a row of a (token, choice) pair's
+ * own; slots are sorted by expert, each expert's from a multiple of 128 on in the
+ * order of its pairs.  Matrices over slots have miaie_experts_rows rows, whatever
+ * the routing; rows of padding and behind the last slot in use are neither read nor
+ * written unless it says so below.  The order is one device array of int32,
+ * miaie_experts_order_bytes long, with the parts
+ *   start [experts + 1]  first slot of each expert; the last: slots in use;
+ *   count [experts]      slots of each expert; the part ends at a multiple of 16;
+ *   slot [tokens][top_k] slot of a pair, -1 without an expert; ends at such too;
+ *   pair [rows]          token * top_k + choice of a slot, -1 in padding, not
+ *                        written behind the slots in use;
+ *   expert [rows / 128]  of 128 slots each, -1 behind those in use.
+ * tokens * top_k in [1, 2^23], experts in [1, MIAIE_MAX_EXPERTS], top_k in [1,
+ * MIAIE_MAX_TOP_K]; sizes of a row in [1, 2^20]. */
+MIAIE_API size_t miaie_experts_rows(int tokens, int top_k, int experts);
+MIAIE_API size_t miaie_experts_order_bytes(int tokens, int top_k, int experts);
+
+/* The order of idx (int32 tokens x top_k; entries outside [0, experts) get no
+ * slot, one that a token has twice gets two).  What reads an order below takes the
+ * tokens, top_k and experts it was made with. */
+MIAIE_API int miaie_experts_order(miaie_ctx* ctx, const int* idx, int* order, int tokens, int top_k, int experts);
+
+/* The MLP of each token's experts and their weighted sum:
+ *   H[slot] = pack(silu(X[t] . Wg^T) * (X[t] . Wu^T)),  Y[slot] = H[slot] . W2^T,
+ *   out[t]  = sum over its slots, in the order of its choices, of w * Y[slot]
+ * X tokens x D packed along its rows (block 1).  W1: the experts' 2 F x D matrices,
+ * gate rows then up rows, each packed with block 128, one after another; W2 likewise
+ * Nout x F.  F is a multiple of 128 (pad with zero rows of W1).  H (Hq, Hs: packed,
+ * rows x F) and Y (rows x Nout, dense, of type dtype, to which it is rounded) are
+ * caller-provided device scratch; out, tokens x Nout of type dtype, row pitch ldo.
+ * Gate, up and their product stay in fp32 until H is packed.  tokens times a packed
+ * row of X, and 2 F times one, are below 2^32 bytes. */
+MIAIE_API int miaie_experts_mlp_fp8(miaie_ctx* ctx, const int* order, const float* w, const uint8_t* Xq, const float* Xs,
+                                    const uint8_t* W1q, const float* W1s, const uint8_t* W2q, const float* W2s,
+                                    uint8_t* Hq, float* Hs, void* Y, void* out, int dtype, int tokens, int top_k,
+                                    int experts, int D, int F, int Nout, int ldo);
+
+/* The parts of a step that trains them.  A product over slots, C[slot] = A[slot] .
+ * B_e^T: A rows x K, or with gather != 0 tokens x K (tokens times a packed row below
+ * 2^32 bytes), packed with block 1; B the experts' N x K matrices packed with block
+ * 128, one after another; C rows x N of type dtype, row pitch ldc. */
+MIAIE_API int miaie_experts_gemm_fp8(miaie_ctx* ctx, const int* order, const uint8_t* Aq, const float* As,
+                                     const uint8_t* Bq, const float* Bs, void* C, int dtype, int tokens, int top_k,
+                                     int experts, int N, int K, int ldc, int gather);
+
+/* Rows of X (tokens x C, row pitch ldx, of type dtype), times w (fp32 tokens x top_k;
+ * NULL: 1), packed by slot along the rows (Q, S: rows x C) and / or along the
+ * slots (Qt, St: C x rows), block 1, as miaie_quant_fp8 does.  Padding up to the
+ * last slot in use is zero; behind it nothing is written. */
+MIAIE_API int miaie_experts_quant_fp8(miaie_ctx* ctx, const int* order, const void* X, int dtype, const float* w,
+                                      uint8_t* Q, float* S, uint8_t* Qt, float* St, int tokens, int top_k, int experts,
+                                      int C, int ldx);
+
+/* silu(gate) * up of GU (rows x 2 F, gate columns then up columns, row pitch ldgu, of
+ * type dtype) packed likewise (rows x F, F x rows). */
+MIAIE_API int miaie_experts_swiglu_fp8(miaie_ctx* ctx, const int* order, const void* GU, int dtype, uint8_t* Q, float* S,
+                                       uint8_t* Qt, float* St, int tokens, int top_k, int experts, int F, int ldgu);
+
+/* Its gradient, of dH (fp32, rows x F, row pitch ldh) with respect to GU, packed
+ * likewise (rows x 2 F, 2 F x rows). */
+MIAIE_API int miaie_experts_swiglu_grad_fp8(miaie_ctx* ctx, const int* order, const void* GU, int dtype, const float* dH,
+                                            uint8_t* Q, float* S, uint8_t* Qt, float* St, int tokens, int top_k,
+                                            int experts, int F, int ldgu, int ldh);
+
+/* Each expert's dW = sum over its slots of A[m][slot] B[n][slot]: At M x rows and Bt
+ * N x rows packed along the slots (block 1, scales powers of two), C experts x M x N
+ * of type dtype, row pitch ldc (an expert's rows follow the one's before); zeros for
+ * an expert without slots. */
+MIAIE_API int miaie_experts_wgrad_fp8(miaie_ctx* ctx, const int* order, const uint8_t* Atq, const float* Ats,
+                                      const uint8_t* Btq, const float* Bts, void* C, int dtype, int tokens, int top_k,
+                                      int experts, int M, int N, int ldc);
+
+/* out[t] = sum over its slots, in the order of its choices, of w * Y[slot] (w NULL:
+ * of Y[slot]), fp32 sums: Y rows x C, row pitch ldy, out tokens x C, row pitch ldo,
+ * both of type dtype.  A pair without a slot adds w * 0. */
+MIAIE_API int miaie_experts_combine(miaie_ctx* ctx, const int* order, const void* Y, const float* w, void* out, int dtype,
+                                    int tokens, int top_k, int experts, int C, int ldy, int ldo);
+/* dw (fp32 tokens x top_k) of it: dw = <dout[t], Y[slot]>, 0 without a slot.  (The
+ * gradient of Y is dout times w: miaie_experts_quant_fp8.) */
+MIAIE_API int miaie_experts_combine_grad(miaie_ctx* ctx, const int* order, const void* Y, const void* dout, float* dw,
+                                         int dtype, int tokens, int top_k, int experts, int C, int ldy, int ldo);
+
 /* ---- synthetic inputs --------------------------------------------------- */
 
 /* Fill dst[0..n) with the seeded int8 stream of tensor `tensor_id`
