@@ -118,21 +118,49 @@ __device__ __forceinline__ void store4(T* C, size_t ldc, int m, int n, int M, in
 }
 
 // ---------------------------------------------------------------- large tiles
-// A workgroup of WAVES_M x WAVES_N waves owns a BM x BN tile, a wave NI x NJ blocks
-// of 16 x 16.  A step is 128 k: whole 128-byte lines of BM + BN rows and their
-// scales, copied into one of STAGES stages of LDS with no registers in between.
-template <int BM_, int BN_, int WAVES_M_, int WAVES_N_, int STAGES_>
+// A workgroup of eight waves owns a BM x BN tile, a wave NI x NJ blocks of 16 x 16.
+// A step is 128 k: whole 128-byte lines of BM + BN rows and their scales, copied
+// into one of STAGES stages of LDS with no registers in between.  A wave keeps its
+// rows' fragments of A through a step and takes those of B column by column.
+//
+// Waves 0-3 (group 0, one on each SIMD) have the first half of B's columns, waves
+// 4-7 the second, half a step behind: while the one group begins a step, with all of
+// A's fragments to read, the matrix units have the middle of the other's.  (All eight
+// in step: 3200 cycles a step of 256 x 256 for 2062 of matrix instructions, whichever
+// number of workgroups runs.)  Two barriers a step:
+//   E0(t), group 0 at the end of its step t, group 1 in the middle of its own: all of
+//     A and the first half of B of step t + 1 are there, B's first half of step t has
+//     been read, and A of step t by both groups, so both take the copies of step
+//     t + STAGES;
+//   E1(t), group 0 in the middle of step t + 1, group 1 at the end of t: the same of
+//     B's second half.
+template <int BM_, int BN_, int WAVES_M_, int STAGES_>
 struct Tile {
-  static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = WAVES_N_, STAGES = STAGES_;
-  static constexpr int WAVES = WAVES_M * WAVES_N, THREADS = 64 * WAVES;
+  static constexpr int BM = BM_, BN = BN_, WAVES_M = WAVES_M_, WAVES_N = 8 / WAVES_M, STAGES = STAGES_;
+  static constexpr int WAVES = 8, THREADS = 512;
   static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, NI = WM / 16, NJ = WN / 16;
   static constexpr int A = 0, B = BM * 128, S = B + BN * 128, STAGE = S + 4 * (BM + BN);
-  static constexpr int A_CP = BM / 8 / WAVES, B_CP = BN / 8 / WAVES;  // copies of a wave in a step
-  static constexpr int S_CP = ((BM + BN) / 64 + WAVES - 1) / WAVES, CP = A_CP + B_CP + S_CP;
+  static constexpr int A_CP = BM / 64, B_CP = BN / 128;  // a wave's copies of A, and of half of B
+  static constexpr int C0 = A_CP + B_CP + 1, C1 = B_CP + 1;  // ... sent after E0 and E1, one of scales in each
   static constexpr int LDS = STAGES * STAGE;
-  static_assert(A_CP >= 1 && B_CP >= 1 && BM % 64 == 0 && BN % 64 == 0 && STAGE % 128 == 0, "copies of whole waves");
+  static_assert(BM % 64 == 0 && BN % 128 == 0 && WAVES_N % 2 == 0 && BM / 64 + BN / 128 <= 8 && STAGE % 128 == 0, "copies of whole waves");
   static_assert(LDS <= 163840, "LDS of a CU");
+  // group 1 has the second half of the columns
+  __device__ static __forceinline__ int wm(int wave) { return (wave & 3) % WAVES_M; }
+  __device__ static __forceinline__ int wn(int wave) { return (wave >> 2) * (WAVES_N / 2) + (wave & 3) / WAVES_M; }
 };
+
+// Waits for what an event makes visible; `left` steps follow the one it is about
+// (t + 1).  Copies that may still be in flight: those sent after it.
+template <class G, int EVENT, int LEFT = G::STAGES - 1>
+__device__ __forceinline__ void wait_event(int left) {
+  constexpr int S = G::STAGES;
+  if constexpr (LEFT > 0) {
+    if (left < LEFT) return wait_event<G, EVENT, LEFT - 1>(left);
+  }
+  constexpr int a = LEFT < S - 2 ? LEFT : S - 2, b = LEFT + (EVENT == 0) < S - 1 ? LEFT + (EVENT == 0) : S - 1;
+  dev::wait_vmcnt<EVENT == 0 ? a * G::C0 + b * G::C1 : b * G::C0 + a * G::C1>();
+}
 
 // Where a tile's operands are: wave-uniform addresses of step 0, a row's offset for
 // each of a wave's copies.
@@ -151,43 +179,57 @@ __device__ __forceinline__ void multiply(int8_t* lds, const Operands& o, uint32_
   constexpr int NI = G::NI, NJ = G::NJ;
   const uint32_t lds0 = dev::lds_addr(lds);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / G::WAVES_N, wn = wave % G::WAVES_N, fr = lane & 15, fg = lane >> 4;
+  const int wm = G::wm(wave), wn = G::wn(wave), fr = lane & 15, fg = lane >> 4;
 
-  uint32_t a_off[G::A_CP], b_off[G::B_CP], s_off[G::S_CP];
+  uint32_t a_off[G::A_CP], b_off[2][G::B_CP], s_off[2];
 #pragma unroll
   for (int x = 0; x < G::A_CP; ++x) {
-    const int r = 8 * (G::WAVES * x + wave) + (lane >> 3);
+    const int r = 8 * (8 * x + wave) + (lane >> 3);
     a_off[x] = row_a(r) * a_pitch + 16 * ((lane & 7) ^ swz(r));
   }
 #pragma unroll
-  for (int x = 0; x < G::B_CP; ++x) {
-    const int r = 8 * (G::WAVES * x + wave) + (lane >> 3);
-    b_off[x] = row_b(r) * b_pitch + 16 * ((lane & 7) ^ swz(r));
-  }
-  // (scales: every wave makes the same number of copies, the last ones again)
-  int s_row[G::S_CP];
+  for (int h = 0; h < 2; ++h)
 #pragma unroll
-  for (int x = 0; x < G::S_CP; ++x) {
-    s_row[x] = 64 * ((G::WAVES * x + wave) % ((G::BM + G::BN) / 64));
-    s_off[x] = 4 * (s_row[x] < G::BM ? row_a(s_row[x] + lane) : scale_b(s_row[x] - G::BM + lane));
-  }
-  const uint8_t *a_src = o.a, *b_src = o.b;
-  const float *as_src = o.as, *bs_src = o.bs;
-  auto copy = [&](uint32_t st) __attribute__((always_inline)) {  // the next step's operands
-#pragma unroll
-    for (int x = 0; x < G::A_CP; ++x)
-      dev::gload_lds16(a_src, a_off[x], lds0 + st + G::A + 1024 * (G::WAVES * x + wave), aq_span);
-#pragma unroll
-    for (int x = 0; x < G::B_CP; ++x)
-      dev::gload_lds16(b_src, b_off[x], lds0 + st + G::B + 1024 * (G::WAVES * x + wave), bq_span);
-#pragma unroll
-    for (int x = 0; x < G::S_CP; ++x) {
-      if (s_row[x] < G::BM)
-        dev::gload_lds4(as_src, s_off[x], lds0 + st + G::S + 4 * s_row[x], as_span);
-      else
-        dev::gload_lds4(bs_src, s_off[x], lds0 + st + G::S + 4 * s_row[x], bs_span);
+    for (int x = 0; x < G::B_CP; ++x) {
+      const int r = h * (G::BN / 2) + 8 * (8 * x + wave) + (lane >> 3);
+      b_off[h][x] = row_b(r) * b_pitch + 16 * ((lane & 7) ^ swz(r));
     }
-    a_src += 128, b_src += 128, as_src += o.as_step, bs_src += o.bs_step;
+  // (scales of 64 rows a wave; every wave makes a copy, some of them the same)
+  int s_row[2];
+  s_row[0] = 64 * (wave % (G::BM / 64 + G::BN / 128));
+  if (s_row[0] >= G::BM) {
+    s_off[0] = 4 * scale_b(s_row[0] - G::BM + lane);
+  } else {
+    s_off[0] = 4 * row_a(s_row[0] + lane);
+  }
+  s_row[1] = G::BM + G::BN / 2 + 64 * (wave % (G::BN / 128));
+  s_off[1] = 4 * scale_b(s_row[1] - G::BM + lane);
+  const uint8_t *a_src = o.a, *b_src[2] = {o.b, o.b};
+  const float *as_src = o.as, *bs_src[2] = {o.bs, o.bs};
+  // Copy c of the next step's operands that follow E0 (0 .. C0 - 1) and E1 (0 .. C1 - 1).
+  auto copy_b = [&](uint32_t st, int h, int x) __attribute__((always_inline)) {
+    dev::gload_lds16(b_src[h], b_off[h][x], lds0 + st + G::B + h * (G::BN / 2 * 128) + 1024 * (8 * x + wave), bq_span);
+  };
+  auto copy0 = [&](uint32_t st, int c) __attribute__((always_inline)) {
+    if (c < G::A_CP) {
+      dev::gload_lds16(a_src, a_off[c], lds0 + st + G::A + 1024 * (8 * c + wave), aq_span);
+    } else if (c < G::A_CP + G::B_CP) {
+      copy_b(st, 0, c - G::A_CP);
+    } else {
+      if (s_row[0] < G::BM)
+        dev::gload_lds4(as_src, s_off[0], lds0 + st + G::S + 4 * s_row[0], as_span);
+      else
+        dev::gload_lds4(bs_src[0], s_off[0], lds0 + st + G::S + 4 * s_row[0], bs_span);
+      a_src += 128, b_src[0] += 128, as_src += o.as_step, bs_src[0] += o.bs_step;
+    }
+  };
+  auto copy1 = [&](uint32_t st, int c) __attribute__((always_inline)) {
+    if (c < G::B_CP) {
+      copy_b(st, 1, c);
+    } else {
+      dev::gload_lds4(bs_src[1], s_off[1], lds0 + st + G::S + 4 * s_row[1], bs_span);
+      b_src[1] += 128, bs_src[1] += o.bs_step;
+    }
   };
 
   const uint32_t a_fo = G::A + (wm * G::WM + fr) * 128 + ((fg ^ swz(fr)) << 4);
@@ -229,17 +271,42 @@ __device__ __forceinline__ void multiply(int8_t* lds, const Operands& o, uint32_
   };
   auto factor = [&](int x) __attribute__((always_inline)) { return s[GLU && x / NI >= NJ / 2][dev::snake_j<NI>(x)]; };
 #pragma unroll
-  for (int k = 0; k < G::STAGES; ++k)
-    if (k < KT) copy(k * G::STAGE);
-  dev::wait_tiles_behind<G::CP, G::STAGES>(min(KT, G::STAGES));
-  dev::barrier();
-  uint32_t st = 0;
-  read_scales(0);
+  for (int k = 0; k < G::STAGES; ++k) {
+    if (k < KT)
 #pragma unroll
-  for (int i = 0; i < NI; ++i) a[i] = read(a_fo, i);
-  read_b(0, 0);
-
-  for (int t = 0; t < KT; ++t) {
+      for (int c = 0; c < G::C0; ++c) copy0(k * G::STAGE, c);
+    if (k < G::STAGES - 1 && k < KT)
+#pragma unroll
+      for (int c = 0; c < G::C1; ++c) copy1(k * G::STAGE, c);
+  }
+  if (KT >= G::STAGES)
+    dev::wait_vmcnt<(G::STAGES - 1) * (G::C0 + G::C1)>();
+  else
+    dev::wait_vmcnt<0>();
+  dev::barrier();  // A and the first half of B of step 0
+  uint32_t st = 0;
+  auto event1 = [&](int t) __attribute__((always_inline)) {  // E1(t)
+    if (t + 1 < KT) wait_event<G, 1>(KT - 2 - t);
+    dev::barrier();
+  };
+  auto event0 = [&](int t) __attribute__((always_inline)) {
+    if (t + 1 < KT) wait_event<G, 0>(KT - 2 - t);
+    dev::barrier();
+  };
+  auto begin = [&](uint32_t st) __attribute__((always_inline)) {
+    read_scales(st);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) a[i] = read(a_fo + st, i);
+    read_b(st, 0);
+  };
+  // A step; its first half sends the copies that follow the event at the end of the
+  // step before (FIRST), its second those that follow the event in the middle, one
+  // now and then: all at once the waves wait for each other's.
+  uint32_t last = (G::STAGES - 1) * G::STAGE;  // stage of step t - 1
+  auto step = [&](auto group_c, auto first_c, auto second_c, int t) __attribute__((always_inline)) {
+    constexpr int GROUP = decltype(group_c)::value;
+    constexpr bool FIRST = decltype(first_c)::value, SECOND = decltype(second_c)::value;
+    constexpr int CF = GROUP == 0 ? G::C0 : G::C1, CS = GROUP == 0 ? G::C1 : G::C0;
     const uint32_t next = st + G::STAGE == G::LDS ? 0 : st + G::STAGE;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
@@ -260,15 +327,20 @@ __device__ __forceinline__ void multiply(int8_t* lds, const Operands& o, uint32_
           eb[j & 1] = (int)(__float_as_uint(sb[j & 1]) >> 23);
           asm volatile("s_nop 2" : "+v"(eb[j & 1]));
         }
+        if (j == NJ / 2) {
+          if constexpr (GROUP == 0)
+            event1(t - 1);
+          else
+            event0(t);
+        }
         if (j + 1 < NJ) {
           read_b(st, j + 1);
         } else {
-          // This step's last fragments are in registers: once every wave is here, and
-          // the next step's operands too, its stage takes the copies of step t + STAGES.
-          dev::waitcnt<63, 0>();
-          if (t + 1 < KT) dev::wait_tiles_behind<G::CP, G::STAGES - 1>(min(KT - 1 - t, G::STAGES - 1));
-          dev::barrier();
-          if (t + G::STAGES < KT) copy(st);
+          dev::waitcnt<63, 0>();  // this step's last fragments are in registers
+          if constexpr (GROUP == 0)
+            event0(t);
+          else
+            event1(t);
           read_scales(next);
           read_b(next, 0);
         }
@@ -280,6 +352,17 @@ __device__ __forceinline__ void multiply(int8_t* lds, const Operands& o, uint32_
         issue_mfma0(p[x % P], b[j & 1], a[i]);
       dev::sched_fence();
       if (j == NJ - 1) a[i] = read(a_fo + next, i);
+      if constexpr (FIRST) {
+#pragma unroll
+        for (int c = 0; c < CF; ++c)
+          if (x == c * (X / 2) / CF) GROUP == 0 ? copy0(last, c) : copy1(last, c);
+      }
+      if constexpr (SECOND) {  // (not with the reads of the last column)
+        constexpr int ROOM = X / 2 - NI;
+#pragma unroll
+        for (int c = 0; c < CS; ++c)
+          if (x == X / 2 + c * ROOM / CS) GROUP == 0 ? copy1(last, c) : copy0(st, c);
+      }
       if constexpr (BBLOCK != 1) {
         if (x < BEHIND)
           add(X - BEHIND + x, s_last[x]);  // (of the step before)
@@ -292,7 +375,34 @@ __device__ __forceinline__ void multiply(int8_t* lds, const Operands& o, uint32_
 #pragma unroll
       for (int k = 0; k < BEHIND; ++k) s_last[k] = factor(X - BEHIND + k);
     }
+    last = st;
     st = next;
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  auto loop = [&](auto group_c) __attribute__((always_inline)) {
+    constexpr int GROUP = decltype(group_c)::value;
+    int t = 0;
+    if constexpr (GROUP == 0) {  // A and B's first half up to step STAGES - 1 are on their way
+      if (G::STAGES - 1 < KT)
+        step(group_c, No{}, Yes{}, t);
+      else
+        step(group_c, No{}, No{}, t);
+      for (t = 1; t - 1 + G::STAGES < KT; ++t) step(group_c, Yes{}, Yes{}, t);
+    } else {
+      for (; t + G::STAGES < KT; ++t) step(group_c, Yes{}, Yes{}, t);
+      if (t - 1 + G::STAGES < KT) step(group_c, Yes{}, No{}, t), ++t;
+    }
+    for (; t < KT; ++t) step(group_c, No{}, No{}, t);
+  };
+  if (wave < 4) {
+    begin(0);
+    loop(std::integral_constant<int, 0>{});
+    dev::barrier();  // E1 of the last step
+  } else {
+    event1(-1);
+    begin(0);
+    loop(std::integral_constant<int, 1>{});
   }
   dev::sched_fence();
   wait_results();
@@ -356,7 +466,7 @@ template <class G>
 __device__ __forceinline__ void store_glu(const Args& p, int8_t* lds, int slot0, int rows, int f0, v4f (&acc)[G::NI][G::NJ]) {
   constexpr int NI = G::NI, HJ = G::NJ / 2;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / G::WAVES_N, wn = wave % G::WAVES_N, fr = lane & 15, fg = lane >> 4;
+  const int wm = G::wm(wave), wn = G::wn(wave), fr = lane & 15, fg = lane >> 4;
   uint32_t* const lmax = reinterpret_cast<uint32_t*>(lds);
   uint32_t mine[NI];
 #pragma unroll
@@ -428,7 +538,7 @@ __global__ __launch_bounds__(G::THREADS) void gemm_tile(Args p, int tiles_m, int
   constexpr bool GLU = OUT == OUT_GLU;
   constexpr int COLS = GLU ? G::BN / 2 : G::BN;  // columns of the result
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave / G::WAVES_N, wn = wave % G::WAVES_N;
+  const int wm = G::wm(wave), wn = G::wn(wave);
   const uint32_t ap = (uint32_t)pitch(p.K), bp = ap;
   Operands o;
   int m0, n0, slot0 = 0;
@@ -745,9 +855,9 @@ __global__ __launch_bounds__(512) void glu_rows(Args p, int tiles_n) {
 }
 
 // ---------------------------------------------------------------- launches
-using Large = Tile<256, 256, 4, 2, 2>;
-using Block = Tile<128, 256, 2, 4, 3>;
-using Small = Tile<128, 128, 2, 2, 4>;
+using Large = Tile<256, 256, 4, 2>;
+using Block = Tile<128, 256, 2, 3>;
+using Small = Tile<128, 128, 4, 4>;
 
 template <class G, Mode MODE, Out OUT, int BBLOCK>
 int run_tile(miaie_ctx* ctx, const Args& p) {
