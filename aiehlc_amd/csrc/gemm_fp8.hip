@@ -150,6 +150,20 @@ struct Tile {
   __device__ static __forceinline__ int wn(int wave) { return (wave >> 2) * (WAVES_N / 2) + (wave & 3) / WAVES_M; }
 };
 
+template <int BM_, int BN_, int STAGES_>
+struct SmallTile {
+  static constexpr int BM = BM_, BN = BN_, WAVES_M = 2, WAVES_N = 2, STAGES = STAGES_;
+  static constexpr int WAVES = 4, THREADS = 256;
+  static constexpr int WM = BM / WAVES_M, WN = BN / WAVES_N, NI = WM / 16, NJ = WN / 16;
+  static constexpr int A = 0, B = BM * 128, S = B + BN * 128, STAGE = S + 4 * (BM + BN);
+  static constexpr int A_CP = BM / 8 / WAVES, B_CP = BN / 8 / WAVES;  // copies of a wave in a step
+  static constexpr int S_CP = ((BM + BN) / 64 + WAVES - 1) / WAVES, CP = A_CP + B_CP + S_CP;
+  static constexpr int LDS = STAGES * STAGE;
+  static_assert(A_CP >= 1 && B_CP >= 1 && BM % 64 == 0 && BN % 64 == 0 && STAGE % 128 == 0, "copies of whole waves");
+  __device__ static __forceinline__ int wm(int wave) { return wave / WAVES_N; }
+  __device__ static __forceinline__ int wn(int wave) { return wave % WAVES_N; }
+};
+
 // Waits for what an event makes visible; `left` steps follow the one it is about
 // (t + 1).  Copies that may still be in flight: those sent after it.
 template <class G, int EVENT, int LEFT = G::STAGES - 1>
@@ -420,6 +434,174 @@ __device__ __forceinline__ void multiply(int8_t* lds, const Operands& o, uint32_
   dev::sched_fence();
 }
 
+// Tiles of few workgroups and short steps: four waves, one on each SIMD, all in step,
+// with one barrier; a workgroup of its own fits beside it.
+template <class G, int BBLOCK, bool GLU, class RowA, class RowB, class ScaleB>
+__device__ __forceinline__ void multiply_small(int8_t* lds, const Operands& o, uint32_t a_pitch, uint32_t b_pitch, RowA row_a, RowB row_b,
+                                         ScaleB scale_b, const dbg::Span& aq_span, const dbg::Span& as_span,
+                                         const dbg::Span& bq_span, const dbg::Span& bs_span, v4f (&acc)[G::NI][G::NJ]) {
+  constexpr int NI = G::NI, NJ = G::NJ;
+  const uint32_t lds0 = dev::lds_addr(lds);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = G::wm(wave), wn = G::wn(wave), fr = lane & 15, fg = lane >> 4;
+
+  uint32_t a_off[G::A_CP], b_off[G::B_CP], s_off[G::S_CP];
+#pragma unroll
+  for (int x = 0; x < G::A_CP; ++x) {
+    const int r = 8 * (G::WAVES * x + wave) + (lane >> 3);
+    a_off[x] = row_a(r) * a_pitch + 16 * ((lane & 7) ^ swz(r));
+  }
+#pragma unroll
+  for (int x = 0; x < G::B_CP; ++x) {
+    const int r = 8 * (G::WAVES * x + wave) + (lane >> 3);
+    b_off[x] = row_b(r) * b_pitch + 16 * ((lane & 7) ^ swz(r));
+  }
+  // (scales: every wave makes the same number of copies, the last ones again)
+  int s_row[G::S_CP];
+#pragma unroll
+  for (int x = 0; x < G::S_CP; ++x) {
+    s_row[x] = 64 * ((G::WAVES * x + wave) % ((G::BM + G::BN) / 64));
+    s_off[x] = 4 * (s_row[x] < G::BM ? row_a(s_row[x] + lane) : scale_b(s_row[x] - G::BM + lane));
+  }
+  const uint8_t *a_src = o.a, *b_src = o.b;
+  const float *as_src = o.as, *bs_src = o.bs;
+  auto copy = [&](uint32_t st) __attribute__((always_inline)) {  // the next step's operands
+#pragma unroll
+    for (int x = 0; x < G::A_CP; ++x)
+      dev::gload_lds16(a_src, a_off[x], lds0 + st + G::A + 1024 * (G::WAVES * x + wave), aq_span);
+#pragma unroll
+    for (int x = 0; x < G::B_CP; ++x)
+      dev::gload_lds16(b_src, b_off[x], lds0 + st + G::B + 1024 * (G::WAVES * x + wave), bq_span);
+#pragma unroll
+    for (int x = 0; x < G::S_CP; ++x) {
+      if (s_row[x] < G::BM)
+        dev::gload_lds4(as_src, s_off[x], lds0 + st + G::S + 4 * s_row[x], as_span);
+      else
+        dev::gload_lds4(bs_src, s_off[x], lds0 + st + G::S + 4 * s_row[x], bs_span);
+    }
+    a_src += 128, b_src += 128, as_src += o.as_step, bs_src += o.bs_step;
+  };
+
+  const uint32_t a_fo = G::A + (wm * G::WM + fr) * 128 + ((fg ^ swz(fr)) << 4);
+  const uint32_t b_fo = G::B + (wn * G::WN + fr) * 128 + ((fg ^ swz(fr)) << 4);
+  auto read = [&](uint32_t at, int block) __attribute__((always_inline)) -> v8i {
+    return join(*reinterpret_cast<const v4i*>(lds + at + 2048 * block), *reinterpret_cast<const v4i*>(lds + (at ^ 64) + 2048 * block));
+  };
+  auto scale = [&](uint32_t st, int row) __attribute__((always_inline)) -> float {
+    return *reinterpret_cast<const float*>(lds + st + G::S + 4 * row);
+  };
+  const int KT = o.steps;
+  constexpr int X = NI * NJ, P = 4, BEHIND = 2;  // a step's products; one is added when two more have been issued
+  static_assert(X % P == 0 && NJ % 2 == 0, "a step begins where the one before began");
+  v8i a[NI], b[2];
+  v4f p[P];
+  float sa[NI], sb[2], s[GLU ? 2 : 1][NI], s_last[BEHIND];
+  int ea[NI], eb[2];
+#pragma unroll
+  for (int k = 0; k < P; ++k) p[k] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int k = 0; k < BEHIND; ++k) s_last[k] = 0.f;
+  auto read_scales = [&](uint32_t st) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) sa[i] = scale(st, wm * G::WM + 16 * i + fr);
+    if constexpr (BBLOCK != 1) {
+      sb[0] = scale(st, G::BM + wn * G::WN);
+      if constexpr (GLU) sb[1] = scale(st, G::BM + wn * G::WN + G::WN / 2);
+    }
+  };
+  auto read_b = [&](uint32_t st, int j) __attribute__((always_inline)) {
+    b[j & 1] = read(b_fo + st, j);
+    if constexpr (BBLOCK == 1) sb[j & 1] = scale(st, G::BM + wn * G::WN + 16 * j + fr);
+  };
+  auto add = [&](int x, float f) __attribute__((always_inline)) {  // a step's x-th product
+    v4f& to = acc[dev::snake_j<NI>(x)][x / NI];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[e] = __builtin_fmaf(p[x % P][e], f, to[e]);
+    asm volatile("" : "+v"(to));  // (added here and not later)
+  };
+  auto factor = [&](int x) __attribute__((always_inline)) { return s[GLU && x / NI >= NJ / 2][dev::snake_j<NI>(x)]; };
+#pragma unroll
+  for (int k = 0; k < G::STAGES; ++k)
+    if (k < KT) copy(k * G::STAGE);
+  dev::wait_tiles_behind<G::CP, G::STAGES>(min(KT, G::STAGES));
+  dev::barrier();
+  uint32_t st = 0;
+  read_scales(0);
+#pragma unroll
+  for (int i = 0; i < NI; ++i) a[i] = read(a_fo, i);
+  read_b(0, 0);
+
+  for (int t = 0; t < KT; ++t) {
+    const uint32_t next = st + G::STAGE == G::LDS ? 0 : st + G::STAGE;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      if constexpr (BBLOCK == 1) {
+        ea[i] = (int)(__float_as_uint(sa[i]) >> 23);
+        asm volatile("" : "+v"(ea[i]));
+      } else {
+        s[0][i] = sa[i] * sb[0];
+        if constexpr (GLU) s[1][i] = sa[i] * sb[1];
+      }
+    }
+    dev::sched_fence();
+#pragma unroll
+    for (int x = 0; x < X; ++x) {
+      const int j = x / NI, i = dev::snake_j<NI>(x);
+      if (x % NI == 0) {
+        if constexpr (BBLOCK == 1) {  // (three wait states from a scale's shift to its use)
+          eb[j & 1] = (int)(__float_as_uint(sb[j & 1]) >> 23);
+          asm volatile("s_nop 2" : "+v"(eb[j & 1]));
+        }
+        if (j + 1 < NJ) {
+          read_b(st, j + 1);
+        } else {
+          // This step's last fragments are in registers: once every wave is here, and
+          // the next step's operands too, its stage takes the copies of step t + STAGES.
+          dev::waitcnt<63, 0>();
+          if (t + 1 < KT) dev::wait_tiles_behind<G::CP, G::STAGES - 1>(min(KT - 1 - t, G::STAGES - 1));
+          dev::barrier();
+          if (t + G::STAGES < KT) copy(st);
+          read_scales(next);
+          read_b(next, 0);
+        }
+        dev::sched_fence();
+      }
+      if constexpr (BBLOCK == 1)
+        issue_mfma_scaled(acc[i][j], b[j & 1], a[i], eb[j & 1], ea[i]);
+      else
+        issue_mfma0(p[x % P], b[j & 1], a[i]);
+      dev::sched_fence();
+      if (j == NJ - 1) a[i] = read(a_fo + next, i);
+      if constexpr (BBLOCK != 1) {
+        if (x < BEHIND)
+          add(X - BEHIND + x, s_last[x]);  // (of the step before)
+        else
+          add(x - BEHIND, factor(x - BEHIND));
+      }
+      dev::sched_fence();
+    }
+    if constexpr (BBLOCK != 1) {
+#pragma unroll
+      for (int k = 0; k < BEHIND; ++k) s_last[k] = factor(X - BEHIND + k);
+    }
+    st = next;
+  }
+  dev::sched_fence();
+  wait_results();
+#pragma unroll
+  for (int k = 0; k < P; ++k) asm volatile("" : "+v"(p[k]));  // (read behind the wait)
+  if constexpr (BBLOCK != 1) {
+#pragma unroll
+    for (int k = 0; k < BEHIND; ++k) add(X - BEHIND + k, s_last[k]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) asm volatile("" : "+v"(acc[i][j]));
+  }
+  dev::sched_fence();
+}
+
 // A wave's part at row 0 and column n0 of C (m < M rows, n0 + .. < N columns of it
 // exist).  In bf16 two blocks beside each other are exchanged between the lanes of a
 // row, so that each holds eight columns of one: 16 bytes a lane in either type.
@@ -515,70 +697,55 @@ __device__ __forceinline__ void store_glu(const Args& p, int8_t* lds, int slot0,
   }
 }
 
-// An expert's tiles are walked blocks of rows first, so that those which share
-// columns of B run beside each other, and the workgroups of one XCD (b % 8) have a
-// contiguous run of all tiles in use: few experts' operands in one L2.  False: no
-// tile is left for this workgroup.
-__device__ __forceinline__ bool slot_tile(const Slots& s, int b, int tiles_n, int& block, int& tn, int& e) {
-  const int tiles = MIAIE_LD(s.start + s.experts) / 128 * tiles_n, each = (tiles + 7) / 8;
+// A tile of ROWS slots (a divisor or multiple of 128) of one expert.  An expert's tiles
+// are walked rows first, so that those which share columns of B run beside each
+// other, and the workgroups of one XCD (b % 8) have a contiguous run of all tiles in
+// use: few experts' operands in one L2.  False: nothing is left for this workgroup.
+struct SlotTile {
+  int e, slot, rows, tn;  // rows: of the expert from this slot on
+};
+template <int ROWS>
+__device__ __forceinline__ bool slot_tile(const Slots& s, int b, int tiles_n, SlotTile& to) {
+  constexpr int UNIT = ROWS < 128 ? ROWS : 128;
+  const int tiles = MIAIE_LD(s.start + s.experts) / UNIT * tiles_n, each = (tiles + 7) / 8;
   if (b / 8 >= each) return false;
   const int logical = b % 8 * each + b / 8;
   if (logical >= tiles) return false;
-  e = MIAIE_LD(s.expert_of + logical / tiles_n);
-  const int first = MIAIE_LD(s.start + e) / 128, n = (MIAIE_LD(s.count + e) + 127) / 128;
-  const int local = logical - first * tiles_n;
-  block = first + local % n;
-  tn = local / n;
+  to.e = MIAIE_LD(s.expert_of + logical / tiles_n / (128 / UNIT));
+  const int start = MIAIE_LD(s.start + to.e), count = MIAIE_LD(s.count + to.e);
+  const int n = (count + 127) / 128 * (128 / UNIT), local = logical - start / UNIT * tiles_n;
+  const int row = local % n * UNIT;
+  if (row >= count || (ROWS > 128 && row % ROWS)) return false;  // (the tile before has these rows)
+  to.slot = start + row, to.rows = count - row, to.tn = local / n;
   return true;
 }
 
+// The tile at row m0 and column n0 of expert e's product (DENSE: e = 0); `rows` of A
+// and C exist from m0 on.
 template <class G, Mode MODE, Out OUT, int BBLOCK>
-__global__ __launch_bounds__(G::THREADS) void gemm_tile(Args p, int tiles_m, int tiles_n) {
-  __shared__ __attribute__((aligned(1024))) int8_t lds[G::LDS];
+__device__ __forceinline__ void run_tile_at(const Args& p, int8_t* lds, int e, int m0, int n0, int rows) {
   constexpr bool GLU = OUT == OUT_GLU;
   constexpr int COLS = GLU ? G::BN / 2 : G::BN;  // columns of the result
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = G::wm(wave), wn = G::wn(wave);
-  const uint32_t ap = (uint32_t)pitch(p.K), bp = ap;
-  Operands o;
-  int m0, n0, slot0 = 0;
-  size_t to = 0;  // first element of the tile's matrix in C
+  const uint32_t pch = (uint32_t)pitch(p.K);
   const int b_rows = GLU ? 2 * p.N : p.N;
   const size_t b_s_rows = BBLOCK == 1 ? (size_t)b_rows : blocks(b_rows);
-  o.a = p.Aq, o.as = p.As, o.b = p.Bq, o.bs = p.Bs;
+  Operands o;
+  o.a = p.Aq, o.as = p.As;
+  o.b = p.Bq + (size_t)n0 * pch, o.bs = p.Bs + (BBLOCK == 1 ? n0 : n0 / 128);
   o.steps = (int)blocks(p.K);
   o.as_step = p.a_rows, o.bs_step = b_s_rows;
-  if constexpr (MODE == DENSE) {
-    int tm, tn;
-    dev::tile_coords<4>(blockIdx.x, tiles_m, tiles_n, tm, tn);
-    m0 = tm * G::BM, n0 = tn * COLS;
-    o.rows = p.M - m0;
-    o.a += (size_t)m0 * ap, o.as += m0;
-  } else if constexpr (MODE == SLOTS) {
-    static_assert(MODE != SLOTS || G::BM == 128, "a block of slots is one expert's");
-    int block, tn, e;
-    if (!slot_tile(p.s, blockIdx.x, tiles_n, block, tn, e)) return;
-    slot0 = 128 * block, m0 = 0, n0 = tn * COLS;
-    o.rows = MIAIE_LD(p.s.start + e) + MIAIE_LD(p.s.count + e) - slot0;
-    if (!p.gather) o.a += (size_t)slot0 * ap, o.as += slot0;
-    o.b += (size_t)e * b_rows * bp, o.bs += (size_t)e * b_s_rows * blocks(p.K);
-    to = (size_t)slot0 * p.ldc;
-  } else {
-    const int each = tiles_m * tiles_n, e = blockIdx.x / each;
-    int tm, tn;
-    dev::tile_coords<4>(blockIdx.x % each, tiles_m, tiles_n, tm, tn);
+  o.rows = min(rows, G::BM), o.cols = min(p.N - n0, COLS);
+  size_t to = 0;  // first element of the product in C
+  if constexpr (MODE == SLOTS) o.b += (size_t)e * b_rows * pch, o.bs += (size_t)e * b_s_rows * blocks(p.K);
+  if (MODE != SLOTS || !p.gather) o.a += (size_t)m0 * pch, o.as += m0;
+  if constexpr (MODE == WGRAD) {  // k: the expert's slots
     const int first = MIAIE_LD(p.s.start + e);
     o.steps = (int)blocks(MIAIE_LD(p.s.count + e));
-    m0 = tm * G::BM, n0 = tn * COLS;
-    o.rows = p.M - m0;
-    o.a += (size_t)m0 * ap + first, o.as += (size_t)(first / 128) * p.M + m0;
+    o.a += first, o.as += (size_t)(first / 128) * p.M;
     o.b += first, o.bs += (size_t)(first / 128) * b_s_rows;
     to = (size_t)e * p.M * p.ldc;
   }
-  o.cols = p.N - n0;
-  o.b += (size_t)n0 * bp;
-  o.bs += BBLOCK == 1 ? n0 : n0 / 128;
-  o.rows = min(o.rows, G::BM), o.cols = min(o.cols, COLS);
   const dbg::Span aq_span = dbg::span_of(p.Aq), as_span = dbg::span_of(p.As), bq_span = dbg::span_of(p.Bq),
                   bs_span = dbg::span_of(p.Bs);  // (debug build only)
   v4f acc[G::NI][G::NJ];
@@ -590,7 +757,7 @@ __global__ __launch_bounds__(G::THREADS) void gemm_tile(Args p, int tiles_m, int
   auto row_a = [&](int r) __attribute__((always_inline)) -> uint32_t {
     r = min(r, o.rows - 1);
     if constexpr (MODE == SLOTS) {
-      if (p.gather) return (uint32_t)(MIAIE_LD(p.s.row_of + slot0 + r) / p.s.top_k);
+      if (p.gather) return (uint32_t)(MIAIE_LD(p.s.row_of + m0 + r) / p.s.top_k);
     }
     return (uint32_t)r;
   };
@@ -605,14 +772,50 @@ __global__ __launch_bounds__(G::THREADS) void gemm_tile(Args p, int tiles_m, int
   auto scale_b = [&](int r) __attribute__((always_inline)) -> uint32_t {
     return BBLOCK == 1 ? row_b(r) : row_b(r) / 128;
   };
-  if (o.steps > 0)
-    multiply<G, BBLOCK, GLU>(lds, o, ap, bp, row_a, row_b, scale_b, aq_span, as_span, bq_span, bs_span, acc);
+  if (o.steps > 0) {
+    if constexpr (G::WAVES == 4)
+      multiply_small<G, BBLOCK, GLU>(lds, o, pch, pch, row_a, row_b, scale_b, aq_span, as_span, bq_span, bs_span, acc);
+    else
+      multiply<G, BBLOCK, GLU>(lds, o, pch, pch, row_a, row_b, scale_b, aq_span, as_span, bq_span, bs_span, acc);
+  }
   if constexpr (GLU) {
-    store_glu<G>(p, lds, slot0, o.rows, n0, acc);
+    store_glu<G>(p, lds, m0, o.rows, n0, acc);
   } else {
     using T = std::conditional_t<OUT == OUT_F32, float, __bf16>;
-    store_part(static_cast<T*>(p.C) + to, p.ldc, m0 + wm * G::WM, n0 + wn * G::WN, m0 + o.rows, p.N, acc);
+    store_part(static_cast<T*>(p.C) + to, p.ldc, m0 + G::wm(wave) * G::WM, n0 + G::wn(wave) * G::WN, m0 + o.rows, p.N, acc);
   }
+}
+
+template <class G, Mode MODE, Out OUT, int BBLOCK>
+__global__ __launch_bounds__(G::THREADS) void gemm_tile(Args p, int tiles_m, int tiles_n) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds[G::LDS];
+  constexpr int COLS = OUT == OUT_GLU ? G::BN / 2 : G::BN;
+  if constexpr (MODE == SLOTS) {
+    static_assert(MODE != SLOTS || 128 % G::BM == 0, "a block of slots is one expert's");
+    SlotTile t;
+    if (!slot_tile<G::BM>(p.s, blockIdx.x, tiles_n, t)) return;
+    run_tile_at<G, MODE, OUT, BBLOCK>(p, lds, t.e, t.slot, t.tn * COLS, t.rows);
+  } else {
+    const int each = tiles_m * tiles_n, e = MODE == WGRAD ? blockIdx.x / each : 0;
+    int tm, tn;
+    dev::tile_coords<4>(MODE == WGRAD ? blockIdx.x % each : blockIdx.x, tiles_m, tiles_n, tm, tn);
+    run_tile_at<G, MODE, OUT, BBLOCK>(p, lds, e, tm * G::BM, tn * COLS, p.M - tm * G::BM);
+  }
+}
+
+// Slots in tiles of 256 rows, an expert's last block of 128 in one of its own where
+// their number is odd.
+template <class G, class H, Out OUT>
+__global__ __launch_bounds__(G::THREADS) void gemm_slots_mixed(Args p, int tiles_n) {
+  static_assert(G::BM == 256 && H::BM == 128 && G::BN == H::BN && G::THREADS == H::THREADS, "tiles of one launch");
+  __shared__ __attribute__((aligned(1024))) int8_t lds[G::LDS > H::LDS ? G::LDS : H::LDS];
+  constexpr int COLS = OUT == OUT_GLU ? G::BN / 2 : G::BN;
+  SlotTile t;
+  if (!slot_tile<256>(p.s, blockIdx.x, tiles_n, t)) return;
+  if (t.rows > 128)
+    run_tile_at<G, SLOTS, OUT, 128>(p, lds, t.e, t.slot, t.tn * COLS, t.rows);
+  else
+    run_tile_at<H, SLOTS, OUT, 128>(p, lds, t.e, t.slot, t.tn * COLS, t.rows);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -739,10 +942,11 @@ __global__ __launch_bounds__(1024) void gemm_rows(Args p, int tiles_n, int waves
   int m0 = 0, n0, rows, slot0 = 0;
   size_t to = 0;
   if constexpr (MODE == SLOTS) {
-    int block, tn, e;
-    if (!slot_tile(p.s, blockIdx.x, tiles_n, block, tn, e)) return;
-    slot0 = 128 * block, n0 = 16 * NJ * tn;
-    rows = min(128, MIAIE_LD(p.s.start + e) + MIAIE_LD(p.s.count + e) - slot0);
+    SlotTile t;
+    if (!slot_tile<128>(p.s, blockIdx.x, tiles_n, t)) return;
+    const int e = t.e;
+    slot0 = t.slot, n0 = 16 * NJ * t.tn;
+    rows = min(128, t.rows);
     if (!p.gather) a += (size_t)slot0 * row_pitch, as += slot0;
     b0 += (size_t)e * p.N * row_pitch, bs0 += (size_t)e * b_s_rows * blocks(p.K);
     to = (size_t)slot0 * p.ldc;
@@ -810,10 +1014,9 @@ __global__ __launch_bounds__(512) void glu_rows(Args p, int tiles_n) {
   const int fr = lane & 15, fg = lane >> 4;
   const uint32_t row_pitch = (uint32_t)pitch(p.K);
   const size_t b_s_rows = blocks(2 * (long)p.N);
-  int block, tn, e;
-  if (!slot_tile(p.s, blockIdx.x, tiles_n, block, tn, e)) return;
-  const int slot0 = 128 * block, f0 = 128 * tn;
-  const int rows = min(128, MIAIE_LD(p.s.start + e) + MIAIE_LD(p.s.count + e) - slot0);
+  SlotTile t;
+  if (!slot_tile<128>(p.s, blockIdx.x, tiles_n, t)) return;
+  const int e = t.e, tn = t.tn, slot0 = t.slot, f0 = 128 * tn, rows = min(128, t.rows);
   const uint8_t* a = p.gather ? p.Aq : p.Aq + (size_t)slot0 * row_pitch;
   const float* as = p.gather ? p.As : p.As + slot0;
   const uint8_t* const gate = p.Bq + ((size_t)e * 2 * p.N + f0 + 16 * wave) * row_pitch;
@@ -857,7 +1060,12 @@ __global__ __launch_bounds__(512) void glu_rows(Args p, int tiles_n) {
 // ---------------------------------------------------------------- launches
 using Large = Tile<256, 256, 4, 2>;
 using Block = Tile<128, 256, 2, 3>;
-using Small = Tile<128, 128, 4, 4>;
+using Square = SmallTile<128, 128, 2>;
+using Flat = SmallTile<64, 128, 3>;
+using Small = SmallTile<64, 64, 3>;
+using Glu = SmallTile<64, 256, 2>;  // (128 columns of H)
+
+constexpr long kThreads = 1l << 32;  // HIP takes fewer in a launch
 
 template <class G, Mode MODE, Out OUT, int BBLOCK>
 int run_tile(miaie_ctx* ctx, const Args& p) {
@@ -868,6 +1076,14 @@ int run_tile(miaie_ctx* ctx, const Args& p) {
   const hipError_t e = launch<gemm_tile<G, MODE, OUT, BBLOCK>>(ctx->device, dim3((unsigned)grid), dim3(G::THREADS), 0, ctx->stream, p,
                                                                (int)tiles_m, (int)tiles_n);
   return check_launch(ctx, e, "gemm_fp8_tile");
+}
+
+template <Out OUT>
+int run_slots_mixed(miaie_ctx* ctx, const Args& p) {
+  const long cols = OUT == OUT_GLU ? Large::BN / 2 : Large::BN, tiles_n = (p.N + cols - 1) / cols, grid = (p.M / 128 * tiles_n + 7) / 8 * 8;
+  const hipError_t e = launch<gemm_slots_mixed<Large, Block, OUT>>(ctx->device, dim3((unsigned)grid), dim3(Large::THREADS), 0, ctx->stream,
+                                                                   p, (int)tiles_n);
+  return check_launch(ctx, e, "gemm_fp8_slots");
 }
 
 template <int MI, int NJ, Mode MODE, Out OUT, int BBLOCK>
@@ -883,17 +1099,50 @@ int run_rows(miaie_ctx* ctx, const Args& p) {
   return check_launch(ctx, e, "gemm_fp8_rows");
 }
 
+// ---- choice of tile: the lowest estimated time.  A CU has `at_once` workgroups of a
+// tile; a workgroup's start and end, and a step's time with one, two, ... of them on
+// the CU while most CUs are at work (the clock falls under that load; with few at
+// work, a step alone takes idle).  Measured at 4096 columns and K = 4096, random
+// elements.  The estimates are for the choice, not for the time.
+struct TileTime {
+  int bm, bn, at_once;
+  double ends, idle, step[3];
+};
+constexpr TileTime kLarge{256, 256, 1, 9.0, 1.05, {1.50}}, kBlock{128, 256, 1, 6.5, 0.72, {0.95}},
+    kSquare{128, 128, 2, 3.3, 0.57, {0.65, 1.09}}, kFlat{64, 128, 2, 2.3, 0.44, {0.47, 0.70}},
+    kSmall{64, 64, 3, 2.0, 0.29, {0.31, 0.44, 0.54}};
+
+double tile_us(const TileTime& t, double tiles, long steps, int cus) {
+  if (2 * tiles <= cus) return 1.0 + t.ends + t.idle * steps;
+  const long each = (long)((tiles + cus - 1) / cus), full = each / t.at_once, rest = each % t.at_once;
+  return 1.0 + full * (t.ends + t.step[t.at_once - 1] * steps) + (rest ? t.ends + t.step[rest - 1] * steps : 0.0);
+}
+double dense_us(const TileTime& t, const Args& p, int cus) {
+  return tile_us(t, (double)((p.M + t.bm - 1l) / t.bm) * (double)((p.N + t.bn - 1l) / t.bn), (long)blocks(p.K), cus);
+}
+// (an expert's last tile is half full on average)
+double slots_us(const TileTime& t, const Args& p, double cols, int cus) {
+  const double n = (double)p.s.tokens * p.s.top_k, used = std::min<double>(p.s.experts, n);
+  return tile_us(t, std::max(used, n / t.bm + used / 2) * ((p.N + cols - 1) / cols), (long)blocks(p.K), cus);
+}
+
 template <Out OUT, int BBLOCK>
 int run_dense(miaie_ctx* ctx, const Args& p) {
   if (p.M <= 16) return run_rows<1, 1, DENSE, OUT, BBLOCK>(ctx, p);
-  const long large = ((p.M + 255l) / 256) * ((p.N + 255l) / 256);
-  if (large >= 128) return run_tile<Large, DENSE, OUT, BBLOCK>(ctx, p);
-  return run_tile<Small, DENSE, OUT, BBLOCK>(ctx, p);
+  const double us[] = {dense_us(kLarge, p, ctx->cus), dense_us(kBlock, p, ctx->cus), dense_us(kSquare, p, ctx->cus),
+                       dense_us(kFlat, p, ctx->cus), dense_us(kSmall, p, ctx->cus)};
+  switch (std::min_element(us, us + 5) - us) {
+    case 0: return run_tile<Large, DENSE, OUT, BBLOCK>(ctx, p);
+    case 1: return run_tile<Block, DENSE, OUT, BBLOCK>(ctx, p);
+    case 2: return run_tile<Square, DENSE, OUT, BBLOCK>(ctx, p);
+    case 3: return run_tile<Flat, DENSE, OUT, BBLOCK>(ctx, p);
+    default: return run_tile<Small, DENSE, OUT, BBLOCK>(ctx, p);
+  }
 }
 
 // Few slots an expert: the waves of gemm_rows and glu_rows have more of B in flight.
 bool few_slots(const Args& p, int cols) {
-  return (long)p.s.tokens * p.s.top_k <= 16l * p.s.experts && p.M / 128 * ((p.N + cols - 1l) / cols) < 1l << 21;
+  return (long)p.s.tokens * p.s.top_k <= 16l * p.s.experts && p.M / 128 * ((p.N + cols - 1l) / cols) < kThreads / 2048;
 }
 
 template <Out OUT>
@@ -904,11 +1153,22 @@ int run_slots(miaie_ctx* ctx, const Args& p) {
       const hipError_t e = launch<glu_rows>(ctx->device, dim3((unsigned)grid), dim3(512), 0, ctx->stream, p, p.N / 128);
       return check_launch(ctx, e, "glu_rows");
     }
+    const double us[] = {slots_us(kLarge, p, 128, ctx->cus), slots_us(kSquare, p, 128, ctx->cus)};
+    if (us[1] < us[0]) return run_tile<Glu, SLOTS, OUT, 128>(ctx, p);
   } else {
     if (few_slots(p, 16)) return run_rows<1, 1, SLOTS, OUT, 128>(ctx, p);
+    const double us[] = {slots_us(kLarge, p, 256, ctx->cus), slots_us(kSquare, p, 128, ctx->cus), slots_us(kSmall, p, 64, ctx->cus)};
+    switch (std::min_element(us, us + 3) - us) {
+      case 1: return run_tile<Square, SLOTS, OUT, 128>(ctx, p);
+      case 2: return run_tile<Small, SLOTS, OUT, 128>(ctx, p);
+      default: break;
+    }
   }
-  return run_tile<Block, SLOTS, OUT, 128>(ctx, p);
+  return run_slots_mixed<OUT>(ctx, p);
 }
+
+template <Out OUT>
+int run_wgrad(miaie_ctx* ctx, const Args& p) { return run_tile<Large, WGRAD, OUT, 1>(ctx, p); }
 
 }  // namespace
 
@@ -934,7 +1194,7 @@ int launch_experts_glu_fp8(miaie_ctx* ctx, const fp8::Slots& s, const uint8_t* X
 int launch_experts_wgrad_fp8(miaie_ctx* ctx, const fp8::Slots& s, const uint8_t* Atq, const float* Ats, const uint8_t* Btq,
                              const float* Bts, void* C, int dtype, int M, int N, int ldc) {
   const Args p{Atq, Ats, Btq, Bts, C, nullptr, nullptr, M, N, s.rows, ldc, M, 0, s};
-  return dtype == MIAIE_BF16 ? run_tile<Large, WGRAD, OUT_BF16, 1>(ctx, p) : run_tile<Large, WGRAD, OUT_F32, 1>(ctx, p);
+  return dtype == MIAIE_BF16 ? run_wgrad<OUT_BF16>(ctx, p) : run_wgrad<OUT_F32>(ctx, p);
 }
 
 }  // namespace miaie

@@ -289,11 +289,26 @@ __global__ __launch_bounds__(64 * kOrderWaves) void order_slots(const int* __res
   for (int i = tid; i < kOrderWaves * experts; i += 64 * kOrderWaves) at[i] = 0;
   for (int i = tid; i < rows / 128; i += 64 * kOrderWaves) MIAIE_ST(expert_of + i, -1);
   __syncthreads();
+  // (a panel of a wave's pairs at a time, its loads in flight together)
+  constexpr int PANEL = 8;
   const int each = (pairs + 64 * kOrderWaves - 1) / (64 * kOrderWaves) * 64, first = wave * each,
             last = min(pairs, first + each);
-  for (int i = first + lane; i < last; i += 64) {
-    const int e = MIAIE_LD(idx + i);
-    if (e >= 0 && e < experts) atomicAdd(at + wave * experts + e, 1);
+  auto load = [&](int i0, int (&e)[PANEL]) {
+#pragma unroll
+    for (int u = 0; u < PANEL; ++u) {
+      const int i = i0 + 64 * u + lane;
+      e[u] = i < last ? MIAIE_LD(idx + i) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < PANEL; ++u)
+      if (e[u] >= experts) e[u] = -1;
+  };
+  for (int i0 = first; i0 < last; i0 += 64 * PANEL) {
+    int e[PANEL];
+    load(i0, e);
+#pragma unroll
+    for (int u = 0; u < PANEL; ++u)
+      if (e[u] >= 0) atomicAdd(at + wave * experts + e[u], 1);
   }
   __syncthreads();
   // thread e: the expert's pairs in each wave, and its place among the experts
@@ -315,7 +330,6 @@ __global__ __launch_bounds__(64 * kOrderWaves) void order_slots(const int* __res
     MIAIE_ST(count + tid, n);
     if (tid == experts - 1) MIAIE_ST(start + experts, upto);
     for (int b = begin / 128; b < upto / 128; ++b) MIAIE_ST(expert_of + b, tid);
-    for (int r = begin + n; r < upto; ++r) MIAIE_ST(row_of + r, -1);
     int next = begin;
     for (int w = 0; w < kOrderWaves; ++w) {
       const int c = at[w * experts + tid];
@@ -323,25 +337,34 @@ __global__ __launch_bounds__(64 * kOrderWaves) void order_slots(const int* __res
       next += c;
     }
   }
+  // padding: thread e's values go round its wave
+  for (int k = 0; k < 64 && 64 * wave + k < experts; ++k) {
+    const int from = __shfl(begin + n, k), to = __shfl(upto, k);
+    for (int r = from + lane; r < to; r += 64) MIAIE_ST(row_of + r, -1);
+  }
   __syncthreads();
-  for (int i0 = first; i0 < last; i0 += 64) {
-    const int i = i0 + lane;
-    int e = i < last ? MIAIE_LD(idx + i) : -1;
-    if (e >= experts) e = -1;
-    unsigned long long same = __ballot(e >= 0);
-    for (int b = 0; b < bits; ++b) {
-      const unsigned long long has = __ballot(e >> b & 1);
-      same &= (e >> b & 1) ? has : ~has;
+  for (int i0 = first; i0 < last; i0 += 64 * PANEL) {
+    int e[PANEL];
+    load(i0, e);
+#pragma unroll
+    for (int u = 0; u < PANEL; ++u) {
+      if (i0 + 64 * u >= last) break;
+      const int i = i0 + 64 * u + lane;
+      unsigned long long same = __ballot(e[u] >= 0);
+      for (int b = 0; b < bits; ++b) {
+        const unsigned long long has = __ballot(e[u] >> b & 1);
+        same &= (e[u] >> b & 1) ? has : ~has;
+      }
+      int slot = -1;
+      if (e[u] >= 0) {
+        const int before = __popcll(same & ((1ull << lane) - 1)), base = at[wave * experts + e[u]];
+        slot = base + before;
+        MIAIE_ST(row_of + slot, i);
+        // (every lane has read its expert's place: one instruction for the wave)
+        if (before == 0) at[wave * experts + e[u]] = base + __popcll(same);
+      }
+      if (i < last) MIAIE_ST(slot_of + i, slot);
     }
-    int slot = -1;
-    if (e >= 0) {
-      const int before = __popcll(same & ((1ull << lane) - 1)), base = at[wave * experts + e];
-      slot = base + before;
-      MIAIE_ST(row_of + slot, i);
-      // (every lane has read its expert's place: one instruction for the wave)
-      if (before == 0) at[wave * experts + e] = base + __popcll(same);
-    }
-    if (i < last) MIAIE_ST(slot_of + i, slot);
   }
 }
 
