@@ -697,7 +697,7 @@ __device__ __forceinline__ void store_glu(const Args& p, int8_t* lds, int slot0,
   }
 }
 
-// A tile of ROWS slots (a divisor or multiple of 128) of one expert.  An expert's tiles
+// A tile of ROWS slots (a divisor of 128) of one expert.  An expert's tiles
 // are walked rows first, so that those which share columns of B run beside each
 // other, and the workgroups of one XCD (b % 8) have a contiguous run of all tiles in
 // use: few experts' operands in one L2.  False: nothing is left for this workgroup.
@@ -706,16 +706,16 @@ struct SlotTile {
 };
 template <int ROWS>
 __device__ __forceinline__ bool slot_tile(const Slots& s, int b, int tiles_n, SlotTile& to) {
-  constexpr int UNIT = ROWS < 128 ? ROWS : 128;
-  const int tiles = MIAIE_LD(s.start + s.experts) / UNIT * tiles_n, each = (tiles + 7) / 8;
+  static_assert(128 % ROWS == 0, "a block of slots is one expert's");
+  const int tiles = MIAIE_LD(s.start + s.experts) / ROWS * tiles_n, each = (tiles + 7) / 8;
   if (b / 8 >= each) return false;
   const int logical = b % 8 * each + b / 8;
   if (logical >= tiles) return false;
-  to.e = MIAIE_LD(s.expert_of + logical / tiles_n / (128 / UNIT));
+  to.e = MIAIE_LD(s.expert_of + logical / tiles_n / (128 / ROWS));
   const int start = MIAIE_LD(s.start + to.e), count = MIAIE_LD(s.count + to.e);
-  const int n = (count + 127) / 128 * (128 / UNIT), local = logical - start / UNIT * tiles_n;
-  const int row = local % n * UNIT;
-  if (row >= count || (ROWS > 128 && row % ROWS)) return false;  // (the tile before has these rows)
+  const int n = (count + 127) / 128 * (128 / ROWS), local = logical - start / ROWS * tiles_n;
+  const int row = local % n * ROWS;
+  if (row >= count) return false;
   to.slot = start + row, to.rows = count - row, to.tn = local / n;
   return true;
 }
@@ -791,7 +791,6 @@ __global__ __launch_bounds__(G::THREADS) void gemm_tile(Args p, int tiles_m, int
   __shared__ __attribute__((aligned(1024))) int8_t lds[G::LDS];
   constexpr int COLS = OUT == OUT_GLU ? G::BN / 2 : G::BN;
   if constexpr (MODE == SLOTS) {
-    static_assert(MODE != SLOTS || 128 % G::BM == 0, "a block of slots is one expert's");
     SlotTile t;
     if (!slot_tile<G::BM>(p.s, blockIdx.x, tiles_n, t)) return;
     run_tile_at<G, MODE, OUT, BBLOCK>(p, lds, t.e, t.slot, t.tn * COLS, t.rows);
@@ -801,21 +800,6 @@ __global__ __launch_bounds__(G::THREADS) void gemm_tile(Args p, int tiles_m, int
     dev::tile_coords<4>(MODE == WGRAD ? blockIdx.x % each : blockIdx.x, tiles_m, tiles_n, tm, tn);
     run_tile_at<G, MODE, OUT, BBLOCK>(p, lds, e, tm * G::BM, tn * COLS, p.M - tm * G::BM);
   }
-}
-
-// Slots in tiles of 256 rows, an expert's last block of 128 in one of its own where
-// their number is odd.
-template <class G, class H, Out OUT>
-__global__ __launch_bounds__(G::THREADS) void gemm_slots_mixed(Args p, int tiles_n) {
-  static_assert(G::BM == 256 && H::BM == 128 && G::BN == H::BN && G::THREADS == H::THREADS, "tiles of one launch");
-  __shared__ __attribute__((aligned(1024))) int8_t lds[G::LDS > H::LDS ? G::LDS : H::LDS];
-  constexpr int COLS = OUT == OUT_GLU ? G::BN / 2 : G::BN;
-  SlotTile t;
-  if (!slot_tile<256>(p.s, blockIdx.x, tiles_n, t)) return;
-  if (t.rows > 128)
-    run_tile_at<G, SLOTS, OUT, 128>(p, lds, t.e, t.slot, t.tn * COLS, t.rows);
-  else
-    run_tile_at<H, SLOTS, OUT, 128>(p, lds, t.e, t.slot, t.tn * COLS, t.rows);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -1078,14 +1062,6 @@ int run_tile(miaie_ctx* ctx, const Args& p) {
   return check_launch(ctx, e, "gemm_fp8_tile");
 }
 
-template <Out OUT>
-int run_slots_mixed(miaie_ctx* ctx, const Args& p) {
-  const long cols = OUT == OUT_GLU ? Large::BN / 2 : Large::BN, tiles_n = (p.N + cols - 1) / cols, grid = (p.M / 128 * tiles_n + 7) / 8 * 8;
-  const hipError_t e = launch<gemm_slots_mixed<Large, Block, OUT>>(ctx->device, dim3((unsigned)grid), dim3(Large::THREADS), 0, ctx->stream,
-                                                                   p, (int)tiles_n);
-  return check_launch(ctx, e, "gemm_fp8_slots");
-}
-
 template <int MI, int NJ, Mode MODE, Out OUT, int BBLOCK>
 int run_rows(miaie_ctx* ctx, const Args& p) {
   using G = RowsGeom<MI, NJ>;
@@ -1110,7 +1086,7 @@ struct TileTime {
 };
 constexpr TileTime kLarge{256, 256, 1, 9.0, 1.05, {1.50}}, kBlock{128, 256, 1, 6.5, 0.72, {0.95}},
     kSquare{128, 128, 2, 3.3, 0.57, {0.65, 1.09}}, kFlat{64, 128, 2, 2.3, 0.44, {0.47, 0.70}},
-    kSmall{64, 64, 3, 2.0, 0.29, {0.31, 0.44, 0.54}};
+    kSmall{64, 64, 3, 2.0, 0.29, {0.31, 0.44, 0.54}}, kGlu{64, 256, 1, 3.0, 0.60, {0.95}};
 
 double tile_us(const TileTime& t, double tiles, long steps, int cus) {
   if (2 * tiles <= cus) return 1.0 + t.ends + t.idle * steps;
@@ -1153,18 +1129,13 @@ int run_slots(miaie_ctx* ctx, const Args& p) {
       const hipError_t e = launch<glu_rows>(ctx->device, dim3((unsigned)grid), dim3(512), 0, ctx->stream, p, p.N / 128);
       return check_launch(ctx, e, "glu_rows");
     }
-    const double us[] = {slots_us(kLarge, p, 128, ctx->cus), slots_us(kSquare, p, 128, ctx->cus)};
-    if (us[1] < us[0]) return run_tile<Glu, SLOTS, OUT, 128>(ctx, p);
+    return slots_us(kGlu, p, 128, ctx->cus) < slots_us(kBlock, p, 128, ctx->cus) ? run_tile<Glu, SLOTS, OUT, 128>(ctx, p)
+                                                                                  : run_tile<Block, SLOTS, OUT, 128>(ctx, p);
   } else {
     if (few_slots(p, 16)) return run_rows<1, 1, SLOTS, OUT, 128>(ctx, p);
-    const double us[] = {slots_us(kLarge, p, 256, ctx->cus), slots_us(kSquare, p, 128, ctx->cus), slots_us(kSmall, p, 64, ctx->cus)};
-    switch (std::min_element(us, us + 3) - us) {
-      case 1: return run_tile<Square, SLOTS, OUT, 128>(ctx, p);
-      case 2: return run_tile<Small, SLOTS, OUT, 128>(ctx, p);
-      default: break;
-    }
+    return slots_us(kSmall, p, 64, ctx->cus) < slots_us(kSquare, p, 128, ctx->cus) ? run_tile<Small, SLOTS, OUT, 128>(ctx, p)
+                                                                                   : run_tile<Square, SLOTS, OUT, 128>(ctx, p);
   }
-  return run_slots_mixed<OUT>(ctx, p);
 }
 
 template <Out OUT>

@@ -285,15 +285,18 @@ __global__ __launch_bounds__(64 * kOrderWaves) void order_slots(const int* __res
                                                                 int pairs, int experts, int rows, int bits) {
   extern __shared__ int at[];  // [waves][experts]: a wave's count of an expert, then its next slot
   __shared__ int wave_sum[kOrderWaves];
+  __shared__ int2 ends[MIAIE_MAX_EXPERTS];  // an expert's last slot in use and in all
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   for (int i = tid; i < kOrderWaves * experts; i += 64 * kOrderWaves) at[i] = 0;
   for (int i = tid; i < rows / 128; i += 64 * kOrderWaves) MIAIE_ST(expert_of + i, -1);
   __syncthreads();
-  // (a panel of a wave's pairs at a time, its loads in flight together)
-  constexpr int PANEL = 8;
+  // a panel of a wave's pairs at a time, its loads in flight together; where there is
+  // one only, it stays in registers
+  constexpr int PANEL = 16;
   const int each = (pairs + 64 * kOrderWaves - 1) / (64 * kOrderWaves) * 64, first = wave * each,
             last = min(pairs, first + each);
-  auto load = [&](int i0, int (&e)[PANEL]) {
+  int e[PANEL];
+  auto load = [&](int i0) {
 #pragma unroll
     for (int u = 0; u < PANEL; ++u) {
       const int i = i0 + 64 * u + lane;
@@ -303,18 +306,22 @@ __global__ __launch_bounds__(64 * kOrderWaves) void order_slots(const int* __res
     for (int u = 0; u < PANEL; ++u)
       if (e[u] >= experts) e[u] = -1;
   };
+  load(first);
   for (int i0 = first; i0 < last; i0 += 64 * PANEL) {
-    int e[PANEL];
-    load(i0, e);
+    if (i0 > first) load(i0);
 #pragma unroll
     for (int u = 0; u < PANEL; ++u)
       if (e[u] >= 0) atomicAdd(at + wave * experts + e[u], 1);
   }
   __syncthreads();
   // thread e: the expert's pairs in each wave, and its place among the experts
-  int n = 0;
-  if (tid < experts)
-    for (int w = 0; w < kOrderWaves; ++w) n += at[w * experts + tid];
+  int n = 0, of_wave[kOrderWaves] = {};
+  if (tid < experts) {
+#pragma unroll
+    for (int w = 0; w < kOrderWaves; ++w) of_wave[w] = at[w * experts + tid];
+#pragma unroll
+    for (int w = 0; w < kOrderWaves; ++w) n += of_wave[w];
+  }
   const int padded = (n + 127) / 128 * 128;
   int upto = padded;
   for (int d = 1; d < 64; d *= 2) {
@@ -329,23 +336,24 @@ __global__ __launch_bounds__(64 * kOrderWaves) void order_slots(const int* __res
     MIAIE_ST(start + tid, begin);
     MIAIE_ST(count + tid, n);
     if (tid == experts - 1) MIAIE_ST(start + experts, upto);
-    for (int b = begin / 128; b < upto / 128; ++b) MIAIE_ST(expert_of + b, tid);
+    ends[tid] = make_int2(begin + n, upto);
     int next = begin;
+#pragma unroll
     for (int w = 0; w < kOrderWaves; ++w) {
-      const int c = at[w * experts + tid];
       at[w * experts + tid] = next;
-      next += c;
+      next += of_wave[w];
     }
   }
-  // padding: thread e's values go round its wave
-  for (int k = 0; k < 64 && 64 * wave + k < experts; ++k) {
-    const int from = __shfl(begin + n, k), to = __shfl(upto, k);
-    for (int r = from + lane; r < to; r += 64) MIAIE_ST(row_of + r, -1);
-  }
   __syncthreads();
+  for (int x = wave; x < experts; x += kOrderWaves) {  // padding, and the blocks' expert
+    const int2 end = ends[x];
+    const int begin_x = x ? ends[x - 1].y : 0;
+    for (int r = end.x + lane; r < end.y; r += 64) MIAIE_ST(row_of + r, -1);
+    for (int b = begin_x / 128 + lane; b < end.y / 128; b += 64) MIAIE_ST(expert_of + b, x);
+  }
+  if (each > 64 * PANEL) load(first);
   for (int i0 = first; i0 < last; i0 += 64 * PANEL) {
-    int e[PANEL];
-    load(i0, e);
+    if (i0 > first) load(i0);
 #pragma unroll
     for (int u = 0; u < PANEL; ++u) {
       if (i0 + 64 * u >= last) break;
