@@ -697,26 +697,55 @@ __device__ __forceinline__ void store_glu(const Args& p, int8_t* lds, int slot0,
   }
 }
 
-// A tile of ROWS slots (a divisor of 128) of one expert.  An expert's tiles
-// are walked rows first, so that those which share columns of B run beside each
-// other, and the workgroups of one XCD (b % 8) have a contiguous run of all tiles in
-// use: few experts' operands in one L2.  False: nothing is left for this workgroup.
+// Inclusive sums over the lanes of a wave.
+__device__ __forceinline__ int scan_wave(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // lane - 1 of sixteen
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // ... - 2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // ... - 4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // ... - 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // the last of the sixteen before
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // the last of the first half
+  return v;
+}
+
+// A tile of up to ROWS slots of one expert: its tiles are ceil(count / ROWS) of rows
+// times tiles_n, walked rows first, so that those which share columns of B run beside
+// each other, and the workgroups of one XCD (b % 8) have a contiguous run of all
+// tiles: few experts' operands in one L2.  Every wave finds its tile from the experts'
+// counts: loads beside each other, where a walk through the order's parts would be
+// three that wait for one another, and no workgroup without a tile among the others
+// (such a one waits for a whole CU's LDS like the rest: 16384 slots of 64 experts at
+// 256 rows a tile 235 us with as many empty ones, 168 without).  False: no tile.
 struct SlotTile {
   int e, slot, rows, tn;  // rows: of the expert from this slot on
 };
 template <int ROWS>
 __device__ __forceinline__ bool slot_tile(const Slots& s, int b, int tiles_n, SlotTile& to) {
-  static_assert(128 % ROWS == 0, "a block of slots is one expert's");
-  const int tiles = MIAIE_LD(s.start + s.experts) / ROWS * tiles_n, each = (tiles + 7) / 8;
-  if (b / 8 >= each) return false;
-  const int logical = b % 8 * each + b / 8;
-  if (logical >= tiles) return false;
-  to.e = MIAIE_LD(s.expert_of + logical / tiles_n / (128 / ROWS));
-  const int start = MIAIE_LD(s.start + to.e), count = MIAIE_LD(s.count + to.e);
-  const int n = (count + 127) / 128 * (128 / ROWS), local = logical - start / ROWS * tiles_n;
-  const int row = local % n * ROWS;
-  if (row >= count) return false;
-  to.slot = start + row, to.rows = count - row, to.tn = local / n;
+  const int lane = threadIdx.x & 63;
+  auto count_of = [&](int e0) { return e0 + lane < s.experts ? MIAIE_LD(s.count + e0 + lane) : 0; };
+  int count = count_of(0), rows = scan_wave((count + ROWS - 1) / ROWS), total = __builtin_amdgcn_readlane(rows, 63);
+  for (int e0 = 64; e0 < s.experts; e0 += 64)
+    total += __builtin_amdgcn_readlane(scan_wave((count_of(e0) + ROWS - 1) / ROWS), 63);
+  const int tiles = total * tiles_n, each = (tiles + 7) / 8, logical = b % 8 * each + b / 8;
+  if (b / 8 >= each || logical >= tiles) return false;
+  const int at = logical / tiles_n;
+  int before = 0, blocks_before = 0, e0 = 0;  // tiles of rows, and blocks of 128 slots, before expert e0
+  int blocks_to = scan_wave((count + 127) / 128);
+  while (before + __builtin_amdgcn_readlane(rows, 63) <= at) {
+    before += __builtin_amdgcn_readlane(rows, 63);
+    blocks_before += __builtin_amdgcn_readlane(blocks_to, 63);
+    e0 += 64;
+    count = count_of(e0);
+    rows = scan_wave((count + ROWS - 1) / ROWS);
+    blocks_to = scan_wave((count + 127) / 128);
+  }
+  const int l = __builtin_ctzll(__ballot(before + rows > at));
+  const int c = __builtin_amdgcn_readlane(count, l), n = (c + ROWS - 1) / ROWS;
+  const int local = logical - (before + __builtin_amdgcn_readlane(rows, l) - n) * tiles_n, row = local % n * ROWS;
+  to.e = e0 + l;
+  to.slot = 128 * (blocks_before + __builtin_amdgcn_readlane(blocks_to, l) - (c + 127) / 128) + row;
+  to.rows = c - row;
+  to.tn = local / n;
   return true;
 }
 
@@ -800,6 +829,20 @@ __global__ __launch_bounds__(G::THREADS) void gemm_tile(Args p, int tiles_m, int
     dev::tile_coords<4>(MODE == WGRAD ? blockIdx.x % each : blockIdx.x, tiles_m, tiles_n, tm, tn);
     run_tile_at<G, MODE, OUT, BBLOCK>(p, lds, e, tm * G::BM, tn * COLS, p.M - tm * G::BM);
   }
+}
+
+// Slots in tiles of 256 rows, the last 128 or fewer of an expert in one of 128.
+template <class G, class H, Out OUT>
+__global__ __launch_bounds__(G::THREADS) void gemm_slots(Args p, int tiles_n) {
+  static_assert(G::BM == 256 && H::BM == 128 && G::BN == H::BN && G::THREADS == H::THREADS, "tiles of one launch");
+  __shared__ __attribute__((aligned(1024))) int8_t lds[G::LDS > H::LDS ? G::LDS : H::LDS];
+  constexpr int COLS = OUT == OUT_GLU ? G::BN / 2 : G::BN;
+  SlotTile t;
+  if (!slot_tile<256>(p.s, blockIdx.x, tiles_n, t)) return;
+  if (t.rows > 128)
+    run_tile_at<G, SLOTS, OUT, 128>(p, lds, t.e, t.slot, t.tn * COLS, t.rows);
+  else
+    run_tile_at<H, SLOTS, OUT, 128>(p, lds, t.e, t.slot, t.tn * COLS, t.rows);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -1051,15 +1094,31 @@ using Glu = SmallTile<64, 256, 2>;  // (128 columns of H)
 
 constexpr long kThreads = 1l << 32;  // HIP takes fewer in a launch
 
+// Most tiles of `rows` slots that a routing can make: one more for each expert than
+// its rows fill.
+long most_slot_tiles(const Slots& s, int rows) {
+  const long n = (long)s.tokens * s.top_k, used = std::min<long>(s.experts, n);
+  return used + (n - used) / rows;
+}
+
 template <class G, Mode MODE, Out OUT, int BBLOCK>
 int run_tile(miaie_ctx* ctx, const Args& p) {
   const long tiles_m = (p.M + G::BM - 1l) / G::BM, cols = OUT == OUT_GLU ? G::BN / 2 : G::BN, tiles_n = (p.N + cols - 1) / cols;
   long grid = tiles_m * tiles_n;
   if (MODE == WGRAD) grid *= p.s.experts;
-  if (MODE == SLOTS) grid = (grid + 7) / 8 * 8;
+  if (MODE == SLOTS) grid = (most_slot_tiles(p.s, G::BM) * tiles_n + 7) / 8 * 8;
   const hipError_t e = launch<gemm_tile<G, MODE, OUT, BBLOCK>>(ctx->device, dim3((unsigned)grid), dim3(G::THREADS), 0, ctx->stream, p,
                                                                (int)tiles_m, (int)tiles_n);
   return check_launch(ctx, e, "gemm_fp8_tile");
+}
+
+template <Out OUT>
+int run_slots_large(miaie_ctx* ctx, const Args& p) {
+  const long cols = OUT == OUT_GLU ? Large::BN / 2 : Large::BN, tiles_n = (p.N + cols - 1) / cols;
+  const long grid = (most_slot_tiles(p.s, 256) * tiles_n + 7) / 8 * 8;
+  const hipError_t e = launch<gemm_slots<Large, Block, OUT>>(ctx->device, dim3((unsigned)grid), dim3(Large::THREADS), 0, ctx->stream, p,
+                                                             (int)tiles_n);
+  return check_launch(ctx, e, "gemm_fp8_slots");
 }
 
 template <int MI, int NJ, Mode MODE, Out OUT, int BBLOCK>
@@ -1068,7 +1127,7 @@ int run_rows(miaie_ctx* ctx, const Args& p) {
   const int groups = ((int)blocks(p.K) + 1) / 2;
   const int most = std::min(16, 163840 / G::REGION), each = (groups + most - 1) / most, waves = (groups + each - 1) / each;
   const long tiles_n = (p.N + 16 * NJ - 1l) / (16 * NJ);
-  const long tiles_m = MODE == SLOTS ? p.M / 128 : (p.M + 16 * MI - 1l) / (16 * MI);
+  const long tiles_m = MODE == SLOTS ? most_slot_tiles(p.s, 128) : (p.M + 16 * MI - 1l) / (16 * MI);
   const long grid = MODE == SLOTS ? (tiles_m * tiles_n + 7) / 8 * 8 : tiles_m * tiles_n;
   const hipError_t e = launch<gemm_rows<MI, NJ, MODE, OUT, BBLOCK>>(ctx->device, dim3((unsigned)grid), dim3(64 * waves),
                                                                     (size_t)waves * G::REGION, ctx->stream, p, (int)tiles_n, waves);
@@ -1125,7 +1184,7 @@ template <Out OUT>
 int run_slots(miaie_ctx* ctx, const Args& p) {
   if constexpr (OUT == OUT_GLU) {
     if (few_slots(p, 128)) {
-      const long grid = ((long)p.M / 128 * (p.N / 128) + 7) / 8 * 8;
+      const long grid = (most_slot_tiles(p.s, 128) * (p.N / 128) + 7) / 8 * 8;
       const hipError_t e = launch<glu_rows>(ctx->device, dim3((unsigned)grid), dim3(512), 0, ctx->stream, p, p.N / 128);
       return check_launch(ctx, e, "glu_rows");
     }
