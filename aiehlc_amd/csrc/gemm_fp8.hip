@@ -79,28 +79,6 @@ __device__ __forceinline__ void wait_results() { asm volatile("s_nop 7\n\ts_nop 
 // fragment read cover all banks.
 __device__ __forceinline__ int swz(int r) { return (r >> 1) & 7; }
 
-// The same block product in bf16, which holds every element: 16 conversions and four
-// instructions an operand's fragment, sums as fp32 has them (few rows; see
-// multiply_rows).
-struct Wide {
-  v8bf v[4];
-  __device__ __forceinline__ explicit Wide(v8i x) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-      const v2bf c0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * q], 1.f, false), c1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * q], 1.f, true),
-                 c2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * q + 1], 1.f, false), c3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * q + 1], 1.f, true);
-      v[q] = v8bf{c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
-    }
-  }
-};
-__device__ __forceinline__ v4f mfma_wide(const Wide& b, const Wide& a) {
-  v4f p = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int q = 0; q < 4; ++q) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.v[q], a.v[q], p, 0, 0, 0);
-  return p;
-}
-
 template <class T>
 __device__ __forceinline__ void store4(T* C, size_t ldc, int m, int n, int M, int N, v4f v) {
   if (m >= M || n >= N) return;
@@ -846,239 +824,240 @@ __global__ __launch_bounds__(G::THREADS) void gemm_slots(Args p, int tiles_n) {
 }
 
 // ---------------------------------------------------------------- few rows
-// A wave copies 256 bytes (two blocks of k, a group) of 16 NJ rows of B and of
-// A's rows into a part of LDS of its own, waits for its own copies (no barriers)
-// and multiplies; the next group is on its way once this one's fragments are in
-// registers.  Bound by reading B, every byte of it once.  Chunk c (16 bytes) of
-// row r lies at c ^ (r % 16).
+// Up to four rows of A at a time by reading B as it lies in memory, straight into
+// registers: a load takes whole lines of eight rows, lane l the 16 bytes l % 8 of row
+// l / 8, and multiplies them in fp32 with those of A, which the workgroup keeps in
+// LDS.  Bound by reading B, every byte of it once; a wave has eight to sixteen lines of
+// eight rows in flight.  (On the matrix instructions, which want 16 rows' 16 bytes
+// side by side, B had to go through LDS: 1 x 11008 x 4096 12.7 us.)
 //
-// With weights the products are taken in bf16: the 8-bit instructions cut products
-// off at 2^-13 of the largest of eight, which moves fp32 sums by 1.5e-5 and with
-// them one in 400 codes of a packed H.  With many rows such steps average out; a
-// token's own MLP had up to 5.7e-3 of its result from a few of them, 2.4e-3 with
-// them gone, and the conversions hide behind the loads.
-template <int MI, int NJ>
-struct RowsGeom {
-  static constexpr int B = 0, A = 4096 * NJ, GROUP = A + 4096 * MI;
-  static constexpr int SUM = MI * NJ * 1024;
-  static constexpr int REGION = GROUP > SUM ? GROUP : SUM;
+// fp32 products are exact here, where the 8-bit matrix instructions cut them off at
+// 2^-13 of the largest of eight.  That moves their sums by 1.5e-5, and one in 400
+// codes of a packed H with them; with many rows such steps average out, while a
+// token's own MLP had up to 5.7e-3 of its result from a few of them (2.4e-3 without).
+constexpr int STREAM_K = 64;  // blocks of k whose A is in LDS at a time
+
+// p += <16 elements of q, 16 elements of x>
+__device__ __forceinline__ float dot16(const float (&b)[16], const float (&a)[16]) {
+  float p0 = b[0] * a[0], p1 = b[1] * a[1];
+#pragma unroll
+  for (int i = 2; i < 16; i += 2) p0 = __builtin_fmaf(b[i], a[i], p0), p1 = __builtin_fmaf(b[i + 1], a[i + 1], p1);
+  return p0 + p1;
+}
+__device__ __forceinline__ void widen(v4u q, float (&x)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const mx::v2f lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)q[i], true);
+    x[4 * i] = lo[0], x[4 * i + 1] = lo[1], x[4 * i + 2] = hi[0], x[4 * i + 3] = hi[1];
+  }
+}
+
+// acc[m][u] += row m of A (in LDS, STREAM_K blocks a row) times this lane's part of
+// row l / 8 of b[u], over the blocks kb0 + first .. kb0 + last - 1.  s[m][u]: lane kb
+// has the scale of block kb0 + kb.
+// D blocks are loaded together, and as many behind them.
+template <int MR, int D>
+__device__ __forceinline__ void stream(const int8_t* lds, const uint8_t* const (&b)[2], int first, int last, const float (&s)[MR][2],
+                                       float (&acc)[MR][2]) {
+  const int lane = threadIdx.x & 63;
+  v4u q[2][D][2];
+  auto load = [&](int kb, v4u (&to)[D][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)  // (blocks behind the last one repeat it)
+        to[d][u] = MIAIE_LD(reinterpret_cast<const v4u*>(b[u] + 128 * (size_t)min(kb + d, last - 1)));
+  };
+  auto multiply = [&](int kb, const v4u (&from)[D][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      if (kb + d >= last) return;
+      float x[2][16];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) widen(from[d][u], x[u]);
+#pragma unroll
+      for (int m = 0; m < MR; ++m) {
+        float a[16];
+        widen(*reinterpret_cast<const v4u*>(lds + 128 * (m * STREAM_K + kb + d) + 16 * (lane & 7)), a);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          acc[m][u] = __builtin_fmaf(dot16(x[u], a), __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s[m][u]), kb + d)), acc[m][u]);
+      }
+    }
+  };
+  if (first >= last) return;
+  load(first, q[0]);
+  for (int kb = first; kb < last; kb += 2 * D) {
+    load(min(kb + D, last - 1), q[1]);
+    multiply(kb, q[0]);
+    if (kb + D >= last) break;
+    load(min(kb + 2 * D, last - 1), q[0]);
+    multiply(kb + D, q[1]);
+  }
+}
+
+// Where a workgroup's rows and columns are.
+struct StreamTile {
+  const uint8_t *a, *b;  // first row of each
+  const float *as, *bs;
+  size_t a_step, b_step;  // floats from one block's scales to the next's
+  int rows;
 };
 
-// acc[i][j] += rows 16 i .. of A times rows of B's j-th sixteen, over the groups
-// first, first + step, ...  a_off, b_off: a lane's offset of the row it copies.
-template <int MI, int NJ, int BBLOCK, class RowA, class RowB>
-__device__ __forceinline__ void multiply_rows(int8_t* mine, const uint8_t* a, const float* as, size_t as_step, const uint8_t* const (&b)[NJ],
-                                              const float* const (&bs)[NJ], size_t bs_step, uint32_t row_pitch, int steps, int rows,
-                                              RowA row_a, RowB row_b, int first, int step, const dbg::Span& aq_span,
-                                              const dbg::Span& bq_span, v4f (&acc)[MI][NJ]) {
-  using G = RowsGeom<MI, NJ>;
-  const int lane = threadIdx.x & 63, fr = lane & 15, fg = lane >> 4;
-  const uint32_t mine0 = dev::lds_addr(mine);
-  const int groups = (steps + 1) / 2;
-  const int a_copies = (min(rows, 16 * MI) + 3) / 4;
-  uint32_t a_off[4 * MI], b_off[4];
+// acc[m][u] of rows r0 .. r0 + MR - 1 (rows behind the last repeat it) and this wave's
+// b0 and b1, the sums over the lanes of a row in each of them.
+template <int MR, int D, class RowA>
+__device__ __forceinline__ void stream_rows(int8_t* lds, const Args& p, const StreamTile& t, const uint8_t* const (&b)[2],
+                                            const float* const (&bs)[2], int r0, RowA row_a, int part, int parts, float (&acc)[MR][2]) {
+  const int tid = threadIdx.x, lane = tid & 63, threads = blockDim.x;
+  const int steps = (int)blocks(p.K);
+  const size_t pch = pitch(p.K);
 #pragma unroll
-  for (int x = 0; x < 4 * MI; ++x) a_off[x] = row_a(min(4 * x + fg, rows - 1)) * row_pitch;
-#pragma unroll
-  for (int x = 0; x < 4; ++x) b_off[x] = row_b(4 * x + fg) * row_pitch;
-  float sa[2][MI], sb[2][NJ];
-  uint32_t a_row[MI], b_row[4];
-#pragma unroll
-  for (int i = 0; i < MI; ++i) a_row[i] = row_a(min(16 * i + fr, rows - 1));
-  b_row[0] = row_b(fr);
-  auto copy = [&](int g) __attribute__((always_inline)) {
-    const uint32_t mask = 2 * g + 1 < steps ? 15 : 7;  // (half a group: its first block again)
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const size_t kb = min(2 * g + k, steps - 1);
-#pragma unroll
-      for (int i = 0; i < MI; ++i) sa[k][i] = MIAIE_LD(as + kb * as_step + a_row[i]);
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) sb[k][j] = MIAIE_LD(bs[j] + kb * bs_step + (BBLOCK == 1 ? b_row[0] : 0u));
+  for (int m = 0; m < MR; ++m) acc[m][0] = acc[m][1] = 0.f;
+  for (int kb0 = 0; kb0 < steps; kb0 += STREAM_K) {
+    const int n = min(STREAM_K, steps - kb0);
+    if (kb0 > 0 || r0 > 0) __syncthreads();
+    for (int i = tid; i < MR * n * 8; i += threads) {
+      const int m = i / (8 * n), c = i % (8 * n);
+      const v4u v = MIAIE_LD(reinterpret_cast<const v4u*>(t.a + row_a(min(r0 + m, t.rows - 1)) * pch + 128 * (size_t)kb0 + 16 * c));
+      *reinterpret_cast<v4u*>(lds + 128 * m * STREAM_K + 16 * c) = v;
     }
+    float s[MR][2];
+    const size_t kb = kb0 + min(lane, n - 1);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+    for (int u = 0; u < 2; ++u) {
+      const float sb = MIAIE_LD(bs[u] + kb * t.b_step);
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        dev::gload_lds16(b[j] + 256 * (size_t)g, b_off[x] + 16 * ((fr ^ (4 * x + fg)) & mask), mine0 + G::B + 4096 * j + 1024 * x, bq_span);
-#pragma unroll
-    for (int x = 0; x < 4 * MI; ++x)
-      if (x < a_copies)
-        dev::gload_lds16(a + 256 * (size_t)g, a_off[x] + 16 * ((fr ^ ((4 * x + fg) & 15)) & mask), mine0 + G::A + 1024 * x, aq_span);
-  };
-  auto half = [&](int k) __attribute__((always_inline)) {
-    v8i fa[MI], fb[NJ];
-    const int c0 = 8 * k + fg, c1 = c0 + 4;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      fb[j] = join(*reinterpret_cast<const v4i*>(mine + G::B + 4096 * j + 256 * fr + 16 * (c0 ^ fr)),
-                   *reinterpret_cast<const v4i*>(mine + G::B + 4096 * j + 256 * fr + 16 * (c1 ^ fr)));
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int r = min(16 * i + fr, 4 * a_copies - 1), x = r & 15;
-      fa[i] = join(*reinterpret_cast<const v4i*>(mine + G::A + 256 * r + 16 * (c0 ^ x)),
-                   *reinterpret_cast<const v4i*>(mine + G::A + 256 * r + 16 * (c1 ^ x)));
+      for (int m = 0; m < MR; ++m) s[m][u] = sb * MIAIE_LD(t.as + kb * t.a_step + row_a(min(r0 + m, t.rows - 1)));
     }
-    if constexpr (BBLOCK == 1) {
-#pragma unroll
-      for (int i = 0; i < MI; ++i)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-          acc[i][j] = mfma_scaled(fb[j], fa[i], acc[i][j], (int)(__float_as_uint(sb[k][j]) >> 23), (int)(__float_as_uint(sa[k][i]) >> 23));
-    } else {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const Wide b(fb[j]);
-#pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          const v4f p = mfma_wide(b, Wide(fa[i]));
-          const float f = sa[k][i] * sb[k][j];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_fmaf(p[e], f, acc[i][j][e]);
-        }
-      }
-    }
-  };
-  if (first < groups) copy(first);
-  for (int g = first; g < groups; g += step) {
-    dev::wait_vmcnt<0>();
-    asm volatile("" ::: "memory");
-    half(0);
-    if (2 * g + 1 < steps) half(1);
-    if (g + step < groups) {
-      dev::waitcnt<63, 0>();
-      asm volatile("" ::: "memory");
-      copy(g + step);
-    }
-  }
-}
-
-// 16 MI rows and 16 NJ columns a workgroup, whose waves share out the groups of k
-// and add their sums in LDS in a fixed order.  SLOTS: a block of 128 slots a
-// workgroup, 16 MI rows at a time (few slots, or B comes out of the L2 again).
-template <int MI, int NJ, Mode MODE, Out OUT, int BBLOCK>
-__global__ __launch_bounds__(1024) void gemm_rows(Args p, int tiles_n, int waves) {
-  using G = RowsGeom<MI, NJ>;
-  extern __shared__ __attribute__((aligned(1024))) int8_t lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int fr = lane & 15, fg = lane >> 4;
-  const uint32_t row_pitch = (uint32_t)pitch(p.K);
-  const size_t b_s_rows = BBLOCK == 1 ? (size_t)p.N : blocks(p.N);
-  const uint8_t *a = p.Aq, *b0 = p.Bq;
-  const float *as = p.As, *bs0 = p.Bs;
-  int m0 = 0, n0, rows, slot0 = 0;
-  size_t to = 0;
-  if constexpr (MODE == SLOTS) {
-    SlotTile t;
-    if (!slot_tile<128>(p.s, blockIdx.x, tiles_n, t)) return;
-    const int e = t.e;
-    slot0 = t.slot, n0 = 16 * NJ * t.tn;
-    rows = min(128, t.rows);
-    if (!p.gather) a += (size_t)slot0 * row_pitch, as += slot0;
-    b0 += (size_t)e * p.N * row_pitch, bs0 += (size_t)e * b_s_rows * blocks(p.K);
-    to = (size_t)slot0 * p.ldc;
-  } else {
-    m0 = 16 * MI * (blockIdx.x / tiles_n), n0 = 16 * NJ * (blockIdx.x % tiles_n);
-    rows = min(16 * MI, p.M - m0);
-    a += (size_t)m0 * row_pitch, as += m0;
-    to = (size_t)m0 * p.ldc;
-  }
-  b0 += (size_t)n0 * row_pitch, bs0 += BBLOCK == 1 ? n0 : n0 / 128;
-  const uint8_t* b[NJ];
-  const float* bs[NJ];
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const int at = min(16 * j, (p.N - 1 - n0) / 16 * 16);  // (sixteens behind the last column repeat the last)
-    b[j] = b0 + (size_t)at * row_pitch;
-    bs[j] = bs0 + (BBLOCK == 1 ? at : 0);
-  }
-  const dbg::Span aq_span = dbg::span_of(p.Aq), bq_span = dbg::span_of(p.Bq);  // (debug build only)
-  const int last = (p.N - 1 - n0) % 16;  // last row of B's last sixteen
-  const bool whole = n0 + 16 * NJ <= p.N;
-  int8_t* const mine = lds + wave * G::REGION;
-  for (int r0 = 0; r0 < rows; r0 += 16 * MI) {
-    v4f acc[MI][NJ];
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-    auto row_a = [&](int r) __attribute__((always_inline)) -> uint32_t {
-      if constexpr (MODE == SLOTS) {
-        if (p.gather) return (uint32_t)(MIAIE_LD(p.s.row_of + slot0 + r0 + r) / p.s.top_k);
-      }
-      return (uint32_t)(r0 + r);
-    };
-    auto row_b = [&](int r) __attribute__((always_inline)) -> uint32_t { return (uint32_t)(whole ? r : min(r, last)); };
-    multiply_rows<MI, NJ, BBLOCK>(mine, a, as, p.a_rows, b, bs, b_s_rows, row_pitch, (int)blocks(p.K), rows - r0, row_a, row_b, wave,
-                                  waves, aq_span, bq_span, acc);
-    if (waves > 1) {
-#pragma unroll
-      for (int f = 0; f < MI * NJ; ++f) *reinterpret_cast<v4f*>(mine + 1024 * f + 16 * lane) = acc[f / NJ][f % NJ];
-      __syncthreads();
-    }
-#pragma unroll
-    for (int u = 0; u < MI * NJ; ++u) {
-      if (u % waves != wave) continue;
-      v4f sum = acc[u / NJ][u % NJ];
-      if (waves > 1) {  // in the order of the waves, whichever of them adds
-        sum = v4f{0.f, 0.f, 0.f, 0.f};
-        for (int w = 0; w < waves; ++w) sum += *reinterpret_cast<const v4f*>(lds + w * G::REGION + 1024 * u + 16 * lane);
-      }
-      using T = std::conditional_t<OUT == OUT_F32, float, __bf16>;
-      store4(static_cast<T*>(p.C) + to, p.ldc, r0 + 16 * (u / NJ) + fr, n0 + 16 * (u % NJ) + 4 * fg, rows, p.N, sum);
-    }
-    if (r0 + 16 * MI < rows) __syncthreads();
-  }
-}
-
-// silu(gate) up of 128 columns of H and a block of slots, 16 rows at a time: eight
-// waves, each with 16 gate and 16 up columns over all of k.
-__global__ __launch_bounds__(512) void glu_rows(Args p, int tiles_n) {
-  using G = RowsGeom<1, 2>;
-  __shared__ __attribute__((aligned(1024))) int8_t lds[8 * G::REGION];
-  __shared__ uint32_t lmax[8][16];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int fr = lane & 15, fg = lane >> 4;
-  const uint32_t row_pitch = (uint32_t)pitch(p.K);
-  const size_t b_s_rows = blocks(2 * (long)p.N);
-  SlotTile t;
-  if (!slot_tile<128>(p.s, blockIdx.x, tiles_n, t)) return;
-  const int e = t.e, tn = t.tn, slot0 = t.slot, f0 = 128 * tn, rows = min(128, t.rows);
-  const uint8_t* a = p.gather ? p.Aq : p.Aq + (size_t)slot0 * row_pitch;
-  const float* as = p.gather ? p.As : p.As + slot0;
-  const uint8_t* const gate = p.Bq + ((size_t)e * 2 * p.N + f0 + 16 * wave) * row_pitch;
-  const uint8_t* const b[2] = {gate, gate + (size_t)p.N * row_pitch};
-  const float* const gate_s = p.Bs + (size_t)e * b_s_rows * blocks(p.K) + f0 / 128;
-  const float* const bs[2] = {gate_s, gate_s + p.N / 128};
-  const dbg::Span aq_span = dbg::span_of(p.Aq), bq_span = dbg::span_of(p.Bq);  // (debug build only)
-  const size_t h_pitch = pitch(p.N);
-  for (int r0 = 0; r0 < rows; r0 += 16) {
-    v4f acc[1][2] = {{v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}}};
-    auto row_a = [&](int r) __attribute__((always_inline)) -> uint32_t {
-      if (p.gather) return (uint32_t)(MIAIE_LD(p.s.row_of + slot0 + r0 + r) / p.s.top_k);
-      return (uint32_t)(r0 + r);
-    };
-    auto row_b = [&](int r) __attribute__((always_inline)) -> uint32_t { return (uint32_t)r; };
-    multiply_rows<1, 2, 128>(lds + wave * G::REGION, a, as, p.a_rows, b, bs, b_s_rows, row_pitch, (int)blocks(p.K), rows - r0, row_a,
-                             row_b, 0, 1, aq_span, bq_span, acc);
-    float h[4];
-    uint32_t m = 0;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      h[x] = swiglu(acc[0][0][x], acc[0][1][x]);
-      m = max(m, abs_bits(h[x]));
-    }
-    m = max_over_16s(m);
-    if (fg == 0) lmax[wave][fr] = m;
     __syncthreads();
-    m = 0;
+    const uint8_t* const from[2] = {b[0] + 128 * (size_t)kb0, b[1] + 128 * (size_t)kb0};
+    const int each = (n + parts - 1) / parts;
+    stream<MR, D>(lds, from, part * each, min(n, (part + 1) * each), s, acc);
+  }
+  // the eight lanes of a row
 #pragma unroll
-    for (int w = 0; w < 8; ++w) m = max(m, lmax[w][fr]);
-    const uint32_t ex = scale_of(m);
-    if (r0 + fr < rows) {
-      const size_t slot = slot0 + r0 + fr;
-      MIAIE_ST(reinterpret_cast<uint32_t*>(p.Hq + slot * h_pitch + f0 + 16 * wave + 4 * fg), pack4(h[0], h[1], h[2], h[3], inverse_f32(ex)));
-      if (wave == 0 && fg == 0) MIAIE_ST(p.Hs + (size_t)tn * p.M + slot, scale_f32(ex));
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      float v = acc[m][u];
+      v += __uint_as_float(mx::quad_swap<0xB1>(__float_as_uint(v)));
+      v += __uint_as_float(mx::quad_swap<0x4E>(__float_as_uint(v)));
+      v += __uint_as_float(mx::quad_swap<0x141>(__float_as_uint(v)));
+      acc[m][u] = v;
+    }
+}
+
+// f(number of rows taken together) for the rows that are left.
+template <class F>
+__device__ __forceinline__ void by_rows(int left, F&& f) {
+  if (left == 1)
+    f(std::integral_constant<int, 1>{});
+  else if (left == 2)
+    f(std::integral_constant<int, 2>{});
+  else
+    f(std::integral_constant<int, 4>{});
+}
+
+// Four waves; 4 / parts of them have 16 columns each, and `parts` share out the blocks
+// of k, whose sums are added in LDS in their order.
+template <Mode MODE, Out OUT>
+__global__ __launch_bounds__(256) void gemm_stream(Args p, int tiles_n, int parts) {
+  __shared__ __attribute__((aligned(16))) int8_t lds[4 * 128 * STREAM_K];
+  __shared__ float sums[4][4][16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = wave % parts, groups = 4 / parts;
+  const size_t pch = pitch(p.K);
+  StreamTile t{p.Aq, p.Bq, p.As, p.Bs, (size_t)p.a_rows, blocks(p.N), p.M};
+  int slot0 = 0, n0;
+  if constexpr (MODE == SLOTS) {
+    SlotTile at;
+    if (!slot_tile<128>(p.s, blockIdx.x, tiles_n, at)) return;
+    slot0 = at.slot, n0 = 16 * groups * at.tn;
+    t.rows = min(128, at.rows);
+    if (!p.gather) t.a += (size_t)slot0 * pch, t.as += slot0;
+    t.b += (size_t)at.e * p.N * pch, t.bs += (size_t)at.e * blocks(p.N) * blocks(p.K);
+  } else {
+    n0 = 16 * groups * blockIdx.x;
+  }
+  const int col = n0 + 16 * (wave / parts);  // of this wave; behind the last one it repeats that
+  const uint8_t* b[2];
+  const float* bs[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    b[u] = t.b + (size_t)min(col + 8 * u + (lane >> 3), p.N - 1) * pch + 16 * (lane & 7);
+    bs[u] = t.bs + min(col, p.N - 1) / 128;
+  }
+  for (int r0 = 0; r0 < t.rows; r0 += 4) {
+    auto row_a = [&](int r) __attribute__((always_inline)) -> size_t {
+      if constexpr (MODE == SLOTS) {
+        if (p.gather) return (size_t)(MIAIE_LD(p.s.row_of + slot0 + r) / p.s.top_k);
+      }
+      return (size_t)r;
+    };
+    by_rows(t.rows - r0, [&](auto mr) __attribute__((always_inline)) {
+      constexpr int MR = decltype(mr)::value;
+      float acc[MR][2];
+      stream_rows<MR, 4>(lds, p, t, b, bs, r0, row_a, part, parts, acc);
+      if ((lane & 7) == 0)
+#pragma unroll
+        for (int m = 0; m < MR; ++m)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) sums[wave][m][8 * u + (lane >> 3)] = acc[m][u];
+    });
+    __syncthreads();
+    // thread: row tid / 64, column tid % 64 of the workgroup's
+    const int m = r0 + wave, n = n0 + lane;
+    if (m < t.rows && lane < 16 * groups && n < p.N) {
+      float sum = 0.f;
+      for (int k = 0; k < parts; ++k) sum += sums[lane / 16 * parts + k][wave][lane % 16];
+      using T = std::conditional_t<OUT == OUT_F32, float, __bf16>;
+      MIAIE_ST(static_cast<T*>(p.C) + (size_t)(slot0 + m) * p.ldc + n, (T)sum);
+    }
+  }
+}
+
+// silu(gate) up of 128 columns of H: sixteen waves, each with eight gate and eight up
+// columns over all of k.
+__global__ __launch_bounds__(1024) void glu_stream(Args p, int tiles_n) {
+  __shared__ __attribute__((aligned(16))) int8_t lds[4 * 128 * STREAM_K];
+  __shared__ __attribute__((aligned(16))) float h[4][128];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const size_t pch = pitch(p.K), b_s_rows = blocks(2 * (long)p.N), h_pitch = pitch(p.N);
+  SlotTile at;
+  if (!slot_tile<128>(p.s, blockIdx.x, tiles_n, at)) return;
+  const int slot0 = at.slot, f0 = 128 * at.tn;
+  StreamTile t{p.gather ? p.Aq : p.Aq + (size_t)slot0 * pch, p.Bq + (size_t)at.e * 2 * p.N * pch, p.gather ? p.As : p.As + slot0,
+               p.Bs + (size_t)at.e * b_s_rows * blocks(p.K), (size_t)p.a_rows, b_s_rows, min(128, at.rows)};
+  const uint8_t* const gate = t.b + (size_t)(f0 + 8 * wave + (lane >> 3)) * pch + 16 * (lane & 7);
+  const uint8_t* const b[2] = {gate, gate + (size_t)p.N * pch};
+  const float* const bs[2] = {t.bs + f0 / 128, t.bs + (p.N + f0) / 128};
+  for (int r0 = 0; r0 < t.rows; r0 += 4) {
+    auto row_a = [&](int r) __attribute__((always_inline)) -> size_t {
+      return p.gather ? (size_t)(MIAIE_LD(p.s.row_of + slot0 + r) / p.s.top_k) : (size_t)r;
+    };
+    by_rows(t.rows - r0, [&](auto mr) __attribute__((always_inline)) {
+      constexpr int MR = decltype(mr)::value;
+      float acc[MR][2];
+      stream_rows<MR, 2>(lds, p, t, b, bs, r0, row_a, 0, 1, acc);
+      if ((lane & 7) == 0)
+#pragma unroll
+        for (int m = 0; m < MR; ++m) h[m][8 * wave + (lane >> 3)] = swiglu(acc[m][0], acc[m][1]);
+    });
+    __syncthreads();
+    if (tid < 128 && r0 + tid / 32 < t.rows) {  // 32 lanes a row, four columns each
+      const v4f v = *reinterpret_cast<const v4f*>(&h[tid / 32][4 * (tid & 31)]);
+      uint32_t m = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
+      m = max(m, mx::quad_swap<0xB1>(m));
+      m = max(m, mx::quad_swap<0x4E>(m));
+      m = max(m, mx::quad_swap<0x141>(m));
+      m = max(m, mx::quad_swap<0x140>(m));
+      uint32_t w = m;
+      swap16(m, w);
+      const uint32_t e = scale_of(max(m, w));
+      const size_t slot = slot0 + r0 + tid / 32;
+      MIAIE_ST(reinterpret_cast<uint32_t*>(p.Hq + slot * h_pitch + f0 + 4 * (tid & 31)), pack4(v[0], v[1], v[2], v[3], inverse_f32(e)));
+      if ((tid & 31) == 0) MIAIE_ST(p.Hs + (size_t)at.tn * p.M + slot, scale_f32(e));
     }
     __syncthreads();
   }
@@ -1121,17 +1100,13 @@ int run_slots_large(miaie_ctx* ctx, const Args& p) {
   return check_launch(ctx, e, "gemm_fp8_slots");
 }
 
-template <int MI, int NJ, Mode MODE, Out OUT, int BBLOCK>
-int run_rows(miaie_ctx* ctx, const Args& p) {
-  using G = RowsGeom<MI, NJ>;
-  const int groups = ((int)blocks(p.K) + 1) / 2;
-  const int most = std::min(16, 163840 / G::REGION), each = (groups + most - 1) / most, waves = (groups + each - 1) / each;
-  const long tiles_n = (p.N + 16 * NJ - 1l) / (16 * NJ);
-  const long tiles_m = MODE == SLOTS ? most_slot_tiles(p.s, 128) : (p.M + 16 * MI - 1l) / (16 * MI);
-  const long grid = MODE == SLOTS ? (tiles_m * tiles_n + 7) / 8 * 8 : tiles_m * tiles_n;
-  const hipError_t e = launch<gemm_rows<MI, NJ, MODE, OUT, BBLOCK>>(ctx->device, dim3((unsigned)grid), dim3(64 * waves),
-                                                                    (size_t)waves * G::REGION, ctx->stream, p, (int)tiles_n, waves);
-  return check_launch(ctx, e, "gemm_fp8_rows");
+template <Mode MODE, Out OUT>
+int run_stream(miaie_ctx* ctx, const Args& p) {
+  const int steps = (int)blocks(p.K), parts = steps >= 32 ? 4 : steps >= 16 ? 2 : 1;
+  const long cols = 16 * (4 / parts), tiles_n = (p.N + cols - 1) / cols;
+  const long grid = MODE == SLOTS ? (most_slot_tiles(p.s, 128) * tiles_n + 7) / 8 * 8 : tiles_n;
+  const hipError_t e = launch<gemm_stream<MODE, OUT>>(ctx->device, dim3((unsigned)grid), dim3(256), 0, ctx->stream, p, (int)tiles_n, parts);
+  return check_launch(ctx, e, "gemm_fp8_stream");
 }
 
 // ---- choice of tile: the lowest estimated time.  A CU has `at_once` workgroups of a
@@ -1163,7 +1138,9 @@ double slots_us(const TileTime& t, const Args& p, double cols, int cus) {
 
 template <Out OUT, int BBLOCK>
 int run_dense(miaie_ctx* ctx, const Args& p) {
-  if (p.M <= 16) return run_rows<1, 1, DENSE, OUT, BBLOCK>(ctx, p);
+  if constexpr (BBLOCK == 128) {
+    if (p.M <= 4) return run_stream<DENSE, OUT>(ctx, p);
+  }
   const double us[] = {dense_us(kLarge, p, ctx->cus), dense_us(kBlock, p, ctx->cus), dense_us(kSquare, p, ctx->cus),
                        dense_us(kFlat, p, ctx->cus), dense_us(kSmall, p, ctx->cus)};
   switch (std::min_element(us, us + 5) - us) {
@@ -1175,9 +1152,9 @@ int run_dense(miaie_ctx* ctx, const Args& p) {
   }
 }
 
-// Few slots an expert: the waves of gemm_rows and glu_rows have more of B in flight.
+// Few slots an expert.  (Beyond four a row tile of 64 is as quick, and reads B once.)
 bool few_slots(const Args& p, int cols) {
-  return (long)p.s.tokens * p.s.top_k <= 16l * p.s.experts && p.M / 128 * ((p.N + cols - 1l) / cols) < kThreads / 2048;
+  return (long)p.s.tokens * p.s.top_k <= 4l * p.s.experts && most_slot_tiles(p.s, 128) * ((p.N + cols - 1l) / cols) < kThreads / 2048;
 }
 
 template <Out OUT>
@@ -1185,15 +1162,23 @@ int run_slots(miaie_ctx* ctx, const Args& p) {
   if constexpr (OUT == OUT_GLU) {
     if (few_slots(p, 128)) {
       const long grid = (most_slot_tiles(p.s, 128) * (p.N / 128) + 7) / 8 * 8;
-      const hipError_t e = launch<glu_rows>(ctx->device, dim3((unsigned)grid), dim3(512), 0, ctx->stream, p, p.N / 128);
-      return check_launch(ctx, e, "glu_rows");
+      const hipError_t e = launch<glu_stream>(ctx->device, dim3((unsigned)grid), dim3(1024), 0, ctx->stream, p, p.N / 128);
+      return check_launch(ctx, e, "glu_stream");
     }
-    return slots_us(kGlu, p, 128, ctx->cus) < slots_us(kBlock, p, 128, ctx->cus) ? run_tile<Glu, SLOTS, OUT, 128>(ctx, p)
-                                                                                  : run_tile<Block, SLOTS, OUT, 128>(ctx, p);
+    const double us[] = {slots_us(kLarge, p, 128, ctx->cus), slots_us(kBlock, p, 128, ctx->cus), slots_us(kGlu, p, 128, ctx->cus)};
+    switch (std::min_element(us, us + 3) - us) {
+      case 1: return run_tile<Block, SLOTS, OUT, 128>(ctx, p);
+      case 2: return run_tile<Glu, SLOTS, OUT, 128>(ctx, p);
+      default: return run_slots_large<OUT>(ctx, p);
+    }
   } else {
-    if (few_slots(p, 16)) return run_rows<1, 1, SLOTS, OUT, 128>(ctx, p);
-    return slots_us(kSmall, p, 64, ctx->cus) < slots_us(kSquare, p, 128, ctx->cus) ? run_tile<Small, SLOTS, OUT, 128>(ctx, p)
-                                                                                   : run_tile<Square, SLOTS, OUT, 128>(ctx, p);
+    if (few_slots(p, 16)) return run_stream<SLOTS, OUT>(ctx, p);
+    const double us[] = {slots_us(kLarge, p, 256, ctx->cus), slots_us(kSquare, p, 128, ctx->cus), slots_us(kSmall, p, 64, ctx->cus)};
+    switch (std::min_element(us, us + 3) - us) {
+      case 1: return run_tile<Square, SLOTS, OUT, 128>(ctx, p);
+      case 2: return run_tile<Small, SLOTS, OUT, 128>(ctx, p);
+      default: return run_slots_large<OUT>(ctx, p);
+    }
   }
 }
 
