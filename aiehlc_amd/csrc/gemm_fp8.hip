@@ -853,35 +853,43 @@ __device__ __forceinline__ void widen(v4u q, float (&x)[16]) {
 }
 
 // acc[m][u] += row m of A (in LDS, STREAM_K blocks a row) times this lane's part of
-// row l / 8 of b[u], over the blocks kb0 + first .. kb0 + last - 1.  s[m][u]: lane kb
-// has the scale of block kb0 + kb.
+// row l / 8 of b[u], over the blocks first .. last - 1 of those in LDS; lane kb of
+// sa[m] and sb[h] has their scales of block kb, h the half of the U that u is in.
 // D blocks are loaded together, and as many behind them.
-template <int MR, int D>
-__device__ __forceinline__ void stream(const int8_t* lds, const uint8_t* const (&b)[2], int first, int last, const float (&s)[MR][2],
-                                       float (&acc)[MR][2]) {
+template <int MR, int U, int D>
+__device__ __forceinline__ void stream(const int8_t* lds, const uint8_t* const (&b)[U], size_t skip, int first, int last,
+                                       const float (&sa)[MR], const float (&sb)[2], float (&acc)[MR][U]) {
   const int lane = threadIdx.x & 63;
-  v4u q[2][D][2];
-  auto load = [&](int kb, v4u (&to)[D][2]) __attribute__((always_inline)) {
+  v4u q[2][D][U];
+  auto load = [&](int kb, v4u (&to)[D][U]) __attribute__((always_inline)) {
 #pragma unroll
     for (int d = 0; d < D; ++d)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)  // (blocks behind the last one repeat it)
-        to[d][u] = MIAIE_LD(reinterpret_cast<const v4u*>(b[u] + 128 * (size_t)min(kb + d, last - 1)));
+      for (int u = 0; u < U; ++u)  // (blocks behind the last one repeat it)
+        to[d][u] = MIAIE_LD(reinterpret_cast<const v4u*>(b[u] + skip + 128 * (size_t)min(kb + d, last - 1)));
   };
-  auto multiply = [&](int kb, const v4u (&from)[D][2]) __attribute__((always_inline)) {
+  auto of_block = [&](float v, int kb) __attribute__((always_inline)) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), kb));
+  };
+  auto multiply = [&](int kb, const v4u (&from)[D][U]) __attribute__((always_inline)) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       if (kb + d >= last) return;
-      float x[2][16];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) widen(from[d][u], x[u]);
+      for (int h = 0; h < 2; ++h) {
+        const float scale = of_block(sb[h], kb + d);
+        float x[U / 2][16];
 #pragma unroll
-      for (int m = 0; m < MR; ++m) {
-        float a[16];
-        widen(*reinterpret_cast<const v4u*>(lds + 128 * (m * STREAM_K + kb + d) + 16 * (lane & 7)), a);
+        for (int u = 0; u < U / 2; ++u) widen(from[d][h * (U / 2) + u], x[u]);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          acc[m][u] = __builtin_fmaf(dot16(x[u], a), __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s[m][u]), kb + d)), acc[m][u]);
+        for (int m = 0; m < MR; ++m) {
+          float a[16];
+          widen(*reinterpret_cast<const v4u*>(lds + 128 * (m * STREAM_K + kb + d) + 16 * (lane & 7)), a);
+          const float f = scale * of_block(sa[m], kb + d);
+#pragma unroll
+          for (int u = 0; u < U / 2; ++u)
+            acc[m][h * (U / 2) + u] = __builtin_fmaf(dot16(x[u], a), f, acc[m][h * (U / 2) + u]);
+        }
       }
     }
   };
@@ -904,16 +912,19 @@ struct StreamTile {
   int rows;
 };
 
-// acc[m][u] of rows r0 .. r0 + MR - 1 (rows behind the last repeat it) and this wave's
-// b0 and b1, the sums over the lanes of a row in each of them.
-template <int MR, int D, class RowA>
-__device__ __forceinline__ void stream_rows(int8_t* lds, const Args& p, const StreamTile& t, const uint8_t* const (&b)[2],
-                                            const float* const (&bs)[2], int r0, RowA row_a, int part, int parts, float (&acc)[MR][2]) {
+// acc[m][u]: the sums of rows r0 .. r0 + MR - 1 of A (rows behind the last repeat it)
+// and this wave's b[u], with the scales bs[0] of the first half of them and bs[1] of
+// the second, over the part of k that is `part` of `parts`; in each of a row's lanes.
+template <int MR, int U, int D, class RowA>
+__device__ __forceinline__ void stream_rows(int8_t* lds, const Args& p, const StreamTile& t, const uint8_t* const (&b)[U],
+                                            const float* const (&bs)[2], int r0, RowA row_a, int part, int parts, float (&acc)[MR][U]) {
   const int tid = threadIdx.x, lane = tid & 63, threads = blockDim.x;
   const int steps = (int)blocks(p.K);
   const size_t pch = pitch(p.K);
 #pragma unroll
-  for (int m = 0; m < MR; ++m) acc[m][0] = acc[m][1] = 0.f;
+  for (int m = 0; m < MR; ++m)
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc[m][u] = 0.f;
   for (int kb0 = 0; kb0 < steps; kb0 += STREAM_K) {
     const int n = min(STREAM_K, steps - kb0);
     if (kb0 > 0 || r0 > 0) __syncthreads();
@@ -922,24 +933,21 @@ __device__ __forceinline__ void stream_rows(int8_t* lds, const Args& p, const St
       const v4u v = MIAIE_LD(reinterpret_cast<const v4u*>(t.a + row_a(min(r0 + m, t.rows - 1)) * pch + 128 * (size_t)kb0 + 16 * c));
       *reinterpret_cast<v4u*>(lds + 128 * m * STREAM_K + 16 * c) = v;
     }
-    float s[MR][2];
+    float sa[MR], sb[2];
     const size_t kb = kb0 + min(lane, n - 1);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const float sb = MIAIE_LD(bs[u] + kb * t.b_step);
+    for (int h = 0; h < 2; ++h) sb[h] = MIAIE_LD(bs[h] + kb * t.b_step);
 #pragma unroll
-      for (int m = 0; m < MR; ++m) s[m][u] = sb * MIAIE_LD(t.as + kb * t.a_step + row_a(min(r0 + m, t.rows - 1)));
-    }
+    for (int m = 0; m < MR; ++m) sa[m] = MIAIE_LD(t.as + kb * t.a_step + row_a(min(r0 + m, t.rows - 1)));
     __syncthreads();
-    const uint8_t* const from[2] = {b[0] + 128 * (size_t)kb0, b[1] + 128 * (size_t)kb0};
     const int each = (n + parts - 1) / parts;
-    stream<MR, D>(lds, from, part * each, min(n, (part + 1) * each), s, acc);
+    stream<MR, U, D>(lds, b, 128 * (size_t)kb0, part * each, min(n, (part + 1) * each), sa, sb, acc);
   }
   // the eight lanes of a row
 #pragma unroll
   for (int m = 0; m < MR; ++m)
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
+    for (int u = 0; u < U; ++u) {
       float v = acc[m][u];
       v += __uint_as_float(mx::quad_swap<0xB1>(__float_as_uint(v)));
       v += __uint_as_float(mx::quad_swap<0x4E>(__float_as_uint(v)));
@@ -998,7 +1006,7 @@ __global__ __launch_bounds__(256) void gemm_stream(Args p, int tiles_n, int part
     by_rows(t.rows - r0, [&](auto mr) __attribute__((always_inline)) {
       constexpr int MR = decltype(mr)::value;
       float acc[MR][2];
-      stream_rows<MR, 4>(lds, p, t, b, bs, r0, row_a, part, parts, acc);
+      stream_rows<MR, 2, 4>(lds, p, t, b, bs, r0, row_a, part, parts, acc);
       if ((lane & 7) == 0)
 #pragma unroll
         for (int m = 0; m < MR; ++m)
@@ -1017,9 +1025,9 @@ __global__ __launch_bounds__(256) void gemm_stream(Args p, int tiles_n, int part
   }
 }
 
-// silu(gate) up of 128 columns of H: sixteen waves, each with eight gate and eight up
-// columns over all of k.
-__global__ __launch_bounds__(1024) void glu_stream(Args p, int tiles_n) {
+// silu(gate) up of 128 columns of H: eight waves, each with sixteen gate and sixteen up
+// columns over all of k; two workgroups fit a CU.
+__global__ __launch_bounds__(512) void glu_stream(Args p, int tiles_n) {
   __shared__ __attribute__((aligned(16))) int8_t lds[4 * 128 * STREAM_K];
   __shared__ __attribute__((aligned(16))) float h[4][128];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1029,8 +1037,10 @@ __global__ __launch_bounds__(1024) void glu_stream(Args p, int tiles_n) {
   const int slot0 = at.slot, f0 = 128 * at.tn;
   StreamTile t{p.gather ? p.Aq : p.Aq + (size_t)slot0 * pch, p.Bq + (size_t)at.e * 2 * p.N * pch, p.gather ? p.As : p.As + slot0,
                p.Bs + (size_t)at.e * b_s_rows * blocks(p.K), (size_t)p.a_rows, b_s_rows, min(128, at.rows)};
-  const uint8_t* const gate = t.b + (size_t)(f0 + 8 * wave + (lane >> 3)) * pch + 16 * (lane & 7);
-  const uint8_t* const b[2] = {gate, gate + (size_t)p.N * pch};
+  const uint8_t* b[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    b[u] = t.b + ((size_t)(u >> 1) * p.N + f0 + 16 * wave + 8 * (u & 1) + (lane >> 3)) * pch + 16 * (lane & 7);
   const float* const bs[2] = {t.bs + f0 / 128, t.bs + (p.N + f0) / 128};
   for (int r0 = 0; r0 < t.rows; r0 += 4) {
     auto row_a = [&](int r) __attribute__((always_inline)) -> size_t {
@@ -1038,11 +1048,13 @@ __global__ __launch_bounds__(1024) void glu_stream(Args p, int tiles_n) {
     };
     by_rows(t.rows - r0, [&](auto mr) __attribute__((always_inline)) {
       constexpr int MR = decltype(mr)::value;
-      float acc[MR][2];
-      stream_rows<MR, 2>(lds, p, t, b, bs, r0, row_a, 0, 1, acc);
+      float acc[MR][4];
+      stream_rows<MR, 4, MR == 4 ? 1 : 2>(lds, p, t, b, bs, r0, row_a, 0, 1, acc);
       if ((lane & 7) == 0)
 #pragma unroll
-        for (int m = 0; m < MR; ++m) h[m][8 * wave + (lane >> 3)] = swiglu(acc[m][0], acc[m][1]);
+        for (int m = 0; m < MR; ++m)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) h[m][16 * wave + 8 * u + (lane >> 3)] = swiglu(acc[m][u], acc[m][2 + u]);
     });
     __syncthreads();
     if (tid < 128 && r0 + tid / 32 < t.rows) {  // 32 lanes a row, four columns each
@@ -1130,10 +1142,12 @@ double tile_us(const TileTime& t, double tiles, long steps, int cus) {
 double dense_us(const TileTime& t, const Args& p, int cus) {
   return tile_us(t, (double)((p.M + t.bm - 1l) / t.bm) * (double)((p.N + t.bn - 1l) / t.bn), (long)blocks(p.K), cus);
 }
-// (an expert's last tile is half full on average)
-double slots_us(const TileTime& t, const Args& p, double cols, int cus) {
+// Slots: an expert's last tile is half full on average; tiles of up to 128 rows and
+// columns take a tenth longer than among dense ones, B coming from memory.
+double slots_us(const TileTime& t, const Args& p, int cols, int cus) {
   const double n = (double)p.s.tokens * p.s.top_k, used = std::min<double>(p.s.experts, n);
-  return tile_us(t, std::max(used, n / t.bm + used / 2) * ((p.N + cols - 1) / cols), (long)blocks(p.K), cus);
+  const double us = tile_us(t, std::max(used, n / t.bm + used / 2) * (double)((p.N + cols - 1l) / cols), (long)blocks(p.K), cus);
+  return t.bn <= 128 ? 1.1 * us : us;
 }
 
 template <Out OUT, int BBLOCK>
@@ -1162,7 +1176,7 @@ int run_slots(miaie_ctx* ctx, const Args& p) {
   if constexpr (OUT == OUT_GLU) {
     if (few_slots(p, 128)) {
       const long grid = (most_slot_tiles(p.s, 128) * (p.N / 128) + 7) / 8 * 8;
-      const hipError_t e = launch<glu_stream>(ctx->device, dim3((unsigned)grid), dim3(1024), 0, ctx->stream, p, p.N / 128);
+      const hipError_t e = launch<glu_stream>(ctx->device, dim3((unsigned)grid), dim3(512), 0, ctx->stream, p, p.N / 128);
       return check_launch(ctx, e, "glu_stream");
     }
     const double us[] = {slots_us(kLarge, p, 128, ctx->cus), slots_us(kBlock, p, 128, ctx->cus), slots_us(kGlu, p, 128, ctx->cus)};
