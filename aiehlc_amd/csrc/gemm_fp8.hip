@@ -853,43 +853,35 @@ __device__ __forceinline__ void widen(v4u q, float (&x)[16]) {
 }
 
 // acc[m][u] += row m of A (in LDS, STREAM_K blocks a row) times this lane's part of
-// row l / 8 of b[u], over the blocks first .. last - 1 of those in LDS; lane kb of
-// sa[m] and sb[h] has their scales of block kb, h the half of the U that u is in.
+// row l / 8 of b[u], over the blocks kb0 + first .. kb0 + last - 1.  s[m][u]: lane kb
+// has the scale of block kb0 + kb.
 // D blocks are loaded together, and as many behind them.
-template <int MR, int U, int D>
-__device__ __forceinline__ void stream(const int8_t* lds, const uint8_t* const (&b)[U], size_t skip, int first, int last,
-                                       const float (&sa)[MR], const float (&sb)[2], float (&acc)[MR][U]) {
+template <int MR, int D>
+__device__ __forceinline__ void stream(const int8_t* lds, const uint8_t* const (&b)[2], int first, int last, const float (&s)[MR][2],
+                                       float (&acc)[MR][2]) {
   const int lane = threadIdx.x & 63;
-  v4u q[2][D][U];
-  auto load = [&](int kb, v4u (&to)[D][U]) __attribute__((always_inline)) {
+  v4u q[2][D][2];
+  auto load = [&](int kb, v4u (&to)[D][2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int d = 0; d < D; ++d)
 #pragma unroll
-      for (int u = 0; u < U; ++u)  // (blocks behind the last one repeat it)
-        to[d][u] = MIAIE_LD(reinterpret_cast<const v4u*>(b[u] + skip + 128 * (size_t)min(kb + d, last - 1)));
+      for (int u = 0; u < 2; ++u)  // (blocks behind the last one repeat it)
+        to[d][u] = MIAIE_LD(reinterpret_cast<const v4u*>(b[u] + 128 * (size_t)min(kb + d, last - 1)));
   };
-  auto of_block = [&](float v, int kb) __attribute__((always_inline)) {
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), kb));
-  };
-  auto multiply = [&](int kb, const v4u (&from)[D][U]) __attribute__((always_inline)) {
+  auto multiply = [&](int kb, const v4u (&from)[D][2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int d = 0; d < D; ++d) {
       if (kb + d >= last) return;
+      float x[2][16];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float scale = of_block(sb[h], kb + d);
-        float x[U / 2][16];
+      for (int u = 0; u < 2; ++u) widen(from[d][u], x[u]);
 #pragma unroll
-        for (int u = 0; u < U / 2; ++u) widen(from[d][h * (U / 2) + u], x[u]);
+      for (int m = 0; m < MR; ++m) {
+        float a[16];
+        widen(*reinterpret_cast<const v4u*>(lds + 128 * (m * STREAM_K + kb + d) + 16 * (lane & 7)), a);
 #pragma unroll
-        for (int m = 0; m < MR; ++m) {
-          float a[16];
-          widen(*reinterpret_cast<const v4u*>(lds + 128 * (m * STREAM_K + kb + d) + 16 * (lane & 7)), a);
-          const float f = scale * of_block(sa[m], kb + d);
-#pragma unroll
-          for (int u = 0; u < U / 2; ++u)
-            acc[m][h * (U / 2) + u] = __builtin_fmaf(dot16(x[u], a), f, acc[m][h * (U / 2) + u]);
-        }
+        for (int u = 0; u < 2; ++u)
+          acc[m][u] = __builtin_fmaf(dot16(x[u], a), __int_as_float(__builtin_amdgcn_readlane(__float_as_int(s[m][u]), kb + d)), acc[m][u]);
       }
     }
   };
@@ -912,19 +904,16 @@ struct StreamTile {
   int rows;
 };
 
-// acc[m][u]: the sums of rows r0 .. r0 + MR - 1 of A (rows behind the last repeat it)
-// and this wave's b[u], with the scales bs[0] of the first half of them and bs[1] of
-// the second, over the part of k that is `part` of `parts`; in each of a row's lanes.
-template <int MR, int U, int D, class RowA>
-__device__ __forceinline__ void stream_rows(int8_t* lds, const Args& p, const StreamTile& t, const uint8_t* const (&b)[U],
-                                            const float* const (&bs)[2], int r0, RowA row_a, int part, int parts, float (&acc)[MR][U]) {
+// acc[m][u] of rows r0 .. r0 + MR - 1 (rows behind the last repeat it) and this wave's
+// b0 and b1, the sums over the lanes of a row in each of them.
+template <int MR, int D, class RowA>
+__device__ __forceinline__ void stream_rows(int8_t* lds, const Args& p, const StreamTile& t, const uint8_t* const (&b)[2],
+                                            const float* const (&bs)[2], int r0, RowA row_a, int part, int parts, float (&acc)[MR][2]) {
   const int tid = threadIdx.x, lane = tid & 63, threads = blockDim.x;
   const int steps = (int)blocks(p.K);
   const size_t pch = pitch(p.K);
 #pragma unroll
-  for (int m = 0; m < MR; ++m)
-#pragma unroll
-    for (int u = 0; u < U; ++u) acc[m][u] = 0.f;
+  for (int m = 0; m < MR; ++m) acc[m][0] = acc[m][1] = 0.f;
   for (int kb0 = 0; kb0 < steps; kb0 += STREAM_K) {
     const int n = min(STREAM_K, steps - kb0);
     if (kb0 > 0 || r0 > 0) __syncthreads();
@@ -933,21 +922,24 @@ __device__ __forceinline__ void stream_rows(int8_t* lds, const Args& p, const St
       const v4u v = MIAIE_LD(reinterpret_cast<const v4u*>(t.a + row_a(min(r0 + m, t.rows - 1)) * pch + 128 * (size_t)kb0 + 16 * c));
       *reinterpret_cast<v4u*>(lds + 128 * m * STREAM_K + 16 * c) = v;
     }
-    float sa[MR], sb[2];
+    float s[MR][2];
     const size_t kb = kb0 + min(lane, n - 1);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) sb[h] = MIAIE_LD(bs[h] + kb * t.b_step);
+    for (int u = 0; u < 2; ++u) {
+      const float sb = MIAIE_LD(bs[u] + kb * t.b_step);
 #pragma unroll
-    for (int m = 0; m < MR; ++m) sa[m] = MIAIE_LD(t.as + kb * t.a_step + row_a(min(r0 + m, t.rows - 1)));
+      for (int m = 0; m < MR; ++m) s[m][u] = sb * MIAIE_LD(t.as + kb * t.a_step + row_a(min(r0 + m, t.rows - 1)));
+    }
     __syncthreads();
+    const uint8_t* const from[2] = {b[0] + 128 * (size_t)kb0, b[1] + 128 * (size_t)kb0};
     const int each = (n + parts - 1) / parts;
-    stream<MR, U, D>(lds, b, 128 * (size_t)kb0, part * each, min(n, (part + 1) * each), sa, sb, acc);
+    stream<MR, D>(lds, from, part * each, min(n, (part + 1) * each), s, acc);
   }
   // the eight lanes of a row
 #pragma unroll
   for (int m = 0; m < MR; ++m)
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < 2; ++u) {
       float v = acc[m][u];
       v += __uint_as_float(mx::quad_swap<0xB1>(__float_as_uint(v)));
       v += __uint_as_float(mx::quad_swap<0x4E>(__float_as_uint(v)));
@@ -1006,7 +998,7 @@ __global__ __launch_bounds__(256) void gemm_stream(Args p, int tiles_n, int part
     by_rows(t.rows - r0, [&](auto mr) __attribute__((always_inline)) {
       constexpr int MR = decltype(mr)::value;
       float acc[MR][2];
-      stream_rows<MR, 2, 4>(lds, p, t, b, bs, r0, row_a, part, parts, acc);
+      stream_rows<MR, 4>(lds, p, t, b, bs, r0, row_a, part, parts, acc);
       if ((lane & 7) == 0)
 #pragma unroll
         for (int m = 0; m < MR; ++m)
@@ -1025,51 +1017,128 @@ __global__ __launch_bounds__(256) void gemm_stream(Args p, int tiles_n, int part
   }
 }
 
-// silu(gate) up of 128 columns of H: eight waves, each with sixteen gate and sixteen up
-// columns over all of k; two workgroups fit a CU.
-__global__ __launch_bounds__(512) void glu_stream(Args p, int tiles_n) {
-  __shared__ __attribute__((aligned(16))) int8_t lds[4 * 128 * STREAM_K];
-  __shared__ __attribute__((aligned(16))) float h[4][128];
+// The block product in bf16, which holds every element: 16 conversions and four
+// instructions a fragment, sums as fp32 has them.
+struct Wide {
+  v8bf v[4];
+  __device__ __forceinline__ explicit Wide(v8i x) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+      const v2bf c0 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * q], 1.f, false), c1 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * q], 1.f, true),
+                 c2 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * q + 1], 1.f, false), c3 = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * q + 1], 1.f, true);
+      v[q] = v8bf{c0[0], c0[1], c1[0], c1[1], c2[0], c2[1], c3[0], c3[1]};
+    }
+  }
+};
+__device__ __forceinline__ v4f mfma_wide(const Wide& b, const Wide& a) {
+  v4f p = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int q = 0; q < 4; ++q) p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b.v[q], a.v[q], p, 0, 0, 0);
+  return p;
+}
+
+// silu(gate) up of 128 columns of H and a block of slots, four rows at a time: eight
+// waves, each with 16 gate and 16 up columns over all of k.  A wave copies 256 bytes
+// (two blocks of k, a group) of its 32 rows of B and of A's rows into a part of LDS of
+// its own, waits for its own copies (no barriers) and multiplies; the next group is on
+// its way once this one's fragments are in registers.  Chunk c (16 bytes) of row r lies
+// at c ^ (r % 16).  Two workgroups fit a CU, so that one starts while another reads
+// (as loads of whole lines into registers, like gemm_stream, one fits: 101 us for 86
+// at 64 experts of 2048 x 4096, eight tokens of eight).
+constexpr int kGluRows = 4, kGluRegion = 2 * 4096 + 256 * kGluRows;
+__global__ __launch_bounds__(512, 4) void glu_rows(Args p, int tiles_n) {
+  __shared__ __attribute__((aligned(1024))) int8_t lds[8 * kGluRegion];
+  __shared__ uint32_t lmax[8][16];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const size_t pch = pitch(p.K), b_s_rows = blocks(2 * (long)p.N), h_pitch = pitch(p.N);
-  SlotTile at;
-  if (!slot_tile<128>(p.s, blockIdx.x, tiles_n, at)) return;
-  const int slot0 = at.slot, f0 = 128 * at.tn;
-  StreamTile t{p.gather ? p.Aq : p.Aq + (size_t)slot0 * pch, p.Bq + (size_t)at.e * 2 * p.N * pch, p.gather ? p.As : p.As + slot0,
-               p.Bs + (size_t)at.e * b_s_rows * blocks(p.K), (size_t)p.a_rows, b_s_rows, min(128, at.rows)};
-  const uint8_t* b[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u)
-    b[u] = t.b + ((size_t)(u >> 1) * p.N + f0 + 16 * wave + 8 * (u & 1) + (lane >> 3)) * pch + 16 * (lane & 7);
-  const float* const bs[2] = {t.bs + f0 / 128, t.bs + (p.N + f0) / 128};
-  for (int r0 = 0; r0 < t.rows; r0 += 4) {
-    auto row_a = [&](int r) __attribute__((always_inline)) -> size_t {
-      return p.gather ? (size_t)(MIAIE_LD(p.s.row_of + slot0 + r) / p.s.top_k) : (size_t)r;
+  const int fr = lane & 15, fg = lane >> 4;
+  const uint32_t row_pitch = (uint32_t)pitch(p.K);
+  const size_t b_s_rows = blocks(2 * (long)p.N);
+  const int steps = (int)blocks(p.K), groups = (steps + 1) / 2;
+  SlotTile t;
+  if (!slot_tile<128>(p.s, blockIdx.x, tiles_n, t)) return;
+  const int e = t.e, tn = t.tn, slot0 = t.slot, f0 = 128 * tn, rows = min(128, t.rows);
+  const uint8_t* const a = p.gather ? p.Aq : p.Aq + (size_t)slot0 * row_pitch;
+  const float* const as = p.gather ? p.As : p.As + slot0;
+  const uint8_t* const gate = p.Bq + ((size_t)e * 2 * p.N + f0 + 16 * wave) * row_pitch;
+  const uint8_t* const b[2] = {gate, gate + (size_t)p.N * row_pitch};
+  const float* const gate_s = p.Bs + (size_t)e * b_s_rows * steps + f0 / 128;
+  const float* const bs[2] = {gate_s, gate_s + p.N / 128};
+  const dbg::Span aq_span = dbg::span_of(p.Aq), bq_span = dbg::span_of(p.Bq);  // (debug build only)
+  const size_t h_pitch = pitch(p.N);
+  int8_t* const mine = lds + wave * kGluRegion;
+  const uint32_t mine0 = dev::lds_addr(mine);
+  for (int r0 = 0; r0 < rows; r0 += kGluRows) {
+    const int n = min(kGluRows, rows - r0);
+    auto row_a = [&](int r) __attribute__((always_inline)) -> uint32_t {
+      r = slot0 + r0 + min(r, n - 1);  // (rows behind the last repeat it)
+      return p.gather ? (uint32_t)(MIAIE_LD(p.s.row_of + r) / p.s.top_k) : (uint32_t)(r - slot0);
     };
-    by_rows(t.rows - r0, [&](auto mr) __attribute__((always_inline)) {
-      constexpr int MR = decltype(mr)::value;
-      float acc[MR][4];
-      stream_rows<MR, 4, MR == 4 ? 1 : 2>(lds, p, t, b, bs, r0, row_a, 0, 1, acc);
-      if ((lane & 7) == 0)
+    const uint32_t a_row = row_a(fg) , s_row = row_a(fr);
+    v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
+    float sa[2], sb[2][2];
+    auto copy = [&](int g) __attribute__((always_inline)) {
+      const uint32_t mask = 2 * g + 1 < steps ? 15 : 7;  // (half a group: its first block again)
 #pragma unroll
-        for (int m = 0; m < MR; ++m)
+      for (int k = 0; k < 2; ++k) {
+        const size_t kb = min(2 * g + k, steps - 1);
+        sa[k] = MIAIE_LD(as + kb * p.a_rows + s_row);
 #pragma unroll
-          for (int u = 0; u < 2; ++u) h[m][16 * wave + 8 * u + (lane >> 3)] = swiglu(acc[m][u], acc[m][2 + u]);
-    });
+        for (int j = 0; j < 2; ++j) sb[k][j] = MIAIE_LD(bs[j] + kb * b_s_rows);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          dev::gload_lds16(b[j] + 256 * (size_t)g, (uint32_t)(4 * x + fg) * row_pitch + 16 * ((fr ^ (4 * x + fg)) & mask),
+                           mine0 + 4096 * j + 1024 * x, bq_span);
+      dev::gload_lds16(a + 256 * (size_t)g, a_row * row_pitch + 16 * ((fr ^ fg) & mask), mine0 + 8192, aq_span);
+    };
+    auto half = [&](int k) __attribute__((always_inline)) {
+      const int c0 = 8 * k + fg, c1 = c0 + 4, r = min(fr, kGluRows - 1);
+      auto fragment = [&](int at, int row) __attribute__((always_inline)) {
+        return Wide(join(*reinterpret_cast<const v4i*>(mine + at + 256 * row + 16 * (c0 ^ row)),
+                         *reinterpret_cast<const v4i*>(mine + at + 256 * row + 16 * (c1 ^ row))));
+      };
+      const Wide fa = fragment(8192, r);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const v4f q = mfma_wide(fragment(4096 * j, fr), fa);
+        const float f = sa[k] * sb[k][j];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[j][x] = __builtin_fmaf(q[x], f, acc[j][x]);
+      }
+    };
+    copy(0);
+    for (int g = 0; g < groups; ++g) {
+      dev::wait_vmcnt<0>();
+      asm volatile("" ::: "memory");
+      half(0);
+      if (2 * g + 1 < steps) half(1);
+      if (g + 1 < groups) {
+        dev::waitcnt<63, 0>();
+        asm volatile("" ::: "memory");
+        copy(g + 1);
+      }
+    }
+    float h[4];
+    uint32_t m = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      h[x] = swiglu(acc[0][x], acc[1][x]);
+      m = max(m, abs_bits(h[x]));
+    }
+    m = max_over_16s(m);
+    if (fg == 0) lmax[wave][fr] = m;
     __syncthreads();
-    if (tid < 128 && r0 + tid / 32 < t.rows) {  // 32 lanes a row, four columns each
-      const v4f v = *reinterpret_cast<const v4f*>(&h[tid / 32][4 * (tid & 31)]);
-      uint32_t m = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
-      m = max(m, mx::quad_swap<0xB1>(m));
-      m = max(m, mx::quad_swap<0x4E>(m));
-      m = max(m, mx::quad_swap<0x141>(m));
-      m = max(m, mx::quad_swap<0x140>(m));
-      uint32_t w = m;
-      swap16(m, w);
-      const uint32_t e = scale_of(max(m, w));
-      const size_t slot = slot0 + r0 + tid / 32;
-      MIAIE_ST(reinterpret_cast<uint32_t*>(p.Hq + slot * h_pitch + f0 + 4 * (tid & 31)), pack4(v[0], v[1], v[2], v[3], inverse_f32(e)));
-      if ((tid & 31) == 0) MIAIE_ST(p.Hs + (size_t)at.tn * p.M + slot, scale_f32(e));
+    m = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) m = max(m, lmax[w][fr]);
+    const uint32_t ex = scale_of(m);
+    if (fr < n) {
+      const size_t slot = slot0 + r0 + fr;
+      MIAIE_ST(reinterpret_cast<uint32_t*>(p.Hq + slot * h_pitch + f0 + 16 * wave + 4 * fg), pack4(h[0], h[1], h[2], h[3], inverse_f32(ex)));
+      if (wave == 0 && fg == 0) MIAIE_ST(p.Hs + (size_t)tn * p.M + slot, scale_f32(ex));
     }
     __syncthreads();
   }
@@ -1176,8 +1245,8 @@ int run_slots(miaie_ctx* ctx, const Args& p) {
   if constexpr (OUT == OUT_GLU) {
     if (few_slots(p, 128)) {
       const long grid = (most_slot_tiles(p.s, 128) * (p.N / 128) + 7) / 8 * 8;
-      const hipError_t e = launch<glu_stream>(ctx->device, dim3((unsigned)grid), dim3(512), 0, ctx->stream, p, p.N / 128);
-      return check_launch(ctx, e, "glu_stream");
+      const hipError_t e = launch<glu_rows>(ctx->device, dim3((unsigned)grid), dim3(512), 0, ctx->stream, p, p.N / 128);
+      return check_launch(ctx, e, "glu_rows");
     }
     const double us[] = {slots_us(kLarge, p, 128, ctx->cus), slots_us(kBlock, p, 128, ctx->cus), slots_us(kGlu, p, 128, ctx->cus)};
     switch (std::min_element(us, us + 3) - us) {

@@ -135,7 +135,6 @@ __global__ __launch_bounds__(256) void route_tokens(const T* __restrict__ logits
   }
 #pragma unroll
   for (int p = 0; p < PER; ++p) {
-    const int e = lane + 64 * p;
     if constexpr (BY_SCORE) {
       of[p] = score_of<SIGMOID>(l[p], largest, total);
       c[p] = of[p] + (double)bias[p];
