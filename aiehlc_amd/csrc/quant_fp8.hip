@@ -15,16 +15,48 @@ namespace {
 
 using namespace fp8;
 
-// ---- where a tile's values come from: eight columns c .. c + 7 of a row
+// ---- where a tile's values come from: eight columns c .. c + 7 of a row.  A source
+// says in turn what a row is (row), loads its columns (fetch) and makes their values
+// (values); a thread does each for its eight rows before the next, so that all loads
+// are in flight together.  (A load and its use in one branch a row wait for each
+// other: 2048 x 4096 bf16 10.3 us.)  fetch takes rows that do not exist, or are
+// padding, from where there is one, and values makes them zero.
+template <class T>
+struct Eight {
+  typedef T V __attribute__((ext_vector_type(8)));
+  V v;
+  // WHOLE: all eight columns exist, of any thread of the workgroup
+  template <bool WHOLE>
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if constexpr (WHOLE) {
+      using P = At<V, T>;
+      v = MIAIE_LD(reinterpret_cast<const P*>(p)).v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < n ? MIAIE_LD(p + i) : (T)0.f;
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
+};
+
 template <class T>
 struct FromMatrix {
   const T* X;
   int R, C, ldx;
+  static constexpr bool TAILS = true;  // tiles whose last columns do not exist
+  using Row = int;
+  using Raw = Eight<T>;
   __device__ __forceinline__ bool tile(int) const { return true; }
-  __device__ __forceinline__ void load(int row, int c, float (&x)[8]) const {
+  __device__ __forceinline__ Row row(int r) const { return r; }
+  template <bool WHOLE>
+  __device__ __forceinline__ Raw fetch(Row r, int c) const {
+    Raw raw;
+    raw.template load<WHOLE>(X + (size_t)min(r, R - 1) * ldx + c, C - c);
+    return raw;
+  }
+  __device__ __forceinline__ void values(Row r, int, const Raw& raw, float (&x)[8]) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (row < R && c < C) mx::load8(X + (size_t)row * ldx + c, C - c, x);
+    for (int i = 0; i < 8; ++i) x[i] = r < R ? raw[i] : 0.f;
   }
 };
 
@@ -35,17 +67,24 @@ struct FromTokens {
   const float* w;
   Slots s;
   int R, C, ldx;
+  static constexpr bool TAILS = true;
+  using Row = int;  // pair
+  struct Raw {
+    Eight<T> x;
+    float f;
+  };
   __device__ __forceinline__ bool tile(int r0) const { return r0 < MIAIE_LD(s.start + s.experts); }
-  __device__ __forceinline__ void load(int row, int c, float (&x)[8]) const {
+  __device__ __forceinline__ Row row(int r) const { return MIAIE_LD(s.row_of + r); }
+  template <bool WHOLE>
+  __device__ __forceinline__ Raw fetch(Row pair, int c) const {
+    Raw raw;
+    raw.x.template load<WHOLE>(X + (size_t)(max(pair, 0) / s.top_k) * ldx + c, C - c);
+    raw.f = w ? MIAIE_LD(w + max(pair, 0)) : 1.f;
+    return raw;
+  }
+  __device__ __forceinline__ void values(Row pair, int c, const Raw& raw, float (&x)[8]) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    const int pair = MIAIE_LD(s.row_of + row);
-    if (pair < 0 || c >= C) return;
-    mx::load8(X + (size_t)(pair / s.top_k) * ldx + c, C - c, x);
-    if (!w) return;
-    const float f = MIAIE_LD(w + pair);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = c + i < C ? x[i] * f : 0.f;  // (no -0 or NaN behind the last column)
+    for (int i = 0; i < 8; ++i) x[i] = pair >= 0 && c + i < C ? raw.x[i] * raw.f : 0.f;  // (no -0 or NaN behind the last column)
   }
 };
 
@@ -55,18 +94,26 @@ struct FromSwiglu {
   const T* GU;
   Slots s;
   int R, C, ldx;  // C = F
+  static constexpr bool TAILS = false;
+  struct Row {
+    int r, pair;
+  };
+  struct Raw {
+    Eight<T> g, u;
+  };
   __device__ __forceinline__ bool tile(int r0) const { return r0 < MIAIE_LD(s.start + s.experts); }
-  __device__ __forceinline__ void load(int row, int c, float (&x)[8]) const {
-    if (MIAIE_LD(s.row_of + row) < 0) {
+  __device__ __forceinline__ Row row(int r) const { return Row{r, MIAIE_LD(s.row_of + r)}; }
+  template <bool WHOLE>
+  __device__ __forceinline__ Raw fetch(Row r, int c) const {
+    static_assert(WHOLE, "F is a multiple of 128");
+    Raw raw;
+    raw.g.template load<true>(GU + (size_t)r.r * ldx + c, 8);
+    raw.u.template load<true>(GU + (size_t)r.r * ldx + C + c, 8);
+    return raw;
+  }
+  __device__ __forceinline__ void values(Row r, int, const Raw& raw, float (&x)[8]) const {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.f;
-      return;
-    }
-    float u[8];
-    mx::load8(GU + (size_t)row * ldx + c, 8, x);
-    mx::load8(GU + (size_t)row * ldx + C + c, 8, u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = swiglu(x[i], u[i]);
+    for (int i = 0; i < 8; ++i) x[i] = r.pair >= 0 ? swiglu(raw.g[i], raw.u[i]) : 0.f;
   }
 };
 
@@ -78,22 +125,33 @@ struct FromSwigluGrad {
   const float* dH;
   Slots s;
   int R, C, ldx, ldh;  // C = 2 F
+  static constexpr bool TAILS = false;
+  struct Row {
+    int r, pair;
+  };
+  struct Raw {
+    Eight<T> g, u;
+    Eight<float> d;
+  };
   __device__ __forceinline__ bool tile(int r0) const { return r0 < MIAIE_LD(s.start + s.experts); }
-  __device__ __forceinline__ void load(int row, int c, float (&x)[8]) const {
-    if (MIAIE_LD(s.row_of + row) < 0) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.f;
-      return;
-    }
+  __device__ __forceinline__ Row row(int r) const { return Row{r, MIAIE_LD(s.row_of + r)}; }
+  template <bool WHOLE>
+  __device__ __forceinline__ Raw fetch(Row r, int c) const {
+    static_assert(WHOLE, "F is a multiple of 128");
     const int F = C / 2, f = c < F ? c : c - F;
-    float g[8], u[8], d[8];
-    mx::load8(GU + (size_t)row * ldx + f, 8, g);
-    if (c < F) mx::load8(GU + (size_t)row * ldx + F + f, 8, u);
-    mx::load8(dH + (size_t)row * ldh + f, 8, d);
+    Raw raw;
+    raw.g.template load<true>(GU + (size_t)r.r * ldx + f, 8);
+    if (c < F) raw.u.template load<true>(GU + (size_t)r.r * ldx + F + f, 8);  // (the same for the workgroup)
+    raw.d.template load<true>(dH + (size_t)r.r * ldh + f, 8);
+    return raw;
+  }
+  __device__ __forceinline__ void values(Row r, int c, const Raw& raw, float (&x)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const Sigmoid y(g[i]);
-      x[i] = c < F ? d[i] * u[i] * y.s * (1.f + g[i] * y.rest) : d[i] * g[i] * y.s;
+      const float g = raw.g[i];
+      const Sigmoid y(g);
+      const float v = c < C / 2 ? raw.d[i] * raw.u[i] * y.s * (1.f + g * y.rest) : raw.d[i] * g * y.s;
+      x[i] = r.pair >= 0 ? v : 0.f;
     }
   }
 };
@@ -114,8 +172,23 @@ __global__ __launch_bounds__(256) void quant_tile(Src src, uint8_t* __restrict__
   const int r0 = 128 * tr + 8 * rg, c = 128 * tc + 8 * cl;
   if (!src.tile(128 * tr)) return;
   float x[8][8];
+  {
+    typename Src::Row row[8];
+    typename Src::Raw raw[8];
 #pragma unroll
-  for (int p = 0; p < 8; ++p) src.load(r0 + p, c, x[p]);
+    for (int p = 0; p < 8; ++p) row[p] = src.row(r0 + p);
+    bool whole = true;
+    if constexpr (Src::TAILS) whole = 128 * tc + 128 <= src.C;
+    if (whole) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p) raw[p] = src.template fetch<true>(row[p], c);
+    } else if constexpr (Src::TAILS) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p) raw[p] = src.template fetch<false>(row[p], c);
+    }
+#pragma unroll
+    for (int p = 0; p < 8; ++p) src.values(row[p], c, raw[p], x[p]);
+  }
   uint32_t e_row[8], e_all = 0;
   if constexpr (BLOCK == 128) {
     uint32_t m = 0;
