@@ -64,9 +64,9 @@ int check_forms(miaie_ctx* ctx, const char* fn, const uint8_t* Q, const float* S
   return MIAIE_OK;
 }
 
-// 256 threads pack 128 x 128; HIP takes fewer than 2^32 threads.
+// 512 threads pack 128 x 128; HIP takes fewer than 2^32 threads.
 int check_tiles(miaie_ctx* ctx, const char* fn, long R, long C) {
-  if (fp8::blocks(R) * fp8::blocks(C) >= 1u << 24)
+  if (fp8::blocks(R) * fp8::blocks(C) >= 1u << 23)
     return fail(ctx, MIAIE_EINVAL, "%s: %ld rows of %ld columns are too large", fn, R, C);
   return MIAIE_OK;
 }

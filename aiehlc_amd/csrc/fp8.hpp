@@ -70,11 +70,12 @@ __device__ __forceinline__ uint32_t max_over_16s(uint32_t v) {
   return max(v, w);
 }
 
-// s = 1 / (1 + e^-g) and 1 - s, from e^-|g|, which does not overflow
+// s = 1 / (1 + e^-g) and 1 - s, from e^-|g|, which does not overflow; the reciprocal is
+// good to a unit in the last place
 struct Sigmoid {
   float s, rest;
   __device__ __forceinline__ explicit Sigmoid(float g) {
-    const float x = expf(-fabsf(g)), big = 1.f / (1.f + x), small = x * big;
+    const float x = expf(-fabsf(g)), big = __builtin_amdgcn_rcpf(1.f + x), small = x * big;
     s = g < 0.f ? small : big, rest = g < 0.f ? big : small;
   }
 };

@@ -156,44 +156,53 @@ struct FromSwigluGrad {
   }
 };
 
-// A workgroup of 256 threads packs 128 rows of 128 columns, whole blocks along
-// either axis: thread t has columns 8 (t % 16) .. + 7 of rows 8 (t / 16) .. + 7.
+// A workgroup of 512 threads packs 128 rows of 128 columns, whole blocks along
+// either axis: thread t has columns 8 (t % 16) .. + 7 of rows 4 (t / 16) .. + 3 (eight
+// rows of half as many threads take 137 to 165 registers along both axes, and a CU
+// has fewer waves of them).
 // A row's block is 16 neighbouring lanes, whose maxima come from four lane
 // permutations; a column's are joined through LDS, and the codes of the transpose
 // leave through LDS as whole lines.  Columns behind C are zero.
 template <class Src, int BLOCK, bool ROWS, bool COLS>
-__global__ __launch_bounds__(256) void quant_tile(Src src, uint8_t* __restrict__ Q, float* __restrict__ S,
+__global__ __launch_bounds__(512) void quant_tile(Src src, uint8_t* __restrict__ Q, float* __restrict__ S,
                                                   uint8_t* __restrict__ Qt, float* __restrict__ St, int tiles_c) {
   __shared__ __attribute__((aligned(16))) uint8_t lq[COLS ? 128 * 128 : 16];
-  __shared__ uint32_t lmax[4][COLS ? 128 : 1];
+  constexpr int N = 4;  // rows of a thread
+  __shared__ uint32_t lmax[8][COLS ? 128 : 1];
   const int tid = threadIdx.x, cl = tid & 15, rg = tid >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int tr = blockIdx.x / tiles_c, tc = blockIdx.x % tiles_c;
-  const int r0 = 128 * tr + 8 * rg, c = 128 * tc + 8 * cl;
+  const int r0 = 128 * tr + N * rg, c = 128 * tc + 8 * cl;
   if (!src.tile(128 * tr)) return;
-  float x[8][8];
-  {
-    typename Src::Row row[8];
-    typename Src::Raw raw[8];
+  auto over_waves = [&](int k) __attribute__((always_inline)) {
+    uint32_t m = lmax[0][k];
 #pragma unroll
-    for (int p = 0; p < 8; ++p) row[p] = src.row(r0 + p);
+    for (int w = 1; w < 8; ++w) m = max(m, lmax[w][k]);
+    return m;
+  };
+  float x[N][8];
+  {
+    typename Src::Row row[N];
+    typename Src::Raw raw[N];
+#pragma unroll
+    for (int p = 0; p < N; ++p) row[p] = src.row(r0 + p);
     bool whole = true;
     if constexpr (Src::TAILS) whole = 128 * tc + 128 <= src.C;
     if (whole) {
 #pragma unroll
-      for (int p = 0; p < 8; ++p) raw[p] = src.template fetch<true>(row[p], c);
+      for (int p = 0; p < N; ++p) raw[p] = src.template fetch<true>(row[p], c);
     } else if constexpr (Src::TAILS) {
 #pragma unroll
-      for (int p = 0; p < 8; ++p) raw[p] = src.template fetch<false>(row[p], c);
+      for (int p = 0; p < N; ++p) raw[p] = src.template fetch<false>(row[p], c);
     }
 #pragma unroll
-    for (int p = 0; p < 8; ++p) src.values(row[p], c, raw[p], x[p]);
+    for (int p = 0; p < N; ++p) src.values(row[p], c, raw[p], x[p]);
   }
-  uint32_t e_row[8], e_all = 0;
+  uint32_t e_row[N], e_all = 0;
   if constexpr (BLOCK == 128) {
     uint32_t m = 0;
 #pragma unroll
-    for (int p = 0; p < 8; ++p)
+    for (int p = 0; p < N; ++p)
 #pragma unroll
       for (int i = 0; i < 8; ++i) m = max(m, abs_bits(x[p][i]));
     m = max(m, mx::quad_swap<0xB1>(m));   // lanes 1 0 3 2
@@ -203,7 +212,7 @@ __global__ __launch_bounds__(256) void quant_tile(Src src, uint8_t* __restrict__
     m = max_over_16s(m);
     if ((tid & 63) == 0) lmax[wave][0] = m;
     __syncthreads();
-    e_all = scale_of(max(max(lmax[0][0], lmax[1][0]), max(lmax[2][0], lmax[3][0])));
+    e_all = scale_of(over_waves(0));
     if (tid == 0) {
       const size_t tiles_r = blocks(src.R);
       if (ROWS) MIAIE_ST(S + tc * tiles_r + tr, scale_f32(e_all));
@@ -213,7 +222,7 @@ __global__ __launch_bounds__(256) void quant_tile(Src src, uint8_t* __restrict__
   if constexpr (ROWS) {
     const size_t row_pitch = pitch(src.C);
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
+    for (int p = 0; p < N; ++p) {
       uint32_t e = e_all;
       if constexpr (BLOCK == 1) {
         uint32_t m = 0;
@@ -233,8 +242,8 @@ __global__ __launch_bounds__(256) void quant_tile(Src src, uint8_t* __restrict__
     if constexpr (BLOCK == 1) {  // lane cl of a row group writes row cl's scale
       uint32_t e = e_row[0];
 #pragma unroll
-      for (int p = 1; p < 8; ++p) e = cl == p ? e_row[p] : e;
-      if (cl < 8 && r0 + cl < src.R) MIAIE_ST(S + (size_t)tc * src.R + r0 + cl, scale_f32(e));
+      for (int p = 1; p < N; ++p) e = cl == p ? e_row[p] : e;
+      if (cl < N && r0 + cl < src.R) MIAIE_ST(S + (size_t)tc * src.R + r0 + cl, scale_f32(e));
     }
   }
   if constexpr (COLS) {
@@ -244,7 +253,7 @@ __global__ __launch_bounds__(256) void quant_tile(Src src, uint8_t* __restrict__
       for (int i = 0; i < 8; ++i) {
         uint32_t m = 0;
 #pragma unroll
-        for (int p = 0; p < 8; ++p) m = max(m, abs_bits(x[p][i]));
+        for (int p = 0; p < N; ++p) m = max(m, abs_bits(x[p][i]));
         m = max_over_16s(m);
         if ((tid & 48) == 0) lmax[wave][8 * cl + i] = m;
       }
@@ -252,7 +261,7 @@ __global__ __launch_bounds__(256) void quant_tile(Src src, uint8_t* __restrict__
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int k = 8 * cl + i;
-        e_col[i] = scale_of(max(max(lmax[0][k], lmax[1][k]), max(lmax[2][k], lmax[3][k])));
+        e_col[i] = scale_of(over_waves(k));
       }
       if (tid < 16) {
 #pragma unroll
@@ -260,22 +269,20 @@ __global__ __launch_bounds__(256) void quant_tile(Src src, uint8_t* __restrict__
           if (c + i < src.C) MIAIE_ST(St + (size_t)tr * src.C + c + i, scale_f32(e_col[i]));
       }
     }
-    // eight rows of a column are eight bytes, at their place xor the column's eight:
-    // the sixteen lanes beside each other write different banks
+    // four rows of a column are four bytes, at their place xor the column's eight: the
+    // lanes beside each other write different banks
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float inv = inverse_f32(BLOCK == 128 ? e_all : e_col[i]);
-      const v2u q = {pack4(x[0][i], x[1][i], x[2][i], x[3][i], inv), pack4(x[4][i], x[5][i], x[6][i], x[7][i], inv)};
-      *reinterpret_cast<v2u*>(lq + 128 * (8 * cl + i) + 8 * (rg ^ cl)) = q;
+      *reinterpret_cast<uint32_t*>(lq + 128 * (8 * cl + i) + 4 * (rg ^ 4 * (cl & 7))) = pack4(x[0][i], x[1][i], x[2][i], x[3][i], inv);
     }
     __syncthreads();
     const size_t col_pitch = pitch(src.R);
 #pragma unroll
-    for (int it = 0; it < 4; ++it) {
-      const int k = 32 * it + (tid >> 3), m = tid & 7, sw = k >> 3;
-      const v4u q = *reinterpret_cast<const v4u*>(lq + 128 * k + 16 * (m ^ (sw >> 1)));
-      const v4u r = (sw & 1) ? v4u{q[2], q[3], q[0], q[1]} : q;
-      if (128 * tc + k < src.C) MIAIE_ST(reinterpret_cast<v4u*>(Qt + (size_t)(128 * tc + k) * col_pitch + 128 * tr + 16 * m), r);
+    for (int it = 0; it < 2; ++it) {
+      const int k = 64 * it + (tid >> 3), m = tid & 7;
+      const v4u q = *reinterpret_cast<const v4u*>(lq + 128 * k + 16 * (m ^ (k >> 3 & 7)));
+      if (128 * tc + k < src.C) MIAIE_ST(reinterpret_cast<v4u*>(Qt + (size_t)(128 * tc + k) * col_pitch + 128 * tr + 16 * m), q);
     }
   }
 }
@@ -306,7 +313,7 @@ int run(miaie_ctx* ctx, const char* what, const Src& src, uint8_t* Q, float* S, 
   const dim3 grid((unsigned)(blocks(src.R) * tiles_c));
   hipError_t e = hipSuccess;
   auto go = [&](auto k) {
-    e = launch<decltype(k)::value>(ctx->device, grid, dim3(256), 0, ctx->stream, src, Q, S, Qt, St, tiles_c);
+    e = launch<decltype(k)::value>(ctx->device, grid, dim3(512), 0, ctx->stream, src, Q, S, Qt, St, tiles_c);
   };
   if (Q && Qt)
     go(kernel_t<quant_tile<Src, BLOCK, true, true>>{});

@@ -434,7 +434,7 @@ MIAIE_API int miaie_norm_block_grad(miaie_ctx* ctx, const void* r, const void* b
  * operands that both have a scale a row (b_block 1) need powers of two from
  * 2^-126 to 2^127 or NaN, as miaie_quant_fp8 makes them (of others the exponent
  * is taken).  The product of two scales is taken in fp32.
- * R and C of a matrix in [1, 2^30] with ceil(R / 128) ceil(C / 128) below 2^24; M
+ * R and C of a matrix in [1, 2^30] with ceil(R / 128) ceil(C / 128) below 2^23; M
  * and N of a product in [1, 2^25] with ceil(M / 256) ceil(N / 256) below 2^23, K
  * in [1, 2^23]. */
 
