@@ -108,6 +108,8 @@ _SIGS = {
     "miaie_quant_fp8": (_i, [_p, _p] + [_i] * 5 + [_p] * 4),
     "miaie_dequant_fp8": (_i, [_p, _p, _p, _i, _p] + [_i] * 4),
     "miaie_gemm_fp8": (_i, [_p] * 5 + [_i, _p] + [_i] * 5),
+    "miaie_plan_gemm_fp8": (_i, [_i] * 5 + [_p]),
+    "miaie_plan_experts_fp8": (_i, [_i] * 7 + [_p]),
     "miaie_route_experts": (_i, [_p, _p, _i, _p, _p, _p] + [_i] * 9 + [_f]),
     "miaie_route_experts_grad": (_i, [_p, _p, _i, _p, _p, _p] + [_i] * 7 + [_f]),
     "miaie_experts_rows": (_sz, [_i] * 3),
@@ -252,6 +254,24 @@ def plan_gemm_mxfp4(M, N, K, out=F32, cus=256) -> dict:
     if rc != MIAIE_OK:
         raise MiaieError(rc, load_library().miaie_last_error_string(None).decode())
     return p.as_dict()
+
+
+def _plan(f, *args) -> dict:
+    p = GemmPlan()
+    rc = f(*args, C.byref(p))
+    if rc != MIAIE_OK:
+        raise MiaieError(rc, load_library().miaie_last_error_string(None).decode())
+    return p.as_dict()
+
+
+def plan_gemm_fp8(M, N, K, b_block=128, cus=256) -> dict:
+    """Which kernel an 8-bit product takes.  A host function: needs no device."""
+    return _plan(load_library().miaie_plan_gemm_fp8, M, N, K, b_block, cus)
+
+
+def plan_experts_fp8(tokens, top_k, experts, N, K, swiglu=False, cus=256) -> dict:
+    """Which kernel a product over slots takes (swiglu: the MLP's first, N = F, K = D).  Needs no device."""
+    return _plan(load_library().miaie_plan_experts_fp8, tokens, top_k, experts, N, K, int(swiglu), cus)
 
 
 class Graph:

@@ -141,15 +141,32 @@ extern "C" int miaie_dequant_fp8(miaie_ctx* ctx, const uint8_t* Q, const float* 
   return launch_dequant_fp8(ctx, Q, S, block, Y, dtype, R, C, ldy);
 }
 
+namespace {
+
+int check_gemm_sizes(miaie_ctx* ctx, const char* fn, int M, int N, int K) {
+  MIAIE_TRY(check_range(ctx, fn, "M", M, kMostMN));
+  MIAIE_TRY(check_range(ctx, fn, "N", N, kMostMN));
+  MIAIE_TRY(check_range(ctx, fn, "K", K, kMostK));
+  if ((long)((M + 255l) / 256) * ((N + 255l) / 256) >= 1l << 23)
+    return fail(ctx, MIAIE_EINVAL, "%s: a product of M=%d N=%d is too large for one launch", fn, M, N);
+  return MIAIE_OK;
+}
+
+}  // namespace
+
+extern "C" int miaie_plan_gemm_fp8(int M, int N, int K, int b_block, int cus, miaie_gemm_plan* plan) {
+  if (!plan) return fail(nullptr, MIAIE_EINVAL, "%s: plan is NULL", __func__);
+  MIAIE_TRY(check_gemm_sizes(nullptr, __func__, M, N, K));
+  MIAIE_TRY(check_block(nullptr, __func__, "b_block", b_block));
+  if (cus < 1) return fail(nullptr, MIAIE_EINVAL, "%s: cus=%d must be >= 1", __func__, cus);
+  return plan_gemm_fp8(M, N, K, b_block, cus, plan);
+}
+
 extern "C" int miaie_gemm_fp8(miaie_ctx* ctx, const uint8_t* Aq, const float* As, const uint8_t* Bq, const float* Bs,
                               int b_block, void* C, int dtype, int M, int N, int K, int ldc) {
   MIAIE_TRY(enter(ctx));
   MIAIE_TRY(check_dtype(ctx, __func__, dtype));
-  MIAIE_TRY(check_range(ctx, __func__, "M", M, kMostMN));
-  MIAIE_TRY(check_range(ctx, __func__, "N", N, kMostMN));
-  MIAIE_TRY(check_range(ctx, __func__, "K", K, kMostK));
-  if ((long)fp8::blocks((M + 1l) / 2) * (long)fp8::blocks((N + 1l) / 2) >= 1l << 23)
-    return fail(ctx, MIAIE_EINVAL, "%s: a product of M=%d N=%d is too large for one launch", __func__, M, N);
+  MIAIE_TRY(check_gemm_sizes(ctx, __func__, M, N, K));
   MIAIE_TRY(check_block(ctx, __func__, "b_block", b_block));
   MIAIE_TRY(check_packed(ctx, __func__, "A", Aq, As));
   MIAIE_TRY(check_packed(ctx, __func__, "B", Bq, Bs));
@@ -278,6 +295,20 @@ extern "C" int miaie_experts_gemm_fp8(miaie_ctx* ctx, const int* order, const ui
   MIAIE_TRY(check_slot_product(ctx, __func__, tokens, top_k, experts, N, K, gather));
   return launch_experts_gemm_fp8(ctx, fp8::slots_of(order, tokens, top_k, experts), Aq, As, gather, Bq, Bs, C, dtype, N, K,
                                  ldc);
+}
+
+extern "C" int miaie_plan_experts_fp8(int tokens, int top_k, int experts, int N, int K, int swiglu, int cus,
+                                      miaie_gemm_plan* plan) {
+  if (!plan) return fail(nullptr, MIAIE_EINVAL, "%s: plan is NULL", __func__);
+  MIAIE_TRY(check_slots(nullptr, __func__, tokens, top_k, experts));
+  if (swiglu != 0 && swiglu != 1) return fail(nullptr, MIAIE_EINVAL, "%s: swiglu=%d must be 0 or 1", __func__, swiglu);
+  MIAIE_TRY(swiglu ? check_hidden(nullptr, __func__, N) : check_width(nullptr, __func__, "N", N));
+  MIAIE_TRY(check_width(nullptr, __func__, "K", K));
+  MIAIE_TRY(check_slot_product(nullptr, __func__, tokens, top_k, experts, swiglu ? 2l * N : N, K, false));
+  if (cus < 1) return fail(nullptr, MIAIE_EINVAL, "%s: cus=%d must be >= 1", __func__, cus);
+  fp8::Slots s{};  // (its sizes alone)
+  s.tokens = tokens, s.top_k = top_k, s.experts = experts;
+  return plan_experts_fp8(s, N, K, swiglu, cus, plan);
 }
 
 extern "C" int miaie_experts_quant_fp8(miaie_ctx* ctx, const int* order, const void* X, int dtype, const float* w,

@@ -56,8 +56,9 @@ __device__ __forceinline__ v8i join(v4i lo, v4i hi) { return v8i{lo[0], lo[1], l
 
 // The same two as the large tiles issue them, in the order that the program has them:
 // the compiler keeps neither a product's place (it starts every product of a step
-// before it adds any, in more registers than there are) nor an accumulator's.  Who
-// reads a result that is not 18 wait states old puts them in between
+// before it adds any, in more registers than there are) nor an accumulator's.  A
+// result is there 8 passes and 3 wait states after its instruction's issue, which the
+// next one's waits 8 passes for: who reads it issues two others before, or waits
 // (tests/test_fp8_asm.py checks the distances in the assembly).
 __device__ __forceinline__ void issue_mfma0(v4f& p, v8i b, v8i a) {
 #if MIAIE_DEVICE_CHECKS
@@ -837,7 +838,7 @@ __global__ __launch_bounds__(G::THREADS) void gemm_slots(Args p, int tiles_n) {
 // token's own MLP had up to 5.7e-3 of its result from a few of them (2.4e-3 without).
 constexpr int STREAM_K = 64;  // blocks of k whose A is in LDS at a time
 
-// p += <16 elements of q, 16 elements of x>
+// <16 elements of a row of B, 16 elements of a row of A>
 __device__ __forceinline__ float dot16(const float (&b)[16], const float (&a)[16]) {
   float p0 = b[0] * a[0], p1 = b[1] * a[1];
 #pragma unroll
@@ -1181,13 +1182,22 @@ int run_slots_large(miaie_ctx* ctx, const Args& p) {
   return check_launch(ctx, e, "gemm_fp8_slots");
 }
 
+// Waves that share out k: at least eight blocks each.
+int stream_parts(int K) { return blocks(K) >= 32 ? 4 : blocks(K) >= 16 ? 2 : 1; }
+
 template <Mode MODE, Out OUT>
 int run_stream(miaie_ctx* ctx, const Args& p) {
-  const int steps = (int)blocks(p.K), parts = steps >= 32 ? 4 : steps >= 16 ? 2 : 1;
+  const int parts = stream_parts(p.K);
   const long cols = 16 * (4 / parts), tiles_n = (p.N + cols - 1) / cols;
   const long grid = MODE == SLOTS ? (most_slot_tiles(p.s, 128) * tiles_n + 7) / 8 * 8 : tiles_n;
   const hipError_t e = launch<gemm_stream<MODE, OUT>>(ctx->device, dim3((unsigned)grid), dim3(256), 0, ctx->stream, p, (int)tiles_n, parts);
   return check_launch(ctx, e, "gemm_fp8_stream");
+}
+
+int run_glu_rows(miaie_ctx* ctx, const Args& p) {
+  const long grid = (most_slot_tiles(p.s, 128) * (p.N / 128) + 7) / 8 * 8;
+  const hipError_t e = launch<glu_rows>(ctx->device, dim3((unsigned)grid), dim3(512), 0, ctx->stream, p, p.N / 128);
+  return check_launch(ctx, e, "glu_rows");
 }
 
 // ---- choice of tile: the lowest estimated time.  A CU has `at_once` workgroups of a
@@ -1203,66 +1213,131 @@ constexpr TileTime kLarge{256, 256, 1, 9.0, 1.05, {1.50}}, kBlock{128, 256, 1, 6
     kSquare{128, 128, 2, 3.3, 0.57, {0.65, 1.09}}, kFlat{64, 128, 2, 2.3, 0.44, {0.47, 0.70}},
     kSmall{64, 64, 3, 2.0, 0.29, {0.31, 0.44, 0.54}}, kGlu{64, 256, 1, 3.0, 0.60, {0.95}};
 
-double tile_us(const TileTime& t, double tiles, long steps, int cus) {
+// (none: a launch of so many tiles would be too large)
+double tile_us(const TileTime& t, double tiles, int threads, long steps, int cus) {
+  if (tiles * threads >= (double)kThreads) return 1e300;
   if (2 * tiles <= cus) return 1.0 + t.ends + t.idle * steps;
   const long each = (long)((tiles + cus - 1) / cus), full = each / t.at_once, rest = each % t.at_once;
   return 1.0 + full * (t.ends + t.step[t.at_once - 1] * steps) + (rest ? t.ends + t.step[rest - 1] * steps : 0.0);
 }
-double dense_us(const TileTime& t, const Args& p, int cus) {
-  return tile_us(t, (double)((p.M + t.bm - 1l) / t.bm) * (double)((p.N + t.bn - 1l) / t.bn), (long)blocks(p.K), cus);
+
+// A kernel of the choice.  T: a tile; Stream, GluRows: few rows.
+template <class T>
+struct On {
+  using type = T;
+};
+struct Stream {};
+struct GluRows {};
+
+// f(the kernel of a dense product)
+template <class F>
+int with_dense(int M, int N, int K, int b_block, int cus, F&& f) {
+  if (b_block == 128 && M <= 4) return f(Stream{});
+  auto us = [&](const TileTime& t, int threads) {
+    return tile_us(t, (double)((M + t.bm - 1l) / t.bm) * (double)((N + t.bn - 1l) / t.bn), threads, (long)blocks(K), cus);
+  };
+  const double times[] = {us(kLarge, 512), us(kBlock, 512), us(kSquare, 256), us(kFlat, 256), us(kSmall, 256)};
+  switch (std::min_element(times, times + 5) - times) {
+    case 0: return f(On<Large>{});
+    case 1: return f(On<Block>{});
+    case 2: return f(On<Square>{});
+    case 3: return f(On<Flat>{});
+    default: return f(On<Small>{});
+  }
 }
-// Slots: an expert's last tile is half full on average; tiles of up to 128 rows and
-// columns take a tenth longer than among dense ones, B coming from memory.
-double slots_us(const TileTime& t, const Args& p, int cols, int cus) {
-  const double n = (double)p.s.tokens * p.s.top_k, used = std::min<double>(p.s.experts, n);
-  const double us = tile_us(t, std::max(used, n / t.bm + used / 2) * (double)((p.N + cols - 1l) / cols), (long)blocks(p.K), cus);
-  return t.bn <= 128 ? 1.1 * us : us;
+
+// f(the kernel of a product over slots of N columns, or of H with N = F).  On<Large>
+// stands for tiles of both 256 and 128 rows.  Four slots an expert or fewer: kernels
+// that read B once for four rows; beyond, a tile of 64 rows is as quick and reads it
+// once for all.  An expert's last tile is half full on average, and tiles of up to 128
+// rows and columns take a tenth longer than among dense ones, B coming from memory.
+template <bool GLU, class F>
+int with_slots(const Slots& s, int N, int K, int cus, F&& f) {
+  const double n = (double)s.tokens * s.top_k, used = std::min<double>(s.experts, n);
+  const long few = GLU ? N / 128 * 512l : (N + 15l) / 16 * 256l;  // threads of a block of slots
+  if (n <= 4.0 * s.experts && most_slot_tiles(s, 128) * few < kThreads) {
+    if constexpr (GLU)
+      return f(GluRows{});
+    else
+      return f(Stream{});
+  }
+  auto us = [&](const TileTime& t, int cols, int threads) {
+    const double tiles_n = (double)((N + cols - 1l) / cols);
+    const double us = tile_us(t, std::max(used, n / t.bm + used / 2) * tiles_n, threads, (long)blocks(K), cus);
+    return most_slot_tiles(s, t.bm) * tiles_n * threads >= (double)kThreads ? 1e300 : t.bn <= 128 ? 1.1 * us : us;
+  };
+  if constexpr (GLU) {
+    const double times[] = {us(kLarge, 128, 512), us(kBlock, 128, 512), us(kGlu, 128, 256)};
+    switch (std::min_element(times, times + 3) - times) {
+      case 1: return f(On<Block>{});
+      case 2: return f(On<Glu>{});
+      default: return f(On<Large>{});
+    }
+  } else {
+    const double times[] = {us(kLarge, 256, 512), us(kSquare, 128, 256), us(kSmall, 64, 256)};
+    switch (std::min_element(times, times + 3) - times) {
+      case 1: return f(On<Square>{});
+      case 2: return f(On<Small>{});
+      default: return f(On<Large>{});
+    }
+  }
 }
 
 template <Out OUT, int BBLOCK>
-int run_dense(miaie_ctx* ctx, const Args& p) {
-  if constexpr (BBLOCK == 128) {
-    if (p.M <= 4) return run_stream<DENSE, OUT>(ctx, p);
+struct RunDense {
+  miaie_ctx* ctx;
+  const Args& p;
+  int operator()(Stream) const {
+    if constexpr (BBLOCK == 128) return run_stream<DENSE, OUT>(ctx, p);
+    return MIAIE_EUNSUPPORTED;  // (not chosen)
   }
-  const double us[] = {dense_us(kLarge, p, ctx->cus), dense_us(kBlock, p, ctx->cus), dense_us(kSquare, p, ctx->cus),
-                       dense_us(kFlat, p, ctx->cus), dense_us(kSmall, p, ctx->cus)};
-  switch (std::min_element(us, us + 5) - us) {
-    case 0: return run_tile<Large, DENSE, OUT, BBLOCK>(ctx, p);
-    case 1: return run_tile<Block, DENSE, OUT, BBLOCK>(ctx, p);
-    case 2: return run_tile<Square, DENSE, OUT, BBLOCK>(ctx, p);
-    case 3: return run_tile<Flat, DENSE, OUT, BBLOCK>(ctx, p);
-    default: return run_tile<Small, DENSE, OUT, BBLOCK>(ctx, p);
-  }
-}
+  template <class T>
+  int operator()(On<T>) const { return run_tile<T, DENSE, OUT, BBLOCK>(ctx, p); }
+};
 
-// Few slots an expert.  (Beyond four a row tile of 64 is as quick, and reads B once.)
-bool few_slots(const Args& p, int cols) {
-  return (long)p.s.tokens * p.s.top_k <= 4l * p.s.experts && most_slot_tiles(p.s, 128) * ((p.N + cols - 1l) / cols) < kThreads / 2048;
+template <Out OUT>
+struct RunSlots {
+  miaie_ctx* ctx;
+  const Args& p;
+  int operator()(Stream) const { return run_stream<SLOTS, OUT>(ctx, p); }
+  int operator()(GluRows) const { return run_glu_rows(ctx, p); }
+  int operator()(On<Large>) const { return run_slots_large<OUT>(ctx, p); }
+  template <class T>
+  int operator()(On<T>) const { return run_tile<T, SLOTS, OUT, 128>(ctx, p); }
+};
+
+// What a plan says of a kernel; `rows` and `cols` tell the workgroups of a tile.
+template <class Rows>
+struct Plan {
+  Rows rows;  // tiles of so many rows
+  int N, K;
+  bool glu;
+  miaie_gemm_plan* to;
+  int fill(int kernel, int tile_m, int tile_n, int threads) const {
+    *to = {kernel, tile_m, tile_n, (int)(rows(tile_m) * ((N + (long)tile_n - 1) / tile_n)), threads};
+    return MIAIE_OK;
+  }
+  int operator()(Stream) const {
+    *to = {MIAIE_KERNEL_ROWS, 4, 16 * (4 / stream_parts(K)), 0, 256};
+    to->workgroups = (int)(rows(128) * ((N + to->tile_n - 1l) / to->tile_n));
+    return MIAIE_OK;
+  }
+  int operator()(GluRows) const {
+    *to = {MIAIE_KERNEL_ROWS, kGluRows, 128, (int)(rows(128) * (N / 128)), 512};
+    return MIAIE_OK;
+  }
+  template <class T>
+  int operator()(On<T>) const { return fill(MIAIE_KERNEL_PIPE, T::BM, glu ? T::BN / 2 : T::BN, T::THREADS); }
+};
+
+template <Out OUT, int BBLOCK>
+int run_dense(miaie_ctx* ctx, const Args& p) {
+  return with_dense(p.M, p.N, p.K, BBLOCK, ctx->cus, RunDense<OUT, BBLOCK>{ctx, p});
 }
 
 template <Out OUT>
 int run_slots(miaie_ctx* ctx, const Args& p) {
-  if constexpr (OUT == OUT_GLU) {
-    if (few_slots(p, 128)) {
-      const long grid = (most_slot_tiles(p.s, 128) * (p.N / 128) + 7) / 8 * 8;
-      const hipError_t e = launch<glu_rows>(ctx->device, dim3((unsigned)grid), dim3(512), 0, ctx->stream, p, p.N / 128);
-      return check_launch(ctx, e, "glu_rows");
-    }
-    const double us[] = {slots_us(kLarge, p, 128, ctx->cus), slots_us(kBlock, p, 128, ctx->cus), slots_us(kGlu, p, 128, ctx->cus)};
-    switch (std::min_element(us, us + 3) - us) {
-      case 1: return run_tile<Block, SLOTS, OUT, 128>(ctx, p);
-      case 2: return run_tile<Glu, SLOTS, OUT, 128>(ctx, p);
-      default: return run_slots_large<OUT>(ctx, p);
-    }
-  } else {
-    if (few_slots(p, 16)) return run_stream<SLOTS, OUT>(ctx, p);
-    const double us[] = {slots_us(kLarge, p, 256, ctx->cus), slots_us(kSquare, p, 128, ctx->cus), slots_us(kSmall, p, 64, ctx->cus)};
-    switch (std::min_element(us, us + 3) - us) {
-      case 1: return run_tile<Square, SLOTS, OUT, 128>(ctx, p);
-      case 2: return run_tile<Small, SLOTS, OUT, 128>(ctx, p);
-      default: return run_slots_large<OUT>(ctx, p);
-    }
-  }
+  return with_slots<OUT == OUT_GLU>(p.s, p.N, p.K, ctx->cus, RunSlots<OUT>{ctx, p});
 }
 
 template <Out OUT>
@@ -1293,6 +1368,17 @@ int launch_experts_wgrad_fp8(miaie_ctx* ctx, const fp8::Slots& s, const uint8_t*
                              const float* Bts, void* C, int dtype, int M, int N, int ldc) {
   const Args p{Atq, Ats, Btq, Bts, C, nullptr, nullptr, M, N, s.rows, ldc, M, 0, s};
   return dtype == MIAIE_BF16 ? run_wgrad<OUT_BF16>(ctx, p) : run_wgrad<OUT_F32>(ctx, p);
+}
+
+int plan_gemm_fp8(int M, int N, int K, int b_block, int cus, miaie_gemm_plan* to) {
+  auto rows = [=](int tile) { return tile == 128 && M <= 4 && b_block == 128 ? 1l : (M + tile - 1l) / tile; };
+  return with_dense(M, N, K, b_block, cus, Plan<decltype(rows)>{rows, N, K, false, to});
+}
+
+int plan_experts_fp8(const fp8::Slots& s, int N, int K, int swiglu, int cus, miaie_gemm_plan* to) {
+  auto rows = [=](int tile) { return most_slot_tiles(s, tile); };
+  if (swiglu) return with_slots<true>(s, N, K, cus, Plan<decltype(rows)>{rows, N, K, true, to});
+  return with_slots<false>(s, N, K, cus, Plan<decltype(rows)>{rows, N, K, false, to});
 }
 
 }  // namespace miaie

@@ -191,6 +191,8 @@ int launch_dequant_fp8(miaie_ctx* ctx, const uint8_t* Q, const float* S, int blo
                        int ldy);
 int launch_gemm_fp8(miaie_ctx* ctx, const uint8_t* Aq, const float* As, const uint8_t* Bq, const float* Bs, int b_block,
                     void* C, int dtype, int M, int N, int K, int ldc);
+int plan_gemm_fp8(int M, int N, int K, int b_block, int cus, miaie_gemm_plan* to);
+int plan_experts_fp8(const fp8::Slots& s, int N, int K, int swiglu, int cus, miaie_gemm_plan* to);
 int launch_route_experts(miaie_ctx* ctx, const void* logits, int dtype, const float* bias, int* idx, float* w, int tokens,
                          int experts, int top_k, int ld, int scoring, int groups, int groups_kept, int group_top,
                          int renormalize, float scale);

@@ -468,6 +468,12 @@ MIAIE_API int miaie_dequant_fp8(miaie_ctx* ctx, const uint8_t* Q, const float* S
 MIAIE_API int miaie_gemm_fp8(miaie_ctx* ctx, const uint8_t* Aq, const float* As, const uint8_t* Bq, const float* Bs,
                              int b_block, void* C, int dtype, int M, int N, int K, int ldc);
 
+/* How miaie_gemm_fp8 runs a product planned for `cus` compute units (256 on an
+ * MI355X; miaie_plan_set_cus on a context): MIAIE_KERNEL_ROWS for up to four rows of
+ * weights, otherwise MIAIE_KERNEL_PIPE with its tile.  A host function: needs no
+ * context and no device.  MIAIE_EINVAL for sizes that the entry point refuses. */
+MIAIE_API int miaie_plan_gemm_fp8(int M, int N, int K, int b_block, int cus, miaie_gemm_plan* plan);
+
 /* ---- routing of tokens to experts ----------------------------------------- */
 
 /* No counterpart in the reference.  logits: tokens x experts, row pitch ld, of type
@@ -510,8 +516,8 @@ MIAIE_API int miaie_route_experts_grad(miaie_ctx* ctx, const void* logits, int d
 /* No counterpart in the reference.  A slot is a row of a (token, choice) pair's
  * own; slots are sorted by expert, each expert's from a multiple of 128 on in the
  * order of its pairs.  Matrices over slots have miaie_experts_rows rows, whatever
- * the routing; rows of padding and behind the last slot in use are neither read nor
- * written unless it says so below.  The order is one device array of int32,
+ * the routing; rows of padding and behind the last slot in use are not written, and
+ * nothing depends on what they hold, unless it says so below.  The order is one device array of int32,
  * miaie_experts_order_bytes long, with the parts
  *   start [experts + 1]  first slot of each expert; the last: slots in use;
  *   count [experts]      slots of each expert; the part ends at a multiple of 16;
@@ -551,6 +557,13 @@ MIAIE_API int miaie_experts_mlp_fp8(miaie_ctx* ctx, const int* order, const floa
 MIAIE_API int miaie_experts_gemm_fp8(miaie_ctx* ctx, const int* order, const uint8_t* Aq, const float* As,
                                      const uint8_t* Bq, const float* Bs, void* C, int dtype, int tokens, int top_k,
                                      int experts, int N, int K, int ldc, int gather);
+
+/* How that runs (swiglu 0), or the first product of miaie_experts_mlp_fp8 (swiglu 1:
+ * N = F, K = D, tile_n columns of H), as miaie_plan_gemm_fp8 says it; workgroups: the
+ * most that a routing can need.  Where tile_m is 256, an expert's last 128 slots or
+ * fewer are a tile of 128 rows. */
+MIAIE_API int miaie_plan_experts_fp8(int tokens, int top_k, int experts, int N, int K, int swiglu, int cus,
+                                     miaie_gemm_plan* plan);
 
 /* Rows of X (tokens x C, row pitch ldx, of type dtype), times w (fp32 tokens x top_k;
  * NULL: 1), packed by slot along the rows (Q, S: rows x C) and / or along the
