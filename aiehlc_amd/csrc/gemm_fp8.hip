@@ -1153,7 +1153,7 @@ using Flat = SmallTile<64, 128, 3>;
 using Small = SmallTile<64, 64, 3>;
 using Glu = SmallTile<64, 256, 2>;  // (128 columns of H)
 
-constexpr long kThreads = 1l << 32;  // HIP takes fewer in a launch
+constexpr long kThreads = (1l << 32) - 8 * 512;  // HIP takes fewer than 2^32 in a launch; slots round up to eight workgroups
 
 // Most tiles of `rows` slots that a routing can make: one more for each expert than
 // its rows fill.
