@@ -226,7 +226,7 @@ inline void mlp_i8(const Buffer<int8_t>& X, const Buffer<int8_t>& W1, const Buff
   ctx.check(miaie_mlp_i8(ctx.get(), X.data(), W1.data(), W2.data(), H.data(), Y.data(), M, K, F, Nout, s1, s2));
 }
 
-// The 4-bit operators and the norms infer sizes, and refuse (miaie::Error,
+// The 4-bit and 8-bit operators, the experts' and the norms infer sizes, and refuse (miaie::Error,
 // MIAIE_EINVAL, before anything is queued) operands that do not fit together and
 // buffers shorter than those sizes.
 namespace detail {
@@ -413,6 +413,217 @@ void norm_before_grad(const Buffer<S>& x, const Buffer<float>& w_before, const B
                                   dy.data(), data(dx), nullptr, nullptr, nullptr, data(dw_before), data(work),
                                   work ? work->bytes() : 0, n.rows, n.cols, n.cols, n.cols, n.rows, dtype_of(x.data()),
                                   dtype_of(dy.data()), 1.f));
+}
+
+// ---- 8-bit matrices with a scale for each block of 128, routing, experts ----
+
+// `count` packed matrices (miaie.h) of rows x cols, one after another: block 1 or
+// 128; count: the experts' matrices.
+struct Fp8Matrix {
+  Fp8Matrix(Context& ctx, int rows, int cols, int block = 1, int count = 1)
+      : rows(rows), cols(cols), block(block), count(count), q(ctx, count * miaie_fp8_q_bytes(rows, cols)),
+        s(ctx, count * miaie_fp8_s_bytes(rows, cols, block) / 4) {}
+  int rows, cols, block, count;
+  Buffer<uint8_t> q;
+  Buffer<float> s;
+};
+
+namespace detail {
+inline bool is(const Fp8Matrix& m, int rows, int cols, int block, int count = 1) {
+  return m.rows == rows && m.cols == cols && m.block == block && m.count == count;
+}
+inline bool is(const Fp8Matrix* m, int rows, int cols) { return !m || is(*m, rows, cols, 1); }
+inline uint8_t* codes(Fp8Matrix* m) { return m ? m->q.data() : nullptr; }
+inline float* scales(Fp8Matrix* m) { return m ? m->s.data() : nullptr; }
+template <typename T>
+T* data(const Buffer<T>* b) { return b ? b->data() : nullptr; }
+}  // namespace detail
+
+// Q = X packed along its rows (X dense, Q.rows x Q.cols).
+template <typename T>
+void quant_fp8(const Buffer<T>& X, Fp8Matrix& Q, Context& ctx = Context::current()) {
+  detail::require(detail::holds(X, Q.rows, Q.cols) && Q.count == 1, "quant_fp8", "X is smaller than Q, or Q several matrices");
+  ctx.check(miaie_quant_fp8(ctx.get(), X.data(), dtype_of(X.data()), Q.rows, Q.cols, Q.cols, Q.block, Q.q.data(), Q.s.data(),
+                            nullptr, nullptr));
+}
+
+// Qt = the transpose of X packed along its rows (X dense, Qt.cols x Qt.rows).
+template <typename T>
+void quant_fp8_t(const Buffer<T>& X, Fp8Matrix& Qt, Context& ctx = Context::current()) {
+  detail::require(detail::holds(X, Qt.cols, Qt.rows) && Qt.count == 1, "quant_fp8_t",
+                  "X is smaller than Qt, or Qt several matrices");
+  ctx.check(miaie_quant_fp8(ctx.get(), X.data(), dtype_of(X.data()), Qt.cols, Qt.rows, Qt.rows, Qt.block, nullptr, nullptr,
+                            Qt.q.data(), Qt.s.data()));
+}
+
+// Both from one read of X.
+template <typename T>
+void quant_fp8_both(const Buffer<T>& X, Fp8Matrix& Q, Fp8Matrix& Qt, Context& ctx = Context::current()) {
+  detail::require(detail::holds(X, Q.rows, Q.cols) && Q.count == 1, "quant_fp8_both",
+                  "X is smaller than Q, or Q several matrices");
+  detail::require(detail::is(Qt, Q.cols, Q.rows, Q.block), "quant_fp8_both", "Qt does not have the shape of Q's transpose");
+  ctx.check(miaie_quant_fp8(ctx.get(), X.data(), dtype_of(X.data()), Q.rows, Q.cols, Q.cols, Q.block, Q.q.data(), Q.s.data(),
+                            Qt.q.data(), Qt.s.data()));
+}
+
+// Y = the values of Q.
+template <typename T>
+void dequant_fp8(const Fp8Matrix& Q, Buffer<T>& Y, Context& ctx = Context::current()) {
+  detail::require(detail::holds(Y, Q.rows, Q.cols) && Q.count == 1, "dequant_fp8", "Y is smaller than Q, or Q several matrices");
+  ctx.check(miaie_dequant_fp8(ctx.get(), Q.q.data(), Q.s.data(), Q.block, Y.data(), dtype_of(Y.data()), Q.rows, Q.cols, Q.cols));
+}
+
+// C = A . B^T (A M x K of block 1, B N x K of either block).
+template <typename T>
+void gemm_fp8(const Fp8Matrix& A, const Fp8Matrix& B, Buffer<T>& C, Context& ctx = Context::current()) {
+  detail::require(A.block == 1 && A.count == 1 && B.count == 1, "gemm_fp8", "A has blocks of 128 rows, or A or B several matrices");
+  detail::require(A.cols == B.cols, "gemm_fp8", "A and B have rows of different lengths");
+  detail::require(detail::holds(C, A.rows, B.rows), "gemm_fp8", "C is smaller than A . B^T");
+  ctx.check(miaie_gemm_fp8(ctx.get(), A.q.data(), A.s.data(), B.q.data(), B.s.data(), B.block, C.data(), dtype_of(C.data()),
+                           A.rows, B.rows, A.cols, B.rows));
+}
+
+// How miaie_route_experts chooses.
+struct Routing {
+  int tokens, top_k, experts;
+  int scoring = MIAIE_SOFTMAX, groups = 1, groups_kept = 1, group_top = 1;
+  bool renormalize = true;
+  float scale = 1.f;
+};
+
+// idx and w (tokens x top_k) from logits (tokens x experts, dense).
+template <typename T>
+void route_experts(const Buffer<T>& logits, const Buffer<float>* bias, Buffer<int32_t>& idx, Buffer<float>& w, const Routing& r,
+                   Context& ctx = Context::current()) {
+  detail::require(detail::holds(logits, r.tokens, r.experts) && (!bias || detail::holds(*bias, 1, r.experts)), "route_experts",
+                  "logits is smaller than tokens x experts, or bias shorter than experts");
+  detail::require(detail::holds(idx, r.tokens, r.top_k) && detail::holds(w, r.tokens, r.top_k), "route_experts",
+                  "idx or w is smaller than tokens x top_k");
+  ctx.check(miaie_route_experts(ctx.get(), logits.data(), dtype_of(logits.data()), detail::data(bias), idx.data(), w.data(),
+                                r.tokens, r.top_k, r.experts, r.experts, r.scoring, r.groups, r.groups_kept, r.group_top,
+                                r.renormalize ? 1 : 0, r.scale));
+}
+
+template <typename T>
+void route_experts_grad(const Buffer<T>& logits, const Buffer<int32_t>& idx, const Buffer<float>& dw, Buffer<float>& dlogits,
+                        const Routing& r, Context& ctx = Context::current()) {
+  detail::require(detail::holds(logits, r.tokens, r.experts) && detail::holds(dlogits, r.tokens, r.experts),
+                  "route_experts_grad", "logits or dlogits is smaller than tokens x experts");
+  detail::require(detail::holds(idx, r.tokens, r.top_k) && detail::holds(dw, r.tokens, r.top_k), "route_experts_grad",
+                  "idx or dw is smaller than tokens x top_k");
+  ctx.check(miaie_route_experts_grad(ctx.get(), logits.data(), dtype_of(logits.data()), idx.data(), dw.data(), dlogits.data(),
+                                     r.tokens, r.top_k, r.experts, r.experts, r.experts, r.scoring, r.renormalize ? 1 : 0,
+                                     r.scale));
+}
+
+// Slots of a routing (miaie_experts_order); matrices over them have rows() rows.
+struct ExpertsOrder {
+  ExpertsOrder(Context& ctx, int tokens, int top_k, int experts)
+      : tokens(tokens), top_k(top_k), experts(experts), order(ctx, miaie_experts_order_bytes(tokens, top_k, experts) / 4) {}
+  int rows() const { return (int)miaie_experts_rows(tokens, top_k, experts); }
+  int tokens, top_k, experts;
+  Buffer<int32_t> order;
+};
+
+inline void experts_order(const Buffer<int32_t>& idx, ExpertsOrder& o, Context& ctx = Context::current()) {
+  detail::require(detail::holds(idx, o.tokens, o.top_k), "experts_order", "idx is smaller than tokens x top_k");
+  ctx.check(miaie_experts_order(ctx.get(), idx.data(), o.order.data(), o.tokens, o.top_k, o.experts));
+}
+
+// out[t] = sum over t's experts of w (H . W2^T), H = pack(silu(gate) up) of X . W1^T.
+template <typename T>
+void experts_mlp_fp8(const ExpertsOrder& o, const Buffer<float>& w, const Fp8Matrix& X, const Fp8Matrix& W1, const Fp8Matrix& W2,
+                     Fp8Matrix& H, Buffer<T>& Y, Buffer<T>& out, Context& ctx = Context::current()) {
+  detail::require(detail::is(X, o.tokens, X.cols, 1), "experts_mlp_fp8", "X is not the tokens' rows");
+  detail::require(detail::is(W1, 2 * W2.cols, X.cols, 128, o.experts) && detail::is(W2, W2.rows, W2.cols, 128, o.experts),
+                  "experts_mlp_fp8", "W1 and W2 are not matrices of each expert that fit X and each other");
+  detail::require(detail::is(H, o.rows(), W2.cols, 1), "experts_mlp_fp8", "H does not have the slots' rows of F columns");
+  detail::require(detail::holds(w, o.tokens, o.top_k) && detail::holds(Y, o.rows(), W2.rows) &&
+                      detail::holds(out, o.tokens, W2.rows),
+                  "experts_mlp_fp8", "w, Y or out is too small");
+  ctx.check(miaie_experts_mlp_fp8(ctx.get(), o.order.data(), w.data(), X.q.data(), X.s.data(), W1.q.data(), W1.s.data(),
+                                  W2.q.data(), W2.s.data(), H.q.data(), H.s.data(), Y.data(), out.data(), dtype_of(out.data()),
+                                  o.tokens, o.top_k, o.experts, X.cols, W2.cols, W2.rows, W2.rows));
+}
+
+// C[slot] = A[slot] . B_e^T; with gather A has the tokens' rows.
+template <typename T>
+void experts_gemm_fp8(const ExpertsOrder& o, const Fp8Matrix& A, const Fp8Matrix& B, Buffer<T>& C, bool gather = false,
+                      Context& ctx = Context::current()) {
+  detail::require(detail::is(A, gather ? o.tokens : o.rows(), A.cols, 1), "experts_gemm_fp8",
+                  gather ? "A is not the tokens' rows" : "A is not the slots' rows");
+  detail::require(detail::is(B, B.rows, A.cols, 128, o.experts), "experts_gemm_fp8", "B is not a matrix of each expert that fits A");
+  detail::require(detail::holds(C, o.rows(), B.rows), "experts_gemm_fp8", "C is smaller than the slots' rows");
+  ctx.check(miaie_experts_gemm_fp8(ctx.get(), o.order.data(), A.q.data(), A.s.data(), B.q.data(), B.s.data(), C.data(),
+                                   dtype_of(C.data()), o.tokens, o.top_k, o.experts, B.rows, A.cols, B.rows, gather ? 1 : 0));
+}
+
+// Conversions over slots: Q (rows() x cols) and / or Qt (its transpose), either NULL.
+template <typename T>
+void experts_quant_fp8(const ExpertsOrder& o, const Buffer<T>& X, const Buffer<float>* w, Fp8Matrix* Q, Fp8Matrix* Qt, int cols,
+                       Context& ctx = Context::current()) {
+  detail::require(detail::holds(X, o.tokens, cols) && (!w || detail::holds(*w, o.tokens, o.top_k)), "experts_quant_fp8",
+                  "X or w is too small");
+  detail::require(detail::is(Q, o.rows(), cols) && detail::is(Qt, cols, o.rows()), "experts_quant_fp8",
+                  "Q or Qt does not have the slots' shape");
+  ctx.check(miaie_experts_quant_fp8(ctx.get(), o.order.data(), X.data(), dtype_of(X.data()), detail::data(w), detail::codes(Q),
+                                    detail::scales(Q), detail::codes(Qt), detail::scales(Qt), o.tokens, o.top_k, o.experts, cols,
+                                    cols));
+}
+
+template <typename T>
+void experts_swiglu_fp8(const ExpertsOrder& o, const Buffer<T>& GU, Fp8Matrix* Q, Fp8Matrix* Qt, int F,
+                        Context& ctx = Context::current()) {
+  detail::require(F < 1 || detail::holds(GU, 2 * o.rows(), F), "experts_swiglu_fp8", "GU is smaller than the slots' 2 F columns");
+  detail::require(detail::is(Q, o.rows(), F) && detail::is(Qt, F, o.rows()), "experts_swiglu_fp8",
+                  "Q or Qt does not have the slots' shape");
+  ctx.check(miaie_experts_swiglu_fp8(ctx.get(), o.order.data(), GU.data(), dtype_of(GU.data()), detail::codes(Q), detail::scales(Q),
+                                     detail::codes(Qt), detail::scales(Qt), o.tokens, o.top_k, o.experts, F, 2 * F));
+}
+
+template <typename T>
+void experts_swiglu_grad_fp8(const ExpertsOrder& o, const Buffer<T>& GU, const Buffer<float>& dH, Fp8Matrix* Q, Fp8Matrix* Qt, int F,
+                             Context& ctx = Context::current()) {
+  detail::require(F < 1 || (detail::holds(GU, 2 * o.rows(), F) && detail::holds(dH, o.rows(), F)), "experts_swiglu_grad_fp8",
+                  "GU or dH is smaller than the slots' columns");
+  detail::require(detail::is(Q, o.rows(), 2 * F) && detail::is(Qt, 2 * F, o.rows()), "experts_swiglu_grad_fp8",
+                  "Q or Qt does not have the slots' shape");
+  ctx.check(miaie_experts_swiglu_grad_fp8(ctx.get(), o.order.data(), GU.data(), dtype_of(GU.data()), dH.data(), detail::codes(Q),
+                                          detail::scales(Q), detail::codes(Qt), detail::scales(Qt), o.tokens, o.top_k, o.experts,
+                                          F, 2 * F, F));
+}
+
+// C (experts x At.rows x Bt.rows): each expert's At . Bt^T over its slots.
+template <typename T>
+void experts_wgrad_fp8(const ExpertsOrder& o, const Fp8Matrix& At, const Fp8Matrix& Bt, Buffer<T>& C,
+                       Context& ctx = Context::current()) {
+  detail::require(detail::is(At, At.rows, o.rows(), 1) && detail::is(Bt, Bt.rows, o.rows(), 1), "experts_wgrad_fp8",
+                  "At or Bt is not packed along the slots");
+  detail::require(At.rows < 1 || Bt.rows < 1 || C.size() / (size_t)At.rows / (size_t)Bt.rows >= (size_t)o.experts,
+                  "experts_wgrad_fp8", "C is smaller than the experts' matrices");
+  ctx.check(miaie_experts_wgrad_fp8(ctx.get(), o.order.data(), At.q.data(), At.s.data(), Bt.q.data(), Bt.s.data(), C.data(),
+                                    dtype_of(C.data()), o.tokens, o.top_k, o.experts, At.rows, Bt.rows, Bt.rows));
+}
+
+// out[t] = sum over t's slots of w Y[slot] (w NULL: of Y[slot]).
+template <typename T>
+void experts_combine(const ExpertsOrder& o, const Buffer<T>& Y, const Buffer<float>* w, Buffer<T>& out, int cols,
+                     Context& ctx = Context::current()) {
+  detail::require(detail::holds(Y, o.rows(), cols) && detail::holds(out, o.tokens, cols) &&
+                      (!w || detail::holds(*w, o.tokens, o.top_k)),
+                  "experts_combine", "Y, out or w is too small");
+  ctx.check(miaie_experts_combine(ctx.get(), o.order.data(), Y.data(), detail::data(w), out.data(), dtype_of(out.data()),
+                                  o.tokens, o.top_k, o.experts, cols, cols, cols));
+}
+
+template <typename T>
+void experts_combine_grad(const ExpertsOrder& o, const Buffer<T>& Y, const Buffer<T>& dout, Buffer<float>& dw, int cols,
+                          Context& ctx = Context::current()) {
+  detail::require(detail::holds(Y, o.rows(), cols) && detail::holds(dout, o.tokens, cols) &&
+                      detail::holds(dw, o.tokens, o.top_k),
+                  "experts_combine_grad", "Y, dout or dw is too small");
+  ctx.check(miaie_experts_combine_grad(ctx.get(), o.order.data(), Y.data(), dout.data(), dw.data(), dtype_of(Y.data()), o.tokens,
+                                       o.top_k, o.experts, cols, cols, cols));
 }
 
 }  // namespace miaie
