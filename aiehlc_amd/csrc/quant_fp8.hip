@@ -7,6 +7,7 @@
 // dY along both axes and X along its columns; the transpose of weights packed in
 // blocks of 128 x 128 has the same codes and scales.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8.hpp"
 
@@ -21,20 +22,54 @@ using namespace fp8;
 // are in flight together.  (A load and its use in one branch a row wait for each
 // other: 2048 x 4096 bf16 10.3 us.)  fetch takes rows that do not exist, or are
 // padding, from where there is one, and values makes them zero.
-template <class T>
-struct Eight {
+template <class T, bool WHOLE>
+struct Eight {  // all eight columns exist, of any thread of the workgroup
   typedef T V __attribute__((ext_vector_type(8)));
   V v;
-  // WHOLE: all eight columns exist, of any thread of the workgroup
-  template <bool WHOLE>
-  __device__ __forceinline__ void load(const T* p, int n) {
-    if constexpr (WHOLE) {
+  __device__ __forceinline__ void load(const T* p, int = 8, int = 8) {
+    using P = At<V, T>;
+    v = MIAIE_LD(reinterpret_cast<const P*>(p)).v;
+  }
+  __device__ __forceinline__ void place() {}
+  __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
+};
+
+// n columns from p on exist of a row of C.  Where that is fewer than eight, the row's
+// last eight are loaded, one vector like the others', and shifted to their places (eight
+// loads and conditions of their own: 333 x 1000 bf16 6.4 us for 3.8, most of the difference
+// the way of so many instructions into the cache).
+template <class T>
+struct Eight<T, false> {
+  typedef T V __attribute__((ext_vector_type(8)));
+  typedef uint32_t W __attribute__((ext_vector_type(2 * sizeof(T))));
+  V v;
+  int shift;
+  __device__ __forceinline__ void load(const T* p, int n, int C) {
+    if (C >= 8) {
       using P = At<V, T>;
-      v = MIAIE_LD(reinterpret_cast<const P*>(p)).v;
+      v = MIAIE_LD(reinterpret_cast<const P*>(p + min(0, n - 8))).v;
+      shift = 8 - n;
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = i < n ? MIAIE_LD(p + i) : (T)0.f;
+      shift = 0;
     }
+  }
+  // (what is behind the last column is anything)
+  __device__ __forceinline__ void place() {
+    if (shift <= 0) return;
+    constexpr int K = 2 * sizeof(T);  // words
+    W w = __builtin_bit_cast(W, v);
+#pragma unroll
+    for (int by = 4; by > 0; by /= 2) {
+      const int words = by * K / 8;
+#pragma unroll
+      for (int i = 0; i < K; ++i) {
+        const uint32_t from = words ? w[min(i + words, K - 1)] : __builtin_amdgcn_alignbit(w[min(i + 1, K - 1)], w[i], 16);
+        w[i] = shift & by ? from : w[i];
+      }
+    }
+    v = __builtin_bit_cast(V, w);
   }
   __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
 };
@@ -45,18 +80,21 @@ struct FromMatrix {
   int R, C, ldx;
   static constexpr bool TAILS = true;  // tiles whose last columns do not exist
   using Row = int;
-  using Raw = Eight<T>;
+  template <bool WHOLE>
+  using Raw = Eight<T, WHOLE>;
   __device__ __forceinline__ bool tile(int) const { return true; }
   __device__ __forceinline__ Row row(int r) const { return r; }
   template <bool WHOLE>
-  __device__ __forceinline__ Raw fetch(Row r, int c) const {
-    Raw raw;
-    raw.template load<WHOLE>(X + (size_t)min(r, R - 1) * ldx + c, C - c);
+  __device__ __forceinline__ Raw<WHOLE> fetch(Row r, int c) const {
+    Raw<WHOLE> raw;
+    raw.load(X + (size_t)min(r, R - 1) * ldx + c, C - c, C);
     return raw;
   }
-  __device__ __forceinline__ void values(Row r, int, const Raw& raw, float (&x)[8]) const {
+  template <bool WHOLE>
+  __device__ __forceinline__ void values(Row r, int c, Raw<WHOLE> raw, float (&x)[8]) const {
+    raw.place();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = r < R ? raw[i] : 0.f;
+    for (int i = 0; i < 8; ++i) x[i] = r < R && (WHOLE || c + i < C) ? raw[i] : 0.f;
   }
 };
 
@@ -69,22 +107,25 @@ struct FromTokens {
   int R, C, ldx;
   static constexpr bool TAILS = true;
   using Row = int;  // pair
+  template <bool WHOLE>
   struct Raw {
-    Eight<T> x;
+    Eight<T, WHOLE> x;
     float f;
   };
   __device__ __forceinline__ bool tile(int r0) const { return r0 < MIAIE_LD(s.start + s.experts); }
   __device__ __forceinline__ Row row(int r) const { return MIAIE_LD(s.row_of + r); }
   template <bool WHOLE>
-  __device__ __forceinline__ Raw fetch(Row pair, int c) const {
-    Raw raw;
-    raw.x.template load<WHOLE>(X + (size_t)(max(pair, 0) / s.top_k) * ldx + c, C - c);
+  __device__ __forceinline__ Raw<WHOLE> fetch(Row pair, int c) const {
+    Raw<WHOLE> raw;
+    raw.x.load(X + (size_t)(max(pair, 0) / s.top_k) * ldx + c, C - c, C);
     raw.f = w ? MIAIE_LD(w + max(pair, 0)) : 1.f;
     return raw;
   }
-  __device__ __forceinline__ void values(Row pair, int c, const Raw& raw, float (&x)[8]) const {
+  template <bool WHOLE>
+  __device__ __forceinline__ void values(Row pair, int c, Raw<WHOLE> raw, float (&x)[8]) const {
+    raw.x.place();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = pair >= 0 && c + i < C ? raw.x[i] * raw.f : 0.f;  // (no -0 or NaN behind the last column)
+    for (int i = 0; i < 8; ++i) x[i] = pair >= 0 && (WHOLE || c + i < C) ? raw.x[i] * raw.f : 0.f;  // (no -0 or NaN behind the last column)
   }
 };
 
@@ -98,20 +139,22 @@ struct FromSwiglu {
   struct Row {
     int r, pair;
   };
+  template <bool WHOLE>
   struct Raw {
-    Eight<T> g, u;
+    Eight<T, WHOLE> g, u;
   };
   __device__ __forceinline__ bool tile(int r0) const { return r0 < MIAIE_LD(s.start + s.experts); }
   __device__ __forceinline__ Row row(int r) const { return Row{r, MIAIE_LD(s.row_of + r)}; }
   template <bool WHOLE>
-  __device__ __forceinline__ Raw fetch(Row r, int c) const {
+  __device__ __forceinline__ Raw<WHOLE> fetch(Row r, int c) const {
     static_assert(WHOLE, "F is a multiple of 128");
-    Raw raw;
-    raw.g.template load<true>(GU + (size_t)r.r * ldx + c, 8);
-    raw.u.template load<true>(GU + (size_t)r.r * ldx + C + c, 8);
+    Raw<WHOLE> raw;
+    raw.g.load(GU + (size_t)r.r * ldx + c);
+    raw.u.load(GU + (size_t)r.r * ldx + C + c);
     return raw;
   }
-  __device__ __forceinline__ void values(Row r, int, const Raw& raw, float (&x)[8]) const {
+  template <bool WHOLE>
+  __device__ __forceinline__ void values(Row r, int, const Raw<WHOLE>& raw, float (&x)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = r.pair >= 0 ? swiglu(raw.g[i], raw.u[i]) : 0.f;
   }
@@ -129,23 +172,25 @@ struct FromSwigluGrad {
   struct Row {
     int r, pair;
   };
+  template <bool WHOLE>
   struct Raw {
-    Eight<T> g, u;
-    Eight<float> d;
+    Eight<T, WHOLE> g, u;
+    Eight<float, WHOLE> d;
   };
   __device__ __forceinline__ bool tile(int r0) const { return r0 < MIAIE_LD(s.start + s.experts); }
   __device__ __forceinline__ Row row(int r) const { return Row{r, MIAIE_LD(s.row_of + r)}; }
   template <bool WHOLE>
-  __device__ __forceinline__ Raw fetch(Row r, int c) const {
+  __device__ __forceinline__ Raw<WHOLE> fetch(Row r, int c) const {
     static_assert(WHOLE, "F is a multiple of 128");
     const int F = C / 2, f = c < F ? c : c - F;
-    Raw raw;
-    raw.g.template load<true>(GU + (size_t)r.r * ldx + f, 8);
-    if (c < F) raw.u.template load<true>(GU + (size_t)r.r * ldx + F + f, 8);  // (the same for the workgroup)
-    raw.d.template load<true>(dH + (size_t)r.r * ldh + f, 8);
+    Raw<WHOLE> raw;
+    raw.g.load(GU + (size_t)r.r * ldx + f);
+    if (c < F) raw.u.load(GU + (size_t)r.r * ldx + F + f);  // (the same for the workgroup)
+    raw.d.load(dH + (size_t)r.r * ldh + f);
     return raw;
   }
-  __device__ __forceinline__ void values(Row r, int c, const Raw& raw, float (&x)[8]) const {
+  template <bool WHOLE>
+  __device__ __forceinline__ void values(Row r, int c, const Raw<WHOLE>& raw, float (&x)[8]) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float g = raw.g[i];
@@ -183,20 +228,24 @@ __global__ __launch_bounds__(512) void quant_tile(Src src, uint8_t* __restrict__
   float x[N][8];
   {
     typename Src::Row row[N];
-    typename Src::Raw raw[N];
 #pragma unroll
     for (int p = 0; p < N; ++p) row[p] = src.row(r0 + p);
-    bool whole = true;
-    if constexpr (Src::TAILS) whole = 128 * tc + 128 <= src.C;
-    if (whole) {
+    auto take = [&](auto whole_c) __attribute__((always_inline)) {
+      constexpr bool WHOLE = decltype(whole_c)::value;
+      typename Src::template Raw<WHOLE> raw[N];
 #pragma unroll
-      for (int p = 0; p < N; ++p) raw[p] = src.template fetch<true>(row[p], c);
-    } else if constexpr (Src::TAILS) {
+      for (int p = 0; p < N; ++p) raw[p] = src.template fetch<WHOLE>(row[p], c);
 #pragma unroll
-      for (int p = 0; p < N; ++p) raw[p] = src.template fetch<false>(row[p], c);
+      for (int p = 0; p < N; ++p) src.template values<WHOLE>(row[p], c, raw[p], x[p]);
+    };
+    if constexpr (Src::TAILS) {
+      if (128 * tc + 128 <= src.C)
+        take(std::true_type{});
+      else
+        take(std::false_type{});
+    } else {
+      take(std::true_type{});
     }
-#pragma unroll
-    for (int p = 0; p < N; ++p) src.values(row[p], c, raw[p], x[p]);
   }
   uint32_t e_row[N], e_all = 0;
   if constexpr (BLOCK == 128) {
