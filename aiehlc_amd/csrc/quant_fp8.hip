@@ -18,7 +18,7 @@ using namespace fp8;
 
 // ---- where a tile's values come from: eight columns c .. c + 7 of a row.  A source
 // says in turn what a row is (row), loads its columns (fetch) and makes their values
-// (values); a thread does each for its eight rows before the next, so that all loads
+// (values); a thread does each for its rows before the next, so that all loads
 // are in flight together.  (A load and its use in one branch a row wait for each
 // other: 2048 x 4096 bf16 10.3 us.)  fetch takes rows that do not exist, or are
 // padding, from where there is one, and values makes them zero.
