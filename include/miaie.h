@@ -425,7 +425,7 @@ MIAIE_API int miaie_norm_block_grad(miaie_ctx* ctx, const void* r, const void* b
 /* ---- 8-bit floating point with a scale for each block of 128 -------------- */
 
 /* No counterpart in the reference.  A packed matrix of R rows and K columns is
- * two device arrays, both 16-byte aligned and dense:
+ * two dense device arrays, Q 16-byte and S 4-byte aligned:
  *   Q  uint8 [R][miaie_fp8_q_pitch(K)]: E4M3 elements (OCP: up to 448, no
  *      infinities), rows of whole 128-byte lines, zero behind column K;
  *   S  fp32 [ceil(K / 128)][ceil(R / block)]: the scale of 128 columns of `block`
@@ -486,7 +486,9 @@ MIAIE_API int miaie_plan_gemm_fp8(int M, int N, int K, int b_block, int cus, mia
  * index, and
  *   w[j] = scale * score[j] / (sum of the token's chosen scores + 1e-20)
  * (scale * score[j] if renormalize is 0) to w (fp32 tokens x top_k).  Scores are
- * computed and compared in 64 bits.
+ * computed in 64 bits.  With a bias or more than one group they are compared as
+ * such; otherwise the choice has the order of the logits, also where scores of
+ * different logits round to the same (above 37 under a sigmoid).
  * An expert whose logit (or bias) is -infinity is never chosen; where a token has
  * fewer than top_k others, idx is -1 and w 0 for the rest (all of them for the
  * padding of a batch).  A NaN among a token's logits or in the choice of an expert

@@ -466,6 +466,18 @@ void quant_fp8_both(const Buffer<T>& X, Fp8Matrix& Q, Fp8Matrix& Qt, Context& ct
                             Qt.q.data(), Qt.s.data()));
 }
 
+// Matrix e of Q, and with Qt that of the transposes: the experts' weights.
+template <typename T>
+void quant_fp8_at(const Buffer<T>& X, Fp8Matrix& Q, int e, Fp8Matrix* Qt = nullptr, Context& ctx = Context::current()) {
+  detail::require(detail::holds(X, Q.rows, Q.cols) && e >= 0 && e < Q.count, "quant_fp8_at", "X is smaller than Q, or Q has no such matrix");
+  detail::require(!Qt || detail::is(*Qt, Q.cols, Q.rows, Q.block, Q.count), "quant_fp8_at",
+                  "Qt does not have the shape of Q's transposes");
+  ctx.check(miaie_quant_fp8(ctx.get(), X.data(), dtype_of(X.data()), Q.rows, Q.cols, Q.cols, Q.block,
+                            Q.q.data() + e * (Q.q.size() / Q.count), Q.s.data() + e * (Q.s.size() / Q.count),
+                            Qt ? Qt->q.data() + e * (Qt->q.size() / Qt->count) : nullptr,
+                            Qt ? Qt->s.data() + e * (Qt->s.size() / Qt->count) : nullptr));
+}
+
 // Y = the values of Q.
 template <typename T>
 void dequant_fp8(const Fp8Matrix& Q, Buffer<T>& Y, Context& ctx = Context::current()) {

@@ -144,6 +144,14 @@ int main() {
   REACHES("quant 1 7 300 300 128", P(h.data(), M(B), M(Bt)), quant_fp8_both(h, B, Bt));
   REFUSED("transpose", quant_fp8_both(h, B, At));
   REFUSED("X is smaller", quant_fp8_both(h1, B, Bt));
+  Fp8Matrix B3(ctx, 7, 300, 128, 3), B3t(ctx, 300, 7, 128, 3);
+  REACHES("quant 1 7 300 300 128", P(h.data(), B3.q.data() + 2 * 7 * 384, B3.s.data() + 2 * 3, nullptr, nullptr), quant_fp8_at(h, B3, 2));
+  REACHES("quant 1 7 300 300 128", P(h.data(), B3.q.data() + 7 * 384, B3.s.data() + 3, B3t.q.data() + 300 * 128, B3t.s.data() + 3),
+          quant_fp8_at(h, B3, 1, &B3t));
+  REFUSED("no such", quant_fp8_at(h, B3, 3));
+  REFUSED("no such", quant_fp8_at(h, B3, -1));
+  REFUSED("X is smaller", quant_fp8_at(h1, B3, 0));
+  REFUSED("transposes", quant_fp8_at(h, B3, 0, &Bt));
   REACHES("dequant 1 1 5 300 300", P(M(A), h.data()), dequant_fp8(A, h));
   REFUSED("Y is smaller", dequant_fp8(A, x1));
   REACHES("gemm 128 0 5 7 300 7", P(M(A), M(B), c.data()), gemm_fp8(A, B, c));

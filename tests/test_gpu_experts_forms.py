@@ -241,6 +241,49 @@ def test_two_streams_at_once(ctx):
         other.close()
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_scores_that_round_to_the_same(ctx, scoring):
+    """Without a bias the larger logit comes first, with one (of zeros) the lower index of equal scores."""
+    _say("equal scores", scoring)
+    if scoring == "sigmoid":
+        row = [40.0, 60.0, -3.0, 50.0, 60.0, 1e30, 2.0]      # 1 in 64 bits above 37
+    else:
+        row = [0.0, 1e-20, -1000.0, -900.0, 1e-30, -800.0, -1e-25]  # e^x is 1, or 0 next to the others
+    E, k = len(row), 6
+    by_logit = sorted(range(E), key=lambda e: (-row[e], e))[:k]
+    s = fp8.scores(np.float64([row]), scoring)[0]
+    by_score = sorted(range(E), key=lambda e: (-s[e], e))[:k]
+    assert by_logit != by_score
+    l, zero = ctx.upload(np.float32([row])), ctx.upload(np.zeros(E, np.float32))
+    idx, w = ctx.empty((1, k), np.int32), ctx.empty((1, k), np.float32)
+    for bias, want in ((None, by_logit), (zero, by_score)):
+        ctx.route_experts(l, bias, idx, w, 1, k, E, scoring=SCORING[scoring], renormalize=False)
+        ctx.wait(60_000)
+        assert ctx.download(idx)[0].tolist() == want
+        assert (np.abs(ctx.download(w)[0] - s[want]) <= 2.0**-23 * s[want]).all()
+    _free(l, zero, idx, w)
+
+
+@pytest.mark.parametrize("R, C", [(40, 70), (384, 300), (128, 128)])
+def test_matrices_of_experts_packed_one_after_another(ctx, R, C):
+    """Along both axes; an expert's scales start wherever the one's before end."""
+    _say("experts' weights", R, C)
+    E = 3
+    W = fp8.bf16(np.random.default_rng(R).standard_normal((E, R, C))).astype(np.float64)
+    (sq, ss), (tq, ts) = mi.fp8_shapes(R, C, 128), mi.fp8_shapes(C, R, 128)
+    d = [_up(ctx, w, "bf16") for w in W]
+    q, s, t, u = (ctx.empty((E, *n), dt) for n, dt in ((sq, np.uint8), (ss, np.float32), (tq, np.uint8), (ts, np.float32)))
+    for e in range(E):
+        ctx.quant_fp8(d[e], R, C, q.ptr + e * np.prod(sq), s.ptr + 4 * e * np.prod(ss), t.ptr + e * np.prod(tq),
+                      u.ptr + 4 * e * np.prod(ts), block=128)
+    ctx.wait(60_000)
+    for e in range(E):
+        for got_q, got_s, x in ((q, s, W[e]), (t, u, W[e].T)):
+            Q, S = fp8.pack(x, 128)
+            assert np.array_equal(ctx.download(got_q)[e], Q) and np.array_equal(ctx.download(got_s)[e], S)
+    _free(*d, q, s, t, u)
+
+
 # ---------------------------------------------------------------- beyond 2^32 bytes
 def _at(ctx, buf, offset, arr):
     """Writes arr at a byte offset of a buffer."""
@@ -367,7 +410,7 @@ def test_refusals(ctx):
                [(0, p + 1, "16-byte"), (1, None, "Xs is NULL"), (2, 0, "block=0"), (3, None, "Y is NULL"), (3, p + 1, "misaligned"),
                 (4, 7, "dtype=7"), (5, -1, "R=-1"), (6, 0, "C=0"), (7, 3, "ldy=3")])
     one_by_one("gemm_fp8", (p, p, p, p, 128, p, BF16, 4, 4, 4, 4),
-               [(0, None, "Aq is NULL"), (1, p + 4, "16-byte"), (2, None, "Bq is NULL"), (3, None, "Bs is NULL"), (4, 2, "b_block=2"),
+               [(0, None, "Aq is NULL"), (1, p + 2, "4-byte"), (2, None, "Bq is NULL"), (3, None, "Bs is NULL"), (4, 2, "b_block=2"),
                 (5, None, "C is NULL"), (5, p + 1, "misaligned"), (6, 4, "dtype=4"), (7, 0, "M=0"), (8, (1 << 25) + 1, "N="),
                 (9, (1 << 23) + 1, "K="), (10, 3, "ldc=3")])
     refused("gemm_fp8", p, p, p, p, 128, p, BF16, 1 << 25, 1 << 25, 4, 1 << 25, text="too large")
@@ -386,7 +429,7 @@ def test_refusals(ctx):
     #            order w  X       W1      W2      H      Y  out dtype T  k  E   D   F  N  ldo
     mlp = (p, p, p, p, p, p, p, p, p, p, p, p, BF16, 4, 2, 8, 16, 128, 16, 16)
     one_by_one("experts_mlp_fp8", mlp,
-               [(0, None, "order is NULL"), (1, None, "w is NULL"), (2, None, "Xq is NULL"), (5, p + 8, "16-byte"), (7, None, "W2s is NULL"),
+               [(0, None, "order is NULL"), (1, None, "w is NULL"), (2, None, "Xq is NULL"), (4, p + 8, "16-byte"), (7, None, "W2s is NULL"),
                 (8, None, "Hq is NULL"), (10, p + 1, "Y"), (11, None, "out is NULL"), (12, 3, "dtype=3"), (13, 0, "tokens=0"),
                 (16, 0, "D=0"), (17, 64, "F=64"), (17, 0, "F=0"), (18, (1 << 20) + 1, "Nout="), (19, 15, "ldo=15")])
     refused("experts_mlp_fp8", *mlp[:13], 1 << 20, 2, 8, 4096, 128, 16, 16, text="2^32 bytes")
@@ -406,7 +449,7 @@ def test_refusals(ctx):
                [(1, p + 1, "GU"), (3, None, "dH is NULL"), (4, None, "Xq is NULL"), (11, 100, "F=100"), (12, 255, "ldgu=255"),
                 (13, 127, "ldh=127")])
     one_by_one("experts_wgrad_fp8", (p, p, p, p, p, p, F32, 4, 2, 8, 16, 16, 16),
-               [(1, None, "Atq is NULL"), (4, p + 4, "16-byte"), (5, None, "C is NULL"), (10, 0, "M=0"), (11, 0, "N=0"), (12, 15, "ldc=15")])
+               [(1, None, "Atq is NULL"), (4, p + 2, "4-byte"), (5, None, "C is NULL"), (10, 0, "M=0"), (11, 0, "N=0"), (12, 15, "ldc=15")])
     refused("experts_wgrad_fp8", p, p, p, p, p, p, F32, 4, 2, 8, 1 << 20, 1 << 20, 1 << 20, text="too large")
     one_by_one("experts_combine", (p, p, p, p, F32, 4, 2, 8, 16, 16, 16),
                [(1, None, "Y is NULL"), (2, p + 2, "w"), (3, None, "out is NULL"), (8, 0, "C=0"), (9, 15, "ldy=15"), (10, 15, "ldo=15")])
