@@ -19,6 +19,7 @@
 // result has row m = l % 16 and the four consecutive columns n = 4 (l / 16) + 0..3
 // of its 16 x 16 block: vectors of a row of C, and one scale of A a lane.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "fp8.hpp"
@@ -689,9 +690,9 @@ __device__ __forceinline__ int scan_wave(int v) {
 
 // A tile of up to ROWS slots of one expert: its tiles are ceil(count / ROWS) of rows
 // times tiles_n, walked rows first, so that those which share columns of B run beside
-// each other, and the workgroups of one XCD (b % 8) have a contiguous run of all
-// tiles: few experts' operands in one L2.  Every wave finds its tile from the experts'
-// counts: loads beside each other, where a walk through the order's parts would be
+// each other, and the workgroups of one XCD have a contiguous run of all tiles, this
+// the i-th of it: few experts' operands in one L2.  Every wave finds its tile from the
+// experts' counts: loads beside each other, where a walk through the order's parts would be
 // three that wait for one another, and no workgroup without a tile among the others
 // (such a one waits for a whole CU's LDS like the rest: 16384 slots of 64 experts at
 // 256 rows a tile 235 us with as many empty ones, 168 without).  False: no tile.
@@ -699,14 +700,14 @@ struct SlotTile {
   int e, slot, rows, tn;  // rows: of the expert from this slot on
 };
 template <int ROWS>
-__device__ __forceinline__ bool slot_tile(const Slots& s, int b, int tiles_n, SlotTile& to) {
+__device__ __forceinline__ bool slot_tile(const Slots& s, int xcd, int i, int tiles_n, SlotTile& to) {
   const int lane = threadIdx.x & 63;
   auto count_of = [&](int e0) { return e0 + lane < s.experts ? MIAIE_LD(s.count + e0 + lane) : 0; };
   int count = count_of(0), rows = scan_wave((count + ROWS - 1) / ROWS), total = __builtin_amdgcn_readlane(rows, 63);
   for (int e0 = 64; e0 < s.experts; e0 += 64)
     total += __builtin_amdgcn_readlane(scan_wave((count_of(e0) + ROWS - 1) / ROWS), 63);
-  const int tiles = total * tiles_n, each = (tiles + 7) / 8, logical = b % 8 * each + b / 8;
-  if (b / 8 >= each || logical >= tiles) return false;
+  const int tiles = total * tiles_n, each = (tiles + 7) / 8, logical = xcd * each + i;
+  if (i >= each || logical >= tiles) return false;
   const int at = logical / tiles_n;
   int before = 0, blocks_before = 0, e0 = 0;  // tiles of rows, and blocks of 128 slots, before expert e0
   int blocks_to = scan_wave((count + 127) / 128);
@@ -800,7 +801,7 @@ __global__ __launch_bounds__(G::THREADS) void gemm_tile(Args p, int tiles_m, int
   constexpr int COLS = OUT == OUT_GLU ? G::BN / 2 : G::BN;
   if constexpr (MODE == SLOTS) {
     SlotTile t;
-    if (!slot_tile<G::BM>(p.s, blockIdx.x, tiles_n, t)) return;
+    if (!slot_tile<G::BM>(p.s, blockIdx.x % 8, blockIdx.x / 8, tiles_n, t)) return;
     run_tile_at<G, MODE, OUT, BBLOCK>(p, lds, t.e, t.slot, t.tn * COLS, t.rows);
   } else {
     const int each = tiles_m * tiles_n, e = MODE == WGRAD ? blockIdx.x / each : 0;
@@ -817,7 +818,7 @@ __global__ __launch_bounds__(G::THREADS) void gemm_slots(Args p, int tiles_n) {
   __shared__ __attribute__((aligned(1024))) int8_t lds[G::LDS > H::LDS ? G::LDS : H::LDS];
   constexpr int COLS = OUT == OUT_GLU ? G::BN / 2 : G::BN;
   SlotTile t;
-  if (!slot_tile<256>(p.s, blockIdx.x, tiles_n, t)) return;
+  if (!slot_tile<256>(p.s, blockIdx.x % 8, blockIdx.x / 8, tiles_n, t)) return;
   if (t.rows > 128)
     run_tile_at<G, SLOTS, OUT, 128>(p, lds, t.e, t.slot, t.tn * COLS, t.rows);
   else
@@ -905,11 +906,12 @@ struct StreamTile {
   int rows;
 };
 
-// acc[m][u] of rows r0 .. r0 + MR - 1 (rows behind the last repeat it) and this wave's
-// b0 and b1, the sums over the lanes of a row in each of them.
+// acc[m][u] of the MR rows (those behind the last repeat it) and this wave's b0 and b1,
+// the sums over the lanes of a row in each of them.  `again`: LDS holds rows that other
+// waves may still read.
 template <int MR, int D, class RowA>
 __device__ __forceinline__ void stream_rows(int8_t* lds, const Args& p, const StreamTile& t, const uint8_t* const (&b)[2],
-                                            const float* const (&bs)[2], int r0, RowA row_a, int part, int parts, float (&acc)[MR][2]) {
+                                            const float* const (&bs)[2], bool again, RowA row_a, int part, int parts, float (&acc)[MR][2]) {
   const int tid = threadIdx.x, lane = tid & 63, threads = blockDim.x;
   const int steps = (int)blocks(p.K);
   const size_t pch = pitch(p.K);
@@ -917,10 +919,10 @@ __device__ __forceinline__ void stream_rows(int8_t* lds, const Args& p, const St
   for (int m = 0; m < MR; ++m) acc[m][0] = acc[m][1] = 0.f;
   for (int kb0 = 0; kb0 < steps; kb0 += STREAM_K) {
     const int n = min(STREAM_K, steps - kb0);
-    if (kb0 > 0 || r0 > 0) __syncthreads();
+    if (kb0 > 0 || again) __syncthreads();
     for (int i = tid; i < MR * n * 8; i += threads) {
       const int m = i / (8 * n), c = i % (8 * n);
-      const v4u v = MIAIE_LD(reinterpret_cast<const v4u*>(t.a + row_a(min(r0 + m, t.rows - 1)) * pch + 128 * (size_t)kb0 + 16 * c));
+      const v4u v = MIAIE_LD(reinterpret_cast<const v4u*>(t.a + row_a(min(m, t.rows - 1)) * pch + 128 * (size_t)kb0 + 16 * c));
       *reinterpret_cast<v4u*>(lds + 128 * m * STREAM_K + 16 * c) = v;
     }
     float s[MR][2];
@@ -929,7 +931,7 @@ __device__ __forceinline__ void stream_rows(int8_t* lds, const Args& p, const St
     for (int u = 0; u < 2; ++u) {
       const float sb = MIAIE_LD(bs[u] + kb * t.b_step);
 #pragma unroll
-      for (int m = 0; m < MR; ++m) s[m][u] = sb * MIAIE_LD(t.as + kb * t.a_step + row_a(min(r0 + m, t.rows - 1)));
+      for (int m = 0; m < MR; ++m) s[m][u] = sb * MIAIE_LD(t.as + kb * t.a_step + row_a(min(m, t.rows - 1)));
     }
     __syncthreads();
     const uint8_t* const from[2] = {b[0] + 128 * (size_t)kb0, b[1] + 128 * (size_t)kb0};
@@ -961,7 +963,10 @@ __device__ __forceinline__ void by_rows(int left, F&& f) {
 }
 
 // Four waves; 4 / parts of them have 16 columns each, and `parts` share out the blocks
-// of k, whose sums are added in LDS in their order.
+// of k, whose sums are added in LDS in their order.  Over slots a workgroup takes four
+// rows of one expert at a time, and the launch's workgroups share out all of these: with
+// an expert's to one workgroup, a popular expert's passes follow one another (256 slots
+// of one expert of 64, 1024 -> 4096 columns: 155 us, 55 shared out).
 template <Mode MODE, Out OUT>
 __global__ __launch_bounds__(256) void gemm_stream(Args p, int tiles_n, int parts) {
   __shared__ __attribute__((aligned(16))) int8_t lds[4 * 128 * STREAM_K];
@@ -969,37 +974,19 @@ __global__ __launch_bounds__(256) void gemm_stream(Args p, int tiles_n, int part
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int part = wave % parts, groups = 4 / parts;
   const size_t pch = pitch(p.K);
-  StreamTile t{p.Aq, p.Bq, p.As, p.Bs, (size_t)p.a_rows, blocks(p.N), p.M};
-  int slot0 = 0, n0;
-  if constexpr (MODE == SLOTS) {
-    SlotTile at;
-    if (!slot_tile<128>(p.s, blockIdx.x, tiles_n, at)) return;
-    slot0 = at.slot, n0 = 16 * groups * at.tn;
-    t.rows = min(128, at.rows);
-    if (!p.gather) t.a += (size_t)slot0 * pch, t.as += slot0;
-    t.b += (size_t)at.e * p.N * pch, t.bs += (size_t)at.e * blocks(p.N) * blocks(p.K);
-  } else {
-    n0 = 16 * groups * blockIdx.x;
-  }
-  const int col = n0 + 16 * (wave / parts);  // of this wave; behind the last one it repeats that
-  const uint8_t* b[2];
-  const float* bs[2];
+  auto pass = [&](const StreamTile& t, int row0, int n0, bool again, auto row_a) __attribute__((always_inline)) {
+    const int col = n0 + 16 * (wave / parts);  // of this wave; behind the last one it repeats that
+    const uint8_t* b[2];
+    const float* bs[2];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    b[u] = t.b + (size_t)min(col + 8 * u + (lane >> 3), p.N - 1) * pch + 16 * (lane & 7);
-    bs[u] = t.bs + min(col, p.N - 1) / 128;
-  }
-  for (int r0 = 0; r0 < t.rows; r0 += 4) {
-    auto row_a = [&](int r) __attribute__((always_inline)) -> size_t {
-      if constexpr (MODE == SLOTS) {
-        if (p.gather) return (size_t)(MIAIE_LD(p.s.row_of + slot0 + r) / p.s.top_k);
-      }
-      return (size_t)r;
-    };
-    by_rows(t.rows - r0, [&](auto mr) __attribute__((always_inline)) {
+    for (int u = 0; u < 2; ++u) {
+      b[u] = t.b + (size_t)min(col + 8 * u + (lane >> 3), p.N - 1) * pch + 16 * (lane & 7);
+      bs[u] = t.bs + min(col, p.N - 1) / 128;
+    }
+    by_rows(t.rows, [&](auto mr) __attribute__((always_inline)) {
       constexpr int MR = decltype(mr)::value;
       float acc[MR][2];
-      stream_rows<MR, 4>(lds, p, t, b, bs, r0, row_a, part, parts, acc);
+      stream_rows<MR, 4>(lds, p, t, b, bs, again, row_a, part, parts, acc);
       if ((lane & 7) == 0)
 #pragma unroll
         for (int m = 0; m < MR; ++m)
@@ -1008,13 +995,28 @@ __global__ __launch_bounds__(256) void gemm_stream(Args p, int tiles_n, int part
     });
     __syncthreads();
     // thread: row tid / 64, column tid % 64 of the workgroup's
-    const int m = r0 + wave, n = n0 + lane;
-    if (m < t.rows && lane < 16 * groups && n < p.N) {
+    const int n = n0 + lane;
+    if (wave < t.rows && lane < 16 * groups && n < p.N) {
       float sum = 0.f;
       for (int k = 0; k < parts; ++k) sum += sums[lane / 16 * parts + k][wave][lane % 16];
       using T = std::conditional_t<OUT == OUT_F32, float, __bf16>;
-      MIAIE_ST(static_cast<T*>(p.C) + (size_t)(slot0 + m) * p.ldc + n, (T)sum);
+      MIAIE_ST(static_cast<T*>(p.C) + (size_t)(row0 + wave) * p.ldc + n, (T)sum);
     }
+  };
+  if constexpr (MODE == SLOTS) {
+    const int first = blockIdx.x / 8;
+    SlotTile at;
+    for (int i = first; slot_tile<4>(p.s, blockIdx.x % 8, i, tiles_n, at); i += gridDim.x / 8) {
+      StreamTile t{p.Aq, p.Bq + (size_t)at.e * p.N * pch, p.As, p.Bs + (size_t)at.e * blocks(p.N) * blocks(p.K), (size_t)p.a_rows,
+                   blocks(p.N), min(4, at.rows)};
+      if (!p.gather) t.a += (size_t)at.slot * pch, t.as += at.slot;
+      pass(t, at.slot, 16 * groups * at.tn, i > first, [&](int r) __attribute__((always_inline)) -> size_t {
+        return p.gather ? (size_t)(MIAIE_LD(p.s.row_of + at.slot + r) / p.s.top_k) : (size_t)r;
+      });
+    }
+  } else {  // (up to four rows)
+    pass(StreamTile{p.Aq, p.Bq, p.As, p.Bs, (size_t)p.a_rows, blocks(p.N), p.M}, 0, 16 * groups * blockIdx.x, false,
+         [&](int r) __attribute__((always_inline)) -> size_t { return (size_t)r; });
   }
 }
 
@@ -1039,12 +1041,13 @@ __device__ __forceinline__ v4f mfma_wide(const Wide& b, const Wide& a) {
   return p;
 }
 
-// silu(gate) up of 128 columns of H and a block of slots, four rows at a time: eight
-// waves, each with 16 gate and 16 up columns over all of k.  A wave copies 256 bytes
-// (two blocks of k, a group) of its 32 rows of B and of A's rows into a part of LDS of
-// its own, waits for its own copies (no barriers) and multiplies; the next group is on
-// its way once this one's fragments are in registers.  Chunk c (16 bytes) of row r lies
-// at c ^ (r % 16).  Two workgroups fit a CU, so that one starts while another reads
+// silu(gate) up of 128 columns of H and four rows of an expert, shared out over the
+// launch's workgroups as in gemm_stream (256 slots of one expert, 4096 x 1024: 470 us by
+// one workgroup a column block, 40 shared out): eight waves, each with 16 gate and 16 up
+// columns over all of k.  A wave copies 256 bytes (two blocks of k, a group) of its 32
+// rows of B and of A's rows into a part of LDS of its own, waits for its own copies (no
+// barriers) and multiplies; the next group is on its way once this one's fragments are
+// in registers.  Chunk c (16 bytes) of row r lies at c ^ (r % 16).  Two workgroups fit a CU, so that one starts while another reads
 // (as loads of whole lines into registers, like gemm_stream, one fits: 101 us for 86
 // at 64 experts of 2048 x 4096, eight tokens of eight).
 constexpr int kGluRows = 4, kGluRegion = 2 * 4096 + 256 * kGluRows;
@@ -1056,26 +1059,24 @@ __global__ __launch_bounds__(512, 4) void glu_rows(Args p, int tiles_n) {
   const uint32_t row_pitch = (uint32_t)pitch(p.K);
   const size_t b_s_rows = blocks(2 * (long)p.N);
   const int steps = (int)blocks(p.K), groups = (steps + 1) / 2;
-  SlotTile t;
-  if (!slot_tile<128>(p.s, blockIdx.x, tiles_n, t)) return;
-  const int e = t.e, tn = t.tn, slot0 = t.slot, f0 = 128 * tn, rows = min(128, t.rows);
-  const uint8_t* const a = p.gather ? p.Aq : p.Aq + (size_t)slot0 * row_pitch;
-  const float* const as = p.gather ? p.As : p.As + slot0;
-  const uint8_t* const gate = p.Bq + ((size_t)e * 2 * p.N + f0 + 16 * wave) * row_pitch;
-  const uint8_t* const b[2] = {gate, gate + (size_t)p.N * row_pitch};
-  const float* const gate_s = p.Bs + (size_t)e * b_s_rows * steps + f0 / 128;
-  const float* const bs[2] = {gate_s, gate_s + p.N / 128};
   const dbg::Span aq_span = dbg::span_of(p.Aq), bq_span = dbg::span_of(p.Bq);  // (debug build only)
   const size_t h_pitch = pitch(p.N);
   int8_t* const mine = lds + wave * kGluRegion;
   const uint32_t mine0 = dev::lds_addr(mine);
-  for (int r0 = 0; r0 < rows; r0 += kGluRows) {
-    const int n = min(kGluRows, rows - r0);
+  SlotTile t;
+  for (int i = blockIdx.x / 8; slot_tile<kGluRows>(p.s, blockIdx.x % 8, i, tiles_n, t); i += gridDim.x / 8) {
+    const int e = t.e, tn = t.tn, slot0 = t.slot, f0 = 128 * tn, n = min(kGluRows, t.rows);
+    const uint8_t* const a = p.gather ? p.Aq : p.Aq + (size_t)slot0 * row_pitch;
+    const float* const as = p.gather ? p.As : p.As + slot0;
+    const uint8_t* const gate = p.Bq + ((size_t)e * 2 * p.N + f0 + 16 * wave) * row_pitch;
+    const uint8_t* const b[2] = {gate, gate + (size_t)p.N * row_pitch};
+    const float* const gate_s = p.Bs + (size_t)e * b_s_rows * steps + f0 / 128;
+    const float* const bs[2] = {gate_s, gate_s + p.N / 128};
     auto row_a = [&](int r) __attribute__((always_inline)) -> uint32_t {
-      r = slot0 + r0 + min(r, n - 1);  // (rows behind the last repeat it)
+      r = slot0 + min(r, n - 1);  // (rows behind the last repeat it)
       return p.gather ? (uint32_t)(MIAIE_LD(p.s.row_of + r) / p.s.top_k) : (uint32_t)(r - slot0);
     };
-    const uint32_t a_row = row_a(fg) , s_row = row_a(fr);
+    const uint32_t a_row = row_a(fg), s_row = row_a(fr);
     v4f acc[2] = {v4f{0.f, 0.f, 0.f, 0.f}, v4f{0.f, 0.f, 0.f, 0.f}};
     float sa[2], sb[2][2];
     auto copy = [&](int g) __attribute__((always_inline)) {
@@ -1137,7 +1138,7 @@ __global__ __launch_bounds__(512, 4) void glu_rows(Args p, int tiles_n) {
     for (int w = 0; w < 8; ++w) m = max(m, lmax[w][fr]);
     const uint32_t ex = scale_of(m);
     if (fr < n) {
-      const size_t slot = slot0 + r0 + fr;
+      const size_t slot = slot0 + fr;
       MIAIE_ST(reinterpret_cast<uint32_t*>(p.Hq + slot * h_pitch + f0 + 16 * wave + 4 * fg), pack4(h[0], h[1], h[2], h[3], inverse_f32(ex)));
       if (wave == 0 && fg == 0) MIAIE_ST(p.Hs + (size_t)tn * p.M + slot, scale_f32(ex));
     }
@@ -1150,8 +1151,8 @@ __global__ __launch_bounds__(512, 4) void glu_rows(Args p, int tiles_n) {
 // us on Block (16 workgroups a row of tiles: one round); 4096 x 4096 over 2048 35 us on
 // Large with a scale a row; 333 x 777 x 1000 5.6 us on Small; 1 x 11008 x 4096 10 us
 // by gemm_stream (4.5 TB/s).  64 experts of 256 slots, 4096 x 1024: gate and up 200 us,
-// down 123 us on Large and Block together; of one slot 86 us by glu_rows, 35 us by
-// gemm_stream.
+// down 123 us on Large and Block together; of one slot 86 us by glu_rows, 27 us on
+// Small.
 using Large = Tile<256, 256, 4, 2>;
 using Block = Tile<128, 256, 2, 3>;
 using Square = SmallTile<128, 128, 2>;
@@ -1235,7 +1236,10 @@ struct On {
 struct Stream {};
 struct GluRows {};
 
-// f(the kernel of a dense product)
+// f(the kernel of a dense product).  Up to four rows of weights: one reading of B by
+// gemm_stream (four rows, 4096 -> 11008, 4096 -> 4096 and 12288 -> 1024 columns: 16.6, 8.5
+// and 16.0 us, where the tile of 64 rows takes 15.3, 11.4 and 29.8 for five to 64; two
+// readings, for five to eight, 32, 16.0 and 31.9).
 template <class F>
 int with_dense(int M, int N, int K, int b_block, int cus, F&& f) {
   if (b_block == 128 && M <= 4) return f(Stream{});
@@ -1252,20 +1256,34 @@ int with_dense(int M, int N, int K, int b_block, int cus, F&& f) {
   }
 }
 
+// gemm_stream over slots: a wave takes half a microsecond for a block of k, and 256 CUs
+// read 4.8 TB/s of B, once for four rows of an expert.
+double stream_us(double passes, int N, int K, int cus) {
+  const double parts = stream_parts(K), bytes = passes * N * (double)pitch(K);
+  return 2.5 + std::max(0.5 * std::ceil(blocks(K) / parts), bytes / (4.8e6 * cus / 256));
+}
+
 // f(the kernel of a product over slots of N columns, or of H with N = F).  On<Large>
-// stands for tiles of both 256 and 128 rows.  Four slots an expert or fewer: kernels
-// that read B once for four rows; beyond, a tile of 64 rows is as quick and reads it
-// once for all.  An expert's last tile is half full on average, and tiles of up to 128
-// rows and columns take a tenth longer than among dense ones, B coming from memory.
+// stands for tiles of both 256 and 128 rows.  An expert's last tile is half full on
+// average, and tiles of up to 128 rows and columns take a tenth longer than among dense
+// ones, B coming from memory.
+//
+// Few slots have kernels that read B once for four rows, and add exact products.
+// glu_rows up to four slots an expert: one code of H that the tiles' cut-off moves weighs
+// most where few rows are added up, and its time is theirs or less but for few experts (H
+// of 64 experts, 4096 x 1024, random choices: 95 us for 115 of the tile of 64 rows at one
+// slot an expert on average, 111 for 130 at two, 133 for 148 at four; 8 experts, 2048 x
+// 1024: 18 for 20 at two, 28 for 20 at four).  gemm_stream where few matrices are read
+// along a long k (8 experts, 4096 -> 4096: 5.4 us for 11.7 of one slot, 12.2 for 12.7 of
+// four, 24 for 16 of eight; 64 experts, 1024 -> 4096: 7 for 6.4 of eight, 35 for 27 of
+// 64), so that its time is estimated too.
 template <bool GLU, class F>
 int with_slots(const Slots& s, int N, int K, int cus, F&& f) {
   const double n = (double)s.tokens * s.top_k, used = std::min<double>(s.experts, n);
   const long few = GLU ? N / 128 * 512l : (N + 15l) / 16 * 256l;  // threads of a block of slots
-  if (n <= 4.0 * s.experts && most_slot_tiles(s, 128) * few < kThreads) {
-    if constexpr (GLU)
-      return f(GluRows{});
-    else
-      return f(Stream{});
+  const bool can = n <= 4.0 * s.experts && most_slot_tiles(s, 128) * few < kThreads;
+  if constexpr (GLU) {
+    if (can) return f(GluRows{});
   }
   auto us = [&](const TileTime& t, int cols, int threads) {
     const double tiles_n = (double)((N + cols - 1l) / cols);
@@ -1280,10 +1298,12 @@ int with_slots(const Slots& s, int N, int K, int cus, F&& f) {
       default: return f(On<Large>{});
     }
   } else {
-    const double times[] = {us(kLarge, 256, 512), us(kSquare, 128, 256), us(kSmall, 64, 256)};
-    switch (std::min_element(times, times + 3) - times) {
+    const double times[] = {us(kLarge, 256, 512), us(kSquare, 128, 256), us(kSmall, 64, 256),
+                            can ? stream_us(used + (n - used) / 4, N, K, cus) : 1e300};
+    switch (std::min_element(times, times + 4) - times) {
       case 1: return f(On<Square>{});
       case 2: return f(On<Small>{});
+      case 3: return f(Stream{});
       default: return f(On<Large>{});
     }
   }

@@ -562,8 +562,9 @@ MIAIE_API int miaie_experts_gemm_fp8(miaie_ctx* ctx, const int* order, const uin
 
 /* How that runs (swiglu 0), or the first product of miaie_experts_mlp_fp8 (swiglu 1:
  * N = F, K = D, tile_n columns of H), as miaie_plan_gemm_fp8 says it; workgroups: the
- * most that a routing can need.  Where tile_m is 256, an expert's last 128 slots or
- * fewer are a tile of 128 rows. */
+ * most that a routing can need; those of MIAIE_KERNEL_ROWS share out all fours of an
+ * expert's rows.  Where tile_m is 256, an expert's last 128 slots or fewer are a tile of
+ * 128 rows. */
 MIAIE_API int miaie_plan_experts_fp8(int tokens, int top_k, int experts, int N, int K, int swiglu, int cus,
                                      miaie_gemm_plan* plan);
 
