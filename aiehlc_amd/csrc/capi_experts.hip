@@ -65,8 +65,10 @@ int check_forms(miaie_ctx* ctx, const char* fn, const uint8_t* Q, const float* S
 }
 
 // 512 threads pack 128 x 128; HIP takes fewer than 2^32 threads.
+bool tiles_fit(long R, long C) { return fp8::blocks(R) * fp8::blocks(C) < 1u << 23; }
+
 int check_tiles(miaie_ctx* ctx, const char* fn, long R, long C) {
-  if (fp8::blocks(R) * fp8::blocks(C) >= 1u << 23)
+  if (!tiles_fit(R, C))
     return fail(ctx, MIAIE_EINVAL, "%s: %ld rows of %ld columns are too large", fn, R, C);
   return MIAIE_OK;
 }
@@ -106,10 +108,12 @@ int check_slot_product(miaie_ctx* ctx, const char* fn, int tokens, int top_k, in
 
 extern "C" size_t miaie_fp8_q_pitch(int K) { return K < 1 || K > kMost ? 0 : fp8::pitch(K); }
 
-extern "C" size_t miaie_fp8_q_bytes(int R, int K) { return R < 1 || R > kMost ? 0 : (size_t)R * miaie_fp8_q_pitch(K); }
+extern "C" size_t miaie_fp8_q_bytes(int R, int K) {
+  return R < 1 || R > kMost || K < 1 || K > kMost || !tiles_fit(R, K) ? 0 : (size_t)R * fp8::pitch(K);
+}
 
 extern "C" size_t miaie_fp8_s_bytes(int R, int K, int block) {
-  if (R < 1 || R > kMost || K < 1 || K > kMost || (block != 1 && block != 128)) return 0;
+  if (!miaie_fp8_q_bytes(R, K) || (block != 1 && block != 128)) return 0;
   return 4 * fp8::blocks(K) * (block == 1 ? (size_t)R : fp8::blocks(R));
 }
 

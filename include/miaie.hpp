@@ -417,12 +417,19 @@ void norm_before_grad(const Buffer<S>& x, const Buffer<float>& w_before, const B
 
 // ---- 8-bit matrices with a scale for each block of 128, routing, experts ----
 
+namespace detail {
+inline size_t times(int count, size_t bytes) {
+  require(bytes > 0 && count > 0 && bytes <= SIZE_MAX / (size_t)count, "Fp8Matrix", "no packed matrices have such sizes");
+  return count * bytes;
+}
+}  // namespace detail
+
 // `count` packed matrices (miaie.h) of rows x cols, one after another: block 1 or
 // 128; count: the experts' matrices.
 struct Fp8Matrix {
   Fp8Matrix(Context& ctx, int rows, int cols, int block = 1, int count = 1)
-      : rows(rows), cols(cols), block(block), count(count), q(ctx, count * miaie_fp8_q_bytes(rows, cols)),
-        s(ctx, count * miaie_fp8_s_bytes(rows, cols, block) / 4) {}
+      : rows(rows), cols(cols), block(block), count(count), q(ctx, detail::times(count, miaie_fp8_q_bytes(rows, cols))),
+        s(ctx, detail::times(count, miaie_fp8_s_bytes(rows, cols, block)) / 4) {}
   int rows, cols, block, count;
   Buffer<uint8_t> q;
   Buffer<float> s;
