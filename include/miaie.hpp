@@ -554,7 +554,8 @@ template <typename T>
 void experts_mlp_fp8(const ExpertsOrder& o, const Buffer<float>& w, const Fp8Matrix& X, const Fp8Matrix& W1, const Fp8Matrix& W2,
                      Fp8Matrix& H, Buffer<T>& Y, Buffer<T>& out, Context& ctx = Context::current()) {
   detail::require(detail::is(X, o.tokens, X.cols, 1), "experts_mlp_fp8", "X is not the tokens' rows");
-  detail::require(detail::is(W1, 2 * W2.cols, X.cols, 128, o.experts) && detail::is(W2, W2.rows, W2.cols, 128, o.experts),
+  detail::require(W1.rows == 2l * W2.cols && detail::is(W1, W1.rows, X.cols, 128, o.experts) &&
+                      detail::is(W2, W2.rows, W2.cols, 128, o.experts),
                   "experts_mlp_fp8", "W1 and W2 are not matrices of each expert that fit X and each other");
   detail::require(detail::is(H, o.rows(), W2.cols, 1), "experts_mlp_fp8", "H does not have the slots' rows of F columns");
   detail::require(detail::holds(w, o.tokens, o.top_k) && detail::holds(Y, o.rows(), W2.rows) &&

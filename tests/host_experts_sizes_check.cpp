@@ -13,6 +13,11 @@ int main() {
   REFUSED("Fp8Matrix", Fp8Matrix(ctx, 5, 300, 1, 0));
   REFUSED("Fp8Matrix", Fp8Matrix(ctx, 5, 300, 1, -1));
   REFUSED("Fp8Matrix", Fp8Matrix(ctx, 1 << 30, 1 << 30, 1, 16));
+  // gate and up of 2^30 columns of H are more rows than an int holds
+  ExpertsOrder o(ctx, 10, 2, 8);
+  Fp8Matrix X(ctx, 10, 40), W1(ctx, 256, 40, 128, 8), W2(ctx, 1, 1 << 30, 128, 8), H(ctx, o.rows(), 128);
+  Buffer<float> w(ctx, 20), Y(ctx, o.rows()), out(ctx, 10);
+  REFUSED("each expert", experts_mlp_fp8(o, w, X, W1, W2, H, Y, out));
   if (!failures) std::printf("ok\n");
   return failures ? 1 : 0;
 }
