@@ -74,6 +74,14 @@ __device__ __forceinline__ V at_lane(V v, int lane) {
   return r;
 }
 
+// What the wave's lanes have written to LDS before, each of them reads behind.  (A wave's
+// LDS instructions stay in order; the compiler is kept from moving or splitting them.)
+__device__ __forceinline__ void wave_lds_order() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <class T>
 __device__ __forceinline__ float load1(const T* p) {
   return (float)MIAIE_LD(p);
@@ -153,9 +161,7 @@ __global__ __launch_bounds__(256) void route_tokens(const T* __restrict__ logits
       const int size = a.E / a.groups;
 #pragma unroll
       for (int p = 0; p < PER; ++p) mine[lane + 64 * p] = c[p];
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      wave_lds_order();
       // `shared` lanes a group, the largest power of two that leaves lanes for all of
       // them; each takes every shared-th member, and their best two are merged
       int shared = 64;
@@ -307,7 +313,10 @@ __global__ __launch_bounds__(256) void route_tokens_grad(const T* __restrict__ l
 // where its own pairs go without waiting for another; then each of its waves places
 // its part of the run in turn, 64 pairs at a time, a pair behind those of the same
 // expert in lower lanes.  (16384 pairs of 64 experts by one workgroup: 17.4 us, most
-// of it the placing.)
+// of it the placing; by 16 of them 6.4.)  Up to some 10^5 pairs the launch is most of the
+// time; beyond, that every workgroup counts all: 131072 pairs of 64 experts 21 us, 2^23 of
+// them 1.2 ms, and 115 us and 7.1 ms where all have one expert, whose count the 64 lanes
+// of a wave raise one by one (products over as many slots take some ten times as long).
 constexpr int kOrderWaves = 16, kOrderThreads = 64 * kOrderWaves, kOrderGroups = 64;
 __global__ __launch_bounds__(kOrderThreads) void order_slots(const int* __restrict__ idx, int* __restrict__ start,
                                                              int* __restrict__ count, int* __restrict__ slot_of,
@@ -405,13 +414,14 @@ __global__ __launch_bounds__(kOrderThreads) void order_slots(const int* __restri
         same &= (e[u] >> b & 1) ? has : ~has;
       }
       int slot = -1;
+      const int ahead = __popcll(same & ((1ull << lane) - 1)), base = e[u] >= 0 ? at[wave * experts + e[u]] : 0;
+      wave_lds_order();  // every lane has read its expert's place, which the first of them moves on
       if (e[u] >= 0) {
-        const int ahead = __popcll(same & ((1ull << lane) - 1)), base = at[wave * experts + e[u]];
         slot = base + ahead;
         MIAIE_ST(row_of + slot, i);
-        // (every lane has read its expert's place: one instruction for the wave)
         if (ahead == 0) at[wave * experts + e[u]] = base + __popcll(same);
       }
+      wave_lds_order();
       if (i < last) MIAIE_ST(slot_of + i, slot);
     }
   }
