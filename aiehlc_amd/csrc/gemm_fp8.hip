@@ -836,7 +836,8 @@ __global__ __launch_bounds__(G::THREADS) void gemm_slots(Args p, int tiles_n) {
 // fp32 products are exact here, where the 8-bit matrix instructions cut them off at
 // 2^-13 of the largest of eight.  That moves their sums by 1.5e-5, and one in 400
 // codes of a packed H with them; with many rows such steps average out, while a
-// token's own MLP had up to 5.7e-3 of its result from a few of them (2.4e-3 without).
+// token's own MLP was up to 5.7e-3 off with a few of them (2.4e-3 without: Y and out are
+// each rounded to bf16).
 constexpr int STREAM_K = 64;  // blocks of k whose A is in LDS at a time
 
 // <16 elements of a row of B, 16 elements of a row of A>

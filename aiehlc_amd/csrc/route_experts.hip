@@ -428,7 +428,10 @@ __global__ __launch_bounds__(kOrderThreads) void order_slots(const int* __restri
 }
 
 // out[t] = sum over the choices j, in their order, of w[t][j] Y[slot]: eight columns
-// a thread.
+// a thread.  Sums are fp32; Y has out's type, so that with bf16 each term has been rounded
+// once before.  That is a choice for bytes: 16384 slots of 4096 columns in fp32 are 134 MB
+// more to write and as many to read, 42 us of an MLP's 423 (64 experts, 4096 x 1024), and
+// who wants them asks for fp32 results.
 template <class T>
 __global__ __launch_bounds__(256) void combine(const T* __restrict__ Y, const float* __restrict__ w, T* __restrict__ out,
                                                Slots s, int C, int ldy, int ldo, int per_row, long units, long stride) {
