@@ -89,7 +89,7 @@ struct Slots {
   const int* count;      // [E]
   const int* slot_of;    // [T k]: slot of a pair, -1 without an expert
   const int* row_of;     // [rows]: pair of a slot (t k + choice), -1 in padding
-  const int* expert_of;  // [rows / 128], -1 behind the last slot in use
+  const int* expert_of;  // [rows / 128], -1 behind the last slot in use (for callers; the kernels go by the counts)
   int tokens, top_k, experts, rows;
 };
 

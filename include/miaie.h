@@ -528,16 +528,20 @@ MIAIE_API int miaie_route_experts_grad(miaie_ctx* ctx, const void* logits, int d
  * own; slots are sorted by expert, each expert's from a multiple of 128 on in the
  * order of its pairs.  Matrices over slots have miaie_experts_rows rows, whatever
  * the routing; rows of padding and behind the last slot in use are not written, and
- * nothing depends on what they hold, unless it says so below.  The order is one device array of int32,
- * miaie_experts_order_bytes long, with the parts
+ * nothing depends on what they hold, unless it says so below.  The order is one device
+ * array of int32, miaie_experts_order_bytes long, with the parts
  *   start [experts + 1]  first slot of each expert; the last: slots in use;
  *   count [experts]      slots of each expert; the part ends at a multiple of 16;
  *   slot [tokens][top_k] slot of a pair, -1 without an expert; ends at such too;
  *   pair [rows]          token * top_k + choice of a slot, -1 in padding, not
  *                        written behind the slots in use;
- *   expert [rows / 128]  of 128 slots each, -1 behind those in use.
+ *   expert [rows / 128]  of 128 slots each, -1 behind those in use (for callers: no
+ *                        entry point reads it).
  * tokens * top_k in [1, 2^23], experts in [1, MIAIE_MAX_EXPERTS], top_k in [1,
- * MIAIE_MAX_TOP_K]; sizes of a row in [1, 2^20]. */
+ * MIAIE_MAX_TOP_K]; sizes of a row in [1, 2^20].  In blocks of 128 x 128, the rows by the
+ * columns of a product's result (the MLP's: 2 F and Nout) are at most 2^22, those of a
+ * conversion's below 2^23; in blocks of 256 x 256, all experts' weight gradients are below
+ * 2^23. */
 MIAIE_API size_t miaie_experts_rows(int tokens, int top_k, int experts);
 MIAIE_API size_t miaie_experts_order_bytes(int tokens, int top_k, int experts);
 
@@ -574,9 +578,9 @@ MIAIE_API int miaie_experts_gemm_fp8(miaie_ctx* ctx, const int* order, const uin
 
 /* How that runs (swiglu 0), or the first product of miaie_experts_mlp_fp8 (swiglu 1:
  * N = F, K = D, tile_n columns of H), as miaie_plan_gemm_fp8 says it; workgroups: the
- * most that a routing can need; those of MIAIE_KERNEL_ROWS share out all fours of an
- * expert's rows.  Where tile_m is 256, an expert's last 128 slots or fewer are a tile of
- * 128 rows. */
+ * most that a routing can need, of which those of MIAIE_KERNEL_ROWS share out all fours
+ * of an expert's rows.  Where tile_m is 256, an expert's last 128 slots or fewer are a
+ * tile of 128 rows.  (The limits of 2^32 bytes are the entry points' own.) */
 MIAIE_API int miaie_plan_experts_fp8(int tokens, int top_k, int experts, int N, int K, int swiglu, int cus,
                                      miaie_gemm_plan* plan);
 

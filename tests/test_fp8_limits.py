@@ -27,6 +27,15 @@ def test_no_sizes_of_larger_ones(R, K):
     assert lib.miaie_fp8_q_bytes(R, K) == lib.miaie_fp8_s_bytes(R, K, 1) == lib.miaie_fp8_s_bytes(R, K, 128) == 0
 
 
+def test_the_largest_products_over_slots():
+    """2^22 blocks of 128 x 128: 8192 of slots by 512 of columns, gate and up counted both; not one more."""
+    assert mi.experts_rows(1 << 20, 1, 1) == 128 * 8192
+    for swiglu, N, unit in ((False, 65536, 1), (True, 32768, 128)):
+        assert mi.plan_experts_fp8(1 << 20, 1, 1, N, 128, swiglu)["workgroups"] > 0
+        with pytest.raises(mi.MiaieError, match="too large"):
+            mi.plan_experts_fp8(1 << 20, 1, 1, N + unit, 128, swiglu)
+
+
 def test_sizes_of_the_wrappers(tmp_path):
     """Undefined arithmetic ends the program."""
     exe = str(tmp_path / "host_experts_sizes_check")
