@@ -42,6 +42,7 @@ B_NN = 0
 B_NT = 1
 F32 = 0   # element types of unpacked matrices (MIAIE_F32, MIAIE_BF16)
 BF16 = 1
+F32_SLOTS = 16  # BF16 | F32_SLOTS: fp32 rows of slots beside a bf16 result (MIAIE_F32_SLOTS)
 MXFP4 = 2  # a packed result, for plan_gemm_mxfp4
 NORM_MAX_COLS = 16384
 SOFTMAX = 0  # scores of route_experts (MIAIE_SOFTMAX, MIAIE_SIGMOID)
@@ -254,6 +255,15 @@ def plan_gemm_mxfp4(M, N, K, out=F32, cus=256) -> dict:
     if rc != MIAIE_OK:
         raise MiaieError(rc, load_library().miaie_last_error_string(None).decode())
     return p.as_dict()
+
+
+def _slots_dtype(dtype: int, y_dtype: int | None) -> int:
+    """The C entries' dtype of a result and of the slots' rows Y behind it."""
+    if y_dtype is None or y_dtype == dtype:
+        return dtype
+    if (dtype, y_dtype) != (BF16, F32):
+        raise ValueError(f"Y of type {y_dtype} beside a result of type {dtype}: it has the result's type, or is F32")
+    return BF16 | F32_SLOTS
 
 
 def _plan(f, *args) -> dict:
@@ -577,10 +587,11 @@ class Context:
         self._compute(self._f_order, idx, order, tokens, top_k, experts)
 
     def experts_mlp_fp8(self, order, w, Xq, Xs, W1q, W1s, W2q, W2s, Hq, Hs, Y, out, tokens, top_k, experts, D, F, Nout,
-                        dtype=BF16, ldo=None) -> None:
-        """out = sum over a token's experts of w * (silu(X . Wg^T) * (X . Wu^T)) . W2^T."""
-        self._compute(self._f_x_mlp, order, w, Xq, Xs, W1q, W1s, W2q, W2s, Hq, Hs, Y, out, dtype, tokens, top_k, experts, D,
-                      F, Nout, Nout if ldo is None else ldo)
+                        dtype=BF16, ldo=None, y_dtype=None) -> None:
+        """out = sum over a token's experts of w * (silu(X . Wg^T) * (X . Wu^T)) . W2^T.  y_dtype: of Y, that of
+        out (dtype) or F32."""
+        self._compute(self._f_x_mlp, order, w, Xq, Xs, W1q, W1s, W2q, W2s, Hq, Hs, Y, out, _slots_dtype(dtype, y_dtype),
+                      tokens, top_k, experts, D, F, Nout, Nout if ldo is None else ldo)
 
     def experts_gemm_fp8(self, order, Aq, As, Bq, Bs, Cm, tokens, top_k, experts, N, K, gather=False, dtype=BF16,
                          ldc=None) -> None:
@@ -607,14 +618,15 @@ class Context:
         self._compute(self._f_x_wgrad, order, Atq, Ats, Btq, Bts, Cm, dtype, tokens, top_k, experts, M, N,
                       N if ldc is None else ldc)
 
-    def experts_combine(self, order, Y, w, out, tokens, top_k, experts, C, dtype=BF16, ldy=None, ldo=None) -> None:
-        """out = sum over a token's slots of w * Y[slot] (w None: of Y[slot])."""
-        self._compute(self._f_x_sum, order, Y, w, out, dtype, tokens, top_k, experts, C, C if ldy is None else ldy,
-                      C if ldo is None else ldo)
+    def experts_combine(self, order, Y, w, out, tokens, top_k, experts, C, dtype=BF16, ldy=None, ldo=None, y_dtype=None) -> None:
+        """out = sum over a token's slots of w * Y[slot] (w None: of Y[slot]).  y_dtype: of Y, that of out (dtype) or F32."""
+        self._compute(self._f_x_sum, order, Y, w, out, _slots_dtype(dtype, y_dtype), tokens, top_k, experts, C,
+                      C if ldy is None else ldy, C if ldo is None else ldo)
 
-    def experts_combine_grad(self, order, Y, dout, dw, tokens, top_k, experts, C, dtype=BF16, ldy=None, ldo=None) -> None:
-        self._compute(self._f_x_sum_grad, order, Y, dout, dw, dtype, tokens, top_k, experts, C, C if ldy is None else ldy,
-                      C if ldo is None else ldo)
+    def experts_combine_grad(self, order, Y, dout, dw, tokens, top_k, experts, C, dtype=BF16, ldy=None, ldo=None,
+                             y_dtype=None) -> None:
+        self._compute(self._f_x_sum_grad, order, Y, dout, dw, _slots_dtype(dtype, y_dtype), tokens, top_k, experts, C,
+                      C if ldy is None else ldy, C if ldo is None else ldo)
 
 
 def version() -> str:

@@ -29,6 +29,14 @@ int check_dtype(miaie_ctx* ctx, const char* fn, int dtype) {
   return MIAIE_OK;
 }
 
+// dtype of a result over tokens, and that of the slots' rows behind it.
+int check_slot_dtypes(miaie_ctx* ctx, const char* fn, int* dtype, int* y_dtype) {
+  const bool wide = *dtype == (MIAIE_BF16 | MIAIE_F32_SLOTS);
+  if (wide) *dtype = MIAIE_BF16;
+  *y_dtype = wide ? MIAIE_F32 : *dtype;
+  return check_dtype(ctx, fn, *dtype);
+}
+
 int check_block(miaie_ctx* ctx, const char* fn, const char* name, int block) {
   if (block != 1 && block != 128) return fail(ctx, MIAIE_EINVAL, "%s: %s=%d is neither 1 nor 128", fn, name, block);
   return MIAIE_OK;
@@ -259,9 +267,10 @@ extern "C" int miaie_experts_mlp_fp8(miaie_ctx* ctx, const int* order, const flo
                                      const uint8_t* W1q, const float* W1s, const uint8_t* W2q, const float* W2s, uint8_t* Hq,
                                      float* Hs, void* Y, void* out, int dtype, int tokens, int top_k, int experts, int D,
                                      int F, int Nout, int ldo) {
+  int y_dtype;
   MIAIE_TRY(enter(ctx));
   MIAIE_TRY(check_order(ctx, __func__, order, tokens, top_k, experts));
-  MIAIE_TRY(check_dtype(ctx, __func__, dtype));
+  MIAIE_TRY(check_slot_dtypes(ctx, __func__, &dtype, &y_dtype));
   MIAIE_TRY(check_width(ctx, __func__, "D", D));
   MIAIE_TRY(check_hidden(ctx, __func__, F));
   MIAIE_TRY(check_width(ctx, __func__, "Nout", Nout));
@@ -270,7 +279,7 @@ extern "C" int miaie_experts_mlp_fp8(miaie_ctx* ctx, const int* order, const flo
   MIAIE_TRY(check_packed(ctx, __func__, "W1", W1q, W1s));
   MIAIE_TRY(check_packed(ctx, __func__, "W2", W2q, W2s));
   MIAIE_TRY(check_packed(ctx, __func__, "H", Hq, Hs));
-  MIAIE_TRY(check_elements(ctx, __func__, "Y", Y, dtype));
+  MIAIE_TRY(check_elements(ctx, __func__, "Y", Y, y_dtype));
   MIAIE_TRY(check_elements(ctx, __func__, "out", out, dtype));
   MIAIE_TRY(check_pitch(ctx, __func__, "ldo", ldo, Nout));
   MIAIE_TRY(check_slot_product(ctx, __func__, tokens, top_k, experts, 2l * F, D, true));
@@ -279,8 +288,8 @@ extern "C" int miaie_experts_mlp_fp8(miaie_ctx* ctx, const int* order, const flo
     return fail(ctx, MIAIE_EINVAL, "%s: 2 F = %d rows of D = %d columns are 2^32 bytes or more", __func__, 2 * F, D);
   const fp8::Slots s = fp8::slots_of(order, tokens, top_k, experts);
   MIAIE_TRY(launch_experts_glu_fp8(ctx, s, Xq, Xs, W1q, W1s, Hq, Hs, D, F));
-  MIAIE_TRY(launch_experts_gemm_fp8(ctx, s, Hq, Hs, 0, W2q, W2s, Y, dtype, Nout, F, Nout));
-  return launch_experts_combine(ctx, s, Y, w, out, dtype, Nout, Nout, ldo);
+  MIAIE_TRY(launch_experts_gemm_fp8(ctx, s, Hq, Hs, 0, W2q, W2s, Y, y_dtype, Nout, F, Nout));
+  return launch_experts_combine(ctx, s, Y, y_dtype, w, out, dtype, Nout, Nout, ldo);
 }
 
 extern "C" int miaie_experts_gemm_fp8(miaie_ctx* ctx, const int* order, const uint8_t* Aq, const float* As,
@@ -379,28 +388,31 @@ extern "C" int miaie_experts_wgrad_fp8(miaie_ctx* ctx, const int* order, const u
 
 extern "C" int miaie_experts_combine(miaie_ctx* ctx, const int* order, const void* Y, const float* w, void* out, int dtype,
                                      int tokens, int top_k, int experts, int C, int ldy, int ldo) {
+  int y_dtype;
   MIAIE_TRY(enter(ctx));
   MIAIE_TRY(check_order(ctx, __func__, order, tokens, top_k, experts));
-  MIAIE_TRY(check_dtype(ctx, __func__, dtype));
+  MIAIE_TRY(check_slot_dtypes(ctx, __func__, &dtype, &y_dtype));
   MIAIE_TRY(check_width(ctx, __func__, "C", C));
-  MIAIE_TRY(check_elements(ctx, __func__, "Y", Y, dtype));
+  MIAIE_TRY(check_elements(ctx, __func__, "Y", Y, y_dtype));
   MIAIE_TRY(check_array(ctx, __func__, "w", w, 4, true));
   MIAIE_TRY(check_elements(ctx, __func__, "out", out, dtype));
   MIAIE_TRY(check_pitch(ctx, __func__, "ldy", ldy, C));
   MIAIE_TRY(check_pitch(ctx, __func__, "ldo", ldo, C));
-  return launch_experts_combine(ctx, fp8::slots_of(order, tokens, top_k, experts), Y, w, out, dtype, C, ldy, ldo);
+  return launch_experts_combine(ctx, fp8::slots_of(order, tokens, top_k, experts), Y, y_dtype, w, out, dtype, C, ldy, ldo);
 }
 
 extern "C" int miaie_experts_combine_grad(miaie_ctx* ctx, const int* order, const void* Y, const void* dout, float* dw,
                                           int dtype, int tokens, int top_k, int experts, int C, int ldy, int ldo) {
+  int y_dtype;
   MIAIE_TRY(enter(ctx));
   MIAIE_TRY(check_order(ctx, __func__, order, tokens, top_k, experts));
-  MIAIE_TRY(check_dtype(ctx, __func__, dtype));
+  MIAIE_TRY(check_slot_dtypes(ctx, __func__, &dtype, &y_dtype));
   MIAIE_TRY(check_width(ctx, __func__, "C", C));
-  MIAIE_TRY(check_elements(ctx, __func__, "Y", Y, dtype));
+  MIAIE_TRY(check_elements(ctx, __func__, "Y", Y, y_dtype));
   MIAIE_TRY(check_elements(ctx, __func__, "dout", dout, dtype));
   MIAIE_TRY(check_array(ctx, __func__, "dw", dw, 4));
   MIAIE_TRY(check_pitch(ctx, __func__, "ldy", ldy, C));
   MIAIE_TRY(check_pitch(ctx, __func__, "ldo", ldo, C));
-  return launch_experts_combine_grad(ctx, fp8::slots_of(order, tokens, top_k, experts), Y, dout, dw, dtype, C, ldy, ldo);
+  return launch_experts_combine_grad(ctx, fp8::slots_of(order, tokens, top_k, experts), Y, y_dtype, dout, dw, dtype, C, ldy,
+                                     ldo);
 }

@@ -212,10 +212,10 @@ int launch_experts_glu_fp8(miaie_ctx* ctx, const fp8::Slots& s, const uint8_t* X
                            const float* W1s, uint8_t* Hq, float* Hs, int D, int F);
 int launch_experts_wgrad_fp8(miaie_ctx* ctx, const fp8::Slots& s, const uint8_t* Atq, const float* Ats, const uint8_t* Btq,
                              const float* Bts, void* C, int dtype, int M, int N, int ldc);
-int launch_experts_combine(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, const float* w, void* out, int dtype, int C,
-                           int ldy, int ldo);
-int launch_experts_combine_grad(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, const void* dout, float* dw, int dtype,
-                                int C, int ldy, int ldo);
+int launch_experts_combine(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, int y_dtype, const float* w, void* out,
+                           int dtype, int C, int ldy, int ldo);
+int launch_experts_combine_grad(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, int y_dtype, const void* dout, float* dw,
+                                int dtype, int C, int ldy, int ldo);
 
 }  // namespace miaie
 

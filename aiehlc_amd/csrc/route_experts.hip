@@ -428,12 +428,10 @@ __global__ __launch_bounds__(kOrderThreads) void order_slots(const int* __restri
 }
 
 // out[t] = sum over the choices j, in their order, of w[t][j] Y[slot]: eight columns
-// a thread.  Sums are fp32; Y has out's type, so that with bf16 each term has been rounded
-// once before.  That is a choice for bytes: 16384 slots of 4096 columns in fp32 are 134 MB
-// more to write and as many to read, 42 us of an MLP's 423 (64 experts, 4096 x 1024), and
-// who wants them asks for fp32 results.
-template <class T>
-__global__ __launch_bounds__(256) void combine(const T* __restrict__ Y, const float* __restrict__ w, T* __restrict__ out,
+// a thread.  Sums are fp32; with Y in bf16 each term has been rounded once before, which
+// the caller chooses.
+template <class TY, class T>
+__global__ __launch_bounds__(256) void combine(const TY* __restrict__ Y, const float* __restrict__ w, T* __restrict__ out,
                                                Slots s, int C, int ldy, int ldo, int per_row, long units, long stride) {
   for (long u = blockIdx.x * 256l + threadIdx.x; u < units; u += stride) {
     const int t = (int)(u / per_row), c = 8 * (int)(u % per_row);
@@ -458,8 +456,8 @@ __global__ __launch_bounds__(256) void combine(const T* __restrict__ Y, const fl
 }
 
 // dw[t][j] = <dout[t], Y[slot]>, a wave a pair; 0 without an expert.
-template <class T>
-__global__ __launch_bounds__(256) void combine_grad(const T* __restrict__ Y, const T* __restrict__ dout,
+template <class TY, class T>
+__global__ __launch_bounds__(256) void combine_grad(const TY* __restrict__ Y, const T* __restrict__ dout,
                                                     float* __restrict__ dw, Slots s, int C, int ldy, int ldo, int pairs) {
   const int lane = threadIdx.x & 63;
   const int pair = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -476,6 +474,13 @@ __global__ __launch_bounds__(256) void combine_grad(const T* __restrict__ Y, con
     }
   sum = over_wave(sum, Add{});
   if (lane == 0) MIAIE_ST(dw + pair, sum);
+}
+
+// f(type of Y, type of the result or its gradient): the same, or fp32 and bf16
+template <class F>
+int with_slot_types(int y_dtype, int dtype, F&& f) {
+  if (dtype != MIAIE_BF16) return f(type_t<float>{}, type_t<float>{});
+  return y_dtype == MIAIE_BF16 ? f(type_t<__bf16>{}, type_t<__bf16>{}) : f(type_t<float>{}, type_t<__bf16>{});
 }
 
 // f(type of the logits, number of a lane's places)
@@ -552,33 +557,33 @@ int launch_experts_order(miaie_ctx* ctx, const fp8::Slots& s, const int* idx) {
   return check_launch(ctx, e, "order_slots");
 }
 
-int launch_experts_combine(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, const float* w, void* out, int dtype, int C,
-                           int ldy, int ldo) {
+int launch_experts_combine(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, int y_dtype, const float* w, void* out,
+                           int dtype, int C, int ldy, int ldo) {
   const int per_row = (C + 7) / 8;
   const long units = (long)s.tokens * per_row, grid = std::min((units + 255) / 256, 1l << 22);
-  auto go = [&](auto t) {
+  return with_slot_types(y_dtype, dtype, [&](auto ty, auto t) {
+    using TY = typename decltype(ty)::type;
     using T = typename decltype(t)::type;
     return check_launch(ctx,
-                        launch<combine<T>>(ctx->device, dim3((unsigned)grid), dim3(256), 0, ctx->stream,
-                                           static_cast<const T*>(Y), w, static_cast<T*>(out), s, C, ldy, ldo, per_row, units,
-                                           256 * grid),
+                        launch<combine<TY, T>>(ctx->device, dim3((unsigned)grid), dim3(256), 0, ctx->stream,
+                                               static_cast<const TY*>(Y), w, static_cast<T*>(out), s, C, ldy, ldo, per_row,
+                                               units, 256 * grid),
                         "experts_combine");
-  };
-  return dtype == MIAIE_BF16 ? go(type_t<__bf16>{}) : go(type_t<float>{});
+  });
 }
 
-int launch_experts_combine_grad(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, const void* dout, float* dw, int dtype,
-                                int C, int ldy, int ldo) {
+int launch_experts_combine_grad(miaie_ctx* ctx, const fp8::Slots& s, const void* Y, int y_dtype, const void* dout, float* dw,
+                                int dtype, int C, int ldy, int ldo) {
   const int pairs = s.tokens * s.top_k;
-  auto go = [&](auto t) {
+  return with_slot_types(y_dtype, dtype, [&](auto ty, auto t) {
+    using TY = typename decltype(ty)::type;
     using T = typename decltype(t)::type;
     return check_launch(ctx,
-                        launch<combine_grad<T>>(ctx->device, dim3((pairs + 3u) / 4), dim3(256), 0, ctx->stream,
-                                                static_cast<const T*>(Y), static_cast<const T*>(dout), dw, s, C, ldy, ldo,
-                                                pairs),
+                        launch<combine_grad<TY, T>>(ctx->device, dim3((pairs + 3u) / 4), dim3(256), 0, ctx->stream,
+                                                    static_cast<const TY*>(Y), static_cast<const T*>(dout), dw, s, C, ldy,
+                                                    ldo, pairs),
                         "experts_combine_grad");
-  };
-  return dtype == MIAIE_BF16 ? go(type_t<__bf16>{}) : go(type_t<float>{});
+  });
 }
 
 }  // namespace miaie

@@ -542,6 +542,7 @@ MIAIE_API int miaie_route_experts_grad(miaie_ctx* ctx, const void* logits, int d
  * columns of a product's result (the MLP's: 2 F and Nout) are at most 2^22, those of a
  * conversion's below 2^23; in blocks of 256 x 256, all experts' weight gradients are below
  * 2^23. */
+#define MIAIE_F32_SLOTS 16 /* MIAIE_BF16 | MIAIE_F32_SLOTS: fp32 Y beside a bf16 result */
 MIAIE_API size_t miaie_experts_rows(int tokens, int top_k, int experts);
 MIAIE_API size_t miaie_experts_order_bytes(int tokens, int top_k, int experts);
 
@@ -556,12 +557,11 @@ MIAIE_API int miaie_experts_order(miaie_ctx* ctx, const int* idx, int* order, in
  * X tokens x D packed along its rows (block 1).  W1: the experts' 2 F x D matrices,
  * gate rows then up rows, each packed with block 128, one after another; W2 likewise
  * Nout x F.  F is a multiple of 128 (pad with zero rows of W1).  H (Hq, Hs: packed,
- * rows x F) and Y (rows x Nout, dense, of type dtype, to which it is rounded) are
- * caller-provided device scratch; out, tokens x Nout of type dtype, row pitch ldo.
- * Gate, up and their product stay in fp32 until H is packed.  With MIAIE_BF16 every Y[slot]
- * is rounded before it is added, and the sum once more (together 0.0024 of the result in
- * the 2-norm, 0.0017 of one rounding alone); with MIAIE_F32 nothing behind H is rounded to
- * fewer bits.  tokens times a packed
+ * rows x F) and Y (rows x Nout, dense) are caller-provided device scratch; out, tokens x
+ * Nout, row pitch ldo.  dtype: MIAIE_F32 or MIAIE_BF16 of both Y and out, or MIAIE_BF16 |
+ * MIAIE_F32_SLOTS: Y fp32, out bf16.  Gate, up and their product stay in fp32 until H is
+ * packed; behind it only what is bf16 is rounded.  (Y in bf16 adds a rounding of each term:
+ * 0.0024 of the result in the 2-norm for 0.0017; Y in fp32 twice the bytes.)  tokens times a packed
  * row of X, and 2 F times one, are below 2^32 bytes. */
 MIAIE_API int miaie_experts_mlp_fp8(miaie_ctx* ctx, const int* order, const float* w, const uint8_t* Xq, const float* Xs,
                                     const uint8_t* W1q, const float* W1s, const uint8_t* W2q, const float* W2s,
@@ -613,11 +613,12 @@ MIAIE_API int miaie_experts_wgrad_fp8(miaie_ctx* ctx, const int* order, const ui
 
 /* out[t] = sum over its slots, in the order of its choices, of w * Y[slot] (w NULL:
  * of Y[slot]), fp32 sums: Y rows x C, row pitch ldy, out tokens x C, row pitch ldo,
- * both of type dtype.  A pair without a slot adds w * 0. */
+ * both of type dtype, or fp32 and bf16 with MIAIE_BF16 | MIAIE_F32_SLOTS.  A pair without a
+ * slot adds w * 0. */
 MIAIE_API int miaie_experts_combine(miaie_ctx* ctx, const int* order, const void* Y, const float* w, void* out, int dtype,
                                     int tokens, int top_k, int experts, int C, int ldy, int ldo);
-/* dw (fp32 tokens x top_k) of it: dw = <dout[t], Y[slot]>, 0 without a slot.  (The
- * gradient of Y is dout times w: miaie_experts_quant_fp8.) */
+/* dw (fp32 tokens x top_k) of it: dw = <dout[t], Y[slot]>, 0 without a slot; dout and Y of
+ * the types of out and Y.  (The gradient of Y is dout times w: miaie_experts_quant_fp8.) */
 MIAIE_API int miaie_experts_combine_grad(miaie_ctx* ctx, const int* order, const void* Y, const void* dout, float* dw,
                                          int dtype, int tokens, int top_k, int experts, int C, int ldy, int ldo);
 

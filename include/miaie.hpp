@@ -27,6 +27,7 @@
 #include <cstdint>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -549,10 +550,20 @@ inline void experts_order(const Buffer<int32_t>& idx, ExpertsOrder& o, Context& 
   ctx.check(miaie_experts_order(ctx.get(), idx.data(), o.order.data(), o.tokens, o.top_k, o.experts));
 }
 
+namespace detail {
+// Y and the result of one type, or fp32 and bf16
+template <typename TY, typename T>
+int slots_dtype(const Buffer<TY>&, const Buffer<T>& out) {
+  constexpr bool wide = std::is_same_v<TY, float> && !std::is_same_v<T, float>;
+  static_assert(wide || std::is_same_v<TY, T>, "Y has the result's type, or is fp32");
+  return dtype_of(out.data()) | (wide ? MIAIE_F32_SLOTS : 0);
+}
+}  // namespace detail
+
 // out[t] = sum over t's experts of w (H . W2^T), H = pack(silu(gate) up) of X . W1^T.
-template <typename T>
+template <typename TY, typename T>
 void experts_mlp_fp8(const ExpertsOrder& o, const Buffer<float>& w, const Fp8Matrix& X, const Fp8Matrix& W1, const Fp8Matrix& W2,
-                     Fp8Matrix& H, Buffer<T>& Y, Buffer<T>& out, Context& ctx = Context::current()) {
+                     Fp8Matrix& H, Buffer<TY>& Y, Buffer<T>& out, Context& ctx = Context::current()) {
   detail::require(detail::is(X, o.tokens, X.cols, 1), "experts_mlp_fp8", "X is not the tokens' rows");
   detail::require(W1.rows == 2l * W2.cols && detail::is(W1, W1.rows, X.cols, 128, o.experts) &&
                       detail::is(W2, W2.rows, W2.cols, 128, o.experts),
@@ -562,8 +573,8 @@ void experts_mlp_fp8(const ExpertsOrder& o, const Buffer<float>& w, const Fp8Mat
                       detail::holds(out, o.tokens, W2.rows),
                   "experts_mlp_fp8", "w, Y or out is too small");
   ctx.check(miaie_experts_mlp_fp8(ctx.get(), o.order.data(), w.data(), X.q.data(), X.s.data(), W1.q.data(), W1.s.data(),
-                                  W2.q.data(), W2.s.data(), H.q.data(), H.s.data(), Y.data(), out.data(), dtype_of(out.data()),
-                                  o.tokens, o.top_k, o.experts, X.cols, W2.cols, W2.rows, W2.rows));
+                                  W2.q.data(), W2.s.data(), H.q.data(), H.s.data(), Y.data(), out.data(),
+                                  detail::slots_dtype(Y, out), o.tokens, o.top_k, o.experts, X.cols, W2.cols, W2.rows, W2.rows));
 }
 
 // C[slot] = A[slot] . B_e^T; with gather A has the tokens' rows.
@@ -626,24 +637,24 @@ void experts_wgrad_fp8(const ExpertsOrder& o, const Fp8Matrix& At, const Fp8Matr
 }
 
 // out[t] = sum over t's slots of w Y[slot] (w NULL: of Y[slot]).
-template <typename T>
-void experts_combine(const ExpertsOrder& o, const Buffer<T>& Y, const Buffer<float>* w, Buffer<T>& out, int cols,
+template <typename TY, typename T>
+void experts_combine(const ExpertsOrder& o, const Buffer<TY>& Y, const Buffer<float>* w, Buffer<T>& out, int cols,
                      Context& ctx = Context::current()) {
   detail::require(detail::holds(Y, o.rows(), cols) && detail::holds(out, o.tokens, cols) &&
                       (!w || detail::holds(*w, o.tokens, o.top_k)),
                   "experts_combine", "Y, out or w is too small");
-  ctx.check(miaie_experts_combine(ctx.get(), o.order.data(), Y.data(), detail::data(w), out.data(), dtype_of(out.data()),
-                                  o.tokens, o.top_k, o.experts, cols, cols, cols));
+  ctx.check(miaie_experts_combine(ctx.get(), o.order.data(), Y.data(), detail::data(w), out.data(),
+                                  detail::slots_dtype(Y, out), o.tokens, o.top_k, o.experts, cols, cols, cols));
 }
 
-template <typename T>
-void experts_combine_grad(const ExpertsOrder& o, const Buffer<T>& Y, const Buffer<T>& dout, Buffer<float>& dw, int cols,
+template <typename TY, typename T>
+void experts_combine_grad(const ExpertsOrder& o, const Buffer<TY>& Y, const Buffer<T>& dout, Buffer<float>& dw, int cols,
                           Context& ctx = Context::current()) {
   detail::require(detail::holds(Y, o.rows(), cols) && detail::holds(dout, o.tokens, cols) &&
                       detail::holds(dw, o.tokens, o.top_k),
                   "experts_combine_grad", "Y, dout or dw is too small");
-  ctx.check(miaie_experts_combine_grad(ctx.get(), o.order.data(), Y.data(), dout.data(), dw.data(), dtype_of(Y.data()), o.tokens,
-                                       o.top_k, o.experts, cols, cols, cols));
+  ctx.check(miaie_experts_combine_grad(ctx.get(), o.order.data(), Y.data(), dout.data(), dw.data(), detail::slots_dtype(Y, dout),
+                                       o.tokens, o.top_k, o.experts, cols, cols, cols));
 }
 
 }  // namespace miaie

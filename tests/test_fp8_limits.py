@@ -36,6 +36,15 @@ def test_the_largest_products_over_slots():
             mi.plan_experts_fp8(1 << 20, 1, 1, N + unit, 128, swiglu)
 
 
+def test_types_of_slots_rows():
+    """What reaches the entry point as its dtype for the types of a result and of the slots' rows."""
+    assert [mi._slots_dtype(*t) for t in ((mi.F32, None), (mi.BF16, None), (mi.F32, mi.F32), (mi.BF16, mi.BF16), (mi.BF16, mi.F32))] \
+        == [mi.F32, mi.BF16, mi.F32, mi.BF16, mi.BF16 | mi.F32_SLOTS]
+    for bad in ((mi.F32, mi.BF16), (mi.BF16, 2), (2, mi.F32)):
+        with pytest.raises(ValueError):
+            mi._slots_dtype(*bad)
+
+
 def test_sizes_of_the_wrappers(tmp_path):
     """Undefined arithmetic ends the program."""
     exe = str(tmp_path / "host_experts_sizes_check")
