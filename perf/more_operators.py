@@ -236,11 +236,11 @@ def prepare(case: dict, seed: int) -> dict:
             s["order"] = _empty(i32, 2 * E + 64 + T * k + R + R // 128)
             if op == "experts":
                 s["Xq"], s["Hq"] = packed(T, D), packed(R, F)
-                s["Y_"], s["out_"] = _empty(bf, R, D), _empty(bf, T, D)
+                s["Y_"], s["out_"] = _empty(f32, R, D), _empty(bf, T, D)
             else:
                 s["dYq"], s["dYt"], s["Ht"], s["Xt"] = packed(R, D), packed(D, R), packed(F, R), packed(D, R)
                 s["dGUq"], s["dGUt"] = packed(R, 2 * F), packed(2 * F, R)
-                s["dH_"], s["dXs_"], s["dX_"] = _empty(f32, R, F), _empty(bf, R, D), _empty(bf, T, D)
+                s["dH_"], s["dXs_"], s["dX_"] = _empty(f32, R, F), _empty(f32, R, D), _empty(bf, T, D)
                 s["dW1_"], s["dW2_"] = _empty(bf, E, 2 * F, D), _empty(bf, E, D, F)
                 s["dw_"], s["dlogits_"] = _empty(f32, T, k), _empty(f32, T, E)
     s["case"] = dict(case)
@@ -334,7 +334,7 @@ def _run_own(s: dict):
         ctx.experts_order(_p(s["idx_"]), order, *n)
         ctx.quant_fp8(_p(s["X"]), T, D, *xq, dtype=_BF16)
         ctx.experts_mlp_fp8(order, _p(s["w_"]), *xq, *_pp(s["W1"]), *_pp(s["W2"]), *_pp(s["Hq"]), _p(s["Y_"]),
-                            _p(s["out_"]), *n, D, F, D, dtype=_BF16)
+                            _p(s["out_"]), *n, D, F, D, dtype=_BF16, y_dtype=_F32)
         return s["idx_"], s["w_"], s["out_"]
     dyq, dyt, dguq, dgut = _pp(s["dYq"]), _pp(s["dYt"]), _pp(s["dGUq"]), _pp(s["dGUt"])
     ht, xt, dh = _pp(s["Ht"]), _pp(s["Xt"]), _p(s["dH_"])
@@ -347,8 +347,8 @@ def _run_own(s: dict):
     ctx.experts_gemm_fp8(order, *dyq, *_pp(s["W2t"]), dh, *n, F, D, dtype=_F32)
     ctx.experts_swiglu_fp8(order, _p(s["GU"]), None, None, *ht, *n, F, dtype=_BF16)
     ctx.experts_swiglu_grad_fp8(order, _p(s["GU"]), dh, *dguq, *dgut, *n, F, dtype=_BF16)
-    ctx.experts_gemm_fp8(order, *dguq, *_pp(s["W1t"]), _p(s["dXs_"]), *n, D, 2 * F, dtype=_BF16)
-    ctx.experts_combine(order, _p(s["dXs_"]), None, _p(s["dX_"]), *n, D, dtype=_BF16)
+    ctx.experts_gemm_fp8(order, *dguq, *_pp(s["W1t"]), _p(s["dXs_"]), *n, D, 2 * F, dtype=_F32)
+    ctx.experts_combine(order, _p(s["dXs_"]), None, _p(s["dX_"]), *n, D, dtype=_BF16, y_dtype=_F32)
     ctx.experts_wgrad_fp8(order, *dyt, *ht, _p(s["dW2_"]), *n, D, F, dtype=_BF16)
     ctx.experts_wgrad_fp8(order, *dgut, *xt, _p(s["dW1_"]), *n, 2 * F, D, dtype=_BF16)
     return s["dX_"], s["dW1_"], s["dW2_"], s["dlogits_"]
