@@ -316,7 +316,7 @@ __global__ __launch_bounds__(256) void route_tokens_grad(const T* __restrict__ l
 // of it the placing; by 16 of them 6.4.)  Up to some 10^5 pairs the launch is most of the
 // time; beyond, that every workgroup counts all: 131072 pairs of 64 experts 21 us, 2^23 of
 // them 1.2 ms, and 115 us and 7.1 ms where all have one expert, whose count the 64 lanes
-// of a wave raise one by one (products over as many slots take some ten times as long).
+// of a wave raise one by one.
 constexpr int kOrderWaves = 16, kOrderThreads = 64 * kOrderWaves, kOrderGroups = 64;
 __global__ __launch_bounds__(kOrderThreads) void order_slots(const int* __restrict__ idx, int* __restrict__ start,
                                                              int* __restrict__ count, int* __restrict__ slot_of,
